@@ -1,0 +1,80 @@
+// kvops.h -- launch interface of the KV-cache operators (kvops.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace s2 {
+
+// Head shape of a handle and its device words.
+struct KvShape {
+  uint32_t H, G, rep;  // query heads, kv heads, H / G
+  float scale;         // of the scores
+  float eps;
+  const double* freq;  // [hd / 2] rope_base^(-2 i / hd)
+  uint32_t* err;       // S2HIP_KV_ERR_* bits are or-ed in
+};
+
+// The caches of a call (strides in elements, all set).
+struct KvCaches {
+  void* k;
+  void* v;
+  const void* pk;
+  const void* pv;
+  const int32_t* lens;
+  const int32_t* new_lens;  // nullable
+  size_t req_stride, head_stride, slot_stride, p_head_stride, p_slot_stride;
+  uint32_t R, cap, P, n;    // requests, capacity, prefix length, tokens per request
+};
+
+struct KvAppendArgs {
+  KvShape s;
+  KvCaches c;
+  const float* qkv;
+  const int32_t* positions;
+  const float* q_norm;  // nullable, with k_norm
+  const float* k_norm;
+  float* q_out;
+  float* scores;            // nullable
+  int32_t* slot_positions;  // nullable
+};
+
+struct KvWorkspace {
+  float* stat;  // [tokens][H][2]: a row's maximum and sum (attention with weights)
+  uint32_t* moves;     // [cap_moves] (from << 16 | to)
+  uint32_t* counts;    // [cap_seqs][2]: moves, slots left
+  size_t cap_moves, cap_seqs;
+};
+
+struct KvAttendArgs {
+  KvShape s;
+  KvCaches c;
+  const float* q;
+  float* out;
+  // with weights (nullable):
+  const float* w_in;   // nullable
+  float* w_out;
+  const float* pw_in;  // nullable
+  float* pw_out;       // nullable
+  uint32_t pw_stride;  // prefix_capacity
+};
+
+struct KvEvictArgs {
+  KvShape s;
+  KvCaches c;
+  size_t layer_stride;
+  uint32_t layers, keep, recent, sinks;
+  const float* scores;
+  const int32_t* positions;
+  float* scores_out;
+  int32_t* positions_out;
+  int32_t* lens_out;
+};
+
+hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStream_t s);
+hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const KvWorkspace& w, hipStream_t s);
+hipError_t launch_kv_evict(uint32_t hd, bool f16, const KvEvictArgs& a, const KvWorkspace& w, hipStream_t s);
+hipError_t launch_kv_take_errors(uint32_t* err, uint32_t* taken, hipStream_t s);
+
+}  // namespace s2

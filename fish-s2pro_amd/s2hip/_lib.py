@@ -79,6 +79,20 @@ class SlowProfile(ctypes.Structure):
                                                "kv_write_ms", "swiglu_ms", "output_head_ms")] + [
         ("steps", ctypes.c_uint32)]
 
+
+class KvConfig(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int32)] + [
+        (n, ctypes.c_uint32) for n in ("heads", "kv_heads", "head_dim", "kv_f16", "max_requests", "max_tokens")] + [
+        (n, ctypes.c_float) for n in ("rope_base", "eps", "scale")]
+
+
+class KvView(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "lens", "new_lens", "prefix_k", "prefix_v")] + [
+        (n, ctypes.c_uint64) for n in ("request_stride", "head_stride", "slot_stride", "prefix_head_stride",
+                                       "prefix_slot_stride")] + [
+        (n, ctypes.c_uint32) for n in ("requests", "capacity", "prefix_len", "prefix_capacity")]
+
+
 _lib = None
 
 
@@ -174,6 +188,18 @@ def load():
     for name in ("s2hip_codec_rvq_lookup", "s2hip_codec_post_module", "s2hip_codec_upsample",
                  "s2hip_codec_decode_latents", "s2hip_codec_decoder", "s2hip_codec_decode_waveform",
                  "s2hip_codec_decode_waveform_device", "s2hip_codec_time"):
+        getattr(L, name).restype = i32
+    view = ctypes.POINTER(KvView)
+    L.s2hip_kv_open.argtypes = [ctypes.POINTER(KvConfig), cp, sz]
+    L.s2hip_kv_open.restype = vp
+    L.s2hip_kv_close.argtypes = [vp]
+    L.s2hip_kv_close.restype = None
+    L.s2hip_kv_errors.argtypes = [vp, vp, ctypes.POINTER(u32), cp, sz]
+    L.s2hip_kv_append.argtypes = [vp, view, vp, u32, vp, vp, vp, vp, vp, vp, vp, cp, sz]
+    L.s2hip_kv_attend.argtypes = [vp, view, vp, u32, vp, vp, cp, sz]
+    L.s2hip_kv_attend_weigh.argtypes = [vp, view, vp, u32, vp, vp, vp, vp, vp, vp, cp, sz]
+    L.s2hip_kv_evict.argtypes = [vp, view, u32, ctypes.c_uint64, u32, u32, u32, vp, vp, vp, vp, vp, vp, cp, sz]
+    for name in ("s2hip_kv_errors", "s2hip_kv_append", "s2hip_kv_attend", "s2hip_kv_attend_weigh", "s2hip_kv_evict"):
         getattr(L, name).restype = i32
     _lib = L
     return L

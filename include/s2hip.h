@@ -8,7 +8,9 @@
  * 1 = success / 0 = failure, and the failure text copied (truncated,
  * NUL-terminated) into a caller-provided err buffer of err_cap bytes.
  * No HIP, torch or device types cross this boundary: inputs are caller-owned
- * host pointers and outputs go to caller-provided host buffers.
+ * host pointers and outputs go to caller-provided host buffers, except where an
+ * entry point says that it takes device memory (the KV-cache operators, the
+ * codec's _device call).
  *
  * Threading: a handle is not thread-safe; the caller serialises calls on one
  * handle, as the reference serialises InferenceEngine behind a Mutex
@@ -382,6 +384,128 @@ void s2hip_codec_snake_host(const float* x, size_t n, const float* alpha, float*
  * No counterpart in the reference (a measurement hook). */
 int32_t s2hip_codec_time(s2hip_codec* codec, const char* what, uint32_t n_frames, uint32_t reps, double* avg_us,
                          double* flops, char* err, size_t err_cap);
+
+/* ---------------------------------------------------------------------------
+ * KV-cache operators on device memory: what a caller that keeps many requests'
+ * caches on the GPU runs per layer, next to the op level above.  No
+ * counterpart in the reference, which keeps one sequence and one cache
+ * (slow_ar.rs:372-438) and refuses a call that would overflow it (:469-474).
+ *
+ * Pointers are device memory of the handle's device, in the caller's hands;
+ * activations are f32, caches f32 or f16 (kv_f16).  Calls launch on `stream`
+ * (a hipStream_t as an opaque pointer; NULL: the default stream), allocate
+ * nothing, wait for nothing and can be captured into a HIP graph; the current
+ * device is the same after a call as before.  A handle's workspace serves one
+ * call at a time: calls on one handle, and replays of graphs captured from it,
+ * have to follow one another on the device (one stream, or ordered by
+ * events); streams and graphs that run side by side take a handle each.
+ *
+ * lens and new_lens are read on the device, so a captured call follows them.
+ * A request whose values are out of range (lens outside [0, capacity];
+ * new_lens outside [0, n_tokens] or above lens) takes no part in the call --
+ * its rows, slots and outputs stay as they were -- and sets
+ * S2HIP_KV_ERR_LENS, which s2hip_kv_errors reports.
+ * ------------------------------------------------------------------------- */
+typedef struct s2hip_kv s2hip_kv;
+
+#define S2HIP_KV_ERR_LENS 1u      /* a request's lens / new_lens out of range: it was left out */
+#define S2HIP_KV_ERR_POSITION 2u  /* append: a negative position: the request's token was left out */
+#define S2HIP_KV_ERR_F16_RANGE 4u /* append: a key or value beyond the f16 range went into an f16 cache */
+
+typedef struct {
+  int32_t device;
+  uint32_t heads, kv_heads; /* heads: a multiple of kv_heads, at most 64 times it */
+  uint32_t head_dim;        /* 64 or 128 */
+  uint32_t kv_f16;          /* 1: caches hold f16 (rounded to nearest even when written), 0: f32 */
+  uint32_t max_requests;    /* 1..256: requests per call */
+  uint32_t max_tokens;      /* 1..65536: requests * n_tokens per call */
+  float rope_base;          /* > 0 */
+  float eps;                /* of the head norms, >= 0 */
+  float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+} s2hip_kv_config;
+
+/* Where the caches are.  Own caches: request b's key of kv head g in slot s is
+ * the head_dim elements at k + b * request_stride + g * head_stride + s *
+ * slot_stride (elements; a multiple of 16 bytes each; 0: [requests]
+ * [kv_heads][capacity][head_dim], dense), its value the same from v.  Shared
+ * prefix (prefix_len 0: none): key i of kv head g at prefix_k + g *
+ * prefix_head_stride + i * prefix_slot_stride (0: [kv_heads][prefix_capacity]
+ * [head_dim], prefix_capacity 0 meaning prefix_len).  A cache that one call
+ * filled as a single request can be the prefix of others.  The own caches of
+ * different requests must not overlap. */
+typedef struct {
+  void* k;
+  void* v;
+  const int32_t* lens;     /* [requests]: slots in use, this call's tokens included */
+  const int32_t* new_lens; /* [requests]: this call's tokens, the last slots in use; NULL: n_tokens of each request, none where lens is 0 */
+  const void* prefix_k;
+  const void* prefix_v;
+  uint64_t request_stride, head_stride, slot_stride;
+  uint64_t prefix_head_stride, prefix_slot_stride;
+  uint32_t requests;
+  uint32_t capacity;        /* 1..32768 slots per request */
+  uint32_t prefix_len;      /* 0..32768 */
+  uint32_t prefix_capacity; /* >= prefix_len, or 0 */
+} s2hip_kv_view;
+
+s2hip_kv* s2hip_kv_open(const s2hip_kv_config* cfg, char* err, size_t err_cap);
+/* The handle's work has to be done (its streams synchronised). */
+void s2hip_kv_close(s2hip_kv* kv);
+/* The S2HIP_KV_ERR_* bits set since the last call, after the work on `stream`
+ * so far: waits for it.  Not for a stream that is being captured. */
+int32_t s2hip_kv_errors(s2hip_kv* kv, void* stream, uint32_t* bits, char* err, size_t err_cap);
+
+/* QK-norm, rotation and cache write of the new tokens: qkv [requests]
+ * [n_tokens][(heads + 2 kv_heads) head_dim] raw products.  With q_norm / k_norm
+ * [head_dim] (both or neither) each q and k head y becomes y / sqrt(mean(y^2)
+ * + eps) * gain; then the pairs (2 i, 2 i + 1) turn by positions[b][t] *
+ * rope_base^(-2 i / head_dim) (apply_rope_normal, attention.rs:172-206; angles
+ * in 64 bits).  q_out [requests][n_tokens][heads head_dim]; token t's key and
+ * value go to slot lens[b] - new_lens[b] + t.  scores and slot_positions
+ * (nullable, [requests][kv_heads][capacity]): there the slot's score becomes 0
+ * and its position the token's.  Positions need not be the slots: after an
+ * eviction they run ahead.  Tokens t >= new_lens[b] are not read and their
+ * rows of q_out stay as they were. */
+int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qkv, uint32_t n_tokens,
+                        const int32_t* positions, const float* q_norm, const float* k_norm, float* q_out,
+                        float* scores, int32_t* slot_positions, void* stream, char* err, size_t err_cap);
+/* Attention of the new tokens' queries q [requests][n_tokens][heads head_dim]:
+ * token t of request b sees the whole shared prefix and its request's slots
+ * 0 .. lens[b] - new_lens[b] + t; query head h reads kv head h / (heads /
+ * kv_heads).  out like q; rows of tokens t >= new_lens[b] stay as they were.
+ * What a token does not see (later slots, other requests, slots not in use)
+ * never reaches its row, whatever bits stand there.  The shared prefix is read
+ * once for several requests' queries.  out must not overlap q. */
+int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
+                        void* stream, char* err, size_t err_cap);
+/* s2hip_kv_attend, and for every slot s < lens[b] of every kv head g
+ *   weights_out[b][g][s] = weights_in[b][g][s] + the weights that the tokens t
+ *   < new_lens[b] and the query heads of g give it
+ * ([requests][kv_heads][capacity] f32; weights_in NULL: 0, or the same array;
+ * other slots stay as they were), and with prefix_weights_out
+ * ([kv_heads][prefix_capacity], nullable) the same for the prefix, summed over
+ * the requests too.  Sums run in a fixed order: the same call gives the same
+ * bits. */
+int32_t s2hip_kv_attend_weigh(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
+                              const float* weights_in, float* weights_out, const float* prefix_weights_in,
+                              float* prefix_weights_out, void* stream, char* err, size_t err_cap);
+/* Cuts every cache with more than `keep` slots in use down to `keep`, each kv
+ * head by its own scores: the slots whose position is among the last `recent`
+ * (above the head's largest position - recent) or below `sinks` stay, then those
+ * with the largest scores (a NaN counts as -infinity), the lower slot first
+ * between equals; where those that stay are more than keep, the heaviest of
+ * them.  Kept rows of slots >= keep move, in order, into the freed slots below
+ * keep, in order; other rows do not move.  1 <= keep, recent <= keep.  scores_out / positions_out receive the scores and positions
+ * of the slots then in use, lens_out their number (they may be the input
+ * arrays; other entries stay as they were).  Rows behind lens_out stay as they
+ * were.  `layers` caches of the same lens are cut in one call, layer l's at k /
+ * v + l * layer_stride elements (0: requests * request_stride); scores and
+ * positions [layers][requests][kv_heads][capacity].  The view's prefix and
+ * new_lens are not looked at. */
+int32_t s2hip_kv_evict(s2hip_kv* kv, const s2hip_kv_view* view, uint32_t layers, uint64_t layer_stride, uint32_t keep,
+                       uint32_t recent, uint32_t sinks, const float* scores, const int32_t* positions,
+                       float* scores_out, int32_t* positions_out, int32_t* lens_out, void* stream, char* err,
+                       size_t err_cap);
 
 #ifdef __cplusplus
 }
