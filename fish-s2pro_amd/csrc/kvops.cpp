@@ -91,7 +91,7 @@ class KvOps {
     shape_.H = c.heads;
     shape_.G = c.kv_heads;
     shape_.rep = c.heads / c.kv_heads;
-    shape_.scale = c.scale != 0.0f ? c.scale : float(1.0 / std::sqrt(double(c.head_dim)));
+    shape_.scale2 = float((c.scale != 0.0f ? double(c.scale) : 1.0 / std::sqrt(double(c.head_dim))) * 1.4426950408889634);
     shape_.eps = c.eps;
     std::vector<double> freq(c.head_dim / 2);
     for (size_t i = 0; i < freq.size(); ++i)
@@ -102,6 +102,9 @@ class KvOps {
     shape_.err = alloc<uint32_t>(2);
     CHK(hipMemset(shape_.err, 0, 2 * sizeof(uint32_t)));
     work_.stat = alloc<float>(size_t(c.max_tokens) * c.heads * 2);
+    work_.cap_parts = 1536;
+    work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
+    work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
     work_.cap_moves = size_t(1) << 23;
     work_.cap_seqs = size_t(1) << 16;
     work_.moves = alloc<uint32_t>(work_.cap_moves);

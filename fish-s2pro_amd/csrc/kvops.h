@@ -10,7 +10,7 @@ namespace s2 {
 // Head shape of a handle and its device words.
 struct KvShape {
   uint32_t H, G, rep;  // query heads, kv heads, H / G
-  float scale;         // of the scores
+  float scale2;        // of the scores, times log2(e)
   float eps;
   const double* freq;  // [hd / 2] rope_base^(-2 i / hd)
   uint32_t* err;       // S2HIP_KV_ERR_* bits are or-ed in
@@ -40,8 +40,18 @@ struct KvAppendArgs {
   int32_t* slot_positions;  // nullable
 };
 
+// Softmax states of 16 rows per (kv head, row tile, split): o [16][hd], (m, l) [16][2].
+struct KvSplit {
+  float* o;
+  float* ml;
+  uint32_t tiles, splits;
+};
+
 struct KvWorkspace {
-  float* stat;  // [tokens][H][2]: a row's maximum and sum (attention with weights)
+  float* stat;  // [tokens][H][2]: a row's m and l (attention with weights)
+  float* part;     // [cap_parts][16][hd]
+  float* part_ml;  // [cap_parts][16][2]
+  size_t cap_parts;
   uint32_t* moves;     // [cap_moves] (from << 16 | to)
   uint32_t* counts;    // [cap_seqs][2]: moves, slots left
   size_t cap_moves, cap_seqs;

@@ -24,6 +24,10 @@ __device__ __forceinline__ Request request_of(const KvCaches& c, uint32_t b, uin
   return ok ? Request{uint32_t(len), uint32_t(fresh)} : Request{0u, 0u};
 }
 
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
 template <bool KH>
 using Elem = std::conditional_t<KH, _Float16, float>;
 
@@ -79,7 +83,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
     const uint32_t g = key ? h - a.s.H : h - a.s.H - a.s.G;
     Elem<KH>* dst = static_cast<Elem<KH>*>(key ? a.c.k : a.c.v) + b * a.c.req_stride + g * a.c.head_stride + slot * a.c.slot_stride + d;
     if constexpr (KH) {
-      typedef _Float16 half4 __attribute__((ext_vector_type(4)));
       const half4 y = {_Float16(x.x), _Float16(x.y), _Float16(x.z), _Float16(x.w)};
       const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
       if (big >= 65520.0f) atomicOr(a.s.err, S2HIP_KV_ERR_F16_RANGE);  // rounds to infinity
@@ -98,6 +101,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
+// Scores are kept in powers of two (q times scale log2(e)), so that a weight is
+// one exp2 of a difference.  A kv head's query rows are packed: row (b n + t)
+// rep + r.  A row's softmax state is (m, l, o): weights 2^(s - m), their sum and
+// their sum with the values; states over disjoint keys join by their m.
+
 template <int HD, class T>
 __device__ __forceinline__ float dot_row(const T* row, const float* q) {
   float s = 0.0f;
@@ -105,71 +113,460 @@ __device__ __forceinline__ float dot_row(const T* row, const float* q) {
   return s;
 }
 
-__device__ __forceinline__ float block_max(float v, float* sh) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
+template <class Op>
+__device__ __forceinline__ float quarter_reduce(float x, Op op) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float block_sum(float v, float* sh) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63u) == 0) sh[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
+__device__ __forceinline__ float quarter_max(float x) {
+  return quarter_reduce(x, [](float p, float q) { return fmaxf(p, q); });
+}
+__device__ __forceinline__ float quarter_sum(float x) {
+  return quarter_reduce(x, [](float p, float q) { return p + q; });
 }
 
-// One block per (token, query head): chunks of 256 keys, one per thread, with
-// the running maximum and sum of the softmax; then a dimension per thread.
+// a power of two r with max / r in [2^13, 2^14), and 1 / r
+__device__ __forceinline__ void pow2_scale(float max, float& r, float& inv) {
+  const int e = int((__float_as_uint(max) >> 23) & 255u) - 13;
+  const uint32_t x = uint32_t(e < 1 ? 1 : e);
+  r = __uint_as_float(x << 23);
+  inv = __uint_as_float((254u - x) << 23);
+}
+
+// Eight halfs of a tile's transposed values: rows (keys) of `row_bytes` bytes in
+// LDS; lane i of 16 reads 8 bytes of row i / 4 and gets column i of four rows.
+typedef __attribute__((address_space(3))) uint8_t lds_byte;
+__device__ __forceinline__ half4 read_tr(lds_byte* p) {
+  typedef short short4v __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
+}
+
+// Few rows over many keys (decode steps).  A wave owns 16 packed rows of a kv
+// head and a run of key tiles out of the shared prefix followed by the own
+// caches of the rows' requests; nothing is exchanged between waves before the
+// end, when the block's four join their states in LDS and, with several blocks
+// per 16 rows, leave them for kv_join_kernel.
+//   Scores transposed, S^T = K Q^T, so a lane holds one row (lane % 16) and some
+// of the tile's keys, and the weights are the B operand of O^T += V^T P^T as
+// they stand in the registers.
+//   f32 caches: v_mfma_f32_16x16x4_f32 (f32 products and sums, 16 keys a tile).
+// It takes one element per lane and step, so K and V go from memory to the
+// operand registers by 16-byte loads in an order of dims of our own choosing.
+//   f16 caches: v_mfma_f32_16x16x32_f16, 32 keys a tile, q and the weights as
+// hi + lo f16 parts (2^-22 of a row's largest q, 2^-22 of a weight; weights are
+// scaled by 2^14 so that small ones keep their lo part); K from memory to
+// registers, V through the wave's own 32 rows of LDS, read transposed.
+//   What a row must not see: scores by select; a value that is no number in a
+// tile that some row does not see in whole takes the tile's product out of the
+// matrix unit (0 x NaN) into a loop over the keys each row sees.
+constexpr int STEP_WAVES = 4;
+
 template <int HD, bool KH>
-__global__ __launch_bounds__(256) void kv_attend_row_kernel(KvAttendArgs a, float* stat) {
+__global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
   using T = Elem<KH>;
-  constexpr uint32_t PARTS = 256 / HD;
-  __shared__ float qs[HD], ps[256], sh[4], os[256];
-  const uint32_t tid = threadIdx.x, h = blockIdx.x % a.s.H, bt = blockIdx.x / a.s.H, b = bt / a.c.n, t = bt % a.c.n;
-  const uint32_t g = h / a.s.rep;
-  const Request r = request_of(a.c, b, tid == 0 && t == 0 && h == 0 ? a.s.err : nullptr);
-  if (t >= r.fresh) return;
-  const uint32_t own = r.len - r.fresh + t + 1, total = a.c.P + own;
-  if (tid < HD) qs[tid] = a.q[size_t(blockIdx.x) * HD + tid];
-  __syncthreads();
-  const T* pk = static_cast<const T*>(a.c.pk) + g * a.c.p_head_stride;
-  const T* pv = static_cast<const T*>(a.c.pv) + g * a.c.p_head_stride;
-  const T* k = static_cast<const T*>(a.c.k) + b * a.c.req_stride + g * a.c.head_stride;
-  const T* v = static_cast<const T*>(a.c.v) + b * a.c.req_stride + g * a.c.head_stride;
-  float m = -INFINITY, l = 0.0f, o = 0.0f;
-  const uint32_t d = tid % HD, part = tid / HD;
-  for (uint32_t k0 = 0; k0 < total; k0 += 256) {
-    const uint32_t i = k0 + tid, nk = min(256u, total - k0);
-    float s = -INFINITY;
-    if (i < total)
-      s = a.s.scale * dot_row<HD>(i < a.c.P ? pk + i * a.c.p_slot_stride : k + (i - a.c.P) * a.c.slot_stride, qs);
-    const float mn = fmaxf(m, block_max(s, sh));
-    const float p = i < total && mn != -INFINITY ? expf(s - mn) : 0.0f;
-    const float corr = m == -INFINITY ? 0.0f : expf(m - mn);
-    l = l * corr + block_sum(p, sh);
-    o *= corr;
-    m = mn;
-    ps[tid] = p;
-    __syncthreads();
-    for (uint32_t j = part; j < nk; j += PARTS) {
-      const uint32_t key = k0 + j;
-      const T* row = key < a.c.P ? pv + key * a.c.p_slot_stride : v + (key - a.c.P) * a.c.slot_stride;
-      o = fmaf(ps[j], float(row[d]), o);
+  constexpr int KT = KH ? 32 : 16;
+  constexpr int OT = HD / 16;                 // 16 x 16 output tiles
+  constexpr int KL = HD * sizeof(T) / 64;     // 16-byte loads of a key row per lane
+  constexpr int OP = HD + 4;                  // padded row of the joined states
+  constexpr float LIFT = KH ? 14.0f : 0.0f;   // weights are 2^(s - m + LIFT)
+  constexpr uint32_t VB = KT * HD * 2;        // bytes of a wave's value tile in LDS
+  constexpr uint32_t JOIN = STEP_WAVES * 16 * OP * 4;
+  constexpr uint32_t LDS = KH && STEP_WAVES * VB > JOIN ? STEP_WAVES * VB : JOIN;
+  __shared__ __align__(16) uint8_t lds[LDS];
+  __shared__ float ml[STEP_WAVES][16][2];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r16 = lane & 15u, q4 = lane >> 4;
+  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
+  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
+
+  // the tile's requests: lane j holds request b_lo + j, the key tiles that its rows need
+  const uint32_t b_lo = tile * 16 / per, b_hi = (min(tile * 16 + 16, rows) - 1) / per;
+  const bool holds = lane <= b_hi - b_lo;
+  Request rq{0, 0};
+  uint32_t seg_keys = 0;
+  if (holds) {
+    const uint32_t b = b_lo + lane;
+    rq = request_of(a.c, b, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+    const uint32_t first = max(tile * 16, b * per) - b * per, last = min(tile * 16 + 16, (b + 1) * per) - 1 - b * per;
+    if (first / a.s.rep < rq.fresh) seg_keys = rq.len - rq.fresh + min(last / a.s.rep, rq.fresh - 1) + 1;
+  }
+  const uint32_t p_tiles = __any(seg_keys != 0) ? (a.c.P + KT - 1) / KT : 0u;
+  uint32_t seg_end = (seg_keys + KT - 1) / KT;  // becomes the end of the lane's segment in the run of tiles
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    const uint32_t y = __shfl_up(seg_end, d, 64);
+    if (lane >= uint32_t(d)) seg_end += y;
+  }
+  seg_end += p_tiles;
+  const uint32_t total = lane_read_u32(seg_end, 15);
+  const uint32_t lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
+  const uint32_t t_lo = uint32_t(uint64_t(total) * lot / lots), t_hi = uint32_t(uint64_t(total) * (lot + 1) / lots);
+
+  // this lane's row
+  const uint32_t row = tile * 16 + r16, b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const uint32_t len_row = __shfl(rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(rq.fresh, int(b_row - b_lo) & 15, 64);
+  const bool live = row < rows && t_row < fresh_row;
+  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
+  const float s2 = a.s.scale2;
+  float qf[KH ? 1 : HD / 4];                                       // f32: dims 16 j + 4 q4 + c
+  half8 qh[KH ? HD / 32 : 1], ql[KH ? HD / 32 : 1];                // f16: dims 32 j + 8 q4 + e
+  float unscale = 1.0f;
+  if constexpr (!KH) {
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+      const float4 x = live ? *reinterpret_cast<const float4*>(a.q + q_at + 16 * j + 4 * q4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      qf[4 * j] = x.x * s2;
+      qf[4 * j + 1] = x.y * s2;
+      qf[4 * j + 2] = x.z * s2;
+      qf[4 * j + 3] = x.w * s2;
     }
-    __syncthreads();
+  } else {
+    float x[HD / 32][8], big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 y = live ? *reinterpret_cast<const float4*>(a.q + q_at + 32 * j + 8 * q4 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[j][e] = y.x * s2;
+        x[j][e + 1] = y.y * s2;
+        x[j][e + 2] = y.z * s2;
+        x[j][e + 3] = y.w * s2;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[j][e]));
+    }
+    float inv;
+    pow2_scale(quarter_max(big), unscale, inv);
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = x[j][e] * inv;
+        qh[j][e] = _Float16(y);
+        ql[j][e] = _Float16(y - float(qh[j][e]));
+      }
   }
-  os[tid] = o;
+
+  // tiles of the run, one after the other: where their rows are and whose they are
+  struct Where {
+    const T* k;
+    const T* v;
+    size_t stride;
+    uint32_t key0, keys;
+    int seg;  // -1: the prefix
+  };
+  uint32_t seg = 0;
+  auto where = [&](uint32_t i) {
+    Where w;
+    if (i < p_tiles) {
+      w.seg = -1;
+      w.key0 = i * KT;
+      w.keys = min(uint32_t(KT), a.c.P - w.key0);
+      w.stride = a.c.p_slot_stride;
+      const size_t at = g * a.c.p_head_stride + w.key0 * w.stride;
+      w.k = static_cast<const T*>(a.c.pk) + at;
+      w.v = static_cast<const T*>(a.c.pv) + at;
+    } else {
+      while (i >= lane_read_u32(seg_end, int(seg))) ++seg;
+      const uint32_t begin = seg ? lane_read_u32(seg_end, int(seg) - 1) : p_tiles;
+      w.seg = int(seg);
+      w.key0 = (i - begin) * KT;
+      w.keys = min(uint32_t(KT), lane_read_u32(seg_keys, int(seg)) - w.key0);
+      w.stride = a.c.slot_stride;
+      const size_t at = (b_lo + seg) * a.c.req_stride + g * a.c.head_stride + w.key0 * w.stride;
+      w.k = static_cast<const T*>(a.c.k) + at;
+      w.v = static_cast<const T*>(a.c.v) + at;
+    }
+    return w;
+  };
+  // f32: K key r16, dims 16 j + 4 q4 ..; V key 4 q4 + i, dims 64 hh + 4 r16 ..
+  // f16: K key 16 kt + r16, dims 32 j + 8 q4 ..; V 16-byte pieces lane + 64 i of the tile
+  uint4 kr[KH ? 2 : 1][KL], vr[KH ? HD / 16 : 4][KH ? 1 : HD / 64];
+  auto load_k = [&](const Where& w) {
+#pragma unroll
+    for (int kt = 0; kt < (KH ? 2 : 1); ++kt) {
+      const T* p = w.k + min(16u * kt + r16, w.keys - 1) * w.stride + (KH ? 8 : 4) * q4;
+#pragma unroll
+      for (int j = 0; j < KL; ++j) kr[kt][j] = *reinterpret_cast<const uint4*>(p + (KH ? 32 : 16) * j);
+    }
+  };
+  auto load_v = [&](const Where& w) {
+    if constexpr (KH) {
+      constexpr uint32_t PR = HD / 8;  // pieces per row
+#pragma unroll
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint32_t p = lane + 64 * i;
+        vr[i][0] = *reinterpret_cast<const uint4*>(w.v + min(p / PR, w.keys - 1) * w.stride + (p % PR) * 8);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const T* p = w.v + min(4 * q4 + i, w.keys - 1) * w.stride + 4 * r16;
+#pragma unroll
+        for (int hh = 0; hh < HD / 64; ++hh) vr[i][hh] = *reinterpret_cast<const uint4*>(p + 64 * hh);
+      }
+    }
+  };
+
+  // f32: o[4 hh + c][j]: dim 64 hh + 16 q4 + 4 j + c; f16: o[dt][j]: dim 16 dt + 4 q4 + j
+  floatx4 o[OT];
+#pragma unroll
+  for (int i = 0; i < OT; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+  lds_byte* v_lds = (lds_byte*)lds + (KH ? wave * VB : 0u);
+  // 16-byte piece p of row `key` stands at piece p ^ swz(key): the 16 rows that a transposed read takes 32 bytes
+  // of then lie in distinct banks
+  auto swz = [](uint32_t key) { return HD == 128 ? 2 * (key & 7u) : 2 * ((key >> 1) & 3u); };
+
+  Where w{};
+  if (t_lo < t_hi) {
+    w = where(t_lo);
+    load_k(w);
+    load_v(w);
+  }
+  for (uint32_t i = t_lo; i < t_hi; ++i) {
+    const bool more = i + 1 < t_hi;
+    const Where next = more ? where(i + 1) : w;
+    constexpr int NS = KH ? 8 : 4;  // scores per lane
+    float s[NS];
+    if constexpr (KH) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        floatx4 hi = floatx4{0.f, 0.f, 0.f, 0.f}, lo = hi;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+          const half8 k8 = __builtin_bit_cast(half8, kr[kt][j]);
+          hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], hi, 0, 0, 0);
+          lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], lo, 0, 0, 0);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[4 * kt + c] = (hi[c] + lo[c]) * unscale;
+      }
+    } else {
+      floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f}, y = x;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j) {
+        const floatx4 k4 = __builtin_bit_cast(floatx4, kr[0][j]);
+        x = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[0], qf[4 * j], x, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[1], qf[4 * j + 1], y, 0, 0, 0);
+        x = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[2], qf[4 * j + 2], x, 0, 0, 0);
+        y = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[3], qf[4 * j + 3], y, 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[c] = x[c] + y[c];
+    }
+    if constexpr (KH) {  // the values go to LDS, their registers take the next tile's
+      constexpr uint32_t PR = HD / 8;
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int p = 0; p < HD / 16; ++p) {
+        const uint32_t x = lane + 64 * p, key = x / PR, piece = x % PR;
+        *reinterpret_cast<uint4*>(lds + wave * VB + key * (HD * 2) + (piece ^ swz(key)) * 16) = vr[p][0];
+      }
+    }
+    if (more) load_k(next);
+    const int limit = w.seg < 0 ? int(a.c.P) - 1 : int(b_row - b_lo) == w.seg ? own_limit : -1;
+    // rows that see the whole tile: nothing to mask
+    const bool whole = __all(limit >= int(w.key0 + KT - 1));
+    if (!whole) {
+#pragma unroll
+      for (int c = 0; c < NS; ++c) {
+        const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
+        if (key > limit) s[c] = -INFINITY;
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int c = 1; c < NS; ++c) top = fmaxf(top, s[c]);
+    const float mn = fmaxf(m, quarter_max(top));
+    if (__any(mn > m)) {
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int c = 0; c < OT; ++c) o[c] *= f;
+      l *= f;
+      m = mn;
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
+#pragma unroll
+    for (int c = 0; c < NS; ++c) {
+      s[c] = __builtin_amdgcn_exp2f(s[c] - base);
+      l += s[c];
+    }
+    bool odd = false;  // a value that is no number, and rows that must not see it
+    if constexpr (KH) {
+      half8 ph, pl;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        ph[c] = _Float16(s[c]);
+        pl[c] = _Float16(s[c] - float(ph[c]));
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      half8 v8[OT];
+#pragma unroll
+      for (int dt = 0; dt < OT; ++dt) {
+        half4 part[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          const uint32_t key = 16 * kt + 4 * q4 + r16 / 4, byte = 32 * dt + 8 * (r16 & 3u);
+          part[kt] = read_tr(v_lds + key * (HD * 2) + (((byte >> 4) ^ swz(key)) << 4) + (byte & 15u));
+        }
+        v8[dt] = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+      if (!whole && w.seg >= 0) {
+        half8 z = v8[0] * _Float16(0);
+#pragma unroll
+        for (int dt = 1; dt < OT; ++dt) z = __builtin_elementwise_fma(v8[dt], half8{}, z);
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) bad |= !(z[c] == _Float16(0));
+        odd = __any(bad);
+      }
+      if (!odd) {
+#pragma unroll
+        for (int dt = 0; dt < OT; ++dt) {
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], ph, o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], pl, o[dt], 0, 0, 0);
+        }
+      }
+    } else {
+      if (!whole && w.seg >= 0) {
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int hh = 0; hh < HD / 64; ++hh) {
+            const floatx4 v4 = __builtin_bit_cast(floatx4, vr[i][hh]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) z = fmaf(v4[c], 0.0f, z);
+          }
+        odd = __any(!(z == 0.0f));
+      }
+      if (!odd) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int hh = 0; hh < HD / 64; ++hh) {
+            const floatx4 v4 = __builtin_bit_cast(floatx4, vr[i][hh]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[4 * hh + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[c], s[i], o[4 * hh + c], 0, 0, 0);
+          }
+      }
+    }
+    if (odd) {
+      for (uint32_t key = 0; key < w.keys; ++key) {
+        const int src = int((key % 16) / 4 * 16 + r16);
+        float p = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NS; ++c) {
+          const float x = __shfl(s[c], src, 64);
+          if (uint32_t(16 * (c / 4) + c % 4) == (key & ~12u)) p = x;
+        }
+        if (int(w.key0 + key) > limit) continue;
+        const T* v = w.v + key * w.stride;
+#pragma unroll
+        for (int c = 0; c < OT; ++c)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            o[c][j] = fmaf(p, float(v[KH ? 16 * c + 4 * q4 + j : 64 * (c / 4) + 16 * q4 + 4 * j + c % 4]), o[c][j]);
+      }
+    }
+    if (more) load_v(next);
+    w = next;
+  }
+
+  // the block's four states as one
+  l = quarter_sum(l);
+  if (q4 == 0) {
+    ml[wave][r16][0] = m;
+    ml[wave][r16][1] = l;
+  }
   __syncthreads();
-  if (tid < HD) {
-    float sum = 0.0f;
-    for (uint32_t j = 0; j < PARTS; ++j) sum += os[tid + HD * j];
-    a.out[size_t(blockIdx.x) * HD + tid] = sum / l;
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i) M = fmaxf(M, ml[i][r16][0]);
+  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  float* os = reinterpret_cast<float*>(lds) + (wave * 16 + r16) * OP;
+#pragma unroll
+  for (int c = 0; c < OT; ++c) {
+    if constexpr (KH) {
+      *reinterpret_cast<floatx4*>(os + 16 * c + 4 * q4) = o[c] * f;
+    } else {
+      const int hh = c / 4, j = c % 4;
+      *reinterpret_cast<floatx4*>(os + 64 * hh + 16 * q4 + 4 * j) =
+          floatx4{o[4 * hh][j] * f, o[4 * hh + 1][j] * f, o[4 * hh + 2][j] * f, o[4 * hh + 3][j] * f};
+    }
   }
+  __syncthreads();
+  const uint32_t jr = tid / 16, d0 = tid % 16 * 4;  // a row per 16 threads
+  const uint32_t out_row = tile * 16 + jr;
+  float M_row = -INFINITY, L_row = 0.0f;
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i) M_row = fmaxf(M_row, ml[i][jr][0]);
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i)
+    if (ml[i][jr][0] != -INFINITY) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_row), L_row);
+  const size_t part = ((size_t(g) * sp.tiles + tile) * sp.splits + split) * 16 + jr;
+  const bool last = sp.splits == 1;
+  const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
+  const bool out_live = out_row < rows && ot < __shfl(rq.fresh, int(ob - b_lo) & 15, 64);
+  if (last && !out_live) return;
+  float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
+  const float inv = last ? (M_row == -INFINITY ? 0.0f : 1.0f / L_row) : 1.0f;
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c) {
+    const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
+    floatx4 x = *reinterpret_cast<const floatx4*>(src);
+#pragma unroll
+    for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * 16 * OP);
+    *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
+  }
+  if (tid % 16 == 0) {
+    float* st = last ? stat + 2 * ((size_t(ob) * a.c.n + ot) * a.s.H + oh) : sp.ml + 2 * part;
+    if (!last || stat) {
+      st[0] = M_row - LIFT;
+      st[1] = L_row;
+    }
+  }
+}
+
+// One block per row of the output: its splits' states joined, a wave per fourth split.
+template <int HD>
+__global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
+  __shared__ float os[4][HD];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t bt = blockIdx.x / a.s.H, h = blockIdx.x % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
+  if (t >= request_of(a.c, b, nullptr).fresh) return;
+  const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
+  const size_t part = (size_t(g) * sp.tiles + tile) * sp.splits * 16 + row % 16;  // + 16 split
+  float M = -INFINITY;
+  for (uint32_t s = lane; s < sp.splits; s += 64) M = fmaxf(M, sp.ml[2 * (part + 16 * s)]);
+  M = wave_max(M);
+  float L = 0.0f;
+  for (uint32_t s = lane; s < sp.splits; s += 64) {
+    const float ms = sp.ml[2 * (part + 16 * s)];
+    if (ms != -INFINITY) L = fmaf(sp.ml[2 * (part + 16 * s) + 1], __builtin_amdgcn_exp2f(ms - M), L);
+  }
+  L = wave_sum(L);
+  constexpr int E = HD / 64;
+  float x[E] = {};
+#pragma unroll 8
+  for (uint32_t s = wave; s < sp.splits; s += 4) {
+    const float ms = sp.ml[2 * (part + 16 * s)];
+    const float f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
+    const float* src = sp.o + (part + 16 * s) * HD + E * lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = fmaf(src[e], f, x[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) os[wave][E * lane + e] = x[e];
+  __syncthreads();
+  if (tid < HD) a.out[size_t(blockIdx.x) * HD + tid] = M == -INFINITY ? 0.0f : ((os[0][tid] + os[1][tid]) + (os[2][tid] + os[3][tid])) / L;
   if (stat && tid == 0) {
-    stat[2 * size_t(blockIdx.x)] = m;
-    stat[2 * size_t(blockIdx.x) + 1] = l;
+    stat[2 * size_t(blockIdx.x)] = M;
+    stat[2 * size_t(blockIdx.x) + 1] = L;
   }
 }
 
@@ -193,10 +590,10 @@ __global__ __launch_bounds__(256) void kv_weigh_row_kernel(KvAttendArgs a, const
       for (uint32_t h = g * a.s.rep; h < (g + 1) * a.s.rep; ++h) {
         const size_t at = (size_t(b) * a.c.n + t) * a.s.H + h;
         __syncthreads();
-        if (tid < HD) qs[tid] = a.q[at * HD + tid];
+        if (tid < HD) qs[tid] = a.q[at * HD + tid] * a.s.scale2;
         if (tid < 2) ml[tid] = stat[2 * at + tid];
         __syncthreads();
-        if (prefix || i <= r.len - r.fresh + t) w += expf(a.s.scale * dot_row<HD>(row, qs) - ml[0]) / ml[1];
+        if (prefix || i <= r.len - r.fresh + t) w += __builtin_amdgcn_exp2f(dot_row<HD>(row, qs) - ml[0]) / ml[1];
       }
   }
   if (i >= n_keys) return;
@@ -408,9 +805,18 @@ hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStr
 }
 
 hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const KvWorkspace& w, hipStream_t s) {
+  KvSplit sp{};
+  sp.o = w.part;
+  sp.ml = w.part_ml;
+  sp.tiles = (a.c.R * a.c.n * a.s.rep + 15) / 16;
+  const uint32_t lots = a.s.G * sp.tiles, kt = f16 ? 32 : 16;
+  const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
+  sp.splits = max(1u, min((512 + lots - 1) / lots, (most + STEP_WAVES - 1) / STEP_WAVES));
+  if (size_t(lots) * sp.splits > w.cap_parts) sp.splits = 1;
+  float* stat = a.w_out ? w.stat : nullptr;
   return by_shape(hd, f16, [&](auto HD, auto KH) {
-    hipLaunchKernelGGL((kv_attend_row_kernel<HD(), KH()>), dim3(a.c.R * a.c.n * a.s.H), dim3(256), 0, s, a,
-                       a.w_out ? w.stat : nullptr);
+    hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat);
+    if (sp.splits > 1) hipLaunchKernelGGL((kv_join_kernel<HD()>), dim3(a.c.R * a.c.n * a.s.H), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
       hipLaunchKernelGGL((kv_weigh_row_kernel<HD(), KH()>), dim3((keys + 255) / 256, a.s.G, a.c.R + (a.pw_out ? 1 : 0)),
