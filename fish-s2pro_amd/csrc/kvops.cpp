@@ -102,7 +102,7 @@ class KvOps {
     shape_.err = alloc<uint32_t>(2);
     CHK(hipMemset(shape_.err, 0, 2 * sizeof(uint32_t)));
     work_.stat = alloc<float>(size_t(c.max_tokens) * c.heads * 2);
-    work_.cap_parts = 1536;
+    work_.cap_parts = 8192;
     work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
     work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
     work_.cap_moves = size_t(1) << 23;

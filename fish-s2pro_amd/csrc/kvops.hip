@@ -26,7 +26,9 @@ __device__ __forceinline__ Request request_of(const KvCaches& c, uint32_t b, uin
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 template <bool KH>
 using Elem = std::conditional_t<KH, _Float16, float>;
@@ -128,10 +130,18 @@ __device__ __forceinline__ float quarter_sum(float x) {
   return quarter_reduce(x, [](float p, float q) { return p + q; });
 }
 
-// a power of two r with max / r in [2^13, 2^14), and 1 / r
+// op over lanes l and l ^ 32
+template <class Op>
+__device__ __forceinline__ float half_reduce(float x, Op op) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// a power of two r with max / r in [2^13, 2^14), and 1 / r; at least 2^-62, so
+// that the product of two is a normal number
 __device__ __forceinline__ void pow2_scale(float max, float& r, float& inv) {
   const int e = int((__float_as_uint(max) >> 23) & 255u) - 13;
-  const uint32_t x = uint32_t(e < 1 ? 1 : e);
+  const uint32_t x = uint32_t(e < 65 ? 65 : e);
   r = __uint_as_float(x << 23);
   inv = __uint_as_float((254u - x) << 23);
 }
@@ -139,9 +149,94 @@ __device__ __forceinline__ void pow2_scale(float max, float& r, float& inv) {
 // Eight halfs of a tile's transposed values: rows (keys) of `row_bytes` bytes in
 // LDS; lane i of 16 reads 8 bytes of row i / 4 and gets column i of four rows.
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
+typedef __attribute__((address_space(3))) half8 lds_half8;
 __device__ __forceinline__ half4 read_tr(lds_byte* p) {
   typedef short short4v __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p));
+}
+
+__device__ __forceinline__ bool not_zero(half8 z) {
+  bool bad = false;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) bad |= !(z[c] == _Float16(0));
+  return bad;
+}
+// Ones where x is no number, which becomes 0 there.
+__device__ __forceinline__ half8 take_odd(half8& x) {
+  half8 marks;
+#pragma unroll
+  for (int c = 0; c < 8; ++c) {
+    const bool bad = !(__builtin_fabsf16(x[c]) < _Float16(INFINITY));
+    marks[c] = bad ? _Float16(1) : _Float16(0);
+    x[c] = bad ? _Float16(0) : x[c];
+  }
+  return marks;
+}
+
+// What `n_rows` packed rows from row0 on attend to, in tiles of KT keys: the
+// shared prefix, then the own caches of their requests, each as far as the last
+// of the rows sees.  Lane j holds request b_lo + j (at most 64 requests).
+struct Run {
+  uint32_t b_lo, p_tiles, total;
+  Request rq;         // the lane's request
+  uint32_t seg_keys;  // keys of it
+  uint32_t seg_end;   // its last tile + 1
+};
+template <int KT>
+__device__ __forceinline__ Run run_of(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows, uint32_t* err) {
+  const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep, row1 = min(row0 + n_rows, a.c.R * per);
+  Run r{};
+  r.b_lo = row0 / per;
+  const uint32_t b = r.b_lo + lane;
+  if (b <= (row1 - 1) / per) {
+    r.rq = request_of(a.c, b, err);
+    const uint32_t first = max(row0, b * per) - b * per, last = min(row1, (b + 1) * per) - 1 - b * per;
+    if (first / a.s.rep < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(last / a.s.rep, r.rq.fresh - 1) + 1;
+  }
+  r.p_tiles = __any(r.seg_keys != 0) ? (a.c.P + KT - 1) / KT : 0u;
+  r.seg_end = (r.seg_keys + KT - 1) / KT;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(r.seg_end, d, 64);
+    if (lane >= uint32_t(d)) r.seg_end += y;
+  }
+  r.seg_end += r.p_tiles;
+  r.total = lane_read_u32(r.seg_end, 63);
+  return r;
+}
+
+// Tile i of a run: where its rows are and whose they are.  `seg` goes up with i.
+template <class T>
+struct Where {
+  const T* k;
+  const T* v;
+  size_t stride;
+  uint32_t key0, keys;
+  int seg;  // -1: the prefix; else request b_lo + seg
+};
+template <class T, int KT>
+__device__ __forceinline__ Where<T> where_of(const KvCaches& c, const Run& r, uint32_t g, uint32_t i, uint32_t& seg) {
+  Where<T> w;
+  if (i < r.p_tiles) {
+    w.seg = -1;
+    w.key0 = i * KT;
+    w.keys = min(uint32_t(KT), c.P - w.key0);
+    w.stride = c.p_slot_stride;
+    const size_t at = g * c.p_head_stride + w.key0 * w.stride;
+    w.k = static_cast<const T*>(c.pk) + at;
+    w.v = static_cast<const T*>(c.pv) + at;
+  } else {
+    while (i >= lane_read_u32(r.seg_end, int(seg))) ++seg;
+    const uint32_t begin = seg ? lane_read_u32(r.seg_end, int(seg) - 1) : r.p_tiles;
+    w.seg = int(seg);
+    w.key0 = (i - begin) * KT;
+    w.keys = min(uint32_t(KT), lane_read_u32(r.seg_keys, int(seg)) - w.key0);
+    w.stride = c.slot_stride;
+    const size_t at = (r.b_lo + seg) * c.req_stride + g * c.head_stride + w.key0 * w.stride;
+    w.k = static_cast<const T*>(c.k) + at;
+    w.v = static_cast<const T*>(c.v) + at;
+  }
+  return w;
 }
 
 // Few rows over many keys (decode steps).  A wave owns 16 packed rows of a kv
@@ -159,9 +254,10 @@ __device__ __forceinline__ half4 read_tr(lds_byte* p) {
 // hi + lo f16 parts (2^-22 of a row's largest q, 2^-22 of a weight; weights are
 // scaled by 2^14 so that small ones keep their lo part); K from memory to
 // registers, V through the wave's own 32 rows of LDS, read transposed.
-//   What a row must not see: scores by select; a value that is no number in a
-// tile that some row does not see in whole takes the tile's product out of the
-// matrix unit (0 x NaN) into a loop over the keys each row sees.
+//   What a row must not see: scores by select; where a tile that some row does
+// not see in whole holds values that are no number (0 x NaN), they count as 0 in
+// the product, and a second product of marks, theirs with the keys each row
+// sees, says which outputs are no number.
 constexpr int STEP_WAVES = 4;
 
 template <int HD, bool KH>
@@ -181,32 +277,14 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
 
-  // the tile's requests: lane j holds request b_lo + j, the key tiles that its rows need
-  const uint32_t b_lo = tile * 16 / per, b_hi = (min(tile * 16 + 16, rows) - 1) / per;
-  const bool holds = lane <= b_hi - b_lo;
-  Request rq{0, 0};
-  uint32_t seg_keys = 0;
-  if (holds) {
-    const uint32_t b = b_lo + lane;
-    rq = request_of(a.c, b, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-    const uint32_t first = max(tile * 16, b * per) - b * per, last = min(tile * 16 + 16, (b + 1) * per) - 1 - b * per;
-    if (first / a.s.rep < rq.fresh) seg_keys = rq.len - rq.fresh + min(last / a.s.rep, rq.fresh - 1) + 1;
-  }
-  const uint32_t p_tiles = __any(seg_keys != 0) ? (a.c.P + KT - 1) / KT : 0u;
-  uint32_t seg_end = (seg_keys + KT - 1) / KT;  // becomes the end of the lane's segment in the run of tiles
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    const uint32_t y = __shfl_up(seg_end, d, 64);
-    if (lane >= uint32_t(d)) seg_end += y;
-  }
-  seg_end += p_tiles;
-  const uint32_t total = lane_read_u32(seg_end, 15);
+  const Run run = run_of<KT>(a, tile * 16, 16, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint32_t b_lo = run.b_lo, total = run.total;
   const uint32_t lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
   const uint32_t t_lo = uint32_t(uint64_t(total) * lot / lots), t_hi = uint32_t(uint64_t(total) * (lot + 1) / lots);
 
   // this lane's row
   const uint32_t row = tile * 16 + r16, b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
-  const uint32_t len_row = __shfl(rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(rq.fresh, int(b_row - b_lo) & 15, 64);
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
   const bool live = row < rows && t_row < fresh_row;
   const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
   const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
@@ -250,63 +328,31 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
       }
   }
 
-  // tiles of the run, one after the other: where their rows are and whose they are
-  struct Where {
-    const T* k;
-    const T* v;
-    size_t stride;
-    uint32_t key0, keys;
-    int seg;  // -1: the prefix
-  };
-  uint32_t seg = 0;
-  auto where = [&](uint32_t i) {
-    Where w;
-    if (i < p_tiles) {
-      w.seg = -1;
-      w.key0 = i * KT;
-      w.keys = min(uint32_t(KT), a.c.P - w.key0);
-      w.stride = a.c.p_slot_stride;
-      const size_t at = g * a.c.p_head_stride + w.key0 * w.stride;
-      w.k = static_cast<const T*>(a.c.pk) + at;
-      w.v = static_cast<const T*>(a.c.pv) + at;
-    } else {
-      while (i >= lane_read_u32(seg_end, int(seg))) ++seg;
-      const uint32_t begin = seg ? lane_read_u32(seg_end, int(seg) - 1) : p_tiles;
-      w.seg = int(seg);
-      w.key0 = (i - begin) * KT;
-      w.keys = min(uint32_t(KT), lane_read_u32(seg_keys, int(seg)) - w.key0);
-      w.stride = a.c.slot_stride;
-      const size_t at = (b_lo + seg) * a.c.req_stride + g * a.c.head_stride + w.key0 * w.stride;
-      w.k = static_cast<const T*>(a.c.k) + at;
-      w.v = static_cast<const T*>(a.c.v) + at;
-    }
-    return w;
-  };
   // f32: K key r16, dims 16 j + 4 q4 ..; V key 4 q4 + i, dims 64 hh + 4 r16 ..
   // f16: K key 16 kt + r16, dims 32 j + 8 q4 ..; V 16-byte pieces lane + 64 i of the tile
-  uint4 kr[KH ? 2 : 1][KL], vr[KH ? HD / 16 : 4][KH ? 1 : HD / 64];
-  auto load_k = [&](const Where& w) {
+  u32x4 kr[KH ? 2 : 1][KL], vr[KH ? HD / 16 : 4][KH ? 1 : HD / 64];
+  auto load_k = [&](const Where<T>& w) {
 #pragma unroll
     for (int kt = 0; kt < (KH ? 2 : 1); ++kt) {
       const T* p = w.k + min(16u * kt + r16, w.keys - 1) * w.stride + (KH ? 8 : 4) * q4;
 #pragma unroll
-      for (int j = 0; j < KL; ++j) kr[kt][j] = *reinterpret_cast<const uint4*>(p + (KH ? 32 : 16) * j);
+      for (int j = 0; j < KL; ++j) kr[kt][j] = *reinterpret_cast<const u32x4*>(p + (KH ? 32 : 16) * j);
     }
   };
-  auto load_v = [&](const Where& w) {
+  auto load_v = [&](const Where<T>& w) {
     if constexpr (KH) {
       constexpr uint32_t PR = HD / 8;  // pieces per row
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
         const uint32_t p = lane + 64 * i;
-        vr[i][0] = *reinterpret_cast<const uint4*>(w.v + min(p / PR, w.keys - 1) * w.stride + (p % PR) * 8);
+        vr[i][0] = *reinterpret_cast<const u32x4*>(w.v + min(p / PR, w.keys - 1) * w.stride + (p % PR) * 8);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const T* p = w.v + min(4 * q4 + i, w.keys - 1) * w.stride + 4 * r16;
 #pragma unroll
-        for (int hh = 0; hh < HD / 64; ++hh) vr[i][hh] = *reinterpret_cast<const uint4*>(p + 64 * hh);
+        for (int hh = 0; hh < HD / 64; ++hh) vr[i][hh] = *reinterpret_cast<const u32x4*>(p + 64 * hh);
       }
     }
   };
@@ -321,15 +367,16 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   // of then lie in distinct banks
   auto swz = [](uint32_t key) { return HD == 128 ? 2 * (key & 7u) : 2 * ((key >> 1) & 3u); };
 
-  Where w{};
+  uint32_t seg = 0;
+  Where<T> w{};
   if (t_lo < t_hi) {
-    w = where(t_lo);
+    w = where_of<T, KT>(a.c, run, g, t_lo, seg);
     load_k(w);
     load_v(w);
   }
   for (uint32_t i = t_lo; i < t_hi; ++i) {
     const bool more = i + 1 < t_hi;
-    const Where next = more ? where(i + 1) : w;
+    const Where<T> next = more ? where_of<T, KT>(a.c, run, g, i + 1, seg) : w;
     constexpr int NS = KH ? 8 : 4;  // scores per lane
     float s[NS];
     if constexpr (KH) {
@@ -364,7 +411,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 #pragma unroll
       for (int p = 0; p < HD / 16; ++p) {
         const uint32_t x = lane + 64 * p, key = x / PR, piece = x % PR;
-        *reinterpret_cast<uint4*>(lds + wave * VB + key * (HD * 2) + (piece ^ swz(key)) * 16) = vr[p][0];
+        *reinterpret_cast<u32x4*>(lds + wave * VB + key * (HD * 2) + (piece ^ swz(key)) * 16) = vr[p][0];
       }
     }
     if (more) load_k(next);
@@ -416,20 +463,27 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
         v8[dt] = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
       }
       if (!whole && w.seg >= 0) {
-        half8 z = v8[0] * _Float16(0);
+        half8 z = half8{};
 #pragma unroll
-        for (int dt = 1; dt < OT; ++dt) z = __builtin_elementwise_fma(v8[dt], half8{}, z);
-        bool bad = false;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) bad |= !(z[c] == _Float16(0));
-        odd = __any(bad);
+        for (int dt = 0; dt < OT; ++dt) z = __builtin_elementwise_fma(v8[dt], half8{}, z);
+        odd = __any(not_zero(z));
       }
-      if (!odd) {
+      if (odd) {
+        half8 seen;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) seen[c] = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4)) <= limit ? _Float16(1) : _Float16(0);
 #pragma unroll
         for (int dt = 0; dt < OT; ++dt) {
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], ph, o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], pl, o[dt], 0, 0, 0);
+          const half8 marks = take_odd(v8[dt]);
+          const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, seen, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[dt][c] = hits[c] > 0.0f ? NAN : o[dt][c];
         }
+      }
+#pragma unroll
+      for (int dt = 0; dt < OT; ++dt) {
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], ph, o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[dt], pl, o[dt], 0, 0, 0);
       }
     } else {
       if (!whole && w.seg >= 0) {
@@ -444,34 +498,30 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
           }
         odd = __any(!(z == 0.0f));
       }
-      if (!odd) {
+      if (odd) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int hh = 0; hh < HD / 64; ++hh)
 #pragma unroll
-          for (int hh = 0; hh < HD / 64; ++hh) {
-            const floatx4 v4 = __builtin_bit_cast(floatx4, vr[i][hh]);
+          for (int c = 0; c < 4; ++c) {
+            floatx4 hits = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) o[4 * hh + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[c], s[i], o[4 * hh + c], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+              const bool bad = !(fabsf(__uint_as_float(vr[i][hh][c])) < INFINITY);
+              if (bad) vr[i][hh][c] = 0;
+              hits = __builtin_amdgcn_mfma_f32_16x16x4f32(bad ? 1.0f : 0.0f, int(w.key0 + 4 * q4 + i) <= limit ? 1.0f : 0.0f, hits, 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[4 * hh + c][j] = hits[j] > 0.0f ? NAN : o[4 * hh + c][j];
           }
       }
-    }
-    if (odd) {
-      for (uint32_t key = 0; key < w.keys; ++key) {
-        const int src = int((key % 16) / 4 * 16 + r16);
-        float p = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NS; ++c) {
-          const float x = __shfl(s[c], src, 64);
-          if (uint32_t(16 * (c / 4) + c % 4) == (key & ~12u)) p = x;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int hh = 0; hh < HD / 64; ++hh) {
+          const floatx4 v4 = __builtin_bit_cast(floatx4, vr[i][hh]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[4 * hh + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[c], s[i], o[4 * hh + c], 0, 0, 0);
         }
-        if (int(w.key0 + key) > limit) continue;
-        const T* v = w.v + key * w.stride;
-#pragma unroll
-        for (int c = 0; c < OT; ++c)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            o[c][j] = fmaf(p, float(v[KH ? 16 * c + 4 * q4 + j : 64 * (c / 4) + 16 * q4 + 4 * j + c % 4]), o[c][j]);
-      }
     }
     if (more) load_v(next);
     w = next;
@@ -511,7 +561,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   const size_t part = ((size_t(g) * sp.tiles + tile) * sp.splits + split) * 16 + jr;
   const bool last = sp.splits == 1;
   const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
-  const bool out_live = out_row < rows && ot < __shfl(rq.fresh, int(ob - b_lo) & 15, 64);
+  const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
   if (last && !out_live) return;
   float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
   const float inv = last ? (M_row == -INFINITY ? 0.0f : 1.0f / L_row) : 1.0f;
@@ -529,6 +579,294 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
       st[0] = M_row - LIFT;
       st[1] = L_row;
     }
+  }
+}
+
+// Many rows (turns, prompts).  A block of four waves owns 128 packed rows of a
+// kv head, 32 per wave, and walks the run of key tiles (64 keys of f16, 32 of
+// f32) that they share through LDS, the next tile's loads in flight meanwhile.
+//   v_mfma_f32_32x32x16_f16 with S^T = K Q^T and O^T += V^T P^T as above: a lane
+// holds one row (lane % 32).  q and the weights are hi + lo f16 parts, f16
+// caches as they are: two products each.
+//   f32 caches: keys and values are split into hi + lo f16 parts as they are
+// staged, scaled by a power of two per 8 keys (the 8 keys of four score
+// registers): three products, 2^-22 of each term, or 2^-39 of the largest value
+// of the run for terms far below it.  (The f32 matrix instructions do a
+// sixteenth of the f16 ones' work per cycle.)
+constexpr int TILE_ROWS = 128;
+
+template <int HD, bool KH>
+__global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
+  using T = Elem<KH>;
+  constexpr int KT = KH ? 64 : 32;
+  constexpr int DS = HD / 16, DT = HD / 32;
+  constexpr uint32_t RB = HD * 2, PLANE = KT * RB;        // bytes of a row and of a plane of a tile in LDS
+  constexpr uint32_t BUF = (KH ? 2 : 4) * PLANE;          // K, V, or K hi, K lo, V hi, V lo
+  constexpr int LD = KT * HD * sizeof(T) / 16 / 256;      // 16-byte loads per thread of a tile's keys
+  constexpr uint32_t PR = HD * sizeof(T) / 16;            // 16-byte pieces of a row in memory
+  constexpr float LIFT = 14.0f;
+  __shared__ __align__(16) uint8_t lds[2 * BUF];
+  __shared__ float scales[2][2][4];  // f32: [buffer][K, V][8 keys]
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r32 = lane & 31u, h2 = lane >> 5;
+  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
+  const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
+  const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
+  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint32_t t_lo = uint32_t(uint64_t(run.total) * split / sp.splits), t_hi = uint32_t(uint64_t(run.total) * (split + 1) / sp.splits);
+
+  // this lane's row
+  const uint32_t row = tile * TILE_ROWS + wave * 32 + r32, b_row = row / per, t_row = row / a.s.rep % a.c.n;
+  const uint32_t h_row = g * a.s.rep + row % a.s.rep;
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
+  const bool live = row < rows && t_row < fresh_row;
+  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
+  half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
+  float unscale;
+  {
+    float x[DS][8], big = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 y = live ? *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[ks][e] = y.x * a.s.scale2;
+        x[ks][e + 1] = y.y * a.s.scale2;
+        x[ks][e + 2] = y.z * a.s.scale2;
+        x[ks][e + 3] = y.w * a.s.scale2;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[ks][e]));
+    }
+    float inv;
+    pow2_scale(half_reduce(big, [](float p, float q) { return fmaxf(p, q); }), unscale, inv);
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = x[ks][e] * inv;
+        qh[ks][e] = _Float16(y);
+        ql[ks][e] = _Float16(y - float(qh[ks][e]));
+      }
+  }
+
+  // thread's pieces of a tile: f16 tid + 256 i; f32 the wave's 8 keys, lane + 64 i of them
+  u32x4 kr[LD], vr[LD];
+  auto key_of = [&](int i) { return KH ? (tid + 256 * i) / PR : 8 * wave + (lane + 64 * i) / PR; };
+  auto piece_of = [&](int i) { return KH ? (tid + 256 * i) % PR : (lane + 64 * i) % PR; };
+  auto load = [&](const Where<T>& w) {
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const size_t at = min(key_of(i), w.keys - 1) * w.stride + piece_of(i) * (16 / sizeof(T));
+      kr[i] = *reinterpret_cast<const u32x4*>(w.k + at);
+      vr[i] = *reinterpret_cast<const u32x4*>(w.v + at);
+    }
+  };
+  // 16-byte piece p of row `key` stands at p ^ swz(key): keys' fragment reads take one piece of 8 rows in a row,
+  // transposed value reads 64 bytes of 4 rows
+  auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
+  auto v_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (HD == 128 ? 4 * (key & 3u) : 4 * ((key >> 1) & 1u))) << 4); };
+  auto store = [&](uint32_t buf) {
+    uint8_t* base = lds + buf * BUF;
+    if constexpr (KH) {
+#pragma unroll
+      for (int i = 0; i < LD; ++i) {
+        *reinterpret_cast<u32x4*>(base + k_at(key_of(i), piece_of(i))) = kr[i];
+        *reinterpret_cast<u32x4*>(base + PLANE + v_at(key_of(i), piece_of(i))) = vr[i];
+      }
+    } else {
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+          const floatx4 x = __builtin_bit_cast(floatx4, which ? vr[i] : kr[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
+        }
+        float r, inv;
+        pow2_scale(wave_max(big), r, inv);
+        if (lane == 0) scales[buf][which][wave] = r;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+          const floatx4 x = __builtin_bit_cast(floatx4, which ? vr[i] : kr[i]) * inv;
+          half4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hi[e] = _Float16(x[e]);
+            lo[e] = _Float16(x[e] - float(hi[e]));
+          }
+          const uint32_t p = piece_of(i), off = (which ? v_at(key_of(i), p / 2) : k_at(key_of(i), p / 2)) + 8 * (p % 2);
+          *reinterpret_cast<half4*>(base + 2 * which * PLANE + off) = hi;
+          *reinterpret_cast<half4*>(base + (2 * which + 1) * PLANE + off) = lo;
+        }
+      }
+    }
+  };
+
+  floatx16 o[DT];  // dim 32 dt + 8 (v / 4) + 4 h2 + v % 4
+#pragma unroll
+  for (int i = 0; i < DT; ++i) o[i] = floatx16{};
+  float m = -INFINITY, l = 0.0f, unit = 0.0f;  // f32: o in units of `unit`
+  uint32_t seg = 0;
+  Where<T> w{};
+  if (t_lo < t_hi) {
+    w = where_of<T, KT>(a.c, run, g, t_lo, seg);
+    load(w);
+    store(0);
+  }
+  __syncthreads();
+  for (uint32_t i = t_lo; i < t_hi; ++i) {
+    const uint32_t buf = (i - t_lo) & 1u;
+    const bool more = i + 1 < t_hi;
+    const Where<T> next = more ? where_of<T, KT>(a.c, run, g, i + 1, seg) : w;
+    if (more) load(next);
+    const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
+#pragma unroll 1
+    for (int sub = 0; sub < KT / 32; ++sub) {
+      const int key0 = int(w.key0) + 32 * sub;
+      if (!__any(limit >= key0)) continue;  // nothing of it for this wave's rows
+      // fragment addresses: the swizzle changes with the low bits of ks and with dt, the rest are constants
+      lds_byte *kp[4], *vp[DT];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) kp[c] = (lds_byte*)lds + (buf * BUF + 32 * sub * RB + k_at(r32, 2 * c + h2));
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint32_t i16 = lane & 15u, byte = 64 * dt + 32 * ((lane >> 4) & 1u) + 8 * (i16 & 3u);
+        vp[dt] = (lds_byte*)lds + (buf * BUF + 32 * sub * RB + v_at(4 * h2 + i16 / 4, byte >> 4) + (byte & 15u));
+      }
+      // the next fragment is read while one multiplies; the barriers keep the compiler from reading all of them
+      // first, for which there are no registers
+      auto key8 = [&](int plane, int ks) { return *reinterpret_cast<const lds_half8*>(kp[ks % 4] + (plane * PLANE + ks / 4 * 128)); };
+      floatx16 s = floatx16{};
+      half8 k8 = key8(0, 0), kl = KH ? half8{} : key8(1, 0);
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks) {
+        const half8 k8n = ks + 1 < DS ? key8(0, ks + 1) : k8, kln = !KH && ks + 1 < DS ? key8(1, ks + 1) : kl;
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[ks], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], s, 0, 0, 0);
+        if constexpr (!KH) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[ks], s, 0, 0, 0);
+        k8 = k8n;
+        kl = kln;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      const bool whole = __all(limit >= key0 + 31);
+      if (!whole) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (key0 + int(8u * (v / 4) + 4u * h2 + (v % 4)) > limit) s[v] = -INFINITY;
+      }
+      float factor[4], top = -INFINITY;  // of the 8 keys of four scores
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        factor[c] = KH ? unscale : unscale * scales[buf][0][c];
+        top = fmaxf(top, fmaxf(fmaxf(s[4 * c], s[4 * c + 1]), fmaxf(s[4 * c + 2], s[4 * c + 3])) * factor[c]);
+      }
+      const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
+      if (__any(mn > m)) {
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+        l *= f;
+        m = mn;
+      }
+      const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], factor[v / 4], bias));
+        l += s[v];
+      }
+      if constexpr (!KH) {
+        const float* vs = scales[buf][1];
+        const float most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        if (most > unit) {
+          const float f = unit / most;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) o[d] *= f;
+          unit = most;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[v] *= vs[v / 4] / unit;  // powers of two
+      }
+      half8 ph[2], pl[2];  // 16 keys each
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        ph[v / 8][v % 8] = _Float16(s[v]);
+        pl[v / 8][v % 8] = _Float16(fmaf(float(ph[v / 8][v % 8]), -1.0f, s[v]));
+      }
+      // 16 keys of 32 dims, transposed; plane 0: the values or their hi parts, 1: the lo parts
+      auto value8 = [&](int plane, int dt, int st) {
+        half4 y[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) y[u] = read_tr(vp[dt] + ((KH ? 1 : 2 + plane) * PLANE + (16 * st + 8 * u) * RB));
+        return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      bool odd = false;  // a value that is no number, and rows that must not see it
+      if (!whole && w.seg >= 0) {
+        half8 z = half8{};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) z = __builtin_elementwise_fma(value8(0, dt, st), half8{}, z);
+        odd = __any(not_zero(z));
+        if (odd) {
+          half8 seen[2];
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            seen[v / 8][v % 8] = key0 + int(8u * (v / 4) + 4u * h2 + (v % 4)) <= limit ? _Float16(1) : _Float16(0);
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) {
+            floatx16 hits = floatx16{};
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              half8 v8 = value8(0, dt, st);
+              hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(take_odd(v8), seen[st], hits, 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[dt][v] = hits[v] > 0.0f ? NAN : o[dt][v];
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+      half8 v8 = value8(0, 0, 0), u8 = KH ? half8{} : value8(1, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 2 * DT; ++c) {
+        const int dt = c / 2, st = c % 2, n = c + 1;
+        const half8 v8n = n < 2 * DT ? value8(0, n / 2, n % 2) : v8, u8n = !KH && n < 2 * DT ? value8(1, n / 2, n % 2) : u8;
+        if (odd) {
+          take_odd(v8);
+          if constexpr (!KH) take_odd(u8);
+        }
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph[st], o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl[st], o[dt], 0, 0, 0);
+        if constexpr (!KH) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8, ph[st], o[dt], 0, 0, 0);
+        v8 = v8n;
+        u8 = u8n;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (more) store(buf ^ 1u);
+    __syncthreads();
+    w = next;
+  }
+
+  l = half_reduce(l, [](float p, float q) { return p + q; });
+  const bool last = sp.splits == 1;
+  if (row >= rows || (last && !live)) return;
+  const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
+  float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
+  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f) * (KH ? 1.0f : unit);
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<floatx4*>(dst + 32 * dt + 8 * c + 4 * h2) =
+          floatx4{o[dt][4 * c] * f, o[dt][4 * c + 1] * f, o[dt][4 * c + 2] * f, o[dt][4 * c + 3] * f};
+  if (h2 == 0 && (!last || stat)) {
+    float* st = last ? stat + 2 * at_row : sp.ml + 2 * part;
+    st[0] = m - LIFT;
+    st[1] = l;
   }
 }
 
@@ -777,10 +1115,10 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvEvictArgs a, uint32_t se
     const size_t d = (tid % LP) * (16 / sizeof(T));
     T* k = static_cast<T*>(a.c.k) + base + d;
     T* v = static_cast<T*>(a.c.v) + base + d;
-    const uint4 x = *reinterpret_cast<const uint4*>(k + from * a.c.slot_stride);
-    const uint4 y = *reinterpret_cast<const uint4*>(v + from * a.c.slot_stride);
-    *reinterpret_cast<uint4*>(k + to * a.c.slot_stride) = x;
-    *reinterpret_cast<uint4*>(v + to * a.c.slot_stride) = y;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(k + from * a.c.slot_stride);
+    const u32x4 y = *reinterpret_cast<const u32x4*>(v + from * a.c.slot_stride);
+    *reinterpret_cast<u32x4*>(k + to * a.c.slot_stride) = x;
+    *reinterpret_cast<u32x4*>(v + to * a.c.slot_stride) = y;
   }
 }
 
@@ -808,14 +1146,19 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   KvSplit sp{};
   sp.o = w.part;
   sp.ml = w.part_ml;
-  sp.tiles = (a.c.R * a.c.n * a.s.rep + 15) / 16;
-  const uint32_t lots = a.s.G * sp.tiles, kt = f16 ? 32 : 16;
+  const uint32_t rows = a.c.R * a.c.n * a.s.rep;
+  sp.tiles = (rows + 15) / 16;
+  const bool many = a.c.n * a.s.rep >= 32;
+  const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
-  sp.splits = max(1u, min((512 + lots - 1) / lots, (most + STEP_WAVES - 1) / STEP_WAVES));
-  if (size_t(lots) * sp.splits > w.cap_parts) sp.splits = 1;
+  sp.splits = max(1u, min((512 + lots - 1) / lots, many ? most / 2 : (most + STEP_WAVES - 1) / STEP_WAVES));
+  if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   float* stat = a.w_out ? w.stat : nullptr;
   return by_shape(hd, f16, [&](auto HD, auto KH) {
-    hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat);
+    if (many)
+      hipLaunchKernelGGL((kv_tile_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(256), 0, s, a, sp, stat);
+    else
+      hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat);
     if (sp.splits > 1) hipLaunchKernelGGL((kv_join_kernel<HD()>), dim3(a.c.R * a.c.n * a.s.H), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
