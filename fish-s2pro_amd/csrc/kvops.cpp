@@ -105,6 +105,8 @@ class KvOps {
     work_.cap_parts = 8192;
     work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
     work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
+    work_.cap_weights = size_t(1) << 24;
+    work_.weights = alloc<float>(work_.cap_weights);
     work_.cap_moves = size_t(1) << 23;
     work_.cap_seqs = size_t(1) << 16;
     work_.moves = alloc<uint32_t>(work_.cap_moves);

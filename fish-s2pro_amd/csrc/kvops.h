@@ -52,6 +52,8 @@ struct KvWorkspace {
   float* part;     // [cap_parts][16][hd]
   float* part_ml;  // [cap_parts][16][2]
   size_t cap_parts;
+  float* weights;  // [cap_weights]: row splits' sums of weights
+  size_t cap_weights;
   uint32_t* moves;     // [cap_moves] (from << 16 | to)
   uint32_t* counts;    // [cap_seqs][2]: moves, slots left
   size_t cap_moves, cap_seqs;

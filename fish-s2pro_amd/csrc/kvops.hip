@@ -108,13 +108,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 // rep + r.  A row's softmax state is (m, l, o): weights 2^(s - m), their sum and
 // their sum with the values; states over disjoint keys join by their m.
 
-template <int HD, class T>
-__device__ __forceinline__ float dot_row(const T* row, const float* q) {
-  float s = 0.0f;
-  for (int d = 0; d < HD; ++d) s = fmaf(float(row[d]), q[d], s);
-  return s;
-}
-
 // max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 template <class Op>
 __device__ __forceinline__ float quarter_reduce(float x, Op op) {
@@ -908,36 +901,216 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp
   }
 }
 
-// A key per thread: its weight in every row that sees it.  blockIdx.z = request,
-// or R for the prefix.
+// ---------------------------------------------------------------------------
+// weights
+// ---------------------------------------------------------------------------
+// A key's weights summed over the rows that see it, from the rows' final (m, l):
+// the scores once more, transposed as above, with the keys in registers for the
+// whole kernel (a wave's 64 of f16, 32 of f32) and the rows passing by in LDS,
+// 32 at a time as hi + lo parts that the block splits.  A lane adds up its row's
+// weights per key; the 32 rows of a wave's lanes are summed at the end, so every
+// sum has one order.  blockIdx.z = request, or R for the prefix with the rows of
+// all requests; with several row splits the sums go to the workspace and
+// kv_weights_join_kernel adds them.
 template <int HD, bool KH>
-__global__ __launch_bounds__(256) void kv_weigh_row_kernel(KvAttendArgs a, const float* stat) {
+__global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const float* stat, float* part, uint32_t splits) {
   using T = Elem<KH>;
-  __shared__ float qs[HD], ml[2];
-  const uint32_t tid = threadIdx.x, g = blockIdx.y, z = blockIdx.z, i = blockIdx.x * 256 + tid;
+  constexpr int KW = KH ? 2 : 1;           // 32-key tiles per wave
+  constexpr int DS = HD / 16;
+  constexpr uint32_t KB = 128 * KW;        // keys per block
+  constexpr uint32_t RB = HD * 2, PLANE = 32 * RB;
+  __shared__ __align__(16) uint8_t lds[2][2 * PLANE];
+  __shared__ float4 info[2][32];           // a row's unscale, m, 1 / l (0: no row), last slot seen
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r32 = lane & 31u, h2 = lane >> 5;
+  const uint32_t g = blockIdx.x % a.s.G, kb = blockIdx.x / a.s.G, split = blockIdx.y, z = blockIdx.z;
   const bool prefix = z == a.c.R;
-  const uint32_t b0 = prefix ? 0 : z, b1 = prefix ? a.c.R : z + 1;
-  const uint32_t n_keys = prefix ? a.c.P : request_of(a.c, z, nullptr).len;
-  if (blockIdx.x * 256 >= n_keys) return;
-  const T* row = prefix ? static_cast<const T*>(a.c.pk) + g * a.c.p_head_stride + min(i, n_keys - 1) * a.c.p_slot_stride
-                        : static_cast<const T*>(a.c.k) + z * a.c.req_stride + g * a.c.head_stride + min(i, n_keys - 1) * a.c.slot_stride;
-  float w = 0.0f;
-  for (uint32_t b = b0; b < b1; ++b) {
-    const Request r = request_of(a.c, b, nullptr);
-    for (uint32_t t = 0; t < r.fresh; ++t)
-      for (uint32_t h = g * a.s.rep; h < (g + 1) * a.s.rep; ++h) {
-        const size_t at = (size_t(b) * a.c.n + t) * a.s.H + h;
-        __syncthreads();
-        if (tid < HD) qs[tid] = a.q[at * HD + tid] * a.s.scale2;
-        if (tid < 2) ml[tid] = stat[2 * at + tid];
-        __syncthreads();
-        if (prefix || i <= r.len - r.fresh + t) w += __builtin_amdgcn_exp2f(dot_row<HD>(row, qs) - ml[0]) / ml[1];
-      }
+  Request rq{a.c.P, 0};
+  if (!prefix) rq = request_of(a.c, z, nullptr);
+  const uint32_t n_keys = rq.len, k0 = kb * KB;
+  if (k0 >= n_keys) return;
+  // rows of this block: packed (b n + t) rep + r, or t rep + r of the request from the first that sees key k0
+  const uint32_t per = a.c.n * a.s.rep;
+  const uint32_t base = prefix ? 0u : rq.len - rq.fresh;
+  const uint32_t row_end = prefix ? a.c.R * per : rq.fresh * a.s.rep;
+  const uint32_t row_begin = !prefix && k0 > base ? min(row_end, (k0 - base) * a.s.rep) / 32 * 32 : 0u;
+  const uint32_t steps = (row_end - row_begin + 31) / 32;
+  const uint32_t s_lo = steps * split / splits, s_hi = steps * (split + 1) / splits;
+
+  // the wave's keys: key 32 kw + r32, dims 16 ks + 8 h2 + e
+  const uint32_t key0 = k0 + wave * 32 * KW;
+  half8 kh[KW][DS], kl[KH ? 1 : KW][DS];
+  float key_scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // f32: of 8 keys each
+#pragma unroll
+  for (int kw = 0; kw < KW; ++kw) {
+    const size_t stride = prefix ? a.c.p_slot_stride : a.c.slot_stride;
+    const T* row = (prefix ? static_cast<const T*>(a.c.pk) + g * a.c.p_head_stride
+                           : static_cast<const T*>(a.c.k) + z * a.c.req_stride + g * a.c.head_stride) +
+                   min(key0 + 32 * kw + r32, n_keys - 1) * stride + 8 * h2;
+    if constexpr (KH) {
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks) kh[kw][ks] = *reinterpret_cast<const half8*>(row + 16 * ks);
+    } else {
+      float x[DS][8], big = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const floatx4 y = *reinterpret_cast<const floatx4*>(row + 16 * ks + e);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            x[ks][e + c] = y[c];
+            big = fmaxf(big, fabsf(y[c]) < INFINITY ? fabsf(y[c]) : 0.0f);
+          }
+        }
+      big = half_reduce(big, [](float p, float q) { return fmaxf(p, q); });
+      big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
+      big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
+      big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
+      float r, inv;
+      pow2_scale(big, r, inv);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) key_scale[c] = lane_read_f32(r, 8 * c);
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[ks][e] * inv;
+          kh[kw][ks][e] = _Float16(y);
+          kl[kw][ks][e] = _Float16(y - float(kh[kw][ks][e]));
+        }
+    }
   }
-  if (i >= n_keys) return;
-  const size_t at = prefix ? size_t(g) * a.pw_stride + i : (size_t(z) * a.s.G + g) * a.c.cap + i;
+
+  // staging: 8 threads per row, HD / 8 dims each
+  constexpr int SD = HD / 8;
+  float4 qr[SD / 4];
+  float4 qi;
+  const uint32_t srow = tid / 8, sd = tid % 8 * SD;
+  auto load = [&](uint32_t step) {
+    const uint32_t row = row_begin + step * 32 + srow;
+    const uint32_t b = prefix ? row / per : z, t = prefix ? row / a.s.rep % a.c.n : row / a.s.rep;
+    const bool live = row < row_end && (!prefix || t < request_of(a.c, b, nullptr).fresh);
+    const size_t at = (size_t(b) * a.c.n + t) * a.s.H + g * a.s.rep + row % a.s.rep;
+#pragma unroll
+    for (int i = 0; i < SD / 4; ++i)
+      qr[i] = live ? *reinterpret_cast<const float4*>(a.q + at * HD + sd + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float2 ml = live ? *reinterpret_cast<const float2*>(stat + 2 * at) : make_float2(0.f, 0.f);
+    qi = make_float4(0.f, ml.x, live ? 1.0f / ml.y : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + t)));
+  };
+  auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
+  auto store = [&](uint32_t buf) {
+    float big = 0.0f;
+#pragma unroll
+    for (int i = 0; i < SD / 4; ++i) {
+      qr[i] = make_float4(qr[i].x * a.s.scale2, qr[i].y * a.s.scale2, qr[i].z * a.s.scale2, qr[i].w * a.s.scale2);
+      big = fmaxf(big, fmaxf(fmaxf(fabsf(qr[i].x), fabsf(qr[i].y)), fmaxf(fabsf(qr[i].z), fabsf(qr[i].w))));
+    }
+    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
+    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
+    big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
+    float inv;
+    pow2_scale(big, qi.x, inv);
+    if (tid % 8 == 0) info[buf][srow] = qi;
+#pragma unroll
+    for (int i = 0; i < SD / 8; ++i) {
+      const float x[8] = {qr[2 * i].x, qr[2 * i].y, qr[2 * i].z, qr[2 * i].w, qr[2 * i + 1].x, qr[2 * i + 1].y, qr[2 * i + 1].z, qr[2 * i + 1].w};
+      half8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        hi[e] = _Float16(x[e] * inv);
+        lo[e] = _Float16(x[e] * inv - float(hi[e]));
+      }
+      const uint32_t off = k_at(srow, sd / 8 + i);
+      *reinterpret_cast<half8*>(&lds[buf][off]) = hi;
+      *reinterpret_cast<half8*>(&lds[buf][PLANE + off]) = lo;
+    }
+  };
+
+  float sum[KW][16];
+#pragma unroll
+  for (int kw = 0; kw < KW; ++kw)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) sum[kw][v] = 0.0f;
+  if (s_lo < s_hi) {
+    load(s_lo);
+    store(0);
+  }
+  __syncthreads();
+  for (uint32_t st = s_lo; st < s_hi; ++st) {
+    const uint32_t buf = (st - s_lo) & 1u;
+    const bool more = st + 1 < s_hi;
+    if (more) load(st + 1);
+    const float4 me = info[buf][r32];
+    const int limit = __float_as_int(me.w);
+    floatx16 s[KW];
+#pragma unroll
+    for (int kw = 0; kw < KW; ++kw) s[kw] = floatx16{};
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks) {
+      const uint32_t off = k_at(r32, 2 * ks + h2);
+      const half8 qh = *reinterpret_cast<const half8*>(&lds[buf][off]), ql = *reinterpret_cast<const half8*>(&lds[buf][PLANE + off]);
+#pragma unroll
+      for (int kw = 0; kw < KW; ++kw) {
+        s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], qh, s[kw], 0, 0, 0);
+        s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
+        if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int kw = 0; kw < KW; ++kw) {
+      const int first = int(key0) + 32 * kw;
+      if (__all(limit >= first + 31)) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
+      } else {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)) * me.z;
+          sum[kw][v] += first + int(8u * (v / 4) + 4u * h2 + (v % 4)) <= limit ? p : 0.0f;
+        }
+      }
+    }
+    if (more) store(buf ^ 1u);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int kw = 0; kw < KW; ++kw) {
+    float mine = 0.0f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float x = row_reduce(sum[kw][v], [](float p, float q) { return p + q; });
+      const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+      x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+      if (r32 == uint32_t(v)) mine = x;
+    }
+    const uint32_t key = key0 + 32 * kw + 8 * (r32 / 4) + 4 * h2 + r32 % 4;
+    if (r32 >= 16 || key >= n_keys) continue;
+    const size_t own = (size_t(z) * a.s.G + g) * a.c.cap + key;
+    if (splits > 1) {
+      const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
+      part[split * all + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own)] = mine;
+    } else if (prefix) {
+      const size_t at = size_t(g) * a.pw_stride + key;
+      a.pw_out[at] = (a.pw_in ? a.pw_in[at] : 0.0f) + mine;
+    } else {
+      a.w_out[own] = (a.w_in ? a.w_in[own] : 0.0f) + mine;
+    }
+  }
+}
+
+// The row splits' sums, in order, and the weights so far.
+__global__ __launch_bounds__(256) void kv_weights_join_kernel(KvAttendArgs a, const float* part, uint32_t splits) {
+  const uint32_t g = blockIdx.y, z = blockIdx.z, key = blockIdx.x * 256 + threadIdx.x;
+  const bool prefix = z == a.c.R;
+  if (key >= (prefix ? a.c.P : request_of(a.c, z, nullptr).len)) return;
+  const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P), own = (size_t(z) * a.s.G + g) * a.c.cap + key;
+  const float* src = part + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own);
+  float x = 0.0f;
+  for (uint32_t i = 0; i < splits; ++i) x += src[i * all];
+  const size_t at = prefix ? size_t(g) * a.pw_stride + key : own;
   const float* in = prefix ? a.pw_in : a.w_in;
-  (prefix ? a.pw_out : a.w_out)[at] = (in ? in[at] : 0.0f) + w;
+  (prefix ? a.pw_out : a.w_out)[at] = (in ? in[at] : 0.0f) + x;
 }
 
 // ---------------------------------------------------------------------------
@@ -1161,9 +1334,15 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat);
     if (sp.splits > 1) hipLaunchKernelGGL((kv_join_kernel<HD()>), dim3(a.c.R * a.c.n * a.s.H), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
+      const uint32_t kb = KH() ? 256 : 128, z = a.c.R + (a.pw_out ? 1 : 0);
       const uint32_t keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
-      hipLaunchKernelGGL((kv_weigh_row_kernel<HD(), KH()>), dim3((keys + 255) / 256, a.s.G, a.c.R + (a.pw_out ? 1 : 0)),
-                         dim3(256), 0, s, a, w.stat);
+      const uint32_t blocks = a.s.G * ((a.c.cap + kb - 1) / kb * a.c.R + (a.pw_out ? (a.c.P + kb - 1) / kb : 0));
+      const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
+      const uint32_t ws = uint32_t(max(size_t(1), min(size_t(min((512 + blocks - 1) / blocks, ((a.pw_out ? rows : a.c.n * a.s.rep) + 31) / 32)),
+                                                      w.cap_weights / all)));
+      hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3((keys + kb - 1) / kb * a.s.G, ws, z), dim3(256), 0, s, a, w.stat, w.weights, ws);
+      if (ws > 1)
+        hipLaunchKernelGGL(kv_weights_join_kernel, dim3((keys + 255) / 256, a.s.G, z), dim3(256), 0, s, a, w.weights, ws);
     }
     return hipGetLastError();
   });
