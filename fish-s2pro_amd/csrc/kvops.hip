@@ -12,16 +12,25 @@
 namespace s2 {
 namespace {
 
-// Slots in use and new tokens of request b; a request out of range has none.
+// Slots in use and new tokens of a request; a request out of range has none.
+// (Loaded and looked at apart, so that other loads can start in between.)
 struct Request {
   uint32_t len, fresh;
 };
-__device__ __forceinline__ Request request_of(const KvCaches& c, uint32_t b, uint32_t* err) {
-  const int32_t len = c.lens[b];
-  const int32_t fresh = c.new_lens ? c.new_lens[b] : len == 0 ? 0 : int32_t(c.n);
-  const bool ok = len >= 0 && len <= int32_t(c.cap) && fresh >= 0 && fresh <= int32_t(c.n) && fresh <= len;
+struct RawRequest {
+  int32_t len, fresh;
+};
+__device__ __forceinline__ RawRequest load_request(const KvCaches& c, uint32_t b) {
+  return {c.lens[b], c.new_lens ? c.new_lens[b] : -1};
+}
+__device__ __forceinline__ Request checked(const KvCaches& c, RawRequest r, uint32_t* err) {
+  if (!c.new_lens) r.fresh = r.len == 0 ? 0 : int32_t(c.n);
+  const bool ok = r.len >= 0 && r.len <= int32_t(c.cap) && r.fresh >= 0 && r.fresh <= int32_t(c.n) && r.fresh <= r.len;
   if (!ok && err) atomicOr(err, S2HIP_KV_ERR_LENS);
-  return ok ? Request{uint32_t(len), uint32_t(fresh)} : Request{0u, 0u};
+  return ok ? Request{uint32_t(r.len), uint32_t(r.fresh)} : Request{0u, 0u};
+}
+__device__ __forceinline__ Request request_of(const KvCaches& c, uint32_t b, uint32_t* err) {
+  return checked(c, load_request(c, b), err);
 }
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -108,6 +117,12 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 // rep + r.  A row's softmax state is (m, l, o): weights 2^(s - m), their sum and
 // their sum with the values; states over disjoint keys join by their m.
 
+// m follows a row's maximum only when it is SLACK behind: weights stay below
+// 2^SLACK and the o registers are hardly ever rescaled.  f16 parts of weights are
+// of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is exact to
+// 2^-25, 2^-31 of the largest.
+constexpr float SLACK = 8.0f, F16_LIFT = 6.0f;
+
 // max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 template <class Op>
 __device__ __forceinline__ float quarter_reduce(float x, Op op) {
@@ -166,39 +181,41 @@ __device__ __forceinline__ half8 take_odd(half8& x) {
   return marks;
 }
 
-// What `n_rows` packed rows from row0 on attend to, in tiles of KT keys: the
-// shared prefix, then the own caches of their requests, each as far as the last
-// of the rows sees.  Lane j holds request b_lo + j (at most 64 requests).
+// The own caches that `n_rows` packed rows from row0 on attend to, in tiles of KT
+// keys, each as far as the last of the rows sees.  Lane j holds request b_lo + j
+// (at most 64 requests).
 struct Run {
-  uint32_t b_lo, p_tiles, total;
+  uint32_t b_lo, tiles;
   Request rq;         // the lane's request
   uint32_t seg_keys;  // keys of it
   uint32_t seg_end;   // its last tile + 1
 };
+__device__ __forceinline__ RawRequest load_requests(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows) {
+  const uint32_t per = a.c.n * a.s.rep, b = row0 / per + (threadIdx.x & 63u);
+  return b <= (min(row0 + n_rows, a.c.R * per) - 1) / per ? load_request(a.c, b) : RawRequest{0, 0};
+}
 template <int KT>
-__device__ __forceinline__ Run run_of(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows, uint32_t* err) {
+__device__ __forceinline__ Run run_of(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows, RawRequest raw, uint32_t* err) {
   const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep, row1 = min(row0 + n_rows, a.c.R * per);
   Run r{};
   r.b_lo = row0 / per;
   const uint32_t b = r.b_lo + lane;
   if (b <= (row1 - 1) / per) {
-    r.rq = request_of(a.c, b, err);
+    r.rq = checked(a.c, raw, err);
     const uint32_t first = max(row0, b * per) - b * per, last = min(row1, (b + 1) * per) - 1 - b * per;
     if (first / a.s.rep < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(last / a.s.rep, r.rq.fresh - 1) + 1;
   }
-  r.p_tiles = __any(r.seg_keys != 0) ? (a.c.P + KT - 1) / KT : 0u;
   r.seg_end = (r.seg_keys + KT - 1) / KT;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint32_t y = __shfl_up(r.seg_end, d, 64);
     if (lane >= uint32_t(d)) r.seg_end += y;
   }
-  r.seg_end += r.p_tiles;
-  r.total = lane_read_u32(r.seg_end, 63);
+  r.tiles = lane_read_u32(r.seg_end, 63);
   return r;
 }
 
-// Tile i of a run: where its rows are and whose they are.  `seg` goes up with i.
+// A tile of keys: where its rows are and whose they are.
 template <class T>
 struct Where {
   const T* k;
@@ -208,27 +225,30 @@ struct Where {
   int seg;  // -1: the prefix; else request b_lo + seg
 };
 template <class T, int KT>
-__device__ __forceinline__ Where<T> where_of(const KvCaches& c, const Run& r, uint32_t g, uint32_t i, uint32_t& seg) {
+__device__ __forceinline__ Where<T> prefix_tile(const KvCaches& c, uint32_t g, uint32_t i) {
   Where<T> w;
-  if (i < r.p_tiles) {
-    w.seg = -1;
-    w.key0 = i * KT;
-    w.keys = min(uint32_t(KT), c.P - w.key0);
-    w.stride = c.p_slot_stride;
-    const size_t at = g * c.p_head_stride + w.key0 * w.stride;
-    w.k = static_cast<const T*>(c.pk) + at;
-    w.v = static_cast<const T*>(c.pv) + at;
-  } else {
-    while (i >= lane_read_u32(r.seg_end, int(seg))) ++seg;
-    const uint32_t begin = seg ? lane_read_u32(r.seg_end, int(seg) - 1) : r.p_tiles;
-    w.seg = int(seg);
-    w.key0 = (i - begin) * KT;
-    w.keys = min(uint32_t(KT), lane_read_u32(r.seg_keys, int(seg)) - w.key0);
-    w.stride = c.slot_stride;
-    const size_t at = (r.b_lo + seg) * c.req_stride + g * c.head_stride + w.key0 * w.stride;
-    w.k = static_cast<const T*>(c.k) + at;
-    w.v = static_cast<const T*>(c.v) + at;
-  }
+  w.seg = -1;
+  w.key0 = i * KT;
+  w.keys = min(uint32_t(KT), c.P - w.key0);
+  w.stride = c.p_slot_stride;
+  const size_t at = g * c.p_head_stride + w.key0 * w.stride;
+  w.k = static_cast<const T*>(c.pk) + at;
+  w.v = static_cast<const T*>(c.pv) + at;
+  return w;
+}
+// tile i of the run; `seg` goes up with i
+template <class T, int KT>
+__device__ __forceinline__ Where<T> own_tile(const KvCaches& c, const Run& r, uint32_t g, uint32_t i, uint32_t& seg) {
+  Where<T> w;
+  while (i >= lane_read_u32(r.seg_end, int(seg))) ++seg;
+  const uint32_t begin = seg ? lane_read_u32(r.seg_end, int(seg) - 1) : 0u;
+  w.seg = int(seg);
+  w.key0 = (i - begin) * KT;
+  w.keys = min(uint32_t(KT), lane_read_u32(r.seg_keys, int(seg)) - w.key0);
+  w.stride = c.slot_stride;
+  const size_t at = (r.b_lo + seg) * c.req_stride + g * c.head_stride + w.key0 * w.stride;
+  w.k = static_cast<const T*>(c.k) + at;
+  w.v = static_cast<const T*>(c.v) + at;
   return w;
 }
 
@@ -260,7 +280,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   constexpr int OT = HD / 16;                 // 16 x 16 output tiles
   constexpr int KL = HD * sizeof(T) / 64;     // 16-byte loads of a key row per lane
   constexpr int OP = HD + 4;                  // padded row of the joined states
-  constexpr float LIFT = KH ? 14.0f : 0.0f;   // weights are 2^(s - m + LIFT)
+  constexpr float LIFT = KH ? F16_LIFT : 0.0f;
   constexpr uint32_t VB = KT * HD * 2;        // bytes of a wave's value tile in LDS
   constexpr uint32_t JOIN = STEP_WAVES * 16 * OP * 4;
   constexpr uint32_t LDS = KH && STEP_WAVES * VB > JOIN ? STEP_WAVES * VB : JOIN;
@@ -270,57 +290,18 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
 
-  const Run run = run_of<KT>(a, tile * 16, 16, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-  const uint32_t b_lo = run.b_lo, total = run.total;
-  const uint32_t lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
-  const uint32_t t_lo = uint32_t(uint64_t(total) * lot / lots), t_hi = uint32_t(uint64_t(total) * (lot + 1) / lots);
-
-  // this lane's row
+  // what needs nothing first: the requests, the row's query, the wave's first tile of the prefix
+  const RawRequest raw = load_requests(a, tile * 16, 16);
   const uint32_t row = tile * 16 + r16, b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
-  const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
-  const bool live = row < rows && t_row < fresh_row;
-  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
   const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
-  const float s2 = a.s.scale2;
-  float qf[KH ? 1 : HD / 4];                                       // f32: dims 16 j + 4 q4 + c
-  half8 qh[KH ? HD / 32 : 1], ql[KH ? HD / 32 : 1];                // f16: dims 32 j + 8 q4 + e
-  float unscale = 1.0f;
-  if constexpr (!KH) {
+  float4 qx[HD / 16];  // f32: dims 16 j + 4 q4 ..; f16: dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
 #pragma unroll
-    for (int j = 0; j < HD / 16; ++j) {
-      const float4 x = live ? *reinterpret_cast<const float4*>(a.q + q_at + 16 * j + 4 * q4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      qf[4 * j] = x.x * s2;
-      qf[4 * j + 1] = x.y * s2;
-      qf[4 * j + 2] = x.z * s2;
-      qf[4 * j + 3] = x.w * s2;
-    }
-  } else {
-    float x[HD / 32][8], big = 0.0f;
-#pragma unroll
-    for (int j = 0; j < HD / 32; ++j) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 y = live ? *reinterpret_cast<const float4*>(a.q + q_at + 32 * j + 8 * q4 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[j][e] = y.x * s2;
-        x[j][e + 1] = y.y * s2;
-        x[j][e + 2] = y.z * s2;
-        x[j][e + 3] = y.w * s2;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[j][e]));
-    }
-    float inv;
-    pow2_scale(quarter_max(big), unscale, inv);
-#pragma unroll
-    for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = x[j][e] * inv;
-        qh[j][e] = _Float16(y);
-        ql[j][e] = _Float16(y - float(qh[j][e]));
-      }
-  }
-
+  for (int j = 0; j < HD / 16; ++j)
+    qx[j] = row < rows ? *reinterpret_cast<const float4*>(a.q + q_at + (KH ? 32 * (j / 2) + 8 * q4 + 4 * (j % 2) : 16 * j + 4 * q4))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+  const uint32_t lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
+  const uint32_t p_tiles = (a.c.P + KT - 1) / KT;
+  const uint32_t p_lo = p_tiles * lot / lots, n_pre = p_tiles * (lot + 1) / lots - p_lo;
   // f32: K key r16, dims 16 j + 4 q4 ..; V key 4 q4 + i, dims 64 hh + 4 r16 ..
   // f16: K key 16 kt + r16, dims 32 j + 8 q4 ..; V 16-byte pieces lane + 64 i of the tile
   u32x4 kr[KH ? 2 : 1][KL], vr[KH ? HD / 16 : 4][KH ? 1 : HD / 64];
@@ -350,6 +331,59 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
     }
   };
 
+  Where<T> w{};
+  if (n_pre) {
+    w = prefix_tile<T, KT>(a.c, g, p_lo);
+    load_k(w);
+    load_v(w);
+  }
+  const Run run = run_of<KT>(a, tile * 16, 16, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint32_t b_lo = run.b_lo;
+  // (the own tiles the other way round: the waves with one more of the prefix get one fewer)
+  const uint32_t o_lo = run.tiles * (lots - 1 - lot) / lots, n_tiles = n_pre + run.tiles * (lots - lot) / lots - o_lo;
+  uint32_t seg = 0;
+  if (n_pre == 0 && n_tiles) {
+    w = own_tile<T, KT>(a.c, run, g, o_lo, seg);
+    load_k(w);
+    load_v(w);
+  }
+
+  // this lane's row
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
+  const bool live = row < rows && t_row < fresh_row;
+  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  float qf[KH ? 1 : HD / 4];                                       // f32: dims 16 j + 4 q4 + c
+  half8 qh[KH ? HD / 32 : 1], ql[KH ? HD / 32 : 1];                // f16: dims 32 j + 8 q4 + e
+  float unscale = 1.0f;
+  {
+    const float s2 = live ? a.s.scale2 : 0.0f;
+    float x[HD / 16][4], big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+      x[j][0] = live ? qx[j].x * s2 : 0.0f;  // (a query of no token may hold anything)
+      x[j][1] = live ? qx[j].y * s2 : 0.0f;
+      x[j][2] = live ? qx[j].z * s2 : 0.0f;
+      x[j][3] = live ? qx[j].w * s2 : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[j][e]));
+    }
+    if constexpr (!KH) {
+#pragma unroll
+      for (int j = 0; j < HD / 4; ++j) qf[j] = x[j / 4][j % 4];
+    } else {
+      float inv;
+      pow2_scale(quarter_max(big), unscale, inv);
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y = x[2 * j + e / 4][e % 4] * inv;
+          qh[j][e] = _Float16(y);
+          ql[j][e] = _Float16(y - float(qh[j][e]));
+        }
+    }
+  }
+
   // f32: o[4 hh + c][j]: dim 64 hh + 16 q4 + 4 j + c; f16: o[dt][j]: dim 16 dt + 4 q4 + j
   floatx4 o[OT];
 #pragma unroll
@@ -360,16 +394,10 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   // of then lie in distinct banks
   auto swz = [](uint32_t key) { return HD == 128 ? 2 * (key & 7u) : 2 * ((key >> 1) & 3u); };
 
-  uint32_t seg = 0;
-  Where<T> w{};
-  if (t_lo < t_hi) {
-    w = where_of<T, KT>(a.c, run, g, t_lo, seg);
-    load_k(w);
-    load_v(w);
-  }
-  for (uint32_t i = t_lo; i < t_hi; ++i) {
-    const bool more = i + 1 < t_hi;
-    const Where<T> next = more ? where_of<T, KT>(a.c, run, g, i + 1, seg) : w;
+  for (uint32_t i = 0; i < n_tiles; ++i) {
+    const bool more = i + 1 < n_tiles;
+    Where<T> next = w;
+    if (more) next = i + 1 < n_pre ? prefix_tile<T, KT>(a.c, g, p_lo + i + 1) : own_tile<T, KT>(a.c, run, g, o_lo + (i + 1 - n_pre), seg);
     constexpr int NS = KH ? 8 : 4;  // scores per lane
     float s[NS];
     if constexpr (KH) {
@@ -422,7 +450,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 #pragma unroll
     for (int c = 1; c < NS; ++c) top = fmaxf(top, s[c]);
     const float mn = fmaxf(m, quarter_max(top));
-    if (__any(mn > m)) {
+    if (__any(mn > m + SLACK)) {
       const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
       for (int c = 0; c < OT; ++c) o[c] *= f;
@@ -597,7 +625,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   constexpr uint32_t BUF = (KH ? 2 : 4) * PLANE;          // K, V, or K hi, K lo, V hi, V lo
   constexpr int LD = KT * HD * sizeof(T) / 16 / 256;      // 16-byte loads per thread of a tile's keys
   constexpr uint32_t PR = HD * sizeof(T) / 16;            // 16-byte pieces of a row in memory
-  constexpr float LIFT = 14.0f;
+  constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
   __shared__ float scales[2][2][4];  // f32: [buffer][K, V][8 keys]
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r32 = lane & 31u, h2 = lane >> 5;
@@ -605,8 +633,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
   const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
-  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-  const uint32_t t_lo = uint32_t(uint64_t(run.total) * split / sp.splits), t_hi = uint32_t(uint64_t(run.total) * (split + 1) / sp.splits);
+  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, load_requests(a, tile * TILE_ROWS, TILE_ROWS),
+                             g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint32_t p_tiles = run.tiles ? (a.c.P + KT - 1) / KT : 0u, total = p_tiles + run.tiles;
+  const uint32_t t_lo = total * split / sp.splits, t_hi = total * (split + 1) / sp.splits;
 
   // this lane's row
   const uint32_t row = tile * TILE_ROWS + wave * 32 + r32, b_row = row / per, t_row = row / a.s.rep % a.c.n;
@@ -703,9 +733,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   for (int i = 0; i < DT; ++i) o[i] = floatx16{};
   float m = -INFINITY, l = 0.0f, unit = 0.0f;  // f32: o in units of `unit`
   uint32_t seg = 0;
+  auto where = [&](uint32_t i) { return i < p_tiles ? prefix_tile<T, KT>(a.c, g, i) : own_tile<T, KT>(a.c, run, g, i - p_tiles, seg); };
   Where<T> w{};
   if (t_lo < t_hi) {
-    w = where_of<T, KT>(a.c, run, g, t_lo, seg);
+    w = where(t_lo);
     load(w);
     store(0);
   }
@@ -713,7 +744,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   for (uint32_t i = t_lo; i < t_hi; ++i) {
     const uint32_t buf = (i - t_lo) & 1u;
     const bool more = i + 1 < t_hi;
-    const Where<T> next = more ? where_of<T, KT>(a.c, run, g, i + 1, seg) : w;
+    const Where<T> next = more ? where(i + 1) : w;
     if (more) load(next);
     const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
 #pragma unroll 1
@@ -757,7 +788,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         top = fmaxf(top, fmaxf(fmaxf(s[4 * c], s[4 * c + 1]), fmaxf(s[4 * c + 2], s[4 * c + 3])) * factor[c]);
       }
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
-      if (__any(mn > m)) {
+      if (__any(mn > m + SLACK)) {
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
@@ -863,41 +894,72 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   }
 }
 
-// One block per row of the output: its splits' states joined, a wave per fourth split.
-template <int HD>
+// The splits' states of the rows of the output joined: HD / 4 threads per row and
+// TEAM teams of them per row, each with every TEAM-th split.  A team loads its
+// states before it looks at their m, and before it knows that the row is one.
+template <int HD, int TEAM>
 __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
-  __shared__ float os[4][HD];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
-  const uint32_t bt = blockIdx.x / a.s.H, h = blockIdx.x % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
-  if (t >= request_of(a.c, b, nullptr).fresh) return;
+  constexpr uint32_t LP = HD / 4, ROWS = 256 / LP / TEAM;
+  __shared__ floatx4 os[TEAM == 1 ? 1 : TEAM][LP];
+  __shared__ float ms[TEAM], ls[TEAM];
+  const uint32_t tid = threadIdx.x, team = tid / LP % TEAM, d = tid % LP;
+  const uint32_t at = blockIdx.x * ROWS + tid / LP / TEAM;
+  const bool is_row = at < a.c.R * a.c.n * a.s.H;
+  const uint32_t out = is_row ? at : 0u, bt = out / a.s.H, h = out % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
+  const RawRequest raw = load_request(a.c, b);
   const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
   const size_t part = (size_t(g) * sp.tiles + tile) * sp.splits * 16 + row % 16;  // + 16 split
-  float M = -INFINITY;
-  for (uint32_t s = lane; s < sp.splits; s += 64) M = fmaxf(M, sp.ml[2 * (part + 16 * s)]);
-  M = wave_max(M);
-  float L = 0.0f;
-  for (uint32_t s = lane; s < sp.splits; s += 64) {
-    const float ms = sp.ml[2 * (part + 16 * s)];
-    if (ms != -INFINITY) L = fmaf(sp.ml[2 * (part + 16 * s) + 1], __builtin_amdgcn_exp2f(ms - M), L);
-  }
-  L = wave_sum(L);
-  constexpr int E = HD / 64;
-  float x[E] = {};
-#pragma unroll 8
-  for (uint32_t s = wave; s < sp.splits; s += 4) {
-    const float ms = sp.ml[2 * (part + 16 * s)];
-    const float f = ms == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ms - M);
-    const float* src = sp.o + (part + 16 * s) * HD + E * lane;
+  float M = -INFINITY, L = 0.0f;
+  floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s0 = team; s0 < sp.splits; s0 += 4 * TEAM) {
+    floatx4 y[4];
+    float2 ml[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = fmaf(src[e], f, x[e]);
-  }
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t s = min(s0 + i * TEAM, sp.splits - 1);
+      ml[i] = *reinterpret_cast<const float2*>(sp.ml + 2 * (part + 16 * s));
+      y[i] = *reinterpret_cast<const floatx4*>(sp.o + (part + 16 * s) * HD + 4 * d);
+    }
 #pragma unroll
-  for (int e = 0; e < E; ++e) os[wave][E * lane + e] = x[e];
-  __syncthreads();
-  if (tid < HD) a.out[size_t(blockIdx.x) * HD + tid] = M == -INFINITY ? 0.0f : ((os[0][tid] + os[1][tid]) + (os[2][tid] + os[3][tid])) / L;
-  if (stat && tid == 0) {
-    stat[2 * size_t(blockIdx.x)] = M;
-    stat[2 * size_t(blockIdx.x) + 1] = L;
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i * TEAM >= sp.splits) continue;
+      if (ml[i].x == -INFINITY) {  // no key, or none but of no number
+        x += y[i];
+        continue;
+      }
+      const float mn = fmaxf(M, ml[i].x);
+      const float f0 = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(ml[i].x - mn);
+      L = L * f0 + ml[i].y * f1;
+      x = x * f0 + y[i] * f1;
+      M = mn;
+    }
+  }
+  if constexpr (TEAM > 1) {
+    os[team][d] = x;
+    if (d == 0) {
+      ms[team] = M;
+      ls[team] = L;
+    }
+    __syncthreads();
+    if (team) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) all = fmaxf(all, ms[i]);
+    x = floatx4{0.f, 0.f, 0.f, 0.f};
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) {
+      const float f = ms[i] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[i] - all);
+      x += os[i][d] * f;
+      L = fmaf(ls[i], f, L);
+    }
+    M = all;
+  }
+  if (!is_row || t >= checked(a.c, raw, nullptr).fresh) return;
+  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? 1.0f : 1.0f / L);
+  if (stat && d == 0) {
+    stat[2 * size_t(out)] = M;
+    stat[2 * size_t(out) + 1] = L;
   }
 }
 
@@ -1324,7 +1386,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   const bool many = a.c.n * a.s.rep >= 32;
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
-  sp.splits = max(1u, min((512 + lots - 1) / lots, many ? most / 2 : (most + STEP_WAVES - 1) / STEP_WAVES));
+  sp.splits = max(1u, min(512 / lots, many ? most / 2 : (most + STEP_WAVES - 1) / STEP_WAVES));
   if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   float* stat = a.w_out ? w.stat : nullptr;
   return by_shape(hd, f16, [&](auto HD, auto KH) {
@@ -1332,7 +1394,11 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_tile_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(256), 0, s, a, sp, stat);
     else
       hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat);
-    if (sp.splits > 1) hipLaunchKernelGGL((kv_join_kernel<HD()>), dim3(a.c.R * a.c.n * a.s.H), dim3(256), 0, s, a, sp, stat);
+    const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
+    if (sp.splits > 1 && out_rows <= 2048)
+      hipLaunchKernelGGL((kv_join_kernel<HD(), 256 / (HD() / 4)>), dim3(out_rows), dim3(256), 0, s, a, sp, stat);
+    else if (sp.splits > 1)
+      hipLaunchKernelGGL((kv_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t kb = KH() ? 256 : 128, z = a.c.R + (a.pw_out ? 1 : 0);
       const uint32_t keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
