@@ -21,7 +21,7 @@ struct RawRequest {
   int32_t len, fresh;
 };
 __device__ __forceinline__ RawRequest load_request(const KvCaches& c, uint32_t b) {
-  return {c.lens[b], c.new_lens ? c.new_lens[b] : -1};
+  return {c.lens[b], (c.new_lens ? c.new_lens : c.lens)[b]};
 }
 __device__ __forceinline__ Request checked(const KvCaches& c, RawRequest r, uint32_t* err) {
   if (!c.new_lens) r.fresh = r.len == 0 ? 0 : int32_t(c.n);
@@ -38,6 +38,9 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// a value that is the same in all lanes, said so
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 
 template <bool KH>
 using Elem = std::conditional_t<KH, _Float16, float>;
@@ -190,9 +193,8 @@ struct Run {
   uint32_t seg_keys;  // keys of it
   uint32_t seg_end;   // its last tile + 1
 };
-__device__ __forceinline__ RawRequest load_requests(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows) {
-  const uint32_t per = a.c.n * a.s.rep, b = row0 / per + (threadIdx.x & 63u);
-  return b <= (min(row0 + n_rows, a.c.R * per) - 1) / per ? load_request(a.c, b) : RawRequest{0, 0};
+__device__ __forceinline__ RawRequest load_requests(const KvAttendArgs& a, uint32_t row0) {
+  return load_request(a.c, min(row0 / (a.c.n * a.s.rep) + (threadIdx.x & 63u), a.c.R - 1));
 }
 template <int KT>
 __device__ __forceinline__ Run run_of(const KvAttendArgs& a, uint32_t row0, uint32_t n_rows, RawRequest raw, uint32_t* err) {
@@ -286,19 +288,18 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   constexpr uint32_t LDS = KH && STEP_WAVES * VB > JOIN ? STEP_WAVES * VB : JOIN;
   __shared__ __align__(16) uint8_t lds[LDS];
   __shared__ float ml[STEP_WAVES][16][2];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r16 = lane & 15u, q4 = lane >> 4;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
 
   // what needs nothing first: the requests, the row's query, the wave's first tile of the prefix
-  const RawRequest raw = load_requests(a, tile * 16, 16);
-  const uint32_t row = tile * 16 + r16, b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const RawRequest raw = load_requests(a, tile * 16);
+  const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
   const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
   float4 qx[HD / 16];  // f32: dims 16 j + 4 q4 ..; f16: dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
 #pragma unroll
   for (int j = 0; j < HD / 16; ++j)
-    qx[j] = row < rows ? *reinterpret_cast<const float4*>(a.q + q_at + (KH ? 32 * (j / 2) + 8 * q4 + 4 * (j % 2) : 16 * j + 4 * q4))
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    qx[j] = *reinterpret_cast<const float4*>(a.q + q_at + (KH ? 32 * (j / 2) + 8 * q4 + 4 * (j % 2) : 16 * j + 4 * q4));
   const uint32_t lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
   const uint32_t p_tiles = (a.c.P + KT - 1) / KT;
   const uint32_t p_lo = p_tiles * lot / lots, n_pre = p_tiles * (lot + 1) / lots - p_lo;
@@ -331,12 +332,12 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
     }
   };
 
-  Where<T> w{};
-  if (n_pre) {
-    w = prefix_tile<T, KT>(a.c, g, p_lo);
-    load_k(w);
-    load_v(w);
-  }
+  // (Loads stand on one path wherever they can: behind a branch the compiler waits for all that may be in flight.
+  // Where there is nothing to load, a row that is there anyway is read again.)
+  Where<T> w{static_cast<const T*>(a.c.k) + g * a.c.head_stride, static_cast<const T*>(a.c.v) + g * a.c.head_stride, 0, 0, 1, -1};
+  if (n_pre) w = prefix_tile<T, KT>(a.c, g, p_lo);
+  load_k(w);
+  load_v(w);
   const Run run = run_of<KT>(a, tile * 16, 16, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint32_t b_lo = run.b_lo;
   // (the own tiles the other way round: the waves with one more of the prefix get one fewer)
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 
   // this lane's row
   const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
-  const bool live = row < rows && t_row < fresh_row;
+  const bool live = tile * 16 + r16 < rows && t_row < fresh_row;
   const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
   float qf[KH ? 1 : HD / 4];                                       // f32: dims 16 j + 4 q4 + c
   half8 qh[KH ? HD / 32 : 1], ql[KH ? HD / 32 : 1];                // f16: dims 32 j + 8 q4 + e
@@ -397,6 +398,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   for (uint32_t i = 0; i < n_tiles; ++i) {
     const bool more = i + 1 < n_tiles;
     Where<T> next = w;
+    next.stride = 0;
     if (more) next = i + 1 < n_pre ? prefix_tile<T, KT>(a.c, g, p_lo + i + 1) : own_tile<T, KT>(a.c, run, g, o_lo + (i + 1 - n_pre), seg);
     constexpr int NS = KH ? 8 : 4;  // scores per lane
     float s[NS];
@@ -435,7 +437,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
         *reinterpret_cast<u32x4*>(lds + wave * VB + key * (HD * 2) + (piece ^ swz(key)) * 16) = vr[p][0];
       }
     }
-    if (more) load_k(next);
+    load_k(next);
     const int limit = w.seg < 0 ? int(a.c.P) - 1 : int(b_row - b_lo) == w.seg ? own_limit : -1;
     // rows that see the whole tile: nothing to mask
     const bool whole = __all(limit >= int(w.key0 + KT - 1));
@@ -544,7 +546,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
           for (int c = 0; c < 4; ++c) o[4 * hh + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v4[c], s[i], o[4 * hh + c], 0, 0, 0);
         }
     }
-    if (more) load_v(next);
+    load_v(next);
     w = next;
   }
 
@@ -576,9 +578,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   float M_row = -INFINITY, L_row = 0.0f;
 #pragma unroll
   for (int i = 0; i < STEP_WAVES; ++i) M_row = fmaxf(M_row, ml[i][jr][0]);
+  const float M_base = M_row == -INFINITY ? 0.0f : M_row;  // (then every l is 0, or no number)
 #pragma unroll
-  for (int i = 0; i < STEP_WAVES; ++i)
-    if (ml[i][jr][0] != -INFINITY) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_row), L_row);
+  for (int i = 0; i < STEP_WAVES; ++i) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_base), L_row);
   const size_t part = ((size_t(g) * sp.tiles + tile) * sp.splits + split) * 16 + jr;
   const bool last = sp.splits == 1;
   const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
@@ -628,12 +630,12 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
   __shared__ float scales[2][2][4];  // f32: [buffer][K, V][8 keys]
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r32 = lane & 31u, h2 = lane >> 5;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5;
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
   const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
-  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, load_requests(a, tile * TILE_ROWS, TILE_ROWS),
+  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, load_requests(a, tile * TILE_ROWS),
                              g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint32_t p_tiles = run.tiles ? (a.c.P + KT - 1) / KT : 0u, total = p_tiles + run.tiles;
   const uint32_t t_lo = total * split / sp.splits, t_hi = total * (split + 1) / sp.splits;
@@ -983,7 +985,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   constexpr uint32_t RB = HD * 2, PLANE = 32 * RB;
   __shared__ __align__(16) uint8_t lds[2][2 * PLANE];
   __shared__ float4 info[2][32];           // a row's unscale, m, 1 / l (0: no row), last slot seen
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, r32 = lane & 31u, h2 = lane >> 5;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5;
   const uint32_t g = blockIdx.x % a.s.G, kb = blockIdx.x / a.s.G, split = blockIdx.y, z = blockIdx.z;
   const bool prefix = z == a.c.R;
   Request rq{a.c.P, 0};
