@@ -47,12 +47,18 @@ struct KvSplit {
   uint32_t tiles, splits;
 };
 
+// A step's scores, kept for the weights (nullable).
+struct KvScores {
+  float* own;     // [R][G][cap][n rep]
+  float* prefix;  // [G][P][R n rep]
+};
+
 struct KvWorkspace {
   float* stat;  // [tokens][H][2]: a row's m and l (attention with weights)
   float* part;     // [cap_parts][16][hd]
   float* part_ml;  // [cap_parts][16][2]
   size_t cap_parts;
-  float* weights;  // [cap_weights]: row splits' sums of weights
+  float* weights;  // [cap_weights]: a step's scores, or the row splits' sums of weights
   size_t cap_weights;
   uint32_t* moves;     // [cap_moves] (from << 16 | to)
   uint32_t* counts;    // [cap_seqs][2]: moves, slots left
