@@ -1184,16 +1184,17 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // row, then takes a key per thread.  Against the scores computed once more: 8
 // requests of 1500 slots, f32, 18 us less; 4 of 20000, f16, 35 us.
 constexpr uint32_t KEPT_ROWS = 512;  // of the prefix, at most
+constexpr uint32_t KEPT_KEYS = 512;  // per block
 template <int HD>
 __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, uint32_t joins, uint32_t key_blocks) {
   if (blockIdx.x < joins) return join_rows<HD, 1024 / HD>(a, sp, nullptr);
   __shared__ float2 ml[KEPT_ROWS];
   const uint32_t tid = threadIdx.x, i = blockIdx.x - joins, kb = i % key_blocks, g = i / key_blocks % a.s.G, z = i / key_blocks / a.s.G;
   const bool prefix = z == a.c.R;
-  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per, key = kb * 256 + tid;
+  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per;
   Request rq{a.c.P, a.c.n};
   if (!prefix) rq = request_of(a.c, z, nullptr);
-  if (kb * 256 >= rq.len) return;
+  if (kb * KEPT_KEYS >= rq.len) return;
   for (uint32_t r0 = 0; r0 < n_rows; r0 += 16) {
     const uint32_t r = r0 + tid / 16, row = min(prefix ? r : z * per + r, a.c.R * per - 1);
     float M = -INFINITY, L = 0.0f;
@@ -1219,18 +1220,25 @@ __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, Kv
     if (tid % 16 == 0 && r < n_rows) ml[r] = live ? make_float2(M, 1.0f / L) : make_float2(0.0f, 0.0f);
   }
   __syncthreads();
-  if (key >= rq.len) return;
-  const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
-  const uint32_t first = prefix || key < rq.len - rq.fresh ? 0u : (key - (rq.len - rq.fresh)) * a.s.rep;  // rows before it do not see the key
-  float w = 0.0f;
-#pragma unroll 4
-  for (uint32_t r = first; r < n_rows; ++r) {
-    const float2 x = ml[r];
-    if (x.y != 0.0f) w = fmaf(__builtin_amdgcn_exp2f(src[r] - x.x), x.y, w);
-  }
-  const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
+  const uint32_t base = prefix ? 0xffffffffu : rq.len - rq.fresh;
   const float* in = prefix ? a.pw_in : a.w_in;
-  (prefix ? a.pw_out : a.w_out)[at] = (in ? in[at] : 0.0f) + w;
+  float* out = prefix ? a.pw_out : a.w_out;
+#pragma unroll
+  for (uint32_t c = 0; c < KEPT_KEYS / 256; ++c) {
+    const uint32_t key = kb * KEPT_KEYS + 256 * c + tid;
+    if (key >= rq.len) break;
+    const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
+    const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
+    const float before = in ? in[at] : 0.0f;
+    float w = 0.0f;
+#pragma unroll 4
+    for (uint32_t r = key <= base ? 0u : (key - base) * a.s.rep; r < n_rows; ++r) {  // earlier rows do not see the key
+      const float2 x = ml[r];
+      const float p = __builtin_amdgcn_exp2f(src[r] - x.x) * x.y;
+      w += x.y != 0.0f ? p : 0.0f;  // (a row of no token left no score)
+    }
+    out[at] = before + w;
+  }
 }
 
 // The row splits' sums, in order, and the weights so far.
@@ -1476,7 +1484,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     const uint32_t z = a.c.R + (a.pw_out ? 1 : 0), keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
     if (keep.own) {
-      const uint32_t joins = sp.splits > 1 ? out_rows : 0, key_blocks = (keys + 255) / 256;
+      const uint32_t joins = sp.splits > 1 ? out_rows : 0, key_blocks = (keys + KEPT_KEYS - 1) / KEPT_KEYS;
       hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(joins + key_blocks * a.s.G * z), dim3(256), 0, s, a, sp, stat, keep, joins, key_blocks);
       return hipGetLastError();
     }
