@@ -247,6 +247,7 @@ class KvOps {
     c.slot_stride = v.slot_stride ? v.slot_stride : cfg_.head_dim;
     c.head_stride = v.head_stride ? v.head_stride : c.slot_stride * v.capacity;
     c.req_stride = v.request_stride ? v.request_stride : c.head_stride * cfg_.kv_heads;
+    if (c.slot_stride >> 24) kfail("kv: slot_stride %llu is not below 2^24", (unsigned long long)c.slot_stride);
     if (c.slot_stride < cfg_.head_dim) kfail("kv: slot_stride %llu is below head_dim %u", (unsigned long long)c.slot_stride, cfg_.head_dim);
     if (c.head_stride < cfg_.head_dim) kfail("kv: head_stride %llu is below head_dim %u", (unsigned long long)c.head_stride, cfg_.head_dim);
     if (c.req_stride < cfg_.head_dim) kfail("kv: request_stride %llu is below head_dim %u", (unsigned long long)c.req_stride, cfg_.head_dim);
@@ -267,6 +268,7 @@ class KvOps {
     c.P = v.prefix_len;
     c.p_slot_stride = v.prefix_slot_stride ? v.prefix_slot_stride : cfg_.head_dim;
     c.p_head_stride = v.prefix_head_stride ? v.prefix_head_stride : c.p_slot_stride * (v.prefix_capacity ? v.prefix_capacity : v.prefix_len);
+    if (c.p_slot_stride >> 24) kfail("kv: prefix_slot_stride %llu is not below 2^24", (unsigned long long)c.p_slot_stride);
     if (c.p_slot_stride < cfg_.head_dim)
       kfail("kv: prefix_slot_stride %llu is below head_dim %u", (unsigned long long)c.p_slot_stride, cfg_.head_dim);
     if (c.p_head_stride < cfg_.head_dim)

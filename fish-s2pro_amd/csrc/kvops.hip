@@ -6,6 +6,7 @@
 #include <type_traits>
 
 #include "kvops.h"
+#include "lds_dma.h"
 #include "s2hip.h"
 #include "wave.h"
 
@@ -686,30 +687,37 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       }
   }
 
-  // thread's pieces of a tile: f16 tid + 256 i; f32 the wave's 8 keys, lane + 64 i of them
-  u32x4 kr[LD], vr[LD];
-  auto key_of = [&](int i) { return KH ? (tid + 256 * i) / PR : 8 * wave + (lane + 64 * i) / PR; };
-  auto piece_of = [&](int i) { return KH ? (tid + 256 * i) % PR : (lane + 64 * i) % PR; };
-  auto load = [&](const Where<T>& w) {
-#pragma unroll
-    for (int i = 0; i < LD; ++i) {
-      const size_t at = min(key_of(i), w.keys - 1) * w.stride + piece_of(i) * (16 / sizeof(T));
-      kr[i] = *reinterpret_cast<const u32x4*>(w.k + at);
-      vr[i] = *reinterpret_cast<const u32x4*>(w.v + at);
-    }
-  };
+  // f32: thread's pieces of a tile, of the wave's 8 keys: lane + 64 i
+  u32x4 kr[KH ? 1 : LD], vr[KH ? 1 : LD];
+  auto key_of = [&](int i) { return 8 * wave + (lane + 64 * i) / PR; };
+  auto piece_of = [&](int i) { return (lane + 64 * i) % PR; };
   // 16-byte piece p of row `key` stands at p ^ swz(key): keys' fragment reads take one piece of 8 rows in a row,
   // transposed value reads 64 bytes of 4 rows
   auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
   auto v_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (HD == 128 ? 4 * (key & 3u) : 4 * ((key >> 1) & 1u))) << 4); };
+  // f16: straight to LDS, a KiB per wave and load, each lane bringing the piece that belongs where its 16 bytes go;
+  // f32: to registers, and to LDS once the other tile is done with
+  const uint32_t lds0 = uint32_t(uintptr_t((lds_byte*)lds));
+  auto load = [&](const Where<T>& w, uint32_t buf) {
+    const uint8_t *k = reinterpret_cast<const uint8_t*>(w.k), *v = reinterpret_cast<const uint8_t*>(w.v);
+    const uint32_t stride = uint32_t(w.stride) * sizeof(T);
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      if constexpr (KH) {
+        const uint32_t x = (wave * LD + i) * 1024 + lane * 16, key = x / RB, off = min(key, w.keys - 1) * stride;
+        dma16(k, off + (k_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + (wave * LD + i) * 1024);
+        dma16(v, off + (v_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + PLANE + (wave * LD + i) * 1024);
+      } else {
+        const uint32_t off = min(key_of(i), w.keys - 1) * stride + piece_of(i) * 16;
+        kr[i] = *reinterpret_cast<const u32x4*>(k + off);
+        vr[i] = *reinterpret_cast<const u32x4*>(v + off);
+      }
+    }
+  };
   auto store = [&](uint32_t buf) {
     uint8_t* base = lds + buf * BUF;
     if constexpr (KH) {
-#pragma unroll
-      for (int i = 0; i < LD; ++i) {
-        *reinterpret_cast<u32x4*>(base + k_at(key_of(i), piece_of(i))) = kr[i];
-        *reinterpret_cast<u32x4*>(base + PLANE + v_at(key_of(i), piece_of(i))) = vr[i];
-      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     } else {
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -749,7 +757,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   Where<T> w{};
   if (t_lo < t_hi) {
     w = where(t_lo);
-    load(w);
+    load(w, 0);
     store(0);
   }
   __syncthreads();
@@ -757,7 +765,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     const uint32_t buf = (i - t_lo) & 1u;
     const bool more = i + 1 < t_hi;
     const Where<T> next = more ? where(i + 1) : w;
-    if (more) load(next);
+    if (more) load(next, buf ^ 1u);
     const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
 #pragma unroll 1
     for (int sub = 0; sub < KT / 32; ++sub) {
@@ -772,19 +780,26 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         const uint32_t i16 = lane & 15u, byte = 64 * dt + 32 * ((lane >> 4) & 1u) + 8 * (i16 & 3u);
         vp[dt] = (lds_byte*)lds + (buf * BUF + 32 * sub * RB + v_at(4 * h2 + i16 / 4, byte >> 4) + (byte & 15u));
       }
-      // the next fragment is read while one multiplies; the barriers keep the compiler from reading all of them
+      // fragments are read two ahead of their products; the barriers keep the compiler from reading all of them
       // first, for which there are no registers
       auto key8 = [&](int plane, int ks) { return *reinterpret_cast<const lds_half8*>(kp[ks % 4] + (plane * PLANE + ks / 4 * 128)); };
       floatx16 s = floatx16{};
-      half8 k8 = key8(0, 0), kl = KH ? half8{} : key8(1, 0);
+      half8 k8[3], kl[3];
+      k8[0] = key8(0, 0);
+      k8[1] = key8(0, 1);
+      if constexpr (!KH) {
+        kl[0] = key8(1, 0);
+        kl[1] = key8(1, 1);
+      }
 #pragma unroll
       for (int ks = 0; ks < DS; ++ks) {
-        const half8 k8n = ks + 1 < DS ? key8(0, ks + 1) : k8, kln = !KH && ks + 1 < DS ? key8(1, ks + 1) : kl;
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, qh[ks], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8, ql[ks], s, 0, 0, 0);
-        if constexpr (!KH) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[ks], s, 0, 0, 0);
-        k8 = k8n;
-        kl = kln;
+        if (ks + 2 < DS) {
+          k8[(ks + 2) % 3] = key8(0, ks + 2);
+          if constexpr (!KH) kl[(ks + 2) % 3] = key8(1, ks + 2);
+        }
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[ks % 3], qh[ks], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[ks % 3], ql[ks], s, 0, 0, 0);
+        if constexpr (!KH) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[ks % 3], qh[ks], s, 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
       const bool whole = __all(limit >= key0 + 31);
@@ -797,8 +812,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         factor[c] = KH ? unscale : unscale * scales[buf][0][c];
-        top = fmaxf(top, fmaxf(fmaxf(s[4 * c], s[4 * c + 1]), fmaxf(s[4 * c + 2], s[4 * c + 3])) * factor[c]);
+        const float x = fmaxf(fmaxf(s[4 * c], s[4 * c + 1]), fmaxf(s[4 * c + 2], s[4 * c + 3]));
+        top = fmaxf(top, KH ? x : x * factor[c]);
       }
+      if constexpr (KH) top *= unscale;
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
       if (__any(mn > m + SLACK)) {
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -827,9 +844,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       }
       half8 ph[2], pl[2];  // 16 keys each
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        ph[v / 8][v % 8] = _Float16(s[v]);
-        pl[v / 8][v % 8] = _Float16(fmaf(float(ph[v / 8][v % 8]), -1.0f, s[v]));
+      for (int v = 0; v < 16; ++v) {  // the upper 11 bits, and the rest
+        const float hi = __uint_as_float(__float_as_uint(s[v]) & 0xffffe000u);
+        ph[v / 8][v % 8] = _Float16(hi);
+        pl[v / 8][v % 8] = _Float16(s[v] - hi);
       }
       // 16 keys of 32 dims, transposed; plane 0: the values or their hi parts, 1: the lo parts
       auto value8 = [&](int plane, int dt, int st) {
@@ -838,7 +856,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         for (int u = 0; u < 2; ++u) y[u] = read_tr(vp[dt] + ((KH ? 1 : 2 + plane) * PLANE + (16 * st + 8 * u) * RB));
         return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
       };
-      bool odd = false;  // a value that is no number, and rows that must not see it
+      int odd = 0;  // a value that is no number, and rows that must not see it
       if (!whole && w.seg >= 0) {
         half8 z = half8{};
 #pragma unroll
@@ -846,40 +864,52 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
           for (int st = 0; st < 2; ++st) z = __builtin_elementwise_fma(value8(0, dt, st), half8{}, z);
         odd = __any(not_zero(z));
-        if (odd) {
-          half8 seen[2];
+      }
+      if (odd) {  // key by key, for the rows that see it
+        const float per_unit = KH ? 1.0f : 1.0f / unit;
+        for (int key = 0; key < 32 && 32 * sub + key < int(w.keys); ++key) {
+          float p = 0.0f;
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            seen[v / 8][v % 8] = key0 + int(8u * (v / 4) + 4u * h2 + (v % 4)) <= limit ? _Float16(1) : _Float16(0);
+          for (int v = 0; v < 16; ++v) {
+            const float x = __shfl(s[v], ((key >> 2) & 1) * 32 + int(r32), 64);
+            if ((v / 4) * 8 + v % 4 == (key & ~4)) p = KH ? x : x / (scales[buf][1][v / 4] * per_unit);
+          }
+          const bool sees = key0 + key <= limit;
+          const T* value = w.v + size_t(32 * sub + key) * w.stride + 4 * h2;
 #pragma unroll
           for (int dt = 0; dt < DT; ++dt) {
-            floatx16 hits = floatx16{};
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-              half8 v8 = value8(0, dt, st);
-              hits = __builtin_amdgcn_mfma_f32_32x32x16_f16(take_odd(v8), seen[st], hits, 0, 0, 0);
+            for (int v = 0; v < 16; ++v) {
+              const float x = fmaf(p * per_unit, float(value[32 * dt + 8 * (v / 4) + v % 4]), o[dt][v]);
+              o[dt][v] = sees ? x : o[dt][v];
             }
-#pragma unroll
-            for (int v = 0; v < 16; ++v) o[dt][v] = hits[v] > 0.0f ? NAN : o[dt][v];
             __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
-      half8 v8 = value8(0, 0, 0), u8 = KH ? half8{} : value8(1, 0, 0);
-#pragma unroll
-      for (int c = 0; c < 2 * DT; ++c) {
-        const int dt = c / 2, st = c % 2, n = c + 1;
-        const half8 v8n = n < 2 * DT ? value8(0, n / 2, n % 2) : v8, u8n = !KH && n < 2 * DT ? value8(1, n / 2, n % 2) : u8;
-        if (odd) {
-          take_odd(v8);
-          if constexpr (!KH) take_odd(u8);
+      odd = __builtin_amdgcn_readfirstlane(odd);
+      asm volatile("" : "+s"(odd));  // (one branch after the other: as two sides of one they would hold two sets of o)
+      if (!odd) {
+        // fragments are read two ahead
+        half8 v8[3], u8[3];
+        v8[0] = value8(0, 0, 0);
+        v8[1] = value8(0, 0, 1);
+        if constexpr (!KH) {
+          u8[0] = value8(1, 0, 0);
+          u8[1] = value8(1, 0, 1);
         }
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph[st], o[dt], 0, 0, 0);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl[st], o[dt], 0, 0, 0);
-        if constexpr (!KH) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8, ph[st], o[dt], 0, 0, 0);
-        v8 = v8n;
-        u8 = u8n;
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < 2 * DT; ++c) {
+          const int dt = c / 2, st = c % 2, n = c + 2;
+          if (n < 2 * DT) {
+            v8[n % 3] = value8(0, n / 2, n % 2);
+            if constexpr (!KH) u8[n % 3] = value8(1, n / 2, n % 2);
+          }
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 3], ph[st], o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 3], pl[st], o[dt], 0, 0, 0);
+          if constexpr (!KH) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[c % 3], ph[st], o[dt], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
     if (more) store(buf ^ 1u);
