@@ -632,7 +632,7 @@ constexpr int TILE_ROWS = 128;
 template <int HD, bool KH>
 __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
   using T = Elem<KH>;
-  constexpr int KT = KH ? 64 : 32;
+  constexpr int KT = KH ? 64 : 32, NSUB = KT / 32;
   constexpr int DS = HD / 16, DT = HD / 32;
   constexpr uint32_t RB = HD * 2, PLANE = KT * RB;        // bytes of a row and of a plane of a tile in LDS
   constexpr uint32_t BUF = (KH ? 2 : 4) * PLANE;          // K, V, or K hi, K lo, V hi, V lo
@@ -767,55 +767,77 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     const Where<T> next = more ? where(i + 1) : w;
     if (more) load(next, buf ^ 1u);
     const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
-#pragma unroll 1
-    for (int sub = 0; sub < KT / 32; ++sub) {
-      const int key0 = int(w.key0) + 32 * sub;
-      if (!__any(limit >= key0)) continue;  // nothing of it for this wave's rows
+    if (__any(limit >= int(w.key0))) {  // else nothing of it is for this wave's rows
       // fragment addresses: the swizzle changes with the low bits of ks and with dt, the rest are constants
       lds_byte *kp[4], *vp[DT];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) kp[c] = (lds_byte*)lds + (buf * BUF + 32 * sub * RB + k_at(r32, 2 * c + h2));
+      for (int c = 0; c < 4; ++c) kp[c] = (lds_byte*)lds + (buf * BUF + k_at(r32, 2 * c + h2));
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         const uint32_t i16 = lane & 15u, byte = 64 * dt + 32 * ((lane >> 4) & 1u) + 8 * (i16 & 3u);
-        vp[dt] = (lds_byte*)lds + (buf * BUF + 32 * sub * RB + v_at(4 * h2 + i16 / 4, byte >> 4) + (byte & 15u));
+        vp[dt] = (lds_byte*)lds + (buf * BUF + v_at(4 * h2 + i16 / 4, byte >> 4) + (byte & 15u));
       }
-      // fragments are read two ahead of their products; the barriers keep the compiler from reading all of them
-      // first, for which there are no registers
-      auto key8 = [&](int plane, int ks) { return *reinterpret_cast<const lds_half8*>(kp[ks % 4] + (plane * PLANE + ks / 4 * 128)); };
-      floatx16 s = floatx16{};
-      half8 k8[3], kl[3];
-      k8[0] = key8(0, 0);
-      k8[1] = key8(0, 1);
-      if constexpr (!KH) {
-        kl[0] = key8(1, 0);
-        kl[1] = key8(1, 1);
-      }
+      // plane 0: the keys or their hi parts, 1: the lo parts; 32 keys from 32 sub
+      auto key8 = [&](int plane, int sub, int ks) {
+        return *reinterpret_cast<const lds_half8*>(kp[ks % 4] + (plane * PLANE + 32 * sub * RB + ks / 4 * 128));
+      };
+      // 16 keys of 32 dims, transposed; plane as above
+      auto value8 = [&](int plane, int sub, int dt, int st) {
+        half4 y[2];
 #pragma unroll
-      for (int ks = 0; ks < DS; ++ks) {
-        if (ks + 2 < DS) {
-          k8[(ks + 2) % 3] = key8(0, ks + 2);
-          if constexpr (!KH) kl[(ks + 2) % 3] = key8(1, ks + 2);
+        for (int u = 0; u < 2; ++u) y[u] = read_tr(vp[dt] + ((KH ? 1 : 2 + plane) * PLANE + (32 * sub + 16 * st + 8 * u) * RB));
+        return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
+      };
+      // Products that follow one another go to different accumulators (f16: the two halves of the tile; f32: the
+      // terms), for one that waits for its own leaves the matrix unit idle.  Fragments are read two ahead; the
+      // barriers keep the compiler from reading all of them first, for which there are no registers.
+      floatx16 s[2] = {};
+      {
+        half8 k8[3][2];
+        auto read = [&](int ks) {
+          k8[ks % 3][0] = key8(0, 0, ks);
+          k8[ks % 3][1] = KH ? key8(0, 1, ks) : key8(1, 0, ks);
+        };
+        read(0);
+        read(1);
+#pragma unroll
+        for (int ks = 0; ks < DS; ++ks) {
+          if (ks + 2 < DS) read(ks + 2);
+          const half8 x = k8[ks % 3][0], y = k8[ks % 3][1];
+          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], s[0], 0, 0, 0);
+          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], s[1], 0, 0, 0);
+          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[ks], s[0], 0, 0, 0);
+          if constexpr (KH) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[ks], s[1], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[ks % 3], qh[ks], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[ks % 3], ql[ks], s, 0, 0, 0);
-        if constexpr (!KH) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[ks % 3], qh[ks], s, 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!KH) s[0] += s[1];
       }
-      const bool whole = __all(limit >= key0 + 31);
+      const bool whole = __all(limit >= int(w.key0) + KT - 1);
       if (!whole) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (key0 + int(8u * (v / 4) + 4u * h2 + (v % 4)) > limit) s[v] = -INFINITY;
-      }
-      float factor[4], top = -INFINITY;  // of the 8 keys of four scores
+        for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        factor[c] = KH ? unscale : unscale * scales[buf][0][c];
-        const float x = fmaxf(fmaxf(s[4 * c], s[4 * c + 1]), fmaxf(s[4 * c + 2], s[4 * c + 3]));
-        top = fmaxf(top, KH ? x : x * factor[c]);
+          for (int v = 0; v < 16; ++v)
+            if (int(w.key0) + int(32u * sub + 8u * (v / 4) + 4u * h2 + (v % 4)) > limit) s[sub][v] = -INFINITY;
       }
-      if constexpr (KH) top *= unscale;
+      float factor[4], top = -INFINITY;  // factor: of the 8 keys of four scores
+      if constexpr (KH) {
+        float top1 = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < 16; v += 2) {
+          top = fmaxf(fmaxf(top, s[0][v]), s[0][v + 1]);
+          top1 = fmaxf(fmaxf(top1, s[1][v]), s[1][v + 1]);
+        }
+        top = fmaxf(top, top1) * unscale;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) factor[c] = unscale;
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          factor[c] = unscale * scales[buf][0][c];
+          top = fmaxf(top, fmaxf(fmaxf(s[0][4 * c], s[0][4 * c + 1]), fmaxf(s[0][4 * c + 2], s[0][4 * c + 3])) * factor[c]);
+        }
+      }
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
       if (__any(mn > m + SLACK)) {
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -825,11 +847,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         m = mn;
       }
       const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        s[v] = __builtin_amdgcn_exp2f(fmaf(s[v], factor[v / 4], bias));
-        l += s[v];
-      }
+      float ratio[4];
       if constexpr (!KH) {
         const float* vs = scales[buf][1];
         const float most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
@@ -840,75 +858,78 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           unit = most;
         }
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s[v] *= vs[v / 4] / unit;  // powers of two
+        for (int c = 0; c < 4; ++c) ratio[c] = vs[c] / unit;  // powers of two
       }
-      half8 ph[2], pl[2];  // 16 keys each
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {  // the upper 11 bits, and the rest
-        const float hi = __uint_as_float(__float_as_uint(s[v]) & 0xffffe000u);
-        ph[v / 8][v % 8] = _Float16(hi);
-        pl[v / 8][v % 8] = _Float16(s[v] - hi);
-      }
-      // 16 keys of 32 dims, transposed; plane 0: the values or their hi parts, 1: the lo parts
-      auto value8 = [&](int plane, int dt, int st) {
-        half4 y[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) y[u] = read_tr(vp[dt] + ((KH ? 1 : 2 + plane) * PLANE + (16 * st + 8 * u) * RB));
-        return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
-      };
       int odd = 0;  // a value that is no number, and rows that must not see it
       if (!whole && w.seg >= 0) {
         half8 z = half8{};
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
+        for (int sub = 0; sub < NSUB; ++sub) {
 #pragma unroll
-          for (int st = 0; st < 2; ++st) z = __builtin_elementwise_fma(value8(0, dt, st), half8{}, z);
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int st = 0; st < 2; ++st) z = __builtin_elementwise_fma(value8(0, sub, dt, st), half8{}, z);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         odd = __any(not_zero(z));
       }
-      if (odd) {  // key by key, for the rows that see it
-        const float per_unit = KH ? 1.0f : 1.0f / unit;
-        for (int key = 0; key < 32 && 32 * sub + key < int(w.keys); ++key) {
-          float p = 0.0f;
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const float x = __shfl(s[v], ((key >> 2) & 1) * 32 + int(r32), 64);
-            if ((v / 4) * 8 + v % 4 == (key & ~4)) p = KH ? x : x / (scales[buf][1][v / 4] * per_unit);
-          }
-          const bool sees = key0 + key <= limit;
-          const T* value = w.v + size_t(32 * sub + key) * w.stride + 4 * h2;
+      for (int sub = 0; sub < NSUB; ++sub) {
+        half8 ph[2], pl[2];  // 16 keys each: the weights' upper 11 bits, and the rest
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) {
+        for (int v = 0; v < 16; ++v) {
+          float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], factor[v / 4], bias));
+          l += p;
+          s[sub][v] = p;
+          if constexpr (!KH) p *= ratio[v / 4];
+          const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
+          ph[v / 8][v % 8] = _Float16(hi);
+          pl[v / 8][v % 8] = _Float16(p - hi);
+        }
+        int slow = __builtin_amdgcn_readfirstlane(odd);
+        if (slow) {  // key by key, for the rows that see it
+          const float per_unit = KH ? 1.0f : 1.0f / unit;
+          for (int key = 0; key < 32 && 32 * sub + key < int(w.keys); ++key) {
+            float p = 0.0f;
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-              const float x = fmaf(p * per_unit, float(value[32 * dt + 8 * (v / 4) + v % 4]), o[dt][v]);
-              o[dt][v] = sees ? x : o[dt][v];
+              const float x = __shfl(s[sub][v], ((key >> 2) & 1) * 32 + int(r32), 64);
+              if ((v / 4) * 8 + v % 4 == (key & ~4)) p = x * per_unit;
             }
+            const bool sees = int(w.key0) + 32 * sub + key <= limit;
+            const T* value = w.v + size_t(32 * sub + key) * w.stride + 4 * h2;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+#pragma unroll
+              for (int v = 0; v < 16; ++v) {
+                const float x = fmaf(p, float(value[32 * dt + 8 * (v / 4) + v % 4]), o[dt][v]);
+                o[dt][v] = sees ? x : o[dt][v];
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        }
+        asm volatile("" : "+s"(slow));  // (one branch after the other: as two sides of one they would hold two sets of o)
+        if (!slow) {
+          // block c: 16 keys (st = c / DT) of 32 dims; its terms are one and two blocks apart
+          constexpr int BL = 2 * DT;
+          half8 v8[4], u8[KH ? 1 : 5];
+          auto read = [&](int c) {
+            v8[c % 4] = value8(0, sub, c % DT, c / DT);
+            if constexpr (!KH) u8[c % 5] = value8(1, sub, c % DT, c / DT);
+          };
+          read(0);
+          read(1);
+#pragma unroll
+          for (int c = 0; c < BL + (KH ? 1 : 2); ++c) {
+            if (c + 2 < BL) read(c + 2);
+            if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[c / DT], o[c % DT], 0, 0, 0);
+            if (c >= 1 && c - 1 < BL)
+              o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
+            if constexpr (!KH)
+              if (c >= 2) o[(c - 2) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[(c - 2) % 5], ph[(c - 2) / DT], o[(c - 2) % DT], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
           }
-        }
-      }
-      odd = __builtin_amdgcn_readfirstlane(odd);
-      asm volatile("" : "+s"(odd));  // (one branch after the other: as two sides of one they would hold two sets of o)
-      if (!odd) {
-        // fragments are read two ahead
-        half8 v8[3], u8[3];
-        v8[0] = value8(0, 0, 0);
-        v8[1] = value8(0, 0, 1);
-        if constexpr (!KH) {
-          u8[0] = value8(1, 0, 0);
-          u8[1] = value8(1, 0, 1);
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * DT; ++c) {
-          const int dt = c / 2, st = c % 2, n = c + 2;
-          if (n < 2 * DT) {
-            v8[n % 3] = value8(0, n / 2, n % 2);
-            if constexpr (!KH) u8[n % 3] = value8(1, n / 2, n % 2);
-          }
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 3], ph[st], o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 3], pl[st], o[dt], 0, 0, 0);
-          if constexpr (!KH) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[c % 3], ph[st], o[dt], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
