@@ -1042,8 +1042,22 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp
 // sum has one order.  blockIdx.z = request, or R for the prefix with the rows of
 // all requests; with several row splits the sums go to the workspace and
 // kv_weights_join_kernel adds them.
+struct RowSteps {
+  uint32_t base, begin, end, steps;
+};
+// The rows that a block of keys from k0 looks at: packed (b n + t) rep + r, or t rep + r of the request from the
+// first that sees key k0.
+__device__ __forceinline__ RowSteps row_steps(const KvAttendArgs& a, Request rq, bool prefix, uint32_t k0) {
+  RowSteps r;
+  r.base = prefix ? 0u : rq.len - rq.fresh;
+  r.end = prefix ? a.c.R * a.c.n * a.s.rep : rq.fresh * a.s.rep;
+  r.begin = !prefix && k0 > r.base ? min(r.end, (k0 - r.base) * a.s.rep) / 32 * 32 : 0u;
+  r.steps = (r.end - r.begin + 31) / 32;
+  return r;
+}
+
 template <int HD, bool KH>
-__global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const float* stat, float* part, uint32_t splits) {
+__global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const float* stat, float* part, uint32_t chunk) {
   using T = Elem<KH>;
   constexpr int KW = KH ? 2 : 1;           // 32-key tiles per wave
   constexpr int DS = HD / 16;
@@ -1058,13 +1072,11 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   if (!prefix) rq = request_of(a.c, z, nullptr);
   const uint32_t n_keys = rq.len, k0 = kb * KB;
   if (k0 >= n_keys) return;
-  // rows of this block: packed (b n + t) rep + r, or t rep + r of the request from the first that sees key k0
   const uint32_t per = a.c.n * a.s.rep;
-  const uint32_t base = prefix ? 0u : rq.len - rq.fresh;
-  const uint32_t row_end = prefix ? a.c.R * per : rq.fresh * a.s.rep;
-  const uint32_t row_begin = !prefix && k0 > base ? min(row_end, (k0 - base) * a.s.rep) / 32 * 32 : 0u;
-  const uint32_t steps = (row_end - row_begin + 31) / 32;
-  const uint32_t s_lo = steps * split / splits, s_hi = steps * (split + 1) / splits;
+  const RowSteps rs = row_steps(a, rq, prefix, k0);
+  const uint32_t base = rs.base, row_begin = rs.begin, row_end = rs.end;
+  const uint32_t s_lo = split * chunk, s_hi = min(s_lo + chunk, rs.steps);
+  if (s_lo >= s_hi && split) return;
 
   // the wave's keys: key 32 kw + r32, dims 16 ks + 8 h2 + e
   const uint32_t key0 = k0 + wave * 32 * KW;
@@ -1111,27 +1123,33 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     }
   }
 
-  // staging: 8 threads per row, HD / 8 dims each
+  // staging: 8 threads per row, HD / 8 dims each; nothing is looked at before it goes to LDS, a step later
   constexpr int SD = HD / 8;
   float4 qr[SD / 4];
-  float4 qi;
-  const uint32_t srow = tid / 8, sd = tid % 8 * SD;
+  float2 q_ml;
+  RawRequest q_rq{0, 0};
+  uint32_t q_t = 0;
+  bool q_row = false;
+  const uint32_t srow = tid / 8, sd = tid % 8 * 4;  // dims sd + 32 i ..: 128 bytes of a row per load
   auto load = [&](uint32_t step) {
-    const uint32_t row = row_begin + step * 32 + srow;
-    const uint32_t b = prefix ? row / per : z, t = prefix ? row / a.s.rep % a.c.n : row / a.s.rep;
-    const bool live = row < row_end && (!prefix || t < request_of(a.c, b, nullptr).fresh);
-    const size_t at = (size_t(b) * a.c.n + t) * a.s.H + g * a.s.rep + row % a.s.rep;
+    const uint32_t at_row = row_begin + step * 32 + srow, row = min(at_row, row_end - 1);
+    const uint32_t b = prefix ? row / per : z;
+    q_row = at_row < row_end;
+    q_t = prefix ? row / a.s.rep % a.c.n : row / a.s.rep;
+    if (prefix) q_rq = load_request(a.c, b);
+    const size_t at = (size_t(b) * a.c.n + q_t) * a.s.H + g * a.s.rep + row % a.s.rep;
 #pragma unroll
-    for (int i = 0; i < SD / 4; ++i)
-      qr[i] = live ? *reinterpret_cast<const float4*>(a.q + at * HD + sd + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-    const float2 ml = live ? *reinterpret_cast<const float2*>(stat + 2 * at) : make_float2(0.f, 0.f);
-    qi = make_float4(0.f, ml.x, live ? 1.0f / ml.y : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + t)));
+    for (int i = 0; i < SD / 4; ++i) qr[i] = *reinterpret_cast<const float4*>(a.q + at * HD + sd + 32 * i);
+    q_ml = *reinterpret_cast<const float2*>(stat + 2 * at);
   };
   auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
   auto store = [&](uint32_t buf) {
+    const bool live = q_row && (!prefix || q_t < checked(a.c, q_rq, nullptr).fresh);
+    float4 qi = make_float4(0.0f, live ? q_ml.x : 0.0f, live ? 1.0f / q_ml.y : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + q_t)));
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < SD / 4; ++i) {
+      if (!live) qr[i] = make_float4(0.f, 0.f, 0.f, 0.f);  // a row of no token may hold anything
       qr[i] = make_float4(qr[i].x * a.s.scale2, qr[i].y * a.s.scale2, qr[i].z * a.s.scale2, qr[i].w * a.s.scale2);
       big = fmaxf(big, fmaxf(fmaxf(fabsf(qr[i].x), fabsf(qr[i].y)), fmaxf(fabsf(qr[i].z), fabsf(qr[i].w))));
     }
@@ -1142,17 +1160,17 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     pow2_scale(big, qi.x, inv);
     if (tid % 8 == 0) info[buf][srow] = qi;
 #pragma unroll
-    for (int i = 0; i < SD / 8; ++i) {
-      const float x[8] = {qr[2 * i].x, qr[2 * i].y, qr[2 * i].z, qr[2 * i].w, qr[2 * i + 1].x, qr[2 * i + 1].y, qr[2 * i + 1].z, qr[2 * i + 1].w};
-      half8 hi, lo;
+    for (int i = 0; i < SD / 4; ++i) {
+      const float x[4] = {qr[i].x, qr[i].y, qr[i].z, qr[i].w};
+      half4 hi, lo;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < 4; ++e) {
         hi[e] = _Float16(x[e] * inv);
         lo[e] = _Float16(x[e] * inv - float(hi[e]));
       }
-      const uint32_t off = k_at(srow, sd / 8 + i);
-      *reinterpret_cast<half8*>(&lds[buf][off]) = hi;
-      *reinterpret_cast<half8*>(&lds[buf][PLANE + off]) = lo;
+      const uint32_t d = sd + 32 * i, off = k_at(srow, d / 8) + d % 8 * 2;
+      *reinterpret_cast<half4*>(&lds[buf][off]) = hi;
+      *reinterpret_cast<half4*>(&lds[buf][PLANE + off]) = lo;
     }
   };
 
@@ -1170,7 +1188,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     const uint32_t buf = (st - s_lo) & 1u;
     const bool more = st + 1 < s_hi;
     if (more) load(st + 1);
-    const float4 me = info[buf][r32];
+    float4 me = info[buf][r32];
     const int limit = __float_as_int(me.w);
     floatx16 s[KW];
 #pragma unroll
@@ -1186,21 +1204,23 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
         if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
       }
     }
+    if (!__all(limit >= int(key0) + 32 * KW - 1)) {
+      const bool lost = !(me.y - me.y == 0.0f) || !(me.z - me.z == 0.0f);  // a row of no number: that of the keys it sees alone
 #pragma unroll
-    for (int kw = 0; kw < KW; ++kw) {
-      const int first = int(key0) + 32 * kw;
-      if (__all(limit >= first + 31)) {
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
-      } else {
+      for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)) * me.z;
-          sum[kw][v] += first + int(8u * (v / 4) + 4u * h2 + (v % 4)) <= limit ? p : 0.0f;
+          const bool sees = int(key0) + int(32u * kw + 8u * (v / 4) + 4u * h2 + (v % 4)) <= limit;
+          if (lost && sees) sum[kw][v] = NAN;
+          if (lost || !sees) s[kw][v] = -INFINITY;
         }
-      }
+      if (lost) me.y = me.z = 0.0f;
     }
+#pragma unroll
+    for (int kw = 0; kw < KW; ++kw)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
     if (more) store(buf ^ 1u);
     __syncthreads();
   }
@@ -1217,7 +1237,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     const uint32_t key = key0 + 32 * kw + 8 * (r32 / 4) + 4 * h2 + r32 % 4;
     if (r32 >= 16 || key >= n_keys) continue;
     const size_t own = (size_t(z) * a.s.G + g) * a.c.cap + key;
-    if (splits > 1) {
+    if (gridDim.y > 1) {
       const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
       part[split * all + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own)] = mine;
     } else if (prefix) {
@@ -1292,15 +1312,18 @@ __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, Kv
   }
 }
 
-// The row splits' sums, in order, and the weights so far.
-__global__ __launch_bounds__(256) void kv_weights_join_kernel(KvAttendArgs a, const float* part, uint32_t splits) {
+// The chunks' sums, in order, and the weights so far.  KB: keys per block of kv_weigh_kernel.
+__global__ __launch_bounds__(256) void kv_weights_join_kernel(KvAttendArgs a, const float* part, uint32_t chunk, uint32_t kb) {
   const uint32_t g = blockIdx.y, z = blockIdx.z, key = blockIdx.x * 256 + threadIdx.x;
   const bool prefix = z == a.c.R;
-  if (key >= (prefix ? a.c.P : request_of(a.c, z, nullptr).len)) return;
+  Request rq{a.c.P, 0};
+  if (!prefix) rq = request_of(a.c, z, nullptr);
+  if (key >= rq.len) return;
+  const uint32_t chunks = max(1u, (row_steps(a, rq, prefix, key / kb * kb).steps + chunk - 1) / chunk);
   const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P), own = (size_t(z) * a.s.G + g) * a.c.cap + key;
   const float* src = part + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own);
   float x = 0.0f;
-  for (uint32_t i = 0; i < splits; ++i) x += src[i * all];
+  for (uint32_t i = 0; i < chunks; ++i) x += src[i * all];
   const size_t at = prefix ? size_t(g) * a.pw_stride + key : own;
   const float* in = prefix ? a.pw_in : a.w_in;
   (prefix ? a.pw_out : a.w_out)[at] = (in ? in[at] : 0.0f) + x;
@@ -1545,13 +1568,16 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t kb = KH() ? 256 : 128;
-      const uint32_t blocks = a.s.G * ((a.c.cap + kb - 1) / kb * a.c.R + (a.pw_out ? (a.c.P + kb - 1) / kb : 0));
+      // steps of 32 rows: half of them, on average, see a key of the turn that they are of
+      const uint32_t own_steps = (a.c.n * a.s.rep + 31) / 32, all_steps = a.pw_out ? (rows + 31) / 32 : own_steps;
+      const size_t work = size_t(a.s.G) * (size_t((a.c.cap + kb - 1) / kb) * a.c.R * own_steps / 2 + (a.pw_out ? size_t((a.c.P + kb - 1) / kb) * all_steps : 0));
       const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
-      const uint32_t ws = uint32_t(max(size_t(1), min(size_t(min((512 + blocks - 1) / blocks, ((a.pw_out ? rows : a.c.n * a.s.rep) + 31) / 32)),
-                                                      w.cap_weights / all)));
-      hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3((keys + kb - 1) / kb * a.s.G, ws, z), dim3(256), 0, s, a, w.stat, w.weights, ws);
-      if (ws > 1)
-        hipLaunchKernelGGL(kv_weights_join_kernel, dim3((keys + 255) / 256, a.s.G, z), dim3(256), 0, s, a, w.weights, ws);
+      const uint32_t room = uint32_t(max(size_t(1), min(size_t(all_steps), w.cap_weights / all)));  // chunks that fit the workspace
+      const uint32_t chunk = max(uint32_t(min(size_t(all_steps), max(size_t(4), work / 512))), (all_steps + room - 1) / room);
+      const uint32_t chunks = (all_steps + chunk - 1) / chunk;
+      hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3((keys + kb - 1) / kb * a.s.G, chunks, z), dim3(256), 0, s, a, w.stat, w.weights, chunk);
+      if (chunks > 1)
+        hipLaunchKernelGGL(kv_weights_join_kernel, dim3((keys + 255) / 256, a.s.G, z), dim3(256), 0, s, a, w.weights, chunk, kb);
     }
     return hipGetLastError();
   });
