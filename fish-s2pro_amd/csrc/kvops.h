@@ -45,6 +45,7 @@ struct KvSplit {
   float* o;
   float* ml;
   uint32_t tiles, splits;
+  uint32_t least;  // key tiles per split, at least (kv_tile_kernel)
 };
 
 // A step's scores, kept for the weights (nullable).

@@ -628,6 +628,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 // of the run for terms far below it.  (The f32 matrix instructions do a
 // sixteenth of the f16 ones' work per cycle.)
 constexpr int TILE_ROWS = 128;
+constexpr float NO_STATE = -1.0f;  // in the place of l: no state here
 
 template <int HD, bool KH>
 __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
@@ -649,7 +650,14 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, load_requests(a, tile * TILE_ROWS),
                              g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint32_t p_tiles = run.tiles ? (a.c.P + KT - 1) / KT : 0u, total = p_tiles + run.tiles;
-  const uint32_t t_lo = total * split / sp.splits, t_hi = total * (split + 1) / sp.splits;
+  // its splits, of sp.least tiles or more; the others, and a tile in one, say so where their state would be
+  const uint32_t splits = min(sp.splits, max(1u, (total + sp.least - 1) / sp.least));
+  const uint32_t t_lo = total * split / splits, t_hi = total * (split + 1) / splits;
+  if (sp.splits > 1 && (split >= splits || splits == 1)) {
+    const uint32_t r = tile * TILE_ROWS + tid;
+    if (tid < TILE_ROWS && r < rows) sp.ml[2 * (((size_t(g) * sp.tiles + r / 16) * sp.splits + split) * 16 + r % 16) + 1] = NO_STATE;
+    if (split >= splits) return;
+  }
 
   // this lane's row
   const uint32_t row = tile * TILE_ROWS + wave * 32 + r32, b_row = row / per, t_row = row / a.s.rep % a.c.n;
@@ -939,7 +947,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   }
 
   l = half_reduce(l, [](float p, float q) { return p + q; });
-  const bool last = sp.splits == 1;
+  const bool last = splits == 1;
   if (row >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
@@ -972,6 +980,7 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
   const RawRequest raw = load_request(a.c, b);
   const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
   const size_t part = (size_t(g) * sp.tiles + tile) * sp.splits * 16 + row % 16;  // + 16 split
+  bool done = false;  // the row has its output
   float M = -INFINITY, L = 0.0f;
   floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
   for (uint32_t s0 = team; s0 < sp.splits; s0 += 4 * TEAM) {
@@ -986,6 +995,10 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (s0 + i * TEAM >= sp.splits) continue;
+      if (ml[i].y == NO_STATE) {
+        done |= s0 + i * TEAM == 0;
+        continue;
+      }
       if (ml[i].x == -INFINITY) {  // no key, or none but of no number
         x += y[i];
         continue;
@@ -1018,7 +1031,7 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
     }
     M = all;
   }
-  if (!is_row || t >= checked(a.c, raw, nullptr).fresh) return;
+  if (done || !is_row || t >= checked(a.c, raw, nullptr).fresh) return;
   *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? 1.0f : 1.0f / L);
   if (stat && d == 0) {
     stat[2 * size_t(out)] = M;
@@ -1541,6 +1554,13 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
   sp.splits = max(1u, min(512 / lots, many ? most / 2 : (most + STEP_WAVES - 1) / STEP_WAVES));
+  sp.least = 2;
+  if (many && lots > 256 && lots <= 448) {
+    // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
+    // A prompt of 1500 tokens (376 row tiles) 81 : 65 us with the join; from 448 on the join costs what it saves.
+    sp.splits = 2;
+    sp.least = 768 / kt;
+  }
   if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   float* stat = a.w_out ? w.stat : nullptr;
   // a step's scores are kept where there is room for them
