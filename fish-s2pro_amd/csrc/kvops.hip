@@ -647,53 +647,16 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
   const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
-  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, load_requests(a, tile * TILE_ROWS),
-                             g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-  const uint32_t p_tiles = run.tiles ? (a.c.P + KT - 1) / KT : 0u, total = p_tiles + run.tiles;
-  // its splits, of sp.least tiles or more; the others, and a tile in one, say so where their state would be
-  const uint32_t splits = min(sp.splits, max(1u, (total + sp.least - 1) / sp.least));
-  const uint32_t t_lo = total * split / splits, t_hi = total * (split + 1) / splits;
-  if (sp.splits > 1 && (split >= splits || splits == 1)) {
-    const uint32_t r = tile * TILE_ROWS + tid;
-    if (tid < TILE_ROWS && r < rows) sp.ml[2 * (((size_t(g) * sp.tiles + r / 16) * sp.splits + split) * 16 + r % 16) + 1] = NO_STATE;
-    if (split >= splits) return;
-  }
-
-  // this lane's row
-  const uint32_t row = tile * TILE_ROWS + wave * 32 + r32, b_row = row / per, t_row = row / a.s.rep % a.c.n;
-  const uint32_t h_row = g * a.s.rep + row % a.s.rep;
-  const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
-  const bool live = row < rows && t_row < fresh_row;
-  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  // what needs nothing first: the requests, the row's query and, where it is known, the first tile of the prefix
+  const RawRequest raw = load_requests(a, tile * TILE_ROWS);
+  const uint32_t at = tile * TILE_ROWS + wave * 32 + r32, row = min(at, rows - 1);
+  const uint32_t b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
   const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
-  half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
-  float unscale;
-  {
-    float x[DS][8], big = 0.0f;
+  float4 qx[DS][2];  // dims 16 ks + 8 h2 ..
 #pragma unroll
-    for (int ks = 0; ks < DS; ++ks) {
+  for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 y = live ? *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + e) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[ks][e] = y.x * a.s.scale2;
-        x[ks][e + 1] = y.y * a.s.scale2;
-        x[ks][e + 2] = y.z * a.s.scale2;
-        x[ks][e + 3] = y.w * a.s.scale2;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[ks][e]));
-    }
-    float inv;
-    pow2_scale(half_reduce(big, [](float p, float q) { return fmaxf(p, q); }), unscale, inv);
-#pragma unroll
-    for (int ks = 0; ks < DS; ++ks)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = x[ks][e] * inv;
-        qh[ks][e] = _Float16(y);
-        ql[ks][e] = _Float16(y - float(qh[ks][e]));
-      }
-  }
+    for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
 
   // f32: thread's pieces of a tile, of the wave's 8 keys: lane + 64 i
   u32x4 kr[KH ? 1 : LD], vr[KH ? 1 : LD];
@@ -756,22 +719,78 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     }
   };
 
+  // The splits of a row tile share its prefix and its own tiles apart, the own ones the other way round; with
+  // sp.least there are only as many splits as it has that many tiles, and they share the run as a whole.
+  const bool whole_run = sp.least != 0;
+  const uint32_t p_all = (a.c.P + KT - 1) / KT;
+  uint32_t p_lo = whole_run ? 0u : p_all * split / sp.splits, n_pre = whole_run ? (split ? 0u : p_all) : p_all * (split + 1) / sp.splits - p_lo;
+  const bool early = n_pre != 0;
+  if (early) load(prefix_tile<T, KT>(a.c, g, p_lo), 0);
+  const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  uint32_t splits = sp.splits, o_lo = run.tiles * (splits - 1 - split) / splits, n_tiles = n_pre + run.tiles * (splits - split) / splits - o_lo;
+  if (whole_run) {
+    const uint32_t total = p_all + run.tiles;
+    splits = min(splits, (total + sp.least - 1) / sp.least);
+    const uint32_t lo = total * split / splits, hi = total * (split + 1) / splits;
+    p_lo = min(lo, p_all);
+    n_pre = min(hi, p_all) - p_lo;
+    o_lo = max(lo, p_all) - p_all;
+    n_tiles = hi - lo;
+    if (sp.splits > 1 && run.tiles && (split >= splits || splits == 1)) {  // no state here: say so in its place
+      const uint32_t r = tile * TILE_ROWS + tid;
+      if (tid < TILE_ROWS && r < rows) sp.ml[2 * (((size_t(g) * sp.tiles + r / 16) * sp.splits + split) * 16 + r % 16) + 1] = NO_STATE;
+    }
+  }
+  if (run.tiles == 0 || split >= splits) {  // no row of a token, or no share of them
+    if constexpr (KH) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (loads to LDS end before the block does)
+    return;
+  }
+
+  // this lane's row
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
+  const bool live = at < rows && t_row < fresh_row;
+  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
+  float unscale;
+  {
+    float big = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float4& y = qx[ks][e];
+        y = live ? make_float4(y.x * a.s.scale2, y.y * a.s.scale2, y.z * a.s.scale2, y.w * a.s.scale2) : make_float4(0.f, 0.f, 0.f, 0.f);
+        big = fmaxf(big, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+      }
+    float inv;
+    pow2_scale(half_reduce(big, [](float p, float q) { return fmaxf(p, q); }), unscale, inv);
+#pragma unroll
+    for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float4 z = qx[ks][e / 4];
+        const float y = (e % 4 == 0 ? z.x : e % 4 == 1 ? z.y : e % 4 == 2 ? z.z : z.w) * inv;
+        qh[ks][e] = _Float16(y);
+        ql[ks][e] = _Float16(y - float(qh[ks][e]));
+      }
+  }
+
   floatx16 o[DT];  // dim 32 dt + 8 (v / 4) + 4 h2 + v % 4
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = floatx16{};
   float m = -INFINITY, l = 0.0f, unit = 0.0f;  // f32: o in units of `unit`
   uint32_t seg = 0;
-  auto where = [&](uint32_t i) { return i < p_tiles ? prefix_tile<T, KT>(a.c, g, i) : own_tile<T, KT>(a.c, run, g, i - p_tiles, seg); };
+  auto where = [&](uint32_t i) { return i < n_pre ? prefix_tile<T, KT>(a.c, g, p_lo + i) : own_tile<T, KT>(a.c, run, g, o_lo + (i - n_pre), seg); };
   Where<T> w{};
-  if (t_lo < t_hi) {
-    w = where(t_lo);
-    load(w, 0);
+  if (n_tiles) {
+    w = where(0);
+    if (!early) load(w, 0);
     store(0);
   }
   __syncthreads();
-  for (uint32_t i = t_lo; i < t_hi; ++i) {
-    const uint32_t buf = (i - t_lo) & 1u;
-    const bool more = i + 1 < t_hi;
+  for (uint32_t i = 0; i < n_tiles; ++i) {
+    const uint32_t buf = i & 1u;
+    const bool more = i + 1 < n_tiles;
     const Where<T> next = more ? where(i + 1) : w;
     if (more) load(next, buf ^ 1u);
     const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
@@ -796,29 +815,29 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         for (int u = 0; u < 2; ++u) y[u] = read_tr(vp[dt] + ((KH ? 1 : 2 + plane) * PLANE + (32 * sub + 16 * st + 8 * u) * RB));
         return __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7);
       };
-      // Products that follow one another go to different accumulators (f16: the two halves of the tile; f32: the
-      // terms), for one that waits for its own leaves the matrix unit idle.  Fragments are read two ahead; the
-      // barriers keep the compiler from reading all of them first, for which there are no registers.
-      floatx16 s[2] = {};
+      // f16: products that follow one another go to different accumulators, for one that waits for its own leaves
+      // the matrix unit idle.  Fragments are read two ahead (f32, short of registers: one); the barriers keep the
+      // compiler from reading all of them first.
+      floatx16 s[NSUB] = {};
       {
+        constexpr int AHEAD = KH ? 2 : 1;
         half8 k8[3][2];
         auto read = [&](int ks) {
           k8[ks % 3][0] = key8(0, 0, ks);
           k8[ks % 3][1] = KH ? key8(0, 1, ks) : key8(1, 0, ks);
         };
-        read(0);
-        read(1);
+#pragma unroll
+        for (int ks = 0; ks < AHEAD; ++ks) read(ks);
 #pragma unroll
         for (int ks = 0; ks < DS; ++ks) {
-          if (ks + 2 < DS) read(ks + 2);
+          if (ks + AHEAD < DS) read(ks + AHEAD);
           const half8 x = k8[ks % 3][0], y = k8[ks % 3][1];
           s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], s[0], 0, 0, 0);
-          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], s[1], 0, 0, 0);
+          s[NSUB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], s[NSUB - 1], 0, 0, 0);
           s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[ks], s[0], 0, 0, 0);
           if constexpr (KH) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[ks], s[1], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!KH) s[0] += s[1];
       }
       const bool whole = __all(limit >= int(w.key0) + KT - 1);
       if (!whole) {
@@ -834,7 +853,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
         for (int v = 0; v < 16; v += 2) {
           top = fmaxf(fmaxf(top, s[0][v]), s[0][v + 1]);
-          top1 = fmaxf(fmaxf(top1, s[1][v]), s[1][v + 1]);
+          top1 = fmaxf(fmaxf(top1, s[NSUB - 1][v]), s[NSUB - 1][v + 1]);
         }
         top = fmaxf(top, top1) * unscale;
 #pragma unroll
@@ -919,23 +938,24 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         }
         asm volatile("" : "+s"(slow));  // (one branch after the other: as two sides of one they would hold two sets of o)
         if (!slow) {
-          // block c: 16 keys (st = c / DT) of 32 dims; its terms are one and two blocks apart
-          constexpr int BL = 2 * DT;
-          half8 v8[4], u8[KH ? 1 : 5];
+          // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind its first
+          constexpr int BL = 2 * DT, AHEAD = KH ? 2 : 1;
+          half8 v8[4], u8[KH ? 1 : 3];
           auto read = [&](int c) {
             v8[c % 4] = value8(0, sub, c % DT, c / DT);
-            if constexpr (!KH) u8[c % 5] = value8(1, sub, c % DT, c / DT);
+            if constexpr (!KH) u8[c % 3] = value8(1, sub, c % DT, c / DT);
           };
-          read(0);
-          read(1);
 #pragma unroll
-          for (int c = 0; c < BL + (KH ? 1 : 2); ++c) {
-            if (c + 2 < BL) read(c + 2);
+          for (int c = 0; c < AHEAD; ++c) read(c);
+#pragma unroll
+          for (int c = 0; c < BL + 1; ++c) {
+            if (c + AHEAD < BL) read(c + AHEAD);
             if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[c / DT], o[c % DT], 0, 0, 0);
-            if (c >= 1 && c - 1 < BL)
-              o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
-            if constexpr (!KH)
-              if (c >= 2) o[(c - 2) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[(c - 2) % 5], ph[(c - 2) / DT], o[(c - 2) % DT], 0, 0, 0);
+            if (c >= 1) {
+              const int b = c - 1;
+              o[b % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[b % 4], pl[b / DT], o[b % DT], 0, 0, 0);
+              if constexpr (!KH) o[b % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[b % 3], ph[b / DT], o[b % DT], 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
           }
         }
@@ -948,7 +968,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 
   l = half_reduce(l, [](float p, float q) { return p + q; });
   const bool last = splits == 1;
-  if (row >= rows || (last && !live)) return;
+  if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
   const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f) * (KH ? 1.0f : unit);
@@ -1553,8 +1573,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   const bool many = a.c.n * a.s.rep >= 32;
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
-  sp.splits = max(1u, min(512 / lots, many ? most / 2 : (most + STEP_WAVES - 1) / STEP_WAVES));
-  sp.least = 2;
+  sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
   if (many && lots > 256 && lots <= 448) {
     // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
     // A prompt of 1500 tokens (376 row tiles) 81 : 65 us with the join; from 448 on the join costs what it saves.
