@@ -1287,7 +1287,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // launch.  A block works out its rows' (m, l) from the splits itself, 16 lanes a
 // row, then takes a key per thread.  Against the scores computed once more: 8
 // requests of 1500 slots, f32, 18 us less; 4 of 20000, f16, 35 us.
-constexpr uint32_t KEPT_ROWS = 512;  // of the prefix, at most
+constexpr uint32_t KEPT_OWN_ROWS = 64, KEPT_ROWS = 512;  // rows of a request and, for the prefix, of all, at most
 constexpr uint32_t KEPT_KEYS = 512;  // per block
 template <int HD>
 __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, uint32_t joins, uint32_t key_blocks) {
@@ -1570,7 +1570,13 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   sp.ml = w.part_ml;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
-  const bool many = a.c.n * a.s.rep >= 32;
+  // Which kernel: by the scores to compute, over all heads and at most (capacities; lengths are on the device), for the
+  // step kernel starts and ends quicker and the tile kernel multiplies quicker.  Both with their join, us, step : tile,
+  // 32 heads over 8: f16 4 requests x 64 tokens over 1500 positions (13M scores) 37 : 39, 8 x 64 over 300 (7M) 27 : 30,
+  // 1 x 130 over 4000 (18M) 80 : 44, 1 x 130 over 100 (1.2M) 12 : 21; f32 8 x 8 over 1500 (3.2M) 32 : 34, 8 x 16 (6.5M)
+  // 51 : 42, 3 x 37 over 1001 (4.2M) 39 : 37, 1 x 130 over 100 18 : 23.  A request of fewer than 32 rows would leave most
+  // of a tile's waves idle in its own cache.
+  const bool many = a.c.n * a.s.rep >= 32 && size_t(a.s.G) * rows * (a.c.P + a.c.cap) > (f16 ? 14000000u : 4000000u);
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
   sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
@@ -1585,7 +1591,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   // a step's scores are kept where there is room for them
   KvScores keep{};
   const size_t own_scores = size_t(rows) * a.s.G * a.c.cap, prefix_scores = a.pw_out ? size_t(rows) * a.s.G * a.c.P : 0;
-  if (a.w_out && !many && own_scores + prefix_scores <= w.cap_weights && (!a.pw_out || rows <= KEPT_ROWS)) {
+  if (a.w_out && !many && own_scores + prefix_scores <= w.cap_weights && a.c.n * a.s.rep <= KEPT_OWN_ROWS && (!a.pw_out || rows <= KEPT_ROWS)) {
     keep.own = w.weights;
     keep.prefix = a.pw_out ? w.weights + own_scores : nullptr;
   }

@@ -108,18 +108,31 @@ def test_attend_requests(requests, f16):
     Batch((32, 8, 128), f16, lens, [1] * requests, cap=96, prefix=333, seed=requests).check_all()
 
 
+# Capacities: of the size of the lengths, and so large that a call counts as much work (it is launched by capacities)
+ROOM = [None, 32768]
+
+
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("n", [2, 3, 4, 5, 7, 8, 9, 16, 31, 32, 33, 64, 65, 130])
-def test_attend_several_tokens(n, f16):
+def test_attend_several_tokens(n, f16, room):
     """Causal within the new tokens; ragged; an idle request between others."""
     new = [n, max(1, n // 2), 0, 1, n]
     lens = [n, n // 2 + 40, 9, 1, n + 77]
-    Batch((8, 2, 128), f16, lens, new, cap=n + 80, prefix=70, seed=n).check_all()
+    Batch((8, 2, 128), f16, lens, new, cap=room or n + 80, prefix=70, seed=n).check_all()
 
 
 @pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n,prefix", [(8, 1000), (9, 2500), (33, 0), (40, 64), (200, 63), (380, 65), (500, 1)])
+def test_attend_splits(n, prefix, f16):
+    """From many splits of a row tile to one, tiles that end inside a split."""
+    Batch((32, 8, 128), f16, [n + 3, n], [n, n - 5], cap=9000, prefix=prefix, seed=n).check_all()
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("case", ["prompt", "turns", "turns64", "mha", "gqa7"])
-def test_attend_many_tokens(case, f16):
+def test_attend_many_tokens(case, f16, room):
     shape, lens, new, P = {
         "prompt": ((8, 2, 128), [517], [517], 0),
         "turns": ((32, 8, 128), [250, 300, 131, 250], [250, 221, 130, 3], 700),
@@ -127,7 +140,7 @@ def test_attend_many_tokens(case, f16):
         "mha": ((4, 4, 64), [300, 129], [300, 128], 33),
         "gqa7": ((14, 2, 128), [200, 77], [190, 77], 100),
     }[case]
-    Batch(shape, f16, lens, new, cap=max(lens) + 5, prefix=P, seed=5).check_all()
+    Batch(shape, f16, lens, new, cap=room or max(lens) + 5, prefix=P, seed=5).check_all()
 
 
 @pytest.mark.parametrize("f16", [False, True])
@@ -136,17 +149,19 @@ def test_attend_long(f16):
     Batch((8, 2, 128), f16, [20011, 3], [1, 1], cap=20100, prefix=9001, seed=3).check_all()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("n", [1, 40])
-def test_attend_sharp_scores(n, f16):
+def test_attend_sharp_scores(n, f16, room):
     """Large scores: one key takes nearly everything."""
-    Batch((8, 2, 128), f16, [n + 60, n + 5], [n, n], prefix=150, seed=8, spread=12.0).check_all()
+    Batch((8, 2, 128), f16, [n + 60, n + 5], [n, n], cap=room, prefix=150, seed=8, spread=12.0).check_all()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("n", [1, 70])
-def test_attend_wide_range_f32(n):
+def test_attend_wide_range_f32(n, room):
     """f32 values far outside the f16 range, keys small to match; rows of very different size."""
-    b = Batch((8, 2, 128), False, [n + 60, n + 5], [n, n], prefix=150, seed=9)
+    b = Batch((8, 2, 128), False, [n + 60, n + 5], [n, n], cap=room, prefix=150, seed=9)
     for x in (b.k, b.pk):
         x.mul_(1e-6)
     b.q.mul_(1e6)
@@ -156,10 +171,12 @@ def test_attend_wide_range_f32(n):
     b.check_all()
 
 
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("n", [1, 70])
-def test_attend_zero_rows(n):
+def test_attend_zero_rows(n, f16, room):
     """Queries, keys or values of zeros: equal weights, outputs of zero."""
-    b = Batch((8, 2, 64), True, [n + 60, n + 5], [n, n], prefix=40, seed=9)
+    b = Batch((8, 2, 64), f16, [n + 60, n + 5], [n, n], cap=room, prefix=40, seed=9)
     b.q[0] = 0
     b.k[1] = 0
     b.v[1] = 0
@@ -170,23 +187,37 @@ def test_attend_zero_rows(n):
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("n", [1, 3, 40, 150])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_attend_does_not_see(bad, n, f16):
+@pytest.mark.parametrize("room", ROOM)
+def test_attend_does_not_see(room, bad, n, f16):
     """Slots not in use, an idle request's cache and later tokens' keys and
     values hold NaN or infinities: rows that do not see them are as without."""
-    b = Batch((8, 2, 128), f16, [n + 21, n, 30, n + 40], [n, n, 0, n], cap=n + 64, prefix=50, seed=n)
+    b = Batch((8, 2, 128), f16, [n + 21, n, 30, n + 40], [n, n, 0, n], cap=room or n + 64, prefix=50, seed=n)
     want = b.expect()
     for r, used in enumerate(b.lens_h):
         b.k[r, :, used:] = bad
         b.v[r, :, used:] = bad
     b.k[2], b.v[2] = bad, bad
     b.check(b.attend(), want)
-    # the last token of request 0 brings a key and value of no number: its own row alone holds one
-    b.k[0, :, n + 20] = math.nan
+    # the last token of request 0 brings a value that is no number: its own row alone holds one, in that dim alone
     b.v[0, :, n + 20, 3] = bad
+    out = b.attend().clone()
+    assert not bool(out[0, n - 1, :, 3].isfinite().any())
+    out[0, n - 1, :, 3] = want[0][0, n - 1, :, 3].float()
+    b.check(out, want)
+    # and a key: its whole row holds none
+    b.k[0, :, n + 20] = math.nan
     out = b.attend().clone()
     assert bool(out[0, n - 1].isnan().all())
     out[0, n - 1] = want[0][0, n - 1].float()
     b.check(out, want)
+    # a value of the prefix: that dim of every row
+    b.k[0, :, n + 20], b.v[0, :, n + 20, 3] = 0.5, 0.5
+    b.pv[1, 49, 7] = bad
+    out = b.attend()
+    live = torch.arange(n, device="cuda")[None] < b.new[:, None]
+    half = b.H // b.G
+    assert not bool(out[live][:, half:, 7].isfinite().any()) and bool(out[live][:, :half].isfinite().all())
+    assert bool(out[live][:, half:, :7].isfinite().all()) and bool(out[live][:, half:, 8:].isfinite().all())
 
 
 @pytest.mark.parametrize("f16", [False, True])
@@ -265,11 +296,13 @@ def test_attend_same_bits(f16):
 # attend_weigh
 # --------------------------------------------------------------------------
 @pytest.mark.parametrize("f16", [False, True])
-@pytest.mark.parametrize("case", ["step", "step_prefix", "step16", "few", "turns", "prompt", "mha", "long"])
-def test_weigh(case, f16):
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("case", ["step", "step_prefix", "step16", "step64", "few", "turns", "prompt", "mha", "long"])
+def test_weigh(case, f16, room):
     shape, lens, new, P = {
         "step": ((32, 8, 128), [1, 2, 70, 129, 300], [1] * 5, 0),
         "step_prefix": ((8, 2, 64), [1, 40, 0, 17], [1, 1, 0, 1], 77),
+        "step64": ((32, 8, 128), [3 + 5 * b for b in range(64)], [1] * 64, 33),
         "step16": ((32, 8, 128), [3 + 5 * b for b in range(16)], [1] * 16, 257),
         "few": ((6, 2, 128), [40, 3, 65], [3, 2, 1], 31),
         "turns": ((8, 2, 128), [150, 90, 33], [130, 77, 33], 100),
@@ -277,7 +310,9 @@ def test_weigh(case, f16):
         "mha": ((4, 4, 64), [70, 150], [64, 150], 129),
         "long": ((8, 2, 128), [9001, 40], [1, 1], 2003),
     }[case]
-    b = Batch(shape, f16, lens, new, cap=max(lens) + 9, prefix=P, seed=12)
+    if room and len(lens) > 16:
+        room = 600  # (as much work, less memory)
+    b = Batch(shape, f16, lens, new, cap=room or max(lens) + 9, prefix=P, seed=12)
     want = b.expect()
     g = gen(3)
     w_in, pw_in = normal(g, b.R, b.G, b.cap).abs(), normal(g, b.G, max(P, 1)).abs()
@@ -316,9 +351,11 @@ def test_weigh(case, f16):
     assert b.ops.errors(stream()) == 0
 
 
-@pytest.mark.parametrize("n", [1, 50])
-def test_weigh_does_not_see(n):
-    b = Batch((8, 2, 128), True, [n + 21, n, 30, n + 40], [n, n, 0, n], cap=n + 64, prefix=50, seed=n)
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 50])
+def test_weigh_does_not_see(n, f16, room):
+    b = Batch((8, 2, 128), f16, [n + 21, n, 30, n + 40], [n, n, 0, n], cap=room or n + 64, prefix=50, seed=n)
     want = b.expect()
     for r, used in enumerate(b.lens_h):
         b.k[r, :, used:] = math.nan
@@ -330,6 +367,17 @@ def test_weigh_does_not_see(n):
     torch.cuda.synchronize()
     b.check(b.out, want)
     assert bool(((w.double() - want[2]).abs() <= want[3]).all()) and bool(((pw.double() - want[4]).abs() <= want[5]).all())
+    # a key that is no number takes with it the weights of the keys that its token sees, and of no others
+    b.k[0, :, n + 20] = math.nan
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), prefix_weights_out=ptr(pw), stream=stream())
+    torch.cuda.synchronize()
+    assert bool(w[0, :, : n + 21].isnan().all()) and bool(pw.isnan().all())
+    assert bool(((w.double() - want[2]).abs() <= want[3])[1:].all())
+    b.k[0, :, n + 20], b.k[1, :, n - 1] = 0.25, math.nan
+    b.new[1] = 0  # the request sits out: no row sees that key
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), prefix_weights_out=ptr(pw), stream=stream())
+    torch.cuda.synchronize()
+    assert bool(pw.isfinite().all()) and bool((w[1, :, :n] == 0).all())
 
 
 # --------------------------------------------------------------------------
