@@ -67,6 +67,12 @@ void may(const void* p, const char* name, size_t align) {
   if (p) need(p, name, align);
 }
 
+// out is in itself, or shares no word of `words` with it.
+void same_or_apart(const void* in, const void* out, size_t words, const char* name) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(in), y = reinterpret_cast<uintptr_t>(out);
+  if (x != y && x < y + 4 * words && y < x + 4 * words) kfail("kv: %s_out overlaps %s without being it", name, name);
+}
+
 class KvOps {
  public:
   explicit KvOps(const s2hip_kv_config& c) {
@@ -163,6 +169,9 @@ class KvOps {
       may(w_in, "weights_in", 4);
       may(pw_in, "prefix_weights_in", 4);
       may(pw_out, "prefix_weights_out", 4);
+      if (w_in) same_or_apart(w_in, w_out, size_t(v.requests) * cfg_.kv_heads * v.capacity, "weights");
+      if (pw_in && pw_out)
+        same_or_apart(pw_in, pw_out, size_t(cfg_.kv_heads) * (v.prefix_capacity ? v.prefix_capacity : v.prefix_len), "prefix_weights");
       if (pw_in && !pw_out) kfail("kv: prefix_weights_in without prefix_weights_out");
       a.w_in = w_in;
       a.w_out = w_out;
@@ -191,6 +200,10 @@ class KvOps {
     need(scores_out, "scores_out", 4);
     need(positions_out, "positions_out", 4);
     need(lens_out, "lens_out", 4);
+    const size_t words = size_t(layers) * v.requests * cfg_.kv_heads * v.capacity;
+    same_or_apart(scores, scores_out, words, "scores");
+    same_or_apart(positions, positions_out, words, "positions");
+    same_or_apart(v.lens, lens_out, v.requests, "lens");
     a.s = shape_;
     a.layer_stride = layer_stride ? layer_stride : a.c.req_stride * v.requests;
     a.layers = layers;
@@ -203,7 +216,8 @@ class KvOps {
     a.positions_out = positions_out;
     a.lens_out = lens_out;
     DeviceScope on(cfg_.device);
-    CHK(launch_kv_evict(cfg_.head_dim, cfg_.kv_f16, a, work_, s));
+    a.elem = cfg_.kv_f16 ? 2 : 4;
+    CHK(launch_kv_evict(a, work_, cfg_.head_dim, s));
   }
 
  private:

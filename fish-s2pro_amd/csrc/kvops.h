@@ -61,7 +61,7 @@ struct KvWorkspace {
   size_t cap_parts;
   float* weights;  // [cap_weights]: a step's scores, or the row splits' sums of weights
   size_t cap_weights;
-  uint32_t* moves;     // [cap_moves] (from << 16 | to)
+  uint32_t* moves;     // [cap_moves] to | from << 16
   uint32_t* counts;    // [cap_seqs][2]: moves, slots left
   size_t cap_moves, cap_seqs;
 };
@@ -84,6 +84,7 @@ struct KvEvictArgs {
   KvCaches c;
   size_t layer_stride;
   uint32_t layers, keep, recent, sinks;
+  uint32_t elem;  // bytes of a cache element
   const float* scores;
   const int32_t* positions;
   float* scores_out;
@@ -93,7 +94,7 @@ struct KvEvictArgs {
 
 hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStream_t s);
 hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const KvWorkspace& w, hipStream_t s);
-hipError_t launch_kv_evict(uint32_t hd, bool f16, const KvEvictArgs& a, const KvWorkspace& w, hipStream_t s);
+hipError_t launch_kv_evict(const KvEvictArgs& a, const KvWorkspace& w, uint32_t hd, hipStream_t s);
 hipError_t launch_kv_take_errors(uint32_t* err, uint32_t* taken, hipStream_t s);
 
 }  // namespace s2

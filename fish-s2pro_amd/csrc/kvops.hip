@@ -1372,10 +1372,12 @@ __device__ __forceinline__ uint32_t score_bits(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the block's 1024 threads in thread order; total for all.
+// Exclusive sum over the block's threads in thread order; total for all.
+template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   uint32_t x = v;
+#pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
     const uint32_t y = __shfl_up(x, d, 64);
     if (lane >= uint32_t(d)) x += y;
@@ -1385,65 +1387,123 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_
   __syncthreads();
   uint32_t before = 0;
   total = 0;
-  for (uint32_t w = 0; w < 16; ++w) {
-    if (w < wave) before += sh[w];
-    total += sh[w];
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; ++w) {
+    const uint32_t y = sh[w];
+    if (w < wave) before += y;
+    total += y;
   }
   return before + x - v;
 }
 
-// One block per (layer, request, kv head): thread t holds slots I t .. I t + I - 1.
-// The k-th largest score among the slots that compete (the safe ones all stay,
+// Rows lo .. hi - 1 of a list (to | from << 16) of cache sg, by `threads` threads; four loads of K and V each in flight.
+__device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, const uint32_t* list, uint32_t lo, uint32_t hi, uint32_t tid,
+                                          uint32_t threads, uint32_t pieces) {
+  const uint32_t g = sg % a.s.G, lb = sg / a.s.G, l = lb / a.c.R, b = lb % a.c.R;
+  const uint32_t shift = 31 - __clz(pieces);
+  const size_t base = (l * a.layer_stride + b * a.c.req_stride + g * a.c.head_stride) * a.elem;
+  uint8_t *k = static_cast<uint8_t*>(a.c.k) + base, *v = static_cast<uint8_t*>(a.c.v) + base;
+  const uint32_t first = lo << shift, last = hi << shift;
+  for (uint32_t i0 = first + tid; i0 < last; i0 += 4 * threads) {
+    u32x4 x[4], y[4];
+    size_t to[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t i = min(i0 + c * threads, last - 1), mv = list[i >> shift], d = (i & (pieces - 1)) * 16;
+      const size_t from = size_t(mv >> 16) * a.c.slot_stride * a.elem + d;
+      to[c] = size_t(mv & 0xffffu) * a.c.slot_stride * a.elem + d;
+      x[c] = *reinterpret_cast<const u32x4*>(k + from);
+      y[c] = *reinterpret_cast<const u32x4*>(v + from);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (i0 + c * threads < last) {
+        *reinterpret_cast<u32x4*>(k + to[c]) = x[c];
+        *reinterpret_cast<u32x4*>(v + to[c]) = y[c];
+      }
+  }
+}
+
+// Eviction: blockIdx.x = (layer, request, kv head) from seq0 on; thread t holds
+// slots I t .. I t + I - 1.
+//   The k-th largest score among the slots that compete (the safe ones all stay,
 // the others compete for the rest) by four digits of 8 bits from the top; of the
 // slots that equal it the lowest stay.  Then the freed slots below m and the
 // kept ones from m on are counted off in slot order: the x-th of one takes the
 // x-th of the other.
-template <int I>
-__global__ __launch_bounds__(1024) void kv_select_kernel(KvEvictArgs a, uint32_t seq0, uint32_t max_moves, uint32_t* moves, uint32_t* counts) {
-  __shared__ uint32_t sh[16], hist[256], pick[2];
-  __shared__ int32_t top[16];
-  const uint32_t tid = threadIdx.x, sg = seq0 + blockIdx.x, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
+//   MOVE: the block then moves the rows, its part blockIdx.y of them, 16 bytes a
+// thread; every part finds the same list (the scores are not written before all
+// have read them: in place, there is one part).  A cache's list takes about 10 us
+// of waiting for LDS and barriers, its rows the memory's time, so with two caches
+// or more per CU one hides the other, and with fewer the parts share the rows
+// without a second launch.  Otherwise the list goes to the workspace for
+// kv_move_kernel.
+struct KvMove {
+  uint32_t seq0, max_moves, pieces;  // pieces: 16-byte pieces of a row
+  uint32_t* moves;
+  uint32_t* counts;
+  bool lens;  // MOVE: write lens_out
+};
+template <int THREADS, int I, bool MOVE>
+__global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMove mv) {
+  constexpr int HIST = 4;  // copies of the digit counts, by lane, for many scores share a digit
+  __shared__ uint32_t sh[THREADS / 64], hist[HIST][256], pick[2];
+  __shared__ int32_t top[THREADS / 64];
+  __shared__ uint32_t list[THREADS * I / 2];  // to | from << 16
+  const uint32_t tid = threadIdx.x, sg = mv.seq0 + blockIdx.x, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
   const uint32_t lane = tid & 63u, wave = tid >> 6;
   const int32_t in_use = a.c.lens[b];
-  const bool ok = in_use >= 0 && in_use <= int32_t(a.c.cap);
-  if (!ok && tid == 0 && lb == b && g == 0) atomicOr(a.s.err, S2HIP_KV_ERR_LENS);
-  const uint32_t n = ok ? uint32_t(in_use) : 0u, m = min(n, a.keep);
-  if (tid == 0) counts[2 * blockIdx.x + 1] = ok ? m : 0xffffffffu;
   const size_t base = size_t(sg) * a.c.cap;
   float sc[I];
   int32_t pos[I];
-  uint32_t bits[I];
-  int32_t newest = INT32_MIN;
 #pragma unroll
-  for (int i = 0; i < I; ++i) {
-    const uint32_t s = tid * I + i;
-    sc[i] = s < n ? a.scores[base + s] : 0.0f;
-    pos[i] = s < n ? a.positions[base + s] : INT32_MIN;
-    bits[i] = score_bits(sc[i]);
-    newest = max(newest, pos[i]);
+  for (int i = 0; i < I; ++i) {  // (slots not in use are loaded and left)
+    const size_t at = base + min(tid * I + i, a.c.cap - 1);
+    sc[i] = a.scores[at];
+    pos[i] = a.positions[at];
+  }
+  const bool ok = in_use >= 0 && in_use <= int32_t(a.c.cap);
+  const uint32_t n = ok ? uint32_t(in_use) : 0u, m = min(n, a.keep);
+  const bool writes = !MOVE || blockIdx.y == 0;
+  if (tid == 0 && writes) {
+    if (!ok && lb == b && g == 0) atomicOr(a.s.err, S2HIP_KV_ERR_LENS);
+    if (!MOVE) mv.counts[2 * blockIdx.x + 1] = ok ? m : 0xffffffffu;
+    if (MOVE && mv.lens && ok && lb == b && g == 0) a.lens_out[b] = int32_t(m);
   }
   if (n <= a.keep) {  // nothing to cut
-    if (tid == 0) counts[2 * blockIdx.x] = 0;
+    if (!MOVE && tid == 0) mv.counts[2 * blockIdx.x] = 0;
+    if (writes) {
 #pragma unroll
-    for (int i = 0; i < I; ++i) {
-      const uint32_t s = tid * I + i;
-      if (s < n) {
-        a.scores_out[base + s] = sc[i];
-        a.positions_out[base + s] = pos[i];
+      for (int i = 0; i < I; ++i) {
+        const uint32_t s = tid * I + i;
+        if (s < n) {
+          a.scores_out[base + s] = sc[i];
+          a.positions_out[base + s] = pos[i];
+        }
       }
     }
     return;
   }
+  uint32_t bits[I];
+  int32_t newest = INT32_MIN;
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    bits[i] = score_bits(sc[i]);
+    if (tid * I + i < n) newest = max(newest, pos[i]);
+  }
+#pragma unroll
   for (int d = 32; d >= 1; d >>= 1) newest = max(newest, __shfl_xor(newest, d, 64));
   if (lane == 0) top[wave] = newest;
+  for (uint32_t i = tid; i < HIST * 256; i += THREADS) hist[0][i] = 0;
   __syncthreads();
-  for (uint32_t w = 0; w < 16; ++w) newest = max(newest, top[w]);
+#pragma unroll
+  for (uint32_t w = 0; w < THREADS / 64; ++w) newest = max(newest, top[w]);
   uint32_t safe = 0, n_safe = 0;  // bit i: slot i of the thread
 #pragma unroll
   for (int i = 0; i < I; ++i)
     if (tid * I + i < n && (int64_t(pos[i]) > int64_t(newest) - int64_t(a.recent) || int64_t(pos[i]) < int64_t(a.sinks))) safe |= 1u << i;
-  block_scan(__popc(safe), sh, n_safe);
-  // who competes for how many places (positions given twice can make more safe slots than there is room)
+  block_scan<THREADS>(__popc(safe), sh, n_safe);
+  // who competes for how many places (positions given twice, or many sinks, can make more safe slots than there is room)
   const bool room = n_safe <= m;
   uint32_t want = room ? m - n_safe : m;
   uint32_t compete = 0;
@@ -1452,23 +1512,33 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvEvictArgs a, uint32_t
     if (tid * I + i < n && (((safe >> i) & 1u) == 0) == room) compete |= 1u << i;
   uint32_t prefix = 0, kept = room ? safe : 0u;
   if (want) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      __syncthreads();
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
+#pragma unroll 1
+    for (int shift = 24; shift >= 0; shift -= 8) {  // (the counts are zero here)
 #pragma unroll
       for (int i = 0; i < I; ++i)
-        if (((compete >> i) & 1u) && (shift == 24 || (bits[i] >> (shift + 8)) == prefix)) atomicAdd(&hist[(bits[i] >> shift) & 255u], 1u);
+        if (((compete >> i) & 1u) && (shift == 24 || (bits[i] >> (shift + 8)) == prefix))
+          atomicAdd(&hist[lane % HIST][(bits[i] >> shift) & 255u], 1u);
       __syncthreads();
       if (tid < 64) {  // digits from the top: lane l holds 255 - 4 l .. 252 - 4 l
         uint32_t c[4], x = 0;
-        for (int j = 0; j < 4; ++j) x += c[j] = hist[255 - 4 * lane - j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          c[j] = 0;
+#pragma unroll
+          for (int h = 0; h < HIST; ++h) {
+            c[j] += hist[h][255 - 4 * lane - j];
+            hist[h][255 - 4 * lane - j] = 0;
+          }
+          x += c[j];
+        }
         uint32_t y = x;
+#pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
           const uint32_t z = __shfl_up(y, d, 64);
           if (lane >= uint32_t(d)) y += z;
         }
         uint32_t above = y - x;
+#pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (above < want && above + c[j] >= want) {
             pick[0] = 255 - 4 * lane - j;
@@ -1488,60 +1558,62 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvEvictArgs a, uint32_t
         if (bits[i] > prefix) kept |= 1u << i;
         if (bits[i] == prefix) equal |= 1u << i;
       }
-    uint32_t rank = block_scan(__popc(equal), sh, dummy);
+    uint32_t rank = block_scan<THREADS>(__popc(equal), sh, dummy);
 #pragma unroll
     for (int i = 0; i < I; ++i)
       if ((equal >> i) & 1u)
         if (rank++ < want) kept |= 1u << i;
   }
-  uint32_t holes = 0, movers = 0;
+  // slots of the thread below m; the rest of them
+  const uint32_t low = tid * I >= m ? 0u : m - tid * I >= 32 ? 0xffffffffu : (1u << (m - tid * I)) - 1u;
+  const uint32_t used = tid * I >= n ? 0u : n - tid * I >= uint32_t(I) ? uint32_t((uint64_t(1) << I) - 1u) : (1u << (n - tid * I)) - 1u;
+  const uint32_t holes = used & low & ~kept, movers = used & ~low & kept;
+  uint32_t both;
+  const uint32_t ranks = block_scan<THREADS>(__popc(holes) | __popc(movers) << 16, sh, both);  // (at most 16384 of each, as many of one as of the other)
+  const uint32_t n_movers = both >> 16;
+  uint32_t hr = ranks & 0xffffu, mr = ranks >> 16;
+  uint16_t* half = reinterpret_cast<uint16_t*>(list);
 #pragma unroll
   for (int i = 0; i < I; ++i) {
-    const uint32_t s = tid * I + i;
-    const bool k = (kept >> i) & 1u;
-    if (s < m && !k) holes |= 1u << i;
-    if (s >= m && s < n && k) movers |= 1u << i;
-    if (s < m && k) {
-      a.scores_out[base + s] = sc[i];
-      a.positions_out[base + s] = pos[i];
+    if ((holes >> i) & 1u) half[2 * hr++] = uint16_t(tid * I + i);
+    if ((movers >> i) & 1u) half[2 * mr++ + 1] = uint16_t(tid * I + i);
+  }
+  __syncthreads();
+  if (writes) {  // scores and positions go from the threads that hold them
+    mr = ranks >> 16;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const bool moves = (movers >> i) & 1u, stays = ((used & low & kept) >> i) & 1u;
+      const uint32_t to = moves ? half[2 * mr++] : tid * I + i;
+      if (moves || stays) {
+        a.scores_out[base + to] = sc[i];
+        a.positions_out[base + to] = pos[i];
+      }
     }
   }
-  uint32_t n_holes, n_movers;
-  uint32_t hr = block_scan(__popc(holes), sh, n_holes), mr = block_scan(__popc(movers), sh, n_movers);
-  uint16_t* list = reinterpret_cast<uint16_t*>(moves + size_t(blockIdx.x) * max_moves);  // (to, from) pairs
-#pragma unroll
-  for (int i = 0; i < I; ++i) {
-    if ((holes >> i) & 1u) list[2 * hr++] = uint16_t(tid * I + i);
-    if ((movers >> i) & 1u) list[2 * mr++ + 1] = uint16_t(tid * I + i);
-  }
-  if (tid == 0) counts[2 * blockIdx.x] = n_movers;
-  __syncthreads();  // the block's own stores to global memory are visible to it
-  for (uint32_t i = tid; i < n_movers; i += 1024) {
-    const uint32_t to = list[2 * i], from = list[2 * i + 1];
-    a.scores_out[base + to] = a.scores[base + from];
-    a.positions_out[base + to] = a.positions[base + from];
+  if constexpr (!MOVE) {
+    if (tid == 0) mv.counts[2 * blockIdx.x] = n_movers;
+    for (uint32_t i = tid; i < n_movers; i += THREADS) mv.moves[size_t(blockIdx.x) * mv.max_moves + i] = list[i];
+  } else {
+    move_rows(a, sg, list, n_movers * blockIdx.y / gridDim.y, n_movers * (blockIdx.y + 1) / gridDim.y, tid, THREADS, mv.pieces);
   }
 }
 
-// Rows of 16-byte pieces; blockIdx.y = (layer, request, kv head) of the launch.
-template <int HD, bool KH>
-__global__ __launch_bounds__(256) void kv_move_kernel(KvEvictArgs a, uint32_t seq0, uint32_t max_moves, const uint32_t* moves, const uint32_t* counts) {
-  using T = Elem<KH>;
-  constexpr uint32_t LP = HD * sizeof(T) / 16, RPB = 256 / LP;
-  const uint32_t tid = threadIdx.x, sg = seq0 + blockIdx.y, g = sg % a.s.G, lb = sg / a.s.G, l = lb / a.c.R, b = lb % a.c.R;
-  const uint32_t n_moves = counts[2 * blockIdx.y], left = counts[2 * blockIdx.y + 1];
-  if (blockIdx.x == 0 && tid == 0 && l == 0 && g == 0 && left != 0xffffffffu) a.lens_out[b] = int32_t(left);
-  const size_t base = l * a.layer_stride + b * a.c.req_stride + g * a.c.head_stride;
-  for (uint32_t i = blockIdx.x * RPB + tid / LP; i < n_moves; i += gridDim.x * RPB) {
-    const uint32_t mv = moves[size_t(blockIdx.y) * max_moves + i], to = mv & 0xffffu, from = mv >> 16;
-    const size_t d = (tid % LP) * (16 / sizeof(T));
-    T* k = static_cast<T*>(a.c.k) + base + d;
-    T* v = static_cast<T*>(a.c.v) + base + d;
-    const u32x4 x = *reinterpret_cast<const u32x4*>(k + from * a.c.slot_stride);
-    const u32x4 y = *reinterpret_cast<const u32x4*>(v + from * a.c.slot_stride);
-    *reinterpret_cast<u32x4*>(k + to * a.c.slot_stride) = x;
-    *reinterpret_cast<u32x4*>(v + to * a.c.slot_stride) = y;
-  }
+// blockIdx.y = (layer, request, kv head) of the launch.
+__global__ __launch_bounds__(256) void kv_move_kernel(KvEvictArgs a, KvMove mv) {
+  const uint32_t sg = mv.seq0 + blockIdx.y, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
+  const uint32_t n_moves = mv.counts[2 * blockIdx.y], left = mv.counts[2 * blockIdx.y + 1];
+  if (blockIdx.x == 0 && threadIdx.x == 0 && lb == b && g == 0 && left != 0xffffffffu) a.lens_out[b] = int32_t(left);
+  move_rows(a, sg, mv.moves + size_t(blockIdx.y) * mv.max_moves, n_moves * blockIdx.x / gridDim.x, n_moves * (blockIdx.x + 1) / gridDim.x,
+            threadIdx.x, 256, mv.pieces);
+}
+
+// lens_out in place of lens, once nothing reads them.
+__global__ __launch_bounds__(256) void kv_lens_kernel(KvEvictArgs a) {
+  const uint32_t b = threadIdx.x;
+  if (b >= a.c.R) return;
+  const int32_t len = a.c.lens[b];
+  if (len >= 0 && len <= int32_t(a.c.cap)) a.lens_out[b] = min(len, int32_t(a.keep));
 }
 
 __global__ void kv_take_errors_kernel(uint32_t* err, uint32_t* taken) { *taken = atomicExch(err, 0u); }
@@ -1628,28 +1700,46 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   });
 }
 
-hipError_t launch_kv_evict(uint32_t hd, bool f16, const KvEvictArgs& a, const KvWorkspace& w, hipStream_t s) {
+template <bool MOVE>
+static void select_launch(const KvEvictArgs& a, const KvMove& mv, dim3 grid, hipStream_t s) {
+  if (a.c.cap <= 2048)
+    hipLaunchKernelGGL((kv_select_kernel<256, 8, MOVE>), grid, dim3(256), 0, s, a, mv);
+  else if (a.c.cap <= 4096)
+    hipLaunchKernelGGL((kv_select_kernel<512, 8, MOVE>), grid, dim3(512), 0, s, a, mv);
+  else if (a.c.cap <= 16384)
+    hipLaunchKernelGGL((kv_select_kernel<1024, 16, MOVE>), grid, dim3(1024), 0, s, a, mv);
+  else
+    hipLaunchKernelGGL((kv_select_kernel<1024, 32, MOVE>), grid, dim3(1024), 0, s, a, mv);
+}
+
+hipError_t launch_kv_evict(const KvEvictArgs& a, const KvWorkspace& w, uint32_t hd, hipStream_t s) {
+  auto meet = [](const void* p, const void* q, size_t n) {  // n words from p, from q
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+    return x < y + 4 * n && y < x + 4 * n;
+  };
   const uint32_t seqs = a.layers * a.c.R * a.s.G;
-  const uint32_t max_moves = a.keep < a.c.cap ? min(a.keep, a.c.cap - a.keep) : 0u;
+  const size_t words = size_t(seqs) * a.c.cap;
+  const bool in_place = meet(a.scores, a.scores_out, words) || meet(a.positions, a.positions_out, words);
+  const bool lens_in_place = meet(a.c.lens, a.lens_out, a.c.R);
+  KvMove mv{};
+  mv.max_moves = a.keep < a.c.cap ? min(a.keep, a.c.cap - a.keep) : 0u;
+  mv.pieces = hd * a.elem / 16;
+  mv.moves = w.moves;
+  mv.counts = w.counts;
+  if (seqs >= 512 || (!in_place && !lens_in_place)) {
+    mv.lens = !lens_in_place;
+    const uint32_t parts = in_place ? 1u : min((512 + seqs - 1) / seqs, max(1u, mv.max_moves / 16));
+    select_launch<true>(a, mv, dim3(seqs, parts), s);
+    if (lens_in_place) hipLaunchKernelGGL(kv_lens_kernel, dim3(1), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
   // as many caches per launch as the lists have room for
-  const uint32_t per = uint32_t(min(max_moves ? w.cap_moves / max_moves : w.cap_seqs, w.cap_seqs));
-  for (uint32_t s0 = 0; s0 < seqs; s0 += per) {
-    const uint32_t ns = min(per, seqs - s0);
-    const dim3 grid(ns), block(1024);
-    if (a.c.cap <= 1024)
-      hipLaunchKernelGGL((kv_select_kernel<1>), grid, block, 0, s, a, s0, max_moves, w.moves, w.counts);
-    else if (a.c.cap <= 4096)
-      hipLaunchKernelGGL((kv_select_kernel<4>), grid, block, 0, s, a, s0, max_moves, w.moves, w.counts);
-    else if (a.c.cap <= 16384)
-      hipLaunchKernelGGL((kv_select_kernel<16>), grid, block, 0, s, a, s0, max_moves, w.moves, w.counts);
-    else
-      hipLaunchKernelGGL((kv_select_kernel<32>), grid, block, 0, s, a, s0, max_moves, w.moves, w.counts);
-    const hipError_t e = by_shape(hd, f16, [&](auto HD, auto KH) {
-      const uint32_t rows = 256 / (HD() * (KH() ? 2 : 4) / 16);
-      hipLaunchKernelGGL((kv_move_kernel<HD(), KH()>), dim3(max(1u, min(64u, (max_moves + rows - 1) / rows)), ns), dim3(256), 0, s, a, s0,
-                         max_moves, w.moves, w.counts);
-      return hipGetLastError();
-    });
+  const uint32_t per = uint32_t(min(mv.max_moves ? w.cap_moves / mv.max_moves : w.cap_seqs, w.cap_seqs));
+  for (mv.seq0 = 0; mv.seq0 < seqs; mv.seq0 += per) {
+    const uint32_t ns = min(per, seqs - mv.seq0);
+    select_launch<false>(a, mv, dim3(ns), s);
+    hipLaunchKernelGGL(kv_move_kernel, dim3(max(1u, min(64u, mv.max_moves * mv.pieces / 256)), ns), dim3(256), 0, s, a, mv);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

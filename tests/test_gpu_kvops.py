@@ -511,6 +511,19 @@ def test_evict_ties_and_odd_scores(values):
     run_evict(ops, k, v, [700, 650, 211], 210, 31, 4, scores, positions)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("layers,cap", [(1, 900), (9, 300), (40, 130), (40, 2100)])
+def test_evict_many_caches(layers, cap, in_place):
+    """From few caches to more than two a compute unit."""
+    g = gen(layers)
+    R, G = 4, 4
+    scores = normal(g, layers * R, G, cap).abs()
+    positions = torch.argsort(torch.rand(layers * R, G, cap, generator=g, device="cuda"), 2).to(torch.int32)
+    k, v = normal(g, layers * R, G, cap, 128).half(), normal(g, layers * R, G, cap, 128).half()
+    ops = KvOps(4, 4, 128, max_requests=R, max_tokens=R, kv_f16=True)
+    run_evict(ops, k, v, [cap, cap // 2, cap // 3, 0], cap // 2 - 5, 20, 4, scores, positions, layers=layers, in_place=in_place)
+
+
 def test_evict_positions_given_twice():
     """More safe slots than room: the heaviest of them stay."""
     g = gen(9)
@@ -802,6 +815,10 @@ def test_refusals():
     refused("recent 6 is more than keep 5", o.evict, v(), 5, 6, 0, *([p["q"]] * 5))
     refused("layers 0", o.evict, v(), 5, 3, 2, *([p["q"]] * 5), layers=0)
     refused("layer_stride 3", o.evict, v(), 5, 3, 2, *([p["q"]] * 5), layers=2, layer_stride=3)
+    refused("scores_out overlaps", o.evict, v(), 5, 3, 2, p["q"], p["k"], p["q"] + 4, p["k"], p["out"])
+    refused("positions_out overlaps", o.evict, v(), 5, 3, 2, p["q"], p["k"], p["q"], p["k"] + 4, p["out"])
+    refused("lens_out overlaps", o.evict, v(), 5, 3, 2, *([p["q"]] * 4), p["lens"] + 4)
+    refused("weights_out overlaps", o.attend_weigh, v(), p["q"], 1, p["out"], p["k"], weights_in=p["k"] + 4)
     refused("lens_out is NULL", o.evict, v(), 5, 3, 2, *([p["q"]] * 4), 0)
     torch.cuda.synchronize()
     b.check(b.attend())  # nothing was launched, the handle works
