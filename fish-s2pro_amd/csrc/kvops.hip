@@ -40,6 +40,22 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 
+// Sum over lanes 0 .. l of the wave (all 64 active): shifts by 1, 2, 4, 8 within
+// each 16 lanes, then their last lanes' sums to the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x += dpp_or_0<0x111, 0xF>(x);  // row_shr:1
+  x += dpp_or_0<0x112, 0xF>(x);
+  x += dpp_or_0<0x114, 0xF>(x);
+  x += dpp_or_0<0x118, 0xF>(x);
+  x += dpp_or_0<0x142, 0xA>(x);  // row_bcast:15 to rows 1 and 3
+  x += dpp_or_0<0x143, 0xC>(x);  // row_bcast:31 to rows 2 and 3
+  return x;
+}
+
 // a value that is the same in all lanes, said so
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return uint32_t(__builtin_amdgcn_readfirstlane(int(x))); }
 
@@ -208,12 +224,7 @@ __device__ __forceinline__ Run run_of(const KvAttendArgs& a, uint32_t row0, uint
     const uint32_t first = max(row0, b * per) - b * per, last = min(row1, (b + 1) * per) - 1 - b * per;
     if (first / a.s.rep < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(last / a.s.rep, r.rq.fresh - 1) + 1;
   }
-  r.seg_end = (r.seg_keys + KT - 1) / KT;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(r.seg_end, d, 64);
-    if (lane >= uint32_t(d)) r.seg_end += y;
-  }
+  r.seg_end = wave_scan((r.seg_keys + KT - 1) / KT);
   r.tiles = lane_read_u32(r.seg_end, 63);
   return r;
 }
@@ -1376,12 +1387,7 @@ __device__ __forceinline__ uint32_t score_bits(float x) {
 template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* sh, uint32_t& total) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  uint32_t x = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(x, d, 64);
-    if (lane >= uint32_t(d)) x += y;
-  }
+  const uint32_t x = wave_scan(v);
   __syncthreads();
   if (lane == 63) sh[wave] = x;
   __syncthreads();
@@ -1491,8 +1497,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
     bits[i] = score_bits(sc[i]);
     if (tid * I + i < n) newest = max(newest, pos[i]);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) newest = max(newest, __shfl_xor(newest, d, 64));
+  newest = int32_t(wave_reduce(uint32_t(newest) ^ 0x80000000u, [](uint32_t p, uint32_t q) { return max(p, q); }) ^ 0x80000000u);
   if (lane == 0) top[wave] = newest;
   for (uint32_t i = tid; i < HIST * 256; i += THREADS) hist[0][i] = 0;
   __syncthreads();
@@ -1531,13 +1536,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
           }
           x += c[j];
         }
-        uint32_t y = x;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const uint32_t z = __shfl_up(y, d, 64);
-          if (lane >= uint32_t(d)) y += z;
-        }
-        uint32_t above = y - x;
+        uint32_t above = wave_scan(x) - x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (above < want && above + c[j] >= want) {
