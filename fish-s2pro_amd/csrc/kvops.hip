@@ -1433,8 +1433,9 @@ __device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, con
 // Eviction: blockIdx.x = (layer, request, kv head) from seq0 on; thread t holds
 // slots I t .. I t + I - 1.
 //   The k-th largest score among the slots that compete (the safe ones all stay,
-// the others compete for the rest) by four digits of 8 bits from the top; of the
-// slots that equal it the lowest stay.  Then the freed slots below m and the
+// the others compete for the rest) by digits of 8 bits from the top, until all
+// scores that share them stay; of the slots that equal it in all four the lowest
+// stay.  Then the freed slots below m and the
 // kept ones from m on are counted off in slot order: the x-th of one takes the
 // x-th of the other.
 //   MOVE: the block then moves the rows, its part blockIdx.y of them, 16 bytes a
@@ -1453,7 +1454,7 @@ struct KvMove {
 template <int THREADS, int I, bool MOVE>
 __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMove mv) {
   constexpr int HIST = 4;  // copies of the digit counts, by lane, for many scores share a digit
-  __shared__ uint32_t sh[THREADS / 64], hist[HIST][256], pick[2];
+  __shared__ uint32_t sh[THREADS / 64], hist[HIST][256], pick[3];
   __shared__ int32_t top[THREADS / 64];
   __shared__ uint32_t list[THREADS * I / 2];  // to | from << 16
   const uint32_t tid = threadIdx.x, sg = mv.seq0 + blockIdx.x, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
@@ -1517,8 +1518,10 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
     if (tid * I + i < n && (((safe >> i) & 1u) == 0) == room) compete |= 1u << i;
   uint32_t prefix = 0, kept = room ? safe : 0u;
   if (want) {
+    int shift = 24;
+    bool all = false;  // every score of the last digit stays: the rest of its bits decides nothing
 #pragma unroll 1
-    for (int shift = 24; shift >= 0; shift -= 8) {  // (the counts are zero here)
+    for (; shift >= 0 && !all; shift -= 8) {  // (the counts are zero here)
 #pragma unroll
       for (int i = 0; i < I; ++i)
         if (((compete >> i) & 1u) && (shift == 24 || (bits[i] >> (shift + 8)) == prefix))
@@ -1542,6 +1545,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
           if (above < want && above + c[j] >= want) {
             pick[0] = 255 - 4 * lane - j;
             pick[1] = want - above;
+            pick[2] = c[j];
           }
           above += c[j];
         }
@@ -1549,19 +1553,25 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
       __syncthreads();
       prefix = (prefix << 8) | pick[0];
       want = pick[1];
+      all = pick[2] == want;
     }
-    uint32_t equal = 0, dummy;
+    shift += 8;
+    uint32_t equal = 0;
 #pragma unroll
     for (int i = 0; i < I; ++i)
       if ((compete >> i) & 1u) {
-        if (bits[i] > prefix) kept |= 1u << i;
-        if (bits[i] == prefix) equal |= 1u << i;
+        if ((bits[i] >> shift) > prefix) kept |= 1u << i;
+        if ((bits[i] >> shift) == prefix) equal |= 1u << i;
       }
-    uint32_t rank = block_scan<THREADS>(__popc(equal), sh, dummy);
+    if (all) {
+      kept |= equal;
+    } else {
+      uint32_t dummy, rank = block_scan<THREADS>(__popc(equal), sh, dummy);
 #pragma unroll
-    for (int i = 0; i < I; ++i)
-      if ((equal >> i) & 1u)
-        if (rank++ < want) kept |= 1u << i;
+      for (int i = 0; i < I; ++i)
+        if ((equal >> i) & 1u)
+          if (rank++ < want) kept |= 1u << i;
+    }
   }
   // slots of the thread below m; the rest of them
   const uint32_t low = tid * I >= m ? 0u : m - tid * I >= 32 ? 0xffffffffu : (1u << (m - tid * I)) - 1u;
