@@ -1659,8 +1659,13 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   // of a tile's waves idle in its own cache.
   const bool many = a.c.n * a.s.rep >= 32 && size_t(a.s.G) * rows * (a.c.P + a.c.cap) > (f16 ? 14000000u : 4000000u);
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
-  const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt;  // key tiles
+  // key tiles of a row tile, at most
+  const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));
   sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
+  // Up to five tiles a wave cost less than a second launch: 4 requests over 200 shared positions, f32 (17 tiles) 11.9 us in
+  // one block a row tile against 8.1 + 3.3 and the time between, over 300 (23 tiles) 13.2 : 8.0 + 3.2; f16 over 400 10.2 :
+  // 7.4 + 3.3, over 600 11.4 : 7.5 + 3.3.
+  if (!many && most <= 20) sp.splits = 1;
   if (many && lots > 256 && lots <= 448) {
     // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
     // A prompt of 1500 tokens (376 row tiles) 81 : 65 us with the join; from 448 on the join costs what it saves.
