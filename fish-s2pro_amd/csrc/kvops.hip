@@ -65,35 +65,42 @@ using Elem = std::conditional_t<KH, _Float16, float>;
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// One block per token: the token's hd / 2 angles once (64-bit product with the
-// position, whole turns taken off in 64 bits, cos and sin of the rest in f32),
-// then 4 elements (two pairs) per thread.
+// One block per token and run of heads (blockIdx.y, every gridDim.y-th 8 or 16):
+// the token's hd / 2 angles once (64-bit product with the position, whole turns
+// taken off in 64 bits, cos and sin of the rest in f32), then 4 elements (two
+// pairs) per thread.  Memory bound: 8 requests x 250 tokens of 32 + 8 + 8 heads
+// read and write 70 MB in 16 us; one step of 8 requests is all latency, so its
+// loads start together and its heads are spread over blocks.
 template <int HD, bool KH>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
   constexpr uint32_t LP = HD / 4;       // lanes per head
   constexpr uint32_t HPB = 256 / LP;    // heads per step of the block
   __shared__ float2 turn[HD / 2];
   const uint32_t tid = threadIdx.x, b = blockIdx.x / a.c.n, t = blockIdx.x % a.c.n;
-  const Request r = request_of(a.c, b, tid == 0 && t == 0 ? a.s.err : nullptr);
+  const RawRequest raw = load_request(a.c, b);
+  const int32_t pos = a.positions[size_t(b) * a.c.n + t];
+  const uint32_t heads = a.s.H + 2 * a.s.G, d = 4 * (tid % LP), h0 = blockIdx.y * HPB + tid / LP;
+  const float* src = a.qkv + (size_t(b) * a.c.n + t) * heads * HD;
+  float4 x = *reinterpret_cast<const float4*>(src + size_t(min(h0, heads - 1)) * HD + d);
+  const double freq = a.s.freq[tid % (HD / 2)];
+  const Request r = checked(a.c, raw, tid == 0 && t == 0 && blockIdx.y == 0 ? a.s.err : nullptr);
   if (t >= r.fresh) return;
   const uint32_t slot = r.len - r.fresh + t;
-  const int32_t pos = a.positions[size_t(b) * a.c.n + t];
   if (pos < 0) {
-    if (tid == 0) atomicOr(a.s.err, S2HIP_KV_ERR_POSITION);
+    if (tid == 0 && blockIdx.y == 0) atomicOr(a.s.err, S2HIP_KV_ERR_POSITION);
     return;
   }
   if (tid < HD / 2) {
-    const double angle = double(pos) * a.s.freq[tid] * 0.15915494309189535;  // in turns
+    const double angle = double(pos) * freq * 0.15915494309189535;  // in turns
     const float rest = float(angle - rint(angle));
     float sn, cs;
     sincospif(2.0f * rest, &sn, &cs);
     turn[tid] = make_float2(cs, sn);
   }
   __syncthreads();
-  const uint32_t heads = a.s.H + 2 * a.s.G, d = 4 * (tid % LP);
-  const float* src = a.qkv + (size_t(b) * a.c.n + t) * heads * HD;
-  for (uint32_t h = tid / LP; h < heads; h += HPB) {  // whole rows of 16 lanes take part
-    float4 x = *reinterpret_cast<const float4*>(src + size_t(h) * HD + d);
+  for (uint32_t h = h0; h < heads;) {  // whole rows of 16 lanes take part
+    const uint32_t next = h + HPB * gridDim.y;
+    const float4 ahead = *reinterpret_cast<const float4*>(src + size_t(min(next, heads - 1)) * HD + d);
     if (h < a.s.H + a.s.G) {
       if (a.q_norm) {
         float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
@@ -108,24 +115,26 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
     }
     if (h < a.s.H) {
       *reinterpret_cast<float4*>(a.q_out + ((size_t(b) * a.c.n + t) * a.s.H + h) * HD + d) = x;
-      continue;
-    }
-    const bool key = h < a.s.H + a.s.G;
-    const uint32_t g = key ? h - a.s.H : h - a.s.H - a.s.G;
-    Elem<KH>* dst = static_cast<Elem<KH>*>(key ? a.c.k : a.c.v) + b * a.c.req_stride + g * a.c.head_stride + slot * a.c.slot_stride + d;
-    if constexpr (KH) {
-      const half4 y = {_Float16(x.x), _Float16(x.y), _Float16(x.z), _Float16(x.w)};
-      const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-      if (big >= 65520.0f) atomicOr(a.s.err, S2HIP_KV_ERR_F16_RANGE);  // rounds to infinity
-      *reinterpret_cast<half4*>(dst) = y;
     } else {
-      *reinterpret_cast<float4*>(dst) = x;
+      const bool key = h < a.s.H + a.s.G;
+      const uint32_t g = key ? h - a.s.H : h - a.s.H - a.s.G;
+      Elem<KH>* dst = static_cast<Elem<KH>*>(key ? a.c.k : a.c.v) + b * a.c.req_stride + g * a.c.head_stride + slot * a.c.slot_stride + d;
+      if constexpr (KH) {
+        const half4 y = {_Float16(x.x), _Float16(x.y), _Float16(x.z), _Float16(x.w)};
+        const float big = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+        if (big >= 65520.0f) atomicOr(a.s.err, S2HIP_KV_ERR_F16_RANGE);  // rounds to infinity
+        *reinterpret_cast<half4*>(dst) = y;
+      } else {
+        *reinterpret_cast<float4*>(dst) = x;
+      }
+      if (!key && tid % LP == 0) {
+        const size_t at = (size_t(b) * a.s.G + g) * a.c.cap + slot;
+        if (a.scores) a.scores[at] = 0.0f;
+        if (a.slot_positions) a.slot_positions[at] = pos;
+      }
     }
-    if (!key && tid % LP == 0) {
-      const size_t at = (size_t(b) * a.s.G + g) * a.c.cap + slot;
-      if (a.scores) a.scores[at] = 0.0f;
-      if (a.slot_positions) a.slot_positions[at] = pos;
-    }
+    x = ahead;
+    h = next;
   }
 }
 
@@ -1640,7 +1649,8 @@ hipError_t by_shape(uint32_t hd, bool f16, F&& f) {
 
 hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStream_t s) {
   return by_shape(hd, f16, [&](auto HD, auto KH) {
-    hipLaunchKernelGGL((kv_append_kernel<HD(), KH()>), dim3(a.c.R * a.c.n), dim3(256), 0, s, a);
+    const uint32_t tokens = a.c.R * a.c.n, steps = (a.s.H + 2 * a.s.G + 1024 / HD() - 1) / (1024 / HD());
+    hipLaunchKernelGGL((kv_append_kernel<HD(), KH()>), dim3(tokens, min(steps, max(1u, 512 / tokens))), dim3(256), 0, s, a);
     return hipGetLastError();
   });
 }

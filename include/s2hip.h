@@ -464,8 +464,8 @@ int32_t s2hip_kv_errors(s2hip_kv* kv, void* stream, uint32_t* bits, char* err, s
  * value go to slot lens[b] - new_lens[b] + t.  scores and slot_positions
  * (nullable, [requests][kv_heads][capacity]): there the slot's score becomes 0
  * and its position the token's.  Positions need not be the slots: after an
- * eviction they run ahead.  Tokens t >= new_lens[b] are not read and their
- * rows of q_out stay as they were. */
+ * eviction they run ahead.  What stands at tokens t >= new_lens[b] does not
+ * matter, and their rows of q_out stay as they were. */
 int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qkv, uint32_t n_tokens,
                         const int32_t* positions, const float* q_norm, const float* k_norm, float* q_out,
                         float* scores, int32_t* slot_positions, void* stream, char* err, size_t err_cap);
