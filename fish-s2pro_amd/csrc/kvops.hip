@@ -1125,7 +1125,6 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   if (!prefix) rq = request_of(a.c, z, nullptr);
   const uint32_t n_keys = rq.len, k0 = kb * KB;
   if (k0 >= n_keys) return;
-  const uint32_t per = a.c.n * a.s.rep;
   const RowSteps rs = row_steps(a, rq, prefix, k0);
   const uint32_t base = rs.base, row_begin = rs.begin, row_end = rs.end;
   const uint32_t s_lo = split * chunk, s_hi = min(s_lo + chunk, rs.steps);
@@ -1184,21 +1183,33 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   uint32_t q_t = 0;
   bool q_row = false;
   const uint32_t srow = tid / 8, sd = tid % 8 * 4;  // dims sd + 32 i ..: 128 bytes of a row per load
-  auto load = [&](uint32_t step) {
-    const uint32_t at_row = row_begin + step * 32 + srow, row = min(at_row, row_end - 1);
-    const uint32_t b = prefix ? row / per : z;
+  // the row of the next load: token (of the request, or b n + t) and head, counted on by 32 rows a step
+  uint32_t at_row = row_begin + s_lo * 32 + srow, token = at_row / a.s.rep, head = at_row % a.s.rep;
+  const uint32_t tokens_on = 32 / a.s.rep, heads_on = 32 % a.s.rep, tokens = row_end / a.s.rep;
+  auto load = [&]() {
     q_row = at_row < row_end;
-    q_t = prefix ? row / a.s.rep % a.c.n : row / a.s.rep;
-    if (prefix) q_rq = load_request(a.c, b);
-    const size_t at = (size_t(b) * a.c.n + q_t) * a.s.H + g * a.s.rep + row % a.s.rep;
+    q_t = min(token, tokens - 1);
+    const size_t at = (prefix ? size_t(q_t) : size_t(z) * a.c.n + q_t) * a.s.H + g * a.s.rep + head;
+    if (prefix) {
+      const uint32_t b = a.c.n == 1 ? q_t : q_t / a.c.n;
+      q_rq = load_request(a.c, b);
+      q_t -= b * a.c.n;
+    }
 #pragma unroll
     for (int i = 0; i < SD / 4; ++i) qr[i] = *reinterpret_cast<const float4*>(a.q + at * HD + sd + 32 * i);
     q_ml = *reinterpret_cast<const float2*>(stat + 2 * at);
+    at_row += 32;
+    token += tokens_on;
+    head += heads_on;
+    if (head >= a.s.rep) {
+      head -= a.s.rep;
+      ++token;
+    }
   };
   auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
   auto store = [&](uint32_t buf) {
     const bool live = q_row && (!prefix || q_t < checked(a.c, q_rq, nullptr).fresh);
-    float4 qi = make_float4(0.0f, live ? q_ml.x : 0.0f, live ? 1.0f / q_ml.y : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + q_t)));
+    float4 qi = make_float4(0.0f, live ? q_ml.x : 0.0f, live ? __builtin_amdgcn_rcpf(q_ml.y) : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + q_t)));
     float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < SD / 4; ++i) {
@@ -1232,15 +1243,15 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
     for (int v = 0; v < 16; ++v) sum[kw][v] = 0.0f;
+  // Rows are loaded two steps ahead, and split for the next step while this one's products run.
   if (s_lo < s_hi) {
-    load(s_lo);
+    load();
     store(0);
+    if (s_lo + 1 < s_hi) load();
   }
   __syncthreads();
   for (uint32_t st = s_lo; st < s_hi; ++st) {
     const uint32_t buf = (st - s_lo) & 1u;
-    const bool more = st + 1 < s_hi;
-    if (more) load(st + 1);
     float4 me = info[buf][r32];
     const int limit = __float_as_int(me.w);
     floatx16 s[KW];
@@ -1256,6 +1267,10 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
         s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
         if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
       }
+    }
+    if (st + 1 < s_hi) {
+      store(buf ^ 1u);
+      if (st + 2 < s_hi) load();
     }
     if (!__all(limit >= int(key0) + 32 * KW - 1)) {
       const bool lost = !(me.y - me.y == 0.0f) || !(me.z - me.z == 0.0f);  // a row of no number: that of the keys it sees alone
@@ -1274,7 +1289,6 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
-    if (more) store(buf ^ 1u);
     __syncthreads();
   }
 #pragma unroll
