@@ -1021,6 +1021,10 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
   const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
   const size_t part = (size_t(g) * sp.tiles + tile) * sp.splits * 16 + row % 16;  // + 16 split
   bool done = false;  // the row has its output
+  if (TEAM == 1) {    // many rows: the state's bytes count, not the wait for its m and l
+    const float2 ml = *reinterpret_cast<const float2*>(sp.ml + 2 * part);
+    if (ml.y == NO_STATE) return;
+  }
   float M = -INFINITY, L = 0.0f;
   floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
   for (uint32_t s0 = team; s0 < sp.splits; s0 += 4 * TEAM) {
@@ -1030,7 +1034,7 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
     for (int i = 0; i < 4; ++i) {
       const uint32_t s = min(s0 + i * TEAM, sp.splits - 1);
       ml[i] = *reinterpret_cast<const float2*>(sp.ml + 2 * (part + 16 * s));
-      y[i] = *reinterpret_cast<const floatx4*>(sp.o + (part + 16 * s) * HD + 4 * d);
+      if (TEAM > 1 || s0 + i < sp.splits) y[i] = *reinterpret_cast<const floatx4*>(sp.o + (part + 16 * s) * HD + 4 * d);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1119,199 +1123,201 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
   __shared__ __align__(16) uint8_t lds[2][2 * PLANE];
   __shared__ float4 info[2][32];           // a row's unscale, m, 1 / l (0: no row), last slot seen
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5;
-  const uint32_t g = blockIdx.x % a.s.G, kb = blockIdx.x / a.s.G, split = blockIdx.y, z = blockIdx.z;
+  const uint32_t g = blockIdx.x % a.s.G, split = blockIdx.y, z = blockIdx.z;
   const bool prefix = z == a.c.R;
   Request rq{a.c.P, 0};
   if (!prefix) rq = request_of(a.c, z, nullptr);
-  const uint32_t n_keys = rq.len, k0 = kb * KB;
-  if (k0 >= n_keys) return;
-  const RowSteps rs = row_steps(a, rq, prefix, k0);
-  const uint32_t base = rs.base, row_begin = rs.begin, row_end = rs.end;
-  const uint32_t s_lo = split * chunk, s_hi = min(s_lo + chunk, rs.steps);
-  if (s_lo >= s_hi && split) return;
+  const uint32_t n_keys = rq.len;
+  for (uint32_t kb = blockIdx.x / a.s.G; kb * KB < n_keys; kb += gridDim.x / a.s.G) {
+    const uint32_t k0 = kb * KB;
+    const RowSteps rs = row_steps(a, rq, prefix, k0);
+    const uint32_t base = rs.base, row_begin = rs.begin, row_end = rs.end;
+    const uint32_t s_lo = split * chunk, s_hi = min(s_lo + chunk, rs.steps);
+    if (s_lo >= s_hi && split) return;  // later keys are seen by fewer rows
 
-  // the wave's keys: key 32 kw + r32, dims 16 ks + 8 h2 + e
-  const uint32_t key0 = k0 + wave * 32 * KW;
-  half8 kh[KW][DS], kl[KH ? 1 : KW][DS];
-  float key_scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // f32: of 8 keys each
+    // the wave's keys: key 32 kw + r32, dims 16 ks + 8 h2 + e
+    const uint32_t key0 = k0 + wave * 32 * KW;
+    half8 kh[KW][DS], kl[KH ? 1 : KW][DS];
+    float key_scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // f32: of 8 keys each
 #pragma unroll
-  for (int kw = 0; kw < KW; ++kw) {
-    const size_t stride = prefix ? a.c.p_slot_stride : a.c.slot_stride;
-    const T* row = (prefix ? static_cast<const T*>(a.c.pk) + g * a.c.p_head_stride
-                           : static_cast<const T*>(a.c.k) + z * a.c.req_stride + g * a.c.head_stride) +
-                   min(key0 + 32 * kw + r32, n_keys - 1) * stride + 8 * h2;
-    if constexpr (KH) {
+    for (int kw = 0; kw < KW; ++kw) {
+      const size_t stride = prefix ? a.c.p_slot_stride : a.c.slot_stride;
+      const T* row = (prefix ? static_cast<const T*>(a.c.pk) + g * a.c.p_head_stride
+                             : static_cast<const T*>(a.c.k) + z * a.c.req_stride + g * a.c.head_stride) +
+                     min(key0 + 32 * kw + r32, n_keys - 1) * stride + 8 * h2;
+      if constexpr (KH) {
 #pragma unroll
-      for (int ks = 0; ks < DS; ++ks) kh[kw][ks] = *reinterpret_cast<const half8*>(row + 16 * ks);
-    } else {
-      float x[DS][8], big = 0.0f;
+        for (int ks = 0; ks < DS; ++ks) kh[kw][ks] = *reinterpret_cast<const half8*>(row + 16 * ks);
+      } else {
+        float x[DS][8], big = 0.0f;
 #pragma unroll
-      for (int ks = 0; ks < DS; ++ks)
+        for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const floatx4 y = *reinterpret_cast<const floatx4*>(row + 16 * ks + e);
+          for (int e = 0; e < 8; e += 4) {
+            const floatx4 y = *reinterpret_cast<const floatx4*>(row + 16 * ks + e);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            x[ks][e + c] = y[c];
-            big = fmaxf(big, fabsf(y[c]) < INFINITY ? fabsf(y[c]) : 0.0f);
+            for (int c = 0; c < 4; ++c) {
+              x[ks][e + c] = y[c];
+              big = fmaxf(big, fabsf(y[c]) < INFINITY ? fabsf(y[c]) : 0.0f);
+            }
           }
-        }
-      big = half_reduce(big, [](float p, float q) { return fmaxf(p, q); });
+        big = half_reduce(big, [](float p, float q) { return fmaxf(p, q); });
+        big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
+        big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
+        big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
+        float r, inv;
+        pow2_scale(big, r, inv);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) key_scale[c] = lane_read_f32(r, 8 * c);
+#pragma unroll
+        for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float y = x[ks][e] * inv;
+            kh[kw][ks][e] = _Float16(y);
+            kl[kw][ks][e] = _Float16(y - float(kh[kw][ks][e]));
+          }
+      }
+    }
+
+    // staging: 8 threads per row, HD / 8 dims each; nothing is looked at before it goes to LDS, a step later
+    constexpr int SD = HD / 8;
+    float4 qr[SD / 4];
+    float2 q_ml;
+    RawRequest q_rq{0, 0};
+    uint32_t q_t = 0;
+    bool q_row = false;
+    const uint32_t srow = tid / 8, sd = tid % 8 * 4;  // dims sd + 32 i ..: 128 bytes of a row per load
+    // the row of the next load: token (of the request, or b n + t) and head, counted on by 32 rows a step
+    uint32_t at_row = row_begin + s_lo * 32 + srow, token = at_row / a.s.rep, head = at_row % a.s.rep;
+    const uint32_t tokens_on = 32 / a.s.rep, heads_on = 32 % a.s.rep, tokens = row_end / a.s.rep;
+    auto load = [&]() {
+      q_row = at_row < row_end;
+      q_t = min(token, tokens - 1);
+      const size_t at = (prefix ? size_t(q_t) : size_t(z) * a.c.n + q_t) * a.s.H + g * a.s.rep + head;
+      if (prefix) {
+        const uint32_t b = a.c.n == 1 ? q_t : q_t / a.c.n;
+        q_rq = load_request(a.c, b);
+        q_t -= b * a.c.n;
+      }
+#pragma unroll
+      for (int i = 0; i < SD / 4; ++i) qr[i] = *reinterpret_cast<const float4*>(a.q + at * HD + sd + 32 * i);
+      q_ml = *reinterpret_cast<const float2*>(stat + 2 * at);
+      at_row += 32;
+      token += tokens_on;
+      head += heads_on;
+      if (head >= a.s.rep) {
+        head -= a.s.rep;
+        ++token;
+      }
+    };
+    auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
+    auto store = [&](uint32_t buf) {
+      const bool live = q_row && (!prefix || q_t < checked(a.c, q_rq, nullptr).fresh);
+      float4 qi = make_float4(0.0f, live ? q_ml.x : 0.0f, live ? __builtin_amdgcn_rcpf(q_ml.y) : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + q_t)));
+      float big = 0.0f;
+#pragma unroll
+      for (int i = 0; i < SD / 4; ++i) {
+        if (!live) qr[i] = make_float4(0.f, 0.f, 0.f, 0.f);  // a row of no token may hold anything
+        qr[i] = make_float4(qr[i].x * a.s.scale2, qr[i].y * a.s.scale2, qr[i].z * a.s.scale2, qr[i].w * a.s.scale2);
+        big = fmaxf(big, fmaxf(fmaxf(fabsf(qr[i].x), fabsf(qr[i].y)), fmaxf(fabsf(qr[i].z), fabsf(qr[i].w))));
+      }
       big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
       big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
       big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
-      float r, inv;
-      pow2_scale(big, r, inv);
+      float inv;
+      pow2_scale(big, qi.x, inv);
+      if (tid % 8 == 0) info[buf][srow] = qi;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) key_scale[c] = lane_read_f32(r, 8 * c);
+      for (int i = 0; i < SD / 4; ++i) {
+        const float x[4] = {qr[i].x, qr[i].y, qr[i].z, qr[i].w};
+        half4 hi, lo;
 #pragma unroll
-      for (int ks = 0; ks < DS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float y = x[ks][e] * inv;
-          kh[kw][ks][e] = _Float16(y);
-          kl[kw][ks][e] = _Float16(y - float(kh[kw][ks][e]));
+        for (int e = 0; e < 4; ++e) {
+          hi[e] = _Float16(x[e] * inv);
+          lo[e] = _Float16(x[e] * inv - float(hi[e]));
         }
-    }
-  }
-
-  // staging: 8 threads per row, HD / 8 dims each; nothing is looked at before it goes to LDS, a step later
-  constexpr int SD = HD / 8;
-  float4 qr[SD / 4];
-  float2 q_ml;
-  RawRequest q_rq{0, 0};
-  uint32_t q_t = 0;
-  bool q_row = false;
-  const uint32_t srow = tid / 8, sd = tid % 8 * 4;  // dims sd + 32 i ..: 128 bytes of a row per load
-  // the row of the next load: token (of the request, or b n + t) and head, counted on by 32 rows a step
-  uint32_t at_row = row_begin + s_lo * 32 + srow, token = at_row / a.s.rep, head = at_row % a.s.rep;
-  const uint32_t tokens_on = 32 / a.s.rep, heads_on = 32 % a.s.rep, tokens = row_end / a.s.rep;
-  auto load = [&]() {
-    q_row = at_row < row_end;
-    q_t = min(token, tokens - 1);
-    const size_t at = (prefix ? size_t(q_t) : size_t(z) * a.c.n + q_t) * a.s.H + g * a.s.rep + head;
-    if (prefix) {
-      const uint32_t b = a.c.n == 1 ? q_t : q_t / a.c.n;
-      q_rq = load_request(a.c, b);
-      q_t -= b * a.c.n;
-    }
-#pragma unroll
-    for (int i = 0; i < SD / 4; ++i) qr[i] = *reinterpret_cast<const float4*>(a.q + at * HD + sd + 32 * i);
-    q_ml = *reinterpret_cast<const float2*>(stat + 2 * at);
-    at_row += 32;
-    token += tokens_on;
-    head += heads_on;
-    if (head >= a.s.rep) {
-      head -= a.s.rep;
-      ++token;
-    }
-  };
-  auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
-  auto store = [&](uint32_t buf) {
-    const bool live = q_row && (!prefix || q_t < checked(a.c, q_rq, nullptr).fresh);
-    float4 qi = make_float4(0.0f, live ? q_ml.x : 0.0f, live ? __builtin_amdgcn_rcpf(q_ml.y) : 0.0f, __int_as_float(!live ? -1 : prefix ? 0x7fffffff : int(base + q_t)));
-    float big = 0.0f;
-#pragma unroll
-    for (int i = 0; i < SD / 4; ++i) {
-      if (!live) qr[i] = make_float4(0.f, 0.f, 0.f, 0.f);  // a row of no token may hold anything
-      qr[i] = make_float4(qr[i].x * a.s.scale2, qr[i].y * a.s.scale2, qr[i].z * a.s.scale2, qr[i].w * a.s.scale2);
-      big = fmaxf(big, fmaxf(fmaxf(fabsf(qr[i].x), fabsf(qr[i].y)), fmaxf(fabsf(qr[i].z), fabsf(qr[i].w))));
-    }
-    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
-    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
-    big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
-    float inv;
-    pow2_scale(big, qi.x, inv);
-    if (tid % 8 == 0) info[buf][srow] = qi;
-#pragma unroll
-    for (int i = 0; i < SD / 4; ++i) {
-      const float x[4] = {qr[i].x, qr[i].y, qr[i].z, qr[i].w};
-      half4 hi, lo;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hi[e] = _Float16(x[e] * inv);
-        lo[e] = _Float16(x[e] * inv - float(hi[e]));
+        const uint32_t d = sd + 32 * i, off = k_at(srow, d / 8) + d % 8 * 2;
+        *reinterpret_cast<half4*>(&lds[buf][off]) = hi;
+        *reinterpret_cast<half4*>(&lds[buf][PLANE + off]) = lo;
       }
-      const uint32_t d = sd + 32 * i, off = k_at(srow, d / 8) + d % 8 * 2;
-      *reinterpret_cast<half4*>(&lds[buf][off]) = hi;
-      *reinterpret_cast<half4*>(&lds[buf][PLANE + off]) = lo;
-    }
-  };
+    };
 
-  float sum[KW][16];
-#pragma unroll
-  for (int kw = 0; kw < KW; ++kw)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) sum[kw][v] = 0.0f;
-  // Rows are loaded two steps ahead, and split for the next step while this one's products run.
-  if (s_lo < s_hi) {
-    load();
-    store(0);
-    if (s_lo + 1 < s_hi) load();
-  }
-  __syncthreads();
-  for (uint32_t st = s_lo; st < s_hi; ++st) {
-    const uint32_t buf = (st - s_lo) & 1u;
-    float4 me = info[buf][r32];
-    const int limit = __float_as_int(me.w);
-    floatx16 s[KW];
-#pragma unroll
-    for (int kw = 0; kw < KW; ++kw) s[kw] = floatx16{};
-#pragma unroll
-    for (int ks = 0; ks < DS; ++ks) {
-      const uint32_t off = k_at(r32, 2 * ks + h2);
-      const half8 qh = *reinterpret_cast<const half8*>(&lds[buf][off]), ql = *reinterpret_cast<const half8*>(&lds[buf][PLANE + off]);
-#pragma unroll
-      for (int kw = 0; kw < KW; ++kw) {
-        s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], qh, s[kw], 0, 0, 0);
-        s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
-        if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
-      }
-    }
-    if (st + 1 < s_hi) {
-      store(buf ^ 1u);
-      if (st + 2 < s_hi) load();
-    }
-    if (!__all(limit >= int(key0) + 32 * KW - 1)) {
-      const bool lost = !(me.y - me.y == 0.0f) || !(me.z - me.z == 0.0f);  // a row of no number: that of the keys it sees alone
-#pragma unroll
-      for (int kw = 0; kw < KW; ++kw)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const bool sees = int(key0) + int(32u * kw + 8u * (v / 4) + 4u * h2 + (v % 4)) <= limit;
-          if (lost && sees) sum[kw][v] = NAN;
-          if (lost || !sees) s[kw][v] = -INFINITY;
-        }
-      if (lost) me.y = me.z = 0.0f;
-    }
+    float sum[KW][16];
 #pragma unroll
     for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int kw = 0; kw < KW; ++kw) {
-    float mine = 0.0f;
-#pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      float x = row_reduce(sum[kw][v], [](float p, float q) { return p + q; });
-      const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-      x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
-      if (r32 == uint32_t(v)) mine = x;
+      for (int v = 0; v < 16; ++v) sum[kw][v] = 0.0f;
+    // Rows are loaded two steps ahead, and split for the next step while this one's products run.
+    if (s_lo < s_hi) {
+      load();
+      store(0);
+      if (s_lo + 1 < s_hi) load();
     }
-    const uint32_t key = key0 + 32 * kw + 8 * (r32 / 4) + 4 * h2 + r32 % 4;
-    if (r32 >= 16 || key >= n_keys) continue;
-    const size_t own = (size_t(z) * a.s.G + g) * a.c.cap + key;
-    if (gridDim.y > 1) {
-      const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
-      part[split * all + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own)] = mine;
-    } else if (prefix) {
-      const size_t at = size_t(g) * a.pw_stride + key;
-      a.pw_out[at] = (a.pw_in ? a.pw_in[at] : 0.0f) + mine;
-    } else {
-      a.w_out[own] = (a.w_in ? a.w_in[own] : 0.0f) + mine;
+    __syncthreads();
+    for (uint32_t st = s_lo; st < s_hi; ++st) {
+      const uint32_t buf = (st - s_lo) & 1u;
+      float4 me = info[buf][r32];
+      const int limit = __float_as_int(me.w);
+      floatx16 s[KW];
+#pragma unroll
+      for (int kw = 0; kw < KW; ++kw) s[kw] = floatx16{};
+#pragma unroll
+      for (int ks = 0; ks < DS; ++ks) {
+        const uint32_t off = k_at(r32, 2 * ks + h2);
+        const half8 qh = *reinterpret_cast<const half8*>(&lds[buf][off]), ql = *reinterpret_cast<const half8*>(&lds[buf][PLANE + off]);
+#pragma unroll
+        for (int kw = 0; kw < KW; ++kw) {
+          s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], qh, s[kw], 0, 0, 0);
+          s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
+          if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
+        }
+      }
+      if (st + 1 < s_hi) {
+        store(buf ^ 1u);
+        if (st + 2 < s_hi) load();
+      }
+      if (!__all(limit >= int(key0) + 32 * KW - 1)) {
+        const bool lost = !(me.y - me.y == 0.0f) || !(me.z - me.z == 0.0f);  // a row of no number: that of the keys it sees alone
+#pragma unroll
+        for (int kw = 0; kw < KW; ++kw)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const bool sees = int(key0) + int(32u * kw + 8u * (v / 4) + 4u * h2 + (v % 4)) <= limit;
+            if (lost && sees) sum[kw][v] = NAN;
+            if (lost || !sees) s[kw][v] = -INFINITY;
+          }
+        if (lost) me.y = me.z = 0.0f;
+      }
+#pragma unroll
+      for (int kw = 0; kw < KW; ++kw)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int kw = 0; kw < KW; ++kw) {
+      float mine = 0.0f;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        float x = row_reduce(sum[kw][v], [](float p, float q) { return p + q; });
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        if (r32 == uint32_t(v)) mine = x;
+      }
+      const uint32_t key = key0 + 32 * kw + 8 * (r32 / 4) + 4 * h2 + r32 % 4;
+      if (r32 >= 16 || key >= n_keys) continue;
+      const size_t own = (size_t(z) * a.s.G + g) * a.c.cap + key;
+      if (gridDim.y > 1) {
+        const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
+        part[split * all + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own)] = mine;
+      } else if (prefix) {
+        const size_t at = size_t(g) * a.pw_stride + key;
+        a.pw_out[at] = (a.pw_in ? a.pw_in[at] : 0.0f) + mine;
+      } else {
+        a.w_out[own] = (a.w_in ? a.w_in[own] : 0.0f) + mine;
+      }
     }
   }
 }
@@ -1327,12 +1333,12 @@ template <int HD>
 __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, uint32_t joins, uint32_t key_blocks) {
   if (blockIdx.x < joins) return join_rows<HD, 1024 / HD>(a, sp, nullptr);
   __shared__ float2 ml[KEPT_ROWS];
-  const uint32_t tid = threadIdx.x, i = blockIdx.x - joins, kb = i % key_blocks, g = i / key_blocks % a.s.G, z = i / key_blocks / a.s.G;
+  const uint32_t tid = threadIdx.x, i = blockIdx.x - joins, kb0 = i % key_blocks, g = i / key_blocks % a.s.G, z = i / key_blocks / a.s.G;
   const bool prefix = z == a.c.R;
   const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per;
   Request rq{a.c.P, a.c.n};
   if (!prefix) rq = request_of(a.c, z, nullptr);
-  if (kb * KEPT_KEYS >= rq.len) return;
+  if (kb0 * KEPT_KEYS >= rq.len) return;
   for (uint32_t r0 = 0; r0 < n_rows; r0 += 16) {
     const uint32_t r = r0 + tid / 16, row = min(prefix ? r : z * per + r, a.c.R * per - 1);
     float M = -INFINITY, L = 0.0f;
@@ -1361,39 +1367,50 @@ __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, Kv
   const uint32_t base = prefix ? 0xffffffffu : rq.len - rq.fresh;
   const float* in = prefix ? a.pw_in : a.w_in;
   float* out = prefix ? a.pw_out : a.w_out;
+  for (uint32_t kb = kb0; kb * KEPT_KEYS < rq.len; kb += key_blocks) {
 #pragma unroll
-  for (uint32_t c = 0; c < KEPT_KEYS / 256; ++c) {
-    const uint32_t key = kb * KEPT_KEYS + 256 * c + tid;
-    if (key >= rq.len) break;
-    const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
-    const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
-    const float before = in ? in[at] : 0.0f;
-    float w = 0.0f;
+    for (uint32_t c = 0; c < KEPT_KEYS / 256; ++c) {
+      const uint32_t key = kb * KEPT_KEYS + 256 * c + tid;
+      if (key >= rq.len) break;
+      const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
+      const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
+      const float before = in ? in[at] : 0.0f;
+      float w = 0.0f;
 #pragma unroll 4
-    for (uint32_t r = key <= base ? 0u : (key - base) * a.s.rep; r < n_rows; ++r) {  // earlier rows do not see the key
-      const float2 x = ml[r];
-      const float p = __builtin_amdgcn_exp2f(src[r] - x.x) * x.y;
-      w += x.y != 0.0f ? p : 0.0f;  // (a row of no token left no score)
+      for (uint32_t r = key <= base ? 0u : (key - base) * a.s.rep; r < n_rows; ++r) {  // earlier rows do not see the key
+        const float2 x = ml[r];
+        const float p = __builtin_amdgcn_exp2f(src[r] - x.x) * x.y;
+        w += x.y != 0.0f ? p : 0.0f;  // (a row of no token left no score)
+      }
+      out[at] = before + w;
     }
-    out[at] = before + w;
   }
 }
 
 // The chunks' sums, in order, and the weights so far.  KB: keys per block of kv_weigh_kernel.
 __global__ __launch_bounds__(256) void kv_weights_join_kernel(KvAttendArgs a, const float* part, uint32_t chunk, uint32_t kb) {
-  const uint32_t g = blockIdx.y, z = blockIdx.z, key = blockIdx.x * 256 + threadIdx.x;
+  const uint32_t g = blockIdx.y, z = blockIdx.z;
   const bool prefix = z == a.c.R;
   Request rq{a.c.P, 0};
   if (!prefix) rq = request_of(a.c, z, nullptr);
-  if (key >= rq.len) return;
-  const uint32_t chunks = max(1u, (row_steps(a, rq, prefix, key / kb * kb).steps + chunk - 1) / chunk);
-  const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P), own = (size_t(z) * a.s.G + g) * a.c.cap + key;
-  const float* src = part + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own);
-  float x = 0.0f;
-  for (uint32_t i = 0; i < chunks; ++i) x += src[i * all];
-  const size_t at = prefix ? size_t(g) * a.pw_stride + key : own;
+  const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
   const float* in = prefix ? a.pw_in : a.w_in;
-  (prefix ? a.pw_out : a.w_out)[at] = (in ? in[at] : 0.0f) + x;
+  float* out = prefix ? a.pw_out : a.w_out;
+  for (uint32_t key = blockIdx.x * 256 + threadIdx.x; key < rq.len; key += gridDim.x * 256) {
+    const uint32_t chunks = max(1u, (row_steps(a, rq, prefix, key / kb * kb).steps + chunk - 1) / chunk);
+    const size_t own = (size_t(z) * a.s.G + g) * a.c.cap + key, at = prefix ? size_t(g) * a.pw_stride + key : own;
+    const float* src = part + (prefix ? size_t(a.c.R) * a.s.G * a.c.cap + size_t(g) * a.c.P + key : own);
+    const float before = in ? in[at] : 0.0f;
+    float x = 0.0f;
+    for (uint32_t i = 0; i < chunks; i += 8) {  // eight loads in flight
+      float y[8];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) y[j] = src[min(i + j, chunks - 1) * all];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) x += i + j < chunks ? y[j] : 0.0f;
+    }
+    out[at] = before + x;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1713,7 +1730,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     const uint32_t z = a.c.R + (a.pw_out ? 1 : 0), keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
     if (keep.own) {
-      const uint32_t joins = sp.splits > 1 ? out_rows : 0, key_blocks = (keys + KEPT_KEYS - 1) / KEPT_KEYS;
+      const uint32_t joins = sp.splits > 1 ? out_rows : 0, key_blocks = min(64u, (keys + KEPT_KEYS - 1) / KEPT_KEYS);
       hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(joins + key_blocks * a.s.G * z), dim3(256), 0, s, a, sp, stat, keep, joins, key_blocks);
       return hipGetLastError();
     }
@@ -1723,16 +1740,18 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t kb = KH() ? 256 : 128;
-      // steps of 32 rows: half of them, on average, see a key of the turn that they are of
+      // Steps of 32 rows: half of them, on average, see a key of their own turn.  Lengths are on the device: chunks are made
+      // for a cache of no more than the turn (longer ones have more key blocks, so the chunks are many enough), and blocks
+      // walk over the keys, so that slots not in use cost no blocks.
       const uint32_t own_steps = (a.c.n * a.s.rep + 31) / 32, all_steps = a.pw_out ? (rows + 31) / 32 : own_steps;
-      const size_t work = size_t(a.s.G) * (size_t((a.c.cap + kb - 1) / kb) * a.c.R * own_steps / 2 + (a.pw_out ? size_t((a.c.P + kb - 1) / kb) * all_steps : 0));
+      const size_t work = size_t(a.s.G) * (size_t((min(a.c.n, a.c.cap) + kb - 1) / kb) * a.c.R * own_steps / 2 + (a.pw_out ? size_t((a.c.P + kb - 1) / kb) * all_steps : 0));
       const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
       const uint32_t room = uint32_t(max(size_t(1), min(size_t(all_steps), w.cap_weights / all)));  // chunks that fit the workspace
-      const uint32_t chunk = max(uint32_t(min(size_t(all_steps), max(size_t(4), work / 512))), (all_steps + room - 1) / room);
+      const uint32_t chunk = max(uint32_t(min(size_t(all_steps), max(size_t(8), work / 320))), (all_steps + room - 1) / room);
       const uint32_t chunks = (all_steps + chunk - 1) / chunk;
-      hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3((keys + kb - 1) / kb * a.s.G, chunks, z), dim3(256), 0, s, a, w.stat, w.weights, chunk);
+      hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3(min(16u, (keys + kb - 1) / kb) * a.s.G, chunks, z), dim3(256), 0, s, a, w.stat, w.weights, chunk);
       if (chunks > 1)
-        hipLaunchKernelGGL(kv_weights_join_kernel, dim3((keys + 255) / 256, a.s.G, z), dim3(256), 0, s, a, w.weights, chunk, kb);
+        hipLaunchKernelGGL(kv_weights_join_kernel, dim3(min(16u, (keys + 255) / 256), a.s.G, z), dim3(256), 0, s, a, w.weights, chunk, kb);
     }
     return hipGetLastError();
   });
