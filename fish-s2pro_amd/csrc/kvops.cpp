@@ -113,10 +113,8 @@ class KvOps {
     work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
     work_.cap_weights = size_t(1) << 24;
     work_.weights = alloc<float>(work_.cap_weights);
-    work_.cap_moves = size_t(1) << 23;
-    work_.cap_seqs = size_t(1) << 16;
-    work_.moves = alloc<uint32_t>(work_.cap_moves);
-    work_.counts = alloc<uint32_t>(2 * work_.cap_seqs);
+    work_.moves = alloc<uint32_t>(size_t(KV_LISTS) * KV_LIST);
+    work_.counts = alloc<uint32_t>(2 * KV_LISTS);
     CHK(hipDeviceSynchronize());
   }
   uint32_t errors(hipStream_t s) {

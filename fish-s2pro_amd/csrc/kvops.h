@@ -54,6 +54,10 @@ struct KvScores {
   float* prefix;  // [G][P][R n rep]
 };
 
+// Caches from which an eviction runs in one launch in place too, and a cache's
+// longest list of moves (half of 32768 slots).
+constexpr uint32_t KV_LISTS = 512, KV_LIST = 16384;
+
 struct KvWorkspace {
   float* stat;  // [tokens][H][2]: a row's m and l (attention with weights)
   float* part;     // [cap_parts][16][hd]
@@ -61,9 +65,8 @@ struct KvWorkspace {
   size_t cap_parts;
   float* weights;  // [cap_weights]: a step's scores, or the row splits' sums of weights
   size_t cap_weights;
-  uint32_t* moves;     // [cap_moves] to | from << 16
-  uint32_t* counts;    // [cap_seqs][2]: moves, slots left
-  size_t cap_moves, cap_seqs;
+  uint32_t* moves;   // [KV_LISTS][KV_LIST]: an eviction's moves (to | from << 16)
+  uint32_t* counts;  // [KV_LISTS][2]: moves, slots left
 };
 
 struct KvAttendArgs {

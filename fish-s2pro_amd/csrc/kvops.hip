@@ -1470,7 +1470,7 @@ __device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, con
   }
 }
 
-// Eviction: blockIdx.x = (layer, request, kv head) from seq0 on; thread t holds
+// Eviction: blockIdx.x = (layer, request, kv head); thread t holds
 // slots I t .. I t + I - 1.
 //   The k-th largest score among the slots that compete (the safe ones all stay,
 // the others compete for the rest) by digits of 8 bits from the top, until all
@@ -1486,7 +1486,7 @@ __device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, con
 // without a second launch.  Otherwise the list goes to the workspace for
 // kv_move_kernel.
 struct KvMove {
-  uint32_t seq0, max_moves, pieces;  // pieces: 16-byte pieces of a row
+  uint32_t max_moves, pieces;  // pieces: 16-byte pieces of a row
   uint32_t* moves;
   uint32_t* counts;
   bool lens;  // MOVE: write lens_out
@@ -1497,7 +1497,7 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
   __shared__ uint32_t sh[THREADS / 64], hist[HIST][256], pick[3];
   __shared__ int32_t top[THREADS / 64];
   __shared__ uint32_t list[THREADS * I / 2];  // to | from << 16
-  const uint32_t tid = threadIdx.x, sg = mv.seq0 + blockIdx.x, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
+  const uint32_t tid = threadIdx.x, sg = blockIdx.x, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
   const uint32_t lane = tid & 63u, wave = tid >> 6;
   const int32_t in_use = a.c.lens[b];
   const size_t base = size_t(sg) * a.c.cap;
@@ -1648,9 +1648,9 @@ __global__ __launch_bounds__(THREADS) void kv_select_kernel(KvEvictArgs a, KvMov
   }
 }
 
-// blockIdx.y = (layer, request, kv head) of the launch.
+// blockIdx.y = (layer, request, kv head).
 __global__ __launch_bounds__(256) void kv_move_kernel(KvEvictArgs a, KvMove mv) {
-  const uint32_t sg = mv.seq0 + blockIdx.y, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
+  const uint32_t sg = blockIdx.y, g = sg % a.s.G, lb = sg / a.s.G, b = lb % a.c.R;
   const uint32_t n_moves = mv.counts[2 * blockIdx.y], left = mv.counts[2 * blockIdx.y + 1];
   if (blockIdx.x == 0 && threadIdx.x == 0 && lb == b && g == 0 && left != 0xffffffffu) a.lens_out[b] = int32_t(left);
   move_rows(a, sg, mv.moves + size_t(blockIdx.y) * mv.max_moves, n_moves * blockIdx.x / gridDim.x, n_moves * (blockIdx.x + 1) / gridDim.x,
@@ -1783,23 +1783,16 @@ hipError_t launch_kv_evict(const KvEvictArgs& a, const KvWorkspace& w, uint32_t 
   mv.pieces = hd * a.elem / 16;
   mv.moves = w.moves;
   mv.counts = w.counts;
-  if (seqs >= 512 || (!in_place && !lens_in_place)) {
+  if (seqs >= KV_LISTS || (!in_place && !lens_in_place)) {
     mv.lens = !lens_in_place;
-    const uint32_t parts = in_place ? 1u : min((512 + seqs - 1) / seqs, max(1u, mv.max_moves / 16));
+    const uint32_t parts = in_place ? 1u : min((KV_LISTS + seqs - 1) / seqs, max(1u, mv.max_moves / 16));
     select_launch<true>(a, mv, dim3(seqs, parts), s);
     if (lens_in_place) hipLaunchKernelGGL(kv_lens_kernel, dim3(1), dim3(256), 0, s, a);
     return hipGetLastError();
   }
-  // as many caches per launch as the lists have room for
-  const uint32_t per = uint32_t(min(mv.max_moves ? w.cap_moves / mv.max_moves : w.cap_seqs, w.cap_seqs));
-  for (mv.seq0 = 0; mv.seq0 < seqs; mv.seq0 += per) {
-    const uint32_t ns = min(per, seqs - mv.seq0);
-    select_launch<false>(a, mv, dim3(ns), s);
-    hipLaunchKernelGGL(kv_move_kernel, dim3(max(1u, min(64u, mv.max_moves * mv.pieces / 256)), ns), dim3(256), 0, s, a, mv);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-  }
-  return hipSuccess;
+  select_launch<false>(a, mv, dim3(seqs), s);  // (fewer than KV_LISTS caches)
+  hipLaunchKernelGGL(kv_move_kernel, dim3(max(1u, min(64u, mv.max_moves * mv.pieces / 256)), seqs), dim3(256), 0, s, a, mv);
+  return hipGetLastError();
 }
 
 hipError_t launch_kv_take_errors(uint32_t* err, uint32_t* taken, hipStream_t s) {
