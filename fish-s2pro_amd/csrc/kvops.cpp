@@ -67,10 +67,31 @@ void may(const void* p, const char* name, size_t align) {
   if (p) need(p, name, align);
 }
 
+// n words from p and m words from q have one in common.
+bool meet(const void* p, size_t n, const void* q, size_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+  return x < y + 4 * m && y < x + 4 * n;
+}
 // out is in itself, or shares no word of `words` with it.
 void same_or_apart(const void* in, const void* out, size_t words, const char* name) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(in), y = reinterpret_cast<uintptr_t>(out);
-  if (x != y && x < y + 4 * words && y < x + 4 * words) kfail("kv: %s_out overlaps %s without being it", name, name);
+  if (in != out && meet(in, words, out, words)) kfail("kv: %s_out overlaps %s without being it", name, name);
+}
+
+// A dimension of the caches' layout.
+struct Dim {
+  uint64_t size, stride;
+};
+// Rows of `row` elements share none: sorted by stride, each dimension steps over all of those before it.
+template <size_t N>
+void check_apart(Dim (&dims)[N], uint64_t row) {
+  std::sort(dims, dims + N, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+  uint64_t extent = row;
+  for (const Dim& d : dims) {
+    if (d.size == 1) continue;
+    if (d.stride < extent) kfail("kv: the strides make caches overlap (one of %llu is less than the %llu elements below it)",
+                                 (unsigned long long)d.stride, (unsigned long long)extent);
+    extent += (d.size - 1) * d.stride;
+  }
 }
 
 class KvOps {
@@ -132,10 +153,13 @@ class KvOps {
   void append(const s2hip_kv_view& v, const float* qkv, uint32_t n, const int32_t* positions, const float* qn,
               const float* kn, float* q_out, float* scores, int32_t* slot_positions, hipStream_t s) {
     KvAppendArgs a{};
-    a.c = caches(v, n, false);
+    a.c = caches(v, n, true, false);
     need(qkv, "qkv", 16);
     need(positions, "positions", 4);
     need(q_out, "q_out", 16);
+    const size_t tokens = size_t(v.requests) * n;
+    if (meet(qkv, tokens * (cfg_.heads + 2 * cfg_.kv_heads) * cfg_.head_dim, q_out, tokens * cfg_.heads * cfg_.head_dim))
+      kfail("kv: q_out overlaps qkv");
     if (!qn != !kn) kfail("kv: q_norm and k_norm go together");
     may(qn, "q_norm", 16);
     may(kn, "k_norm", 16);
@@ -156,12 +180,11 @@ class KvOps {
   void attend(const s2hip_kv_view& v, const float* q, uint32_t n, float* out, bool weigh, const float* w_in, float* w_out,
               const float* pw_in, float* pw_out, hipStream_t s) {
     KvAttendArgs a{};
-    a.c = caches(v, n, true);
+    a.c = caches(v, n, true, true);
     need(q, "q", 16);
     need(out, "out", 16);
-    const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
-    const size_t bytes = size_t(v.requests) * n * cfg_.heads * cfg_.head_dim * sizeof(float);
-    if (q0 < o0 + bytes && o0 < q0 + bytes) kfail("kv: out overlaps q");
+    const size_t words = size_t(v.requests) * n * cfg_.heads * cfg_.head_dim;
+    if (meet(q, words, out, words)) kfail("kv: out overlaps q");
     if (weigh) {
       need(w_out, "weights_out", 4);
       may(w_in, "weights_in", 4);
@@ -188,7 +211,7 @@ class KvOps {
              const float* scores, const int32_t* positions, float* scores_out, int32_t* positions_out, int32_t* lens_out,
              hipStream_t s) {
     KvEvictArgs a{};
-    a.c = caches(v, 1, false);
+    a.c = caches(v, 0, false, false);
     if (layers == 0 || layers > KV_MAX_LAYERS) kfail("kv: layers %u is not in 1..%u", layers, KV_MAX_LAYERS);
     if (keep == 0) kfail("kv: keep is 0");
     if (recent > keep) kfail("kv: recent %u is more than keep %u", recent, keep);
@@ -203,7 +226,9 @@ class KvOps {
     same_or_apart(positions, positions_out, words, "positions");
     same_or_apart(v.lens, lens_out, v.requests, "lens");
     a.s = shape_;
-    a.layer_stride = layer_stride ? layer_stride : a.c.req_stride * v.requests;
+    a.layer_stride = layer_stride ? layer_stride : std::max({a.c.req_stride * v.requests, a.c.head_stride * cfg_.kv_heads, a.c.slot_stride * v.capacity});
+    Dim dims[] = {{layers, a.layer_stride}, {v.requests, a.c.req_stride}, {cfg_.kv_heads, a.c.head_stride}, {v.capacity, a.c.slot_stride}};
+    check_apart(dims, cfg_.head_dim);
     a.layers = layers;
     a.keep = keep;
     a.recent = recent;
@@ -237,11 +262,11 @@ class KvOps {
     if (n >> 40) kfail("kv: %s %llu is too large", name, (unsigned long long)n);
   }
 
-  // The view's checks; strides of 0 become the dense ones.
-  KvCaches caches(const s2hip_kv_view& v, uint32_t n, bool prefix) const {
+  // The view's checks; strides of 0 become those that step over all below.  tokens: a call with n per request.
+  KvCaches caches(const s2hip_kv_view& v, uint32_t n, bool tokens, bool prefix) const {
     if (v.requests == 0 || v.requests > cfg_.max_requests)
       kfail("kv: requests %u is not in 1..max_requests %u", v.requests, cfg_.max_requests);
-    if (n == 0 || uint64_t(v.requests) * n > cfg_.max_tokens)
+    if (tokens && (n == 0 || uint64_t(v.requests) * n > cfg_.max_tokens))
       kfail("kv: %u requests of n_tokens %u are not in 1..max_tokens %u", v.requests, n, cfg_.max_tokens);
     if (v.capacity == 0 || v.capacity > KV_MAX_SLOTS) kfail("kv: capacity %u is not in 1..%u", v.capacity, KV_MAX_SLOTS);
     need(v.k, "k", 16);
@@ -258,11 +283,13 @@ class KvOps {
     c.new_lens = v.new_lens;
     c.slot_stride = v.slot_stride ? v.slot_stride : cfg_.head_dim;
     c.head_stride = v.head_stride ? v.head_stride : c.slot_stride * v.capacity;
-    c.req_stride = v.request_stride ? v.request_stride : c.head_stride * cfg_.kv_heads;
+    c.req_stride = v.request_stride ? v.request_stride : std::max(c.head_stride * cfg_.kv_heads, c.slot_stride * v.capacity);
     if (c.slot_stride >> 24) kfail("kv: slot_stride %llu is not below 2^24", (unsigned long long)c.slot_stride);
     if (c.slot_stride < cfg_.head_dim) kfail("kv: slot_stride %llu is below head_dim %u", (unsigned long long)c.slot_stride, cfg_.head_dim);
     if (c.head_stride < cfg_.head_dim) kfail("kv: head_stride %llu is below head_dim %u", (unsigned long long)c.head_stride, cfg_.head_dim);
     if (c.req_stride < cfg_.head_dim) kfail("kv: request_stride %llu is below head_dim %u", (unsigned long long)c.req_stride, cfg_.head_dim);
+    Dim dims[] = {{v.requests, c.req_stride}, {cfg_.kv_heads, c.head_stride}, {v.capacity, c.slot_stride}};
+    check_apart(dims, cfg_.head_dim);
     c.R = v.requests;
     c.cap = v.capacity;
     c.n = n;

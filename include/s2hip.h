@@ -426,13 +426,15 @@ typedef struct {
 
 /* Where the caches are.  Own caches: request b's key of kv head g in slot s is
  * the head_dim elements at k + b * request_stride + g * head_stride + s *
- * slot_stride (elements; a multiple of 16 bytes each; 0: [requests]
- * [kv_heads][capacity][head_dim], dense), its value the same from v.  Shared
+ * slot_stride (elements; a multiple of 16 bytes each; slot strides below 2^24),
+ * its value the same from v.  Strides of 0: [requests][kv_heads][capacity]
+ * [head_dim], dense; a request_stride of 0 steps over the heads and slots as
+ * the other two lay them out.  Any order of the dimensions that makes no two
+ * rows overlap (sorted by stride, each steps over all before it).  Shared
  * prefix (prefix_len 0: none): key i of kv head g at prefix_k + g *
  * prefix_head_stride + i * prefix_slot_stride (0: [kv_heads][prefix_capacity]
  * [head_dim], prefix_capacity 0 meaning prefix_len).  A cache that one call
- * filled as a single request can be the prefix of others.  The own caches of
- * different requests must not overlap. */
+ * filled as a single request can be the prefix of others. */
 typedef struct {
   void* k;
   void* v;
@@ -465,7 +467,8 @@ int32_t s2hip_kv_errors(s2hip_kv* kv, void* stream, uint32_t* bits, char* err, s
  * (nullable, [requests][kv_heads][capacity]): there the slot's score becomes 0
  * and its position the token's.  Positions need not be the slots: after an
  * eviction they run ahead.  What stands at tokens t >= new_lens[b] does not
- * matter, and their rows of q_out stay as they were. */
+ * matter, and their rows of q_out stay as they were.  q_out must not overlap
+ * qkv. */
 int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qkv, uint32_t n_tokens,
                         const int32_t* positions, const float* q_norm, const float* k_norm, float* q_out,
                         float* scores, int32_t* slot_positions, void* stream, char* err, size_t err_cap);
@@ -474,8 +477,13 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * 0 .. lens[b] - new_lens[b] + t; query head h reads kv head h / (heads /
  * kv_heads).  out like q; rows of tokens t >= new_lens[b] stay as they were.
  * What a token does not see (later slots, other requests, slots not in use)
- * never reaches its row, whatever bits stand there.  The shared prefix is read
- * once for several requests' queries.  out must not overlap q. */
+ * never reaches its row, whatever bits stand there; an infinity or NaN that it
+ * sees makes the elements of its row that it takes part in no number.  The
+ * shared prefix is read once for several requests' queries.  out must not
+ * overlap q.
+ *   Products and sums are f32 or better, except for calls of many tokens over
+ * f32 caches: there each term is exact to 2^-22, or to 2^-39 of the largest
+ * value among the keys that its block of rows reads. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                         void* stream, char* err, size_t err_cap);
 /* s2hip_kv_attend, and for every slot s < lens[b] of every kv head g
@@ -484,8 +492,8 @@ int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q,
  * ([requests][kv_heads][capacity] f32; weights_in NULL: 0, or the same array;
  * other slots stay as they were), and with prefix_weights_out
  * ([kv_heads][prefix_capacity], nullable) the same for the prefix, summed over
- * the requests too.  Sums run in a fixed order: the same call gives the same
- * bits. */
+ * the requests too.  An array in is the array out or shares nothing with it.
+ * Sums run in a fixed order: the same call gives the same bits. */
 int32_t s2hip_kv_attend_weigh(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                               const float* weights_in, float* weights_out, const float* prefix_weights_in,
                               float* prefix_weights_out, void* stream, char* err, size_t err_cap);
@@ -495,11 +503,12 @@ int32_t s2hip_kv_attend_weigh(s2hip_kv* kv, const s2hip_kv_view* view, const flo
  * with the largest scores (a NaN counts as -infinity), the lower slot first
  * between equals; where those that stay are more than keep, the heaviest of
  * them.  Kept rows of slots >= keep move, in order, into the freed slots below
- * keep, in order; other rows do not move.  1 <= keep, recent <= keep.  scores_out / positions_out receive the scores and positions
- * of the slots then in use, lens_out their number (they may be the input
- * arrays; other entries stay as they were).  Rows behind lens_out stay as they
- * were.  `layers` caches of the same lens are cut in one call, layer l's at k /
- * v + l * layer_stride elements (0: requests * request_stride); scores and
+ * keep, in order; other rows do not move.  1 <= keep, recent <= keep.
+ *   scores_out / positions_out receive the scores and positions of the slots
+ * then in use, lens_out their number; each is its input array or shares nothing
+ * with it, and other entries stay as they were.  Rows behind lens_out stay as
+ * they were.  `layers` caches of the same lens are cut in one call, layer l's at k /
+ * v + l * layer_stride elements (0: stepping over one layer's); scores and
  * positions [layers][requests][kv_heads][capacity].  The view's prefix and
  * new_lens are not looked at. */
 int32_t s2hip_kv_evict(s2hip_kv* kv, const s2hip_kv_view* view, uint32_t layers, uint64_t layer_stride, uint32_t keep,

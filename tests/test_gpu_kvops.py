@@ -822,3 +822,57 @@ def test_refusals():
     refused("lens_out is NULL", o.evict, v(), 5, 3, 2, *([p["q"]] * 4), 0)
     torch.cuda.synchronize()
     b.check(b.attend())  # nothing was launched, the handle works
+
+
+def test_refusals_of_layouts():
+    """Strides that make rows overlap, or that are too large; arrays that overlap."""
+    b = Batch((8, 2, 64), True, [4, 4], [2, 2], cap=8, prefix=5, seed=1)
+    o, v = b.ops, b.view
+    p = {n: ptr(getattr(b, n)) for n in ("k", "v", "q", "out", "lens")}
+    call = (p["q"], 1, p["out"])
+    refused("slot_stride 16777216 is not below", o.attend, v(slot_stride=1 << 24), *call)
+    refused("prefix_slot_stride 16777216 is not below", o.attend, v(prefix_slot_stride=1 << 24), *call)
+    refused("request_stride 1099511627776 is too large", o.attend, v(request_stride=1 << 40), *call)
+    refused("overlap", o.attend, v(request_stride=1016), *call)
+    refused("overlap", o.attend, v(head_stride=504), *call)
+    refused("overlap", o.attend, v(slot_stride=128, head_stride=120), *call)
+    refused("overlap", o.append, v(slot_stride=128, head_stride=64, request_stride=128), p["k"], 1, p["lens"], p["q"])
+    five = (p["q"], p["k"], p["q"], p["k"], p["out"])
+    refused("overlap", o.evict, v(), 5, 3, 2, *five, layers=2, layer_stride=2040)
+    refused("overlap", o.evict, v(slot_stride=256, head_stride=64, request_stride=128), 5, 3, 2, *five, layers=2, layer_stride=256)
+    refused("q_out overlaps qkv", o.append, v(), p["q"], 1, p["lens"], p["q"])
+    refused("q_out overlaps qkv", o.append, v(), p["q"], 1, p["lens"], p["q"] + 4 * 2 * 12 * 64 - 16)
+    torch.cuda.synchronize()
+    b.check(b.attend())
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_strides_left_out(f16):
+    """Slots before heads: the strides left out step over what the given ones lay out."""
+    b = Batch((8, 2, 64), f16, [30, 41, 9], [2, 3, 1], cap=48, seed=12)
+    dense = b.attend().clone()
+    k, v = b.k.transpose(1, 2).contiguous(), b.v.transpose(1, 2).contiguous()
+    out = torch.full_like(b.q, 7.0)
+    view = b.ops.view(ptr(k), ptr(v), ptr(b.lens), 3, 48, new_lens=ptr(b.new), head_stride=64, slot_stride=128)
+    b.ops.attend(view, ptr(b.q), b.n, ptr(out), stream=stream())
+    torch.cuda.synchronize()
+    assert torch.equal(out, dense)
+
+
+def test_evict_layer_stride_left_out():
+    """Layers of [slot][request][kv head] rows, and more requests than tokens of a call."""
+    g = gen(13)
+    L, R, G, cap = 3, 2, 2, 100
+    scores = normal(g, L * R, G, cap).abs()
+    positions = torch.arange(cap, dtype=torch.int32, device="cuda").expand(L * R, G, cap).contiguous()
+    k, v = normal(g, L * R, G, cap, 64), normal(g, L * R, G, cap, 64)
+    ops = KvOps(2, 2, 64, max_requests=2, max_tokens=1)
+    k2, v2 = (x.reshape(L, R, G, cap, 64).permute(0, 3, 1, 2, 4).contiguous() for x in (k, v))
+    s2, p2, lens, lo = scores.clone(), positions.clone(), dev([100, 61], torch.int32), dev([0, 0], torch.int32)
+    run_evict(ops, k, v, [100, 61], 40, 8, 2, scores, positions, layers=L)
+    view = ops.view(ptr(k2), ptr(v2), ptr(lens), R, cap, request_stride=128, head_stride=64, slot_stride=256)
+    ops.evict(view, 40, 8, 2, ptr(s2), ptr(p2), ptr(s2), ptr(p2), ptr(lo), layers=L, stream=stream())
+    torch.cuda.synchronize()
+    for x, y in ((k, k2), (v, v2)):
+        assert torch.equal(x.reshape(L, R, G, cap, 64).permute(0, 3, 1, 2, 4), y)
+    assert lo.tolist() == [40, 40]
