@@ -1324,67 +1324,112 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 
 // Weights of a step whose scores kv_step_kernel kept (own [b][g][slot][row of the
 // request], prefix [g][key][row]): the last block of rows' joins and these in one
-// launch.  A block works out its rows' (m, l) from the splits itself, 16 lanes a
-// row, then takes a key per thread.  Against the scores computed once more: 8
-// requests of 1500 slots, f32, 18 us less; 4 of 20000, f16, 35 us.
+// launch.  A block works out its rows' (m, l) from the splits itself, the more
+// lanes a row the fewer rows, then sums a key's weights per thread, or, of many
+// rows, per 16 lanes.  Against the scores computed once more, the whole call, us:
+// 8 requests of 1500 slots, f32, 24 : 40; 4 of 20000, f16, 74 : 95; 8 x 14 tokens
+// of 8 heads over 2 after 666 positions 32 : 23, 12 x 4 of 32 over 8 after 2900
+// 38 : 45.
 constexpr uint32_t KEPT_OWN_ROWS = 64, KEPT_ROWS = 512;  // rows of a request and, for the prefix, of all, at most
-constexpr uint32_t KEPT_KEYS = 512;  // per block
+constexpr uint32_t KEPT_TEAM_ROWS = 32;                  // from here on 16 lanes a key: 3 x 3 tokens of 14 heads over 2 after 2800 positions, 17 : 23 us a call
+__host__ __device__ constexpr uint32_t kept_keys(uint32_t rows) { return rows >= KEPT_TEAM_ROWS ? 128 : 256; }  // per block
+struct KvKeptGrid {
+  uint32_t joins, prefix, own;  // blocks: of joins, per kv head of the prefix, per cache (a cache's walk over its keys)
+};
 template <int HD>
-__global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, uint32_t joins, uint32_t key_blocks) {
-  if (blockIdx.x < joins) return join_rows<HD, 1024 / HD>(a, sp, nullptr);
+__global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, KvKeptGrid grid) {
+  if (blockIdx.x < grid.joins) return join_rows<HD, 1024 / HD>(a, sp, nullptr);
   __shared__ float2 ml[KEPT_ROWS];
-  const uint32_t tid = threadIdx.x, i = blockIdx.x - joins, kb0 = i % key_blocks, g = i / key_blocks % a.s.G, z = i / key_blocks / a.s.G;
-  const bool prefix = z == a.c.R;
-  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per;
+  const uint32_t tid = threadIdx.x, i = blockIdx.x - grid.joins;
+  const bool prefix = i < grid.prefix * a.s.G;
+  const uint32_t j = prefix ? i : i - grid.prefix * a.s.G, blocks = prefix ? grid.prefix : grid.own;
+  const uint32_t kb0 = j % blocks, g = j / blocks % a.s.G, z = j / blocks / a.s.G;
+  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per, keys = kept_keys(n_rows);
   Request rq{a.c.P, a.c.n};
   if (!prefix) rq = request_of(a.c, z, nullptr);
-  if (kb0 * KEPT_KEYS >= rq.len) return;
-  for (uint32_t r0 = 0; r0 < n_rows; r0 += 16) {
-    const uint32_t r = r0 + tid / 16, row = min(prefix ? r : z * per + r, a.c.R * per - 1);
-    float M = -INFINITY, L = 0.0f;
-    if (sp.splits == 1) {
-      const size_t at = size_t(row / a.s.rep) * a.s.H + g * a.s.rep + row % a.s.rep;
-      M = stat[2 * at];
-      L = stat[2 * at + 1];
-    } else {
-      const float* src = sp.ml + 2 * ((size_t(g) * sp.tiles + row / 16) * sp.splits * 16 + row % 16);
-      for (uint32_t s = tid % 16; s < sp.splits; s += 16) {
-        const float2 x = *reinterpret_cast<const float2*>(src + 32 * s);
-        const float mn = fmaxf(M, x.x), base = mn == -INFINITY ? 0.0f : mn;
-        L = L * __builtin_amdgcn_exp2f(M - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
-        M = mn;
+  if (kb0 * keys >= rq.len) return;
+  auto states = [&](auto LN) {
+    constexpr uint32_t L = LN();  // lanes per row
+    for (uint32_t r0 = 0; r0 < n_rows; r0 += 256 / L) {
+      const uint32_t r = r0 + tid / L, row = min(prefix ? r : z * per + r, a.c.R * per - 1);
+      float M = -INFINITY, S = 0.0f;
+      if (sp.splits == 1) {
+        const size_t at = size_t(row / a.s.rep) * a.s.H + g * a.s.rep + row % a.s.rep;
+        M = stat[2 * at];
+        S = stat[2 * at + 1];
+      } else {
+        const float* src = sp.ml + 2 * ((size_t(g) * sp.tiles + row / 16) * sp.splits * 16 + row % 16);
+#pragma unroll 4
+        for (uint32_t s = tid % L; s < sp.splits; s += L) {
+          const float2 x = *reinterpret_cast<const float2*>(src + 32 * s);
+          const float mn = fmaxf(M, x.x), base = mn == -INFINITY ? 0.0f : mn;
+          S = S * __builtin_amdgcn_exp2f(M - base) + x.y * __builtin_amdgcn_exp2f(x.x - base);
+          M = mn;
+        }
+        if constexpr (L > 1) {
+          auto reduce = [](float x, auto op) {
+            x = op(x, dpp_f32<DPP_QUAD_XOR1>(x));
+            x = op(x, dpp_f32<DPP_QUAD_XOR2>(x));
+            if constexpr (L == 16) {
+              x = op(x, dpp_f32<DPP_ROW_HALF_MIRROR>(x));
+              x = op(x, dpp_f32<DPP_ROW_MIRROR>(x));
+            }
+            return x;
+          };
+          const float all = reduce(M, [](float p, float q) { return fmaxf(p, q); });
+          S = reduce(S * __builtin_amdgcn_exp2f(M - (all == -INFINITY ? 0.0f : all)), [](float p, float q) { return p + q; });
+          M = all;
+        }
       }
-      const float all = row_reduce(M, [](float p, float q) { return fmaxf(p, q); });
-      L = row_reduce(L * __builtin_amdgcn_exp2f(M - (all == -INFINITY ? 0.0f : all)), [](float p, float q) { return p + q; });
-      M = all;
+      // rows of no token give nothing
+      const uint32_t b = row / per, t = row / a.s.rep % a.c.n;
+      const bool live = r < n_rows && t < (prefix ? request_of(a.c, b, nullptr).fresh : rq.fresh);
+      if (tid % L == 0 && r < n_rows) ml[r] = live ? make_float2(M, 1.0f / S) : make_float2(0.0f, 0.0f);
     }
-    // rows of no token give nothing
-    const uint32_t b = row / per, t = row / a.s.rep % a.c.n;
-    const bool live = r < n_rows && t < (prefix ? request_of(a.c, b, nullptr).fresh : rq.fresh);
-    if (tid % 16 == 0 && r < n_rows) ml[r] = live ? make_float2(M, 1.0f / L) : make_float2(0.0f, 0.0f);
-  }
+  };
+  if (n_rows <= 16)
+    states(std::integral_constant<uint32_t, 16>());
+  else if (n_rows <= 64)
+    states(std::integral_constant<uint32_t, 4>());
+  else
+    states(std::integral_constant<uint32_t, 1>());
   __syncthreads();
   const uint32_t base = prefix ? 0xffffffffu : rq.len - rq.fresh;
   const float* in = prefix ? a.pw_in : a.w_in;
   float* out = prefix ? a.pw_out : a.w_out;
-  for (uint32_t kb = kb0; kb * KEPT_KEYS < rq.len; kb += key_blocks) {
+  auto sums = [&](auto LN) {
+    constexpr uint32_t L = LN(), U = L == 1 ? 4 : 8;  // lanes per key, loads in flight
+    const uint32_t lane = tid % L;
+    for (uint32_t kb = kb0; kb * keys < rq.len; kb += blocks) {
+      for (uint32_t c = 0; c < keys; c += 256 / L) {
+        const uint32_t key = kb * keys + c + tid / L;
+        if (key >= rq.len) break;  // (a key's lanes as one)
+        const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
+        const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
+        const float before = in ? in[at] : 0.0f;
+        const uint32_t first = key <= base ? 0u : (key - base) * a.s.rep;  // earlier rows do not see the key
+        float w = 0.0f;
+        for (uint32_t r0 = first; r0 < n_rows; r0 += U * L) {
+          float y[U];
 #pragma unroll
-    for (uint32_t c = 0; c < KEPT_KEYS / 256; ++c) {
-      const uint32_t key = kb * KEPT_KEYS + 256 * c + tid;
-      if (key >= rq.len) break;
-      const float* src = prefix ? keep.prefix + (size_t(g) * a.c.P + key) * n_rows : keep.own + ((size_t(z) * a.s.G + g) * a.c.cap + key) * per;
-      const size_t at = prefix ? size_t(g) * a.pw_stride + key : (size_t(z) * a.s.G + g) * a.c.cap + key;
-      const float before = in ? in[at] : 0.0f;
-      float w = 0.0f;
-#pragma unroll 4
-      for (uint32_t r = key <= base ? 0u : (key - base) * a.s.rep; r < n_rows; ++r) {  // earlier rows do not see the key
-        const float2 x = ml[r];
-        const float p = __builtin_amdgcn_exp2f(src[r] - x.x) * x.y;
-        w += x.y != 0.0f ? p : 0.0f;  // (a row of no token left no score)
+          for (uint32_t u = 0; u < U; ++u) y[u] = src[min(r0 + u * L + lane, n_rows - 1)];
+#pragma unroll
+          for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t r = r0 + u * L + lane;
+            const float2 x = ml[min(r, n_rows - 1)];
+            const float p = __builtin_amdgcn_exp2f(y[u] - x.x) * x.y;
+            w += r < n_rows && x.y != 0.0f ? p : 0.0f;  // (a row of no token left no score)
+          }
+        }
+        if constexpr (L == 16) w = row_reduce(w, [](float p, float q) { return p + q; });
+        if (lane == 0) out[at] = before + w;
       }
-      out[at] = before + w;
     }
-  }
+  };
+  if (n_rows >= KEPT_TEAM_ROWS)
+    sums(std::integral_constant<uint32_t, 16>());
+  else
+    sums(std::integral_constant<uint32_t, 1>());
 }
 
 // The chunks' sums, in order, and the weights so far.  KB: keys per block of kv_weigh_kernel.
@@ -1696,9 +1741,10 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   // step kernel starts and ends quicker and the tile kernel multiplies quicker.  Both with their join, us, step : tile,
   // 32 heads over 8: f16 4 requests x 64 tokens over 1500 positions (13M scores) 37 : 39, 8 x 64 over 300 (7M) 27 : 30,
   // 1 x 130 over 4000 (18M) 80 : 44, 1 x 130 over 100 (1.2M) 12 : 21; f32 8 x 8 over 1500 (3.2M) 32 : 34, 8 x 16 (6.5M)
-  // 51 : 42, 3 x 37 over 1001 (4.2M) 39 : 37, 1 x 130 over 100 18 : 23.  A request of fewer than 32 rows would leave most
-  // of a tile's waves idle in its own cache.
-  const bool many = a.c.n * a.s.rep >= 32 && size_t(a.s.G) * rows * (a.c.P + a.c.cap) > (f16 ? 14000000u : 4000000u);
+  // 51 : 42, 3 x 37 over 1001 (4.2M) 39 : 37, 1 x 130 over 100 18 : 23; heads of 64 count half: 16 over 16, f16 8 x 96 over
+  // 838 (15M) 20 : 28, f32 8 over 2, 2 x 150 over 1500 (4.1M) 21 : 26, 3 x 436 over 1155 (17M) 55 : 38.  A request of fewer
+  // than 32 rows would leave most of a tile's waves idle in its own cache.
+  const bool many = a.c.n * a.s.rep >= 32 && size_t(a.s.G) * rows * (a.c.P + a.c.cap) * hd > (f16 ? 14000000u : 4000000u) * size_t(128);
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   // key tiles of a row tile, at most
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));
@@ -1730,8 +1776,11 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     const uint32_t z = a.c.R + (a.pw_out ? 1 : 0), keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
     if (keep.own) {
-      const uint32_t joins = sp.splits > 1 ? out_rows : 0, key_blocks = min(64u, (keys + KEPT_KEYS - 1) / KEPT_KEYS);
-      hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(joins + key_blocks * a.s.G * z), dim3(256), 0, s, a, sp, stat, keep, joins, key_blocks);
+      KvKeptGrid grid{sp.splits > 1 ? out_rows : 0, 0, 0};
+      const uint32_t own_keys = kept_keys(a.c.n * a.s.rep), prefix_keys = kept_keys(rows);
+      grid.own = min(128u, (a.c.cap + own_keys - 1) / own_keys);
+      if (a.pw_out) grid.prefix = (a.c.P + prefix_keys - 1) / prefix_keys;
+      hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(grid.joins + a.s.G * (grid.prefix + grid.own * a.c.R)), dim3(256), 0, s, a, sp, stat, keep, grid);
       return hipGetLastError();
     }
     if (sp.splits > 1 && out_rows <= 2048)
@@ -1740,14 +1789,19 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t kb = KH() ? 256 : 128;
-      // Steps of 32 rows: half of them, on average, see a key of their own turn.  Lengths are on the device: chunks are made
-      // for a cache of no more than the turn (longer ones have more key blocks, so the chunks are many enough), and blocks
-      // walk over the keys, so that slots not in use cost no blocks.
+      // Steps of 32 rows.  Lengths are on the device: chunks are made for a cache of no more than the turn, whose key block i
+      // is seen from its row i kb rep on (longer ones have more key blocks, so the chunks are many enough), and blocks walk
+      // over the keys, so that slots not in use cost no blocks.  A block costs its start (keys, and f32 ones split) and 1.3
+      // us a step, the join 64 chunks with ease.  Chunks of 2 : 3 : 5 : 8 : 13 steps, the whole call, 32 heads over 8, us:
+      // f16 1 request x 1500 tokens (5184 steps) 132 : 121 : 113 : 112 : 102, 1 x 126 over 1500 (896) 42 : 43 : 46 : 48 : 56;
+      // f32 5 x 243 (1840) 85 : 77 : 75 : 69 : 77, 2 x 157 over 32 (704) 34 : 35 : 37 : 39 : 44.
       const uint32_t own_steps = (a.c.n * a.s.rep + 31) / 32, all_steps = a.pw_out ? (rows + 31) / 32 : own_steps;
-      const size_t work = size_t(a.s.G) * (size_t((min(a.c.n, a.c.cap) + kb - 1) / kb) * a.c.R * own_steps / 2 + (a.pw_out ? size_t((a.c.P + kb - 1) / kb) * all_steps : 0));
+      const size_t own_blocks = (min(a.c.n, a.c.cap) + kb - 1) / kb, p_blocks = a.pw_out ? (a.c.P + kb - 1) / kb : 0;
+      const size_t work = a.s.G * (a.c.R * (own_blocks * own_steps - own_blocks * (own_blocks - 1) / 2 * (kb * a.s.rep / 32)) + p_blocks * all_steps);
       const size_t all = size_t(a.s.G) * (size_t(a.c.R) * a.c.cap + a.c.P);
       const uint32_t room = uint32_t(max(size_t(1), min(size_t(all_steps), w.cap_weights / all)));  // chunks that fit the workspace
-      const uint32_t chunk = max(uint32_t(min(size_t(all_steps), max(size_t(8), work / 320))), (all_steps + room - 1) / room);
+      const size_t blocks = !KH() && HD() == 128 ? 256 : 430;
+      const uint32_t chunk = max(max(uint32_t(min(size_t(all_steps), max(size_t(2), (work + blocks - 1) / blocks))), (all_steps + 63) / 64), (all_steps + room - 1) / room);
       const uint32_t chunks = (all_steps + chunk - 1) / chunk;
       hipLaunchKernelGGL((kv_weigh_kernel<HD(), KH()>), dim3(min(16u, (keys + kb - 1) / kb) * a.s.G, chunks, z), dim3(256), 0, s, a, w.stat, w.weights, chunk);
       if (chunks > 1)
