@@ -694,48 +694,57 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     const uint32_t stride = uint32_t(w.stride) * sizeof(T);
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
-      if constexpr (KH) {
-        const uint32_t x = (wave * LD + i) * 1024 + lane * 16, key = x / RB, off = min(key, w.keys - 1) * stride;
-        dma16(k, off + (k_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + (wave * LD + i) * 1024);
-        dma16(v, off + (v_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + PLANE + (wave * LD + i) * 1024);
-      } else {
-        const uint32_t off = min(key_of(i), w.keys - 1) * stride + piece_of(i) * 16;
-        kr[i] = *reinterpret_cast<const u32x4*>(k + off);
-        vr[i] = *reinterpret_cast<const u32x4*>(v + off);
-      }
+      const uint32_t x = (wave * LD + i) * 1024 + lane * 16, key = x / RB, off = min(key, w.keys - 1) * stride;
+      dma16(k, off + (k_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + (wave * LD + i) * 1024);
+      dma16(v, off + (v_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + PLANE + (wave * LD + i) * 1024);
     }
   };
-  auto store = [&](uint32_t buf) {
+  auto load_f32 = [&](const Where<T>& w, const T* from, u32x4* r) {
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(from);
+    const uint32_t stride = uint32_t(w.stride) * sizeof(T);
+#pragma unroll
+    for (int i = 0; i < LD; ++i) r[i] = *reinterpret_cast<const u32x4*>(src + (min(key_of(i), w.keys - 1) * stride + piece_of(i) * 16));
+  };
+  auto store_f32 = [&](uint32_t buf, int which, const u32x4* r) {
     uint8_t* base = lds + buf * BUF;
-    if constexpr (KH) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    } else {
+    float big = 0.0f;
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        float big = 0.0f;
+    for (int i = 0; i < LD; ++i) {
+      const floatx4 x = __builtin_bit_cast(floatx4, r[i]);
 #pragma unroll
-        for (int i = 0; i < LD; ++i) {
-          const floatx4 x = __builtin_bit_cast(floatx4, which ? vr[i] : kr[i]);
+      for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]));
+    }
+    big = wave_max(big);
+    if (!(big < INFINITY)) {  // the largest number, then
+      big = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
-        }
-        float r, inv;
-        pow2_scale(wave_max(big), r, inv);
-        if (lane == 0) scales[buf][which][wave] = r;
+      for (int i = 0; i < LD; ++i) {
+        const floatx4 x = __builtin_bit_cast(floatx4, r[i]);
 #pragma unroll
-        for (int i = 0; i < LD; ++i) {
-          const floatx4 x = __builtin_bit_cast(floatx4, which ? vr[i] : kr[i]) * inv;
-          half4 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            hi[e] = _Float16(x[e]);
-            lo[e] = _Float16(x[e] - float(hi[e]));
-          }
-          const uint32_t p = piece_of(i), off = (which ? v_at(key_of(i), p / 2) : k_at(key_of(i), p / 2)) + 8 * (p % 2);
-          *reinterpret_cast<half4*>(base + 2 * which * PLANE + off) = hi;
-          *reinterpret_cast<half4*>(base + (2 * which + 1) * PLANE + off) = lo;
-        }
+        for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
       }
+      big = wave_max(big);
+    }
+    float scale, inv;
+    pow2_scale(big, scale, inv);
+    if (lane == 0) scales[buf][which][wave] = scale;
+#pragma unroll
+    for (int i = 0; i < LD; ++i) {
+      const floatx4 x = __builtin_bit_cast(floatx4, r[i]) * inv;
+      const half4 hi = __builtin_convertvector(x, half4);
+      const half4 lo = __builtin_convertvector(x - __builtin_convertvector(hi, floatx4), half4);
+      const uint32_t p = piece_of(i), off = (which ? v_at(key_of(i), p / 2) : k_at(key_of(i), p / 2)) + 8 * (p % 2);
+      *reinterpret_cast<half4*>(base + 2 * which * PLANE + off) = hi;
+      *reinterpret_cast<half4*>(base + (2 * which + 1) * PLANE + off) = lo;
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto load_first = [&](const Where<T>& w) {
+    if constexpr (KH) {
+      load(w, 0);
+    } else {
+      load_f32(w, w.k, kr);
+      load_f32(w, w.v, vr);
     }
   };
 
@@ -745,7 +754,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   const uint32_t p_all = (a.c.P + KT - 1) / KT;
   uint32_t p_lo = whole_run ? 0u : p_all * split / sp.splits, n_pre = whole_run ? (split ? 0u : p_all) : p_all * (split + 1) / sp.splits - p_lo;
   const bool early = n_pre != 0;
-  if (early) load(prefix_tile<T, KT>(a.c, g, p_lo), 0);
+  if (early) load_first(prefix_tile<T, KT>(a.c, g, p_lo));
   const Run run = run_of<KT>(a, tile * TILE_ROWS, TILE_ROWS, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   uint32_t splits = sp.splits, o_lo = run.tiles * (splits - 1 - split) / splits, n_tiles = n_pre + run.tiles * (splits - split) / splits - o_lo;
   if (whole_run) {
@@ -769,7 +778,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   // this lane's row
   const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
   const bool live = at < rows && t_row < fresh_row;
-  const int own_limit = live ? int(len_row - fresh_row + t_row) : -1;
+  const uint32_t own_rows = live ? (b_row - run.b_lo) << 16 | (len_row - fresh_row + t_row) : 0u;  // segment, last slot seen
   half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
   float unscale;
   {
@@ -798,22 +807,36 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   floatx16 o[DT];  // dim 32 dt + 8 (v / 4) + 4 h2 + v % 4
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = floatx16{};
-  float m = -INFINITY, l = 0.0f, unit = 0.0f;  // f32: o in units of `unit`
+  float m = -INFINITY, l = 0.0f;
+  uint32_t unit = 0;  // f32: o is in units of this (its bits)
+  auto quotient = [](uint32_t p, uint32_t q) { return __uint_as_float(uint32_t(max(int(p - q + 0x3f800000u), 0))); };
   uint32_t seg = 0;
   auto where = [&](uint32_t i) { return i < n_pre ? prefix_tile<T, KT>(a.c, g, p_lo + i) : own_tile<T, KT>(a.c, run, g, o_lo + (i - n_pre), seg); };
   Where<T> w{};
   if (n_tiles) {
     w = where(0);
-    if (!early) load(w, 0);
-    store(0);
+    if (!early) load_first(w);
+    if constexpr (KH) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else {
+      store_f32(0, 0, kr);
+      store_f32(0, 1, vr);
+    }
   }
   __syncthreads();
   for (uint32_t i = 0; i < n_tiles; ++i) {
     const uint32_t buf = i & 1u;
     const bool more = i + 1 < n_tiles;
     const Where<T> next = more ? where(i + 1) : w;
-    if (more) load(next, buf ^ 1u);
-    const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : int(b_row - run.b_lo) == w.seg ? own_limit : -1;
+    if constexpr (KH) {
+      if (more) load(next, buf ^ 1u);
+    } else {
+      if (more) {
+        load_f32(next, next.k, kr);
+        load_f32(next, next.v, vr);
+      }
+    }
+    const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : uint32_t(w.seg) == own_rows >> 16 ? int(own_rows & 0xffffu) : -1;
     if (__any(limit >= int(w.key0))) {  // else nothing of it is for this wave's rows
       // fragment addresses: the swizzle changes with the low bits of ks and with dt, the rest are constants
       lds_byte *kp[4], *vp[DT];
@@ -842,6 +865,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       {
         constexpr int AHEAD = KH ? 2 : 1;
         half8 k8[3][2];
+        floatx16 s_lo = {};
         auto read = [&](int ks) {
           k8[ks % 3][0] = key8(0, 0, ks);
           k8[ks % 3][1] = KH ? key8(0, 1, ks) : key8(1, 0, ks);
@@ -852,12 +876,20 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         for (int ks = 0; ks < DS; ++ks) {
           if (ks + AHEAD < DS) read(ks + AHEAD);
           const half8 x = k8[ks % 3][0], y = k8[ks % 3][1];
-          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], s[0], 0, 0, 0);
-          s[NSUB - 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], s[NSUB - 1], 0, 0, 0);
-          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[ks], s[0], 0, 0, 0);
-          if constexpr (KH) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[ks], s[1], 0, 0, 0);
+          if constexpr (KH) {
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], s[1], 0, 0, 0);
+            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[ks], s[0], 0, 0, 0);
+            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, ql[ks], s[1], 0, 0, 0);
+          } else {
+            floatx16 &p = ks % 2 ? s_lo : s[0], &q = ks % 2 ? s[0] : s_lo;
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, qh[ks], p, 0, 0, 0);
+            q = __builtin_amdgcn_mfma_f32_32x32x16_f16(y, qh[ks], q, 0, 0, 0);
+            p = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, ql[ks], p, 0, 0, 0);
+          }
           __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (!KH) s[0] += s_lo;
       }
       const bool whole = __all(limit >= int(w.key0) + KT - 1);
       if (!whole) {
@@ -896,16 +928,21 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
       float ratio[4];
       if constexpr (!KH) {
-        const float* vs = scales[buf][1];
-        const float most = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        // (all powers of two, and quotients by their exponents: 0 below the normal numbers)
+        uint32_t vs[4], most = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          vs[c] = uniform(__float_as_uint(scales[buf][1][c]));
+          most = max(most, vs[c]);
+        }
         if (most > unit) {
-          const float f = unit / most;
+          const float f = quotient(unit, most);
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[d] *= f;
           unit = most;
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) ratio[c] = vs[c] / unit;  // powers of two
+        for (int c = 0; c < 4; ++c) ratio[c] = quotient(vs[c], unit);
       }
       int odd = 0;  // a value that is no number, and rows that must not see it
       if (!whole && w.seg >= 0) {
@@ -923,19 +960,22 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub) {
         half8 ph[2], pl[2];  // 16 keys each: the weights' upper 11 bits, and the rest
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
           float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], factor[v / 4], bias));
-          l += p;
+          sum[v % 2] += p;
           s[sub][v] = p;
           if constexpr (!KH) p *= ratio[v / 4];
           const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
           ph[v / 8][v % 8] = _Float16(hi);
           pl[v / 8][v % 8] = _Float16(p - hi);
         }
+        l += sum[0] + sum[1];
+        if constexpr (!KH) asm volatile("" : "+v"(l));  // (here, or the sums hold all the weights' registers to the end)
         int slow = __builtin_amdgcn_readfirstlane(odd);
         if (slow) {  // key by key, for the rows that see it
-          const float per_unit = KH ? 1.0f : 1.0f / unit;
+          const float per_unit = KH ? 1.0f : quotient(0x3f800000u, unit);
           for (int key = 0; key < 32 && 32 * sub + key < int(w.keys); ++key) {
             float p = 0.0f;
 #pragma unroll
@@ -958,30 +998,43 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         }
         asm volatile("" : "+s"(slow));  // (one branch after the other: as two sides of one they would hold two sets of o)
         if (!slow) {
-          // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind its first
-          constexpr int BL = 2 * DT, AHEAD = KH ? 2 : 1;
-          half8 v8[4], u8[KH ? 1 : 3];
+          // block c: 16 keys (st = c / DT) of 32 dims; its second and third terms come a block and two later, not right
+          // behind the one before
+          constexpr int BL = 2 * DT, AHEAD = KH ? 2 : 1, TERMS = KH ? 2 : 3;
+          half8 v8[4], u8[KH ? 1 : 4];
           auto read = [&](int c) {
             v8[c % 4] = value8(0, sub, c % DT, c / DT);
-            if constexpr (!KH) u8[c % 3] = value8(1, sub, c % DT, c / DT);
+            if constexpr (!KH) u8[c % 4] = value8(1, sub, c % DT, c / DT);
           };
 #pragma unroll
           for (int c = 0; c < AHEAD; ++c) read(c);
 #pragma unroll
-          for (int c = 0; c < BL + 1; ++c) {
+          for (int c = 0; c < BL + TERMS - 1; ++c) {
             if (c + AHEAD < BL) read(c + AHEAD);
             if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[c / DT], o[c % DT], 0, 0, 0);
-            if (c >= 1) {
+            if (c >= 1 && c <= BL) {
               const int b = c - 1;
               o[b % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[b % 4], pl[b / DT], o[b % DT], 0, 0, 0);
-              if constexpr (!KH) o[b % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[b % 3], ph[b / DT], o[b % DT], 0, 0, 0);
+            }
+            if constexpr (!KH) {
+              if (c >= 2) {
+                const int b = c - 2;
+                o[b % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(u8[b % 4], ph[b / DT], o[b % DT], 0, 0, 0);
+              }
             }
             __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
     }
-    if (more) store(buf ^ 1u);
+    if (more) {
+      if constexpr (KH) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      } else {
+        store_f32(buf ^ 1u, 0, kr);
+        store_f32(buf ^ 1u, 1, vr);
+      }
+    }
     __syncthreads();
     w = next;
   }
@@ -991,7 +1044,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
-  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f) * (KH ? 1.0f : unit);
+  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f) * (KH ? 1.0f : __uint_as_float(unit));
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
