@@ -1801,11 +1801,15 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   // key tiles of a row tile, at most
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));
-  sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
-  // Up to five tiles a wave cost less than a second launch: 4 requests over 200 shared positions, f32 (17 tiles) 11.9 us in
-  // one block a row tile against 8.1 + 3.3 and the time between, over 300 (23 tiles) 13.2 : 8.0 + 3.2; f16 over 400 10.2 :
-  // 7.4 + 3.3, over 600 11.4 : 7.5 + 3.3.
-  if (!many && most <= 20) sp.splits = 1;
+  // Step kernel: a block per CU, for more blocks' states cost the join more than they save (8 requests over 1500 + 512
+  // slots, f32: 256 blocks 14.6 us, 512 16.8; 4 over 20000 with weights, f16: 70 : 75), but two where one each would leave
+  // a third of the CUs idle (2 x 150 tokens of 8 heads over 2, 150 row tiles: 26.6 : 21.8).  Tile kernel: two.
+  const uint32_t fill = many || (lots > 128 && lots <= 170) ? 512 : 256;
+  sp.splits = max(1u, min(fill / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
+  // Up to six tiles a wave (twelve of heads of 64) cost less than a second launch, which weights have anyhow: 6 requests x
+  // 3 tokens, 300 slots, f16 (24 tiles) 6.8 : 10.3 us, 3 x 22 over 207, f32 (21) 10.9 : 13.4, 7 x 2 over 307 (29) 13.6 :
+  // 10.3; of heads of 64, 6 x 13 over 432, f16 (26) 6.8 : 9.1, 7 x 1 over 500 (32) 7.6 : 9.2, 2 x 4 over 1000 (53) 13.1 : 9.9.
+  if (!many && most <= (a.w_out ? 20u : 24u * 128 / hd)) sp.splits = 1;
   if (many && lots > 256 && lots <= 448) {
     // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
     // A prompt of 1500 tokens (376 row tiles) 81 : 65 us with the join; from 448 on the join costs what it saves.
