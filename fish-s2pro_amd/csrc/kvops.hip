@@ -150,7 +150,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 // 2^SLACK and the o registers are hardly ever rescaled.  f16 parts of weights are
 // of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is exact to
 // 2^-25, 2^-31 of the largest.
-constexpr float SLACK = 8.0f, F16_LIFT = 6.0f;
+// Weights of f32 values are of 2^(s - m + F32_LIFT): 65536 of up to 2^SLACK sum up
+// to no more than 1, and o to no more than the largest value.
+constexpr float SLACK = 8.0f, F16_LIFT = 6.0f, F32_LIFT = -24.0f;
 
 // max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 template <class Op>
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   constexpr int OT = HD / 16;                 // 16 x 16 output tiles
   constexpr int KL = HD * sizeof(T) / 64;     // 16-byte loads of a key row per lane
   constexpr int OP = HD + 4;                  // padded row of the joined states
-  constexpr float LIFT = KH ? F16_LIFT : 0.0f;
+  constexpr float LIFT = KH ? F16_LIFT : F32_LIFT;
   constexpr uint32_t VB = KT * HD * 2;        // bytes of a wave's value tile in LDS
   constexpr uint32_t JOIN = STEP_WAVES * 16 * OP * 4;
   constexpr uint32_t LDS = KH && STEP_WAVES * VB > JOIN ? STEP_WAVES * VB : JOIN;
@@ -1044,7 +1046,9 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
-  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : 1.0f) * (KH ? 1.0f : __uint_as_float(unit));
+  // (a state of f32 values leaves with F32_LIFT)
+  const float down = KH || last ? 1.0f : __builtin_amdgcn_exp2f(F32_LIFT - LIFT);
+  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : down) * (KH ? 1.0f : __uint_as_float(unit));
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1053,8 +1057,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           floatx4{o[dt][4 * c] * f, o[dt][4 * c + 1] * f, o[dt][4 * c + 2] * f, o[dt][4 * c + 3] * f};
   if (h2 == 0 && (!last || stat)) {
     float* st = last ? stat + 2 * at_row : sp.ml + 2 * part;
-    st[0] = m - LIFT;
-    st[1] = l;
+    st[0] = m - (KH || last ? LIFT : F32_LIFT);
+    st[1] = l * down;
   }
 }
 

@@ -876,3 +876,57 @@ def test_evict_layer_stride_left_out():
     for x, y in ((k, k2), (v, v2)):
         assert torch.equal(x.reshape(L, R, G, cap, 64).permute(0, 3, 1, 2, 4), y)
     assert lo.tolist() == [40, 40]
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("requests,n,heads,kv,prefix,length", [
+    (4, 4, 4, 4, 700, 140), (17, 1, 2, 2, 130, 300), (31, 1, 2, 2, 129, 5), (8, 1, 8, 2, 127, 1), (8, 4, 4, 4, 128, 257), (33, 1, 3, 3, 300, 70),
+    (4, 16, 4, 4, 100, 129), (5, 13, 2, 2, 90, 260), (2, 32, 4, 4, 0, 128), (1, 33, 4, 4, 65, 40), (16, 4, 32, 8, 2000, 33), (51, 5, 2, 2, 40, 6),
+    (257 // 2, 2, 4, 2, 50, 3), (171, 3, 2, 2, 30, 3)])
+def test_weigh_rows(requests, n, heads, kv, prefix, length, f16):
+    """Numbers of rows around those where a key's rows are summed by more lanes, or the scores are computed once more; some idle."""
+    lens = [max(1, length - b % 5) for b in range(requests)]
+    new = [min(lens[b], n - b % n) if b % 4 != 3 else 0 for b in range(requests)]
+    b = Batch((heads, kv, 64), f16, lens, new, prefix=prefix, seed=requests + n, rows=n, cap=max(lens) + 3)
+    ref = b.expect()
+    w, pw = torch.full((b.R, b.G, b.cap), 5.0, device="cuda"), torch.full((b.G, max(prefix, 1)), 5.0, device="cuda")
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), prefix_weights_out=ptr(pw) if prefix else 0, stream=stream())
+    torch.cuda.synchronize()
+    b.check(b.out, ref)
+    used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+    assert bool((w[~used] == 5.0).all())
+    assert bool(((w.double() - ref[2]).abs() <= ref[3] + U * ref[2])[used].all())
+    assert not prefix or bool(((pw.double() - ref[4]).abs() <= ref[5] + U * ref[4]).all())
+    assert b.ops.errors(stream()) == 0
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("shape", ["gqa4", "mha", "gqa7"])
+@pytest.mark.parametrize("n", [40, 255, 256, 257, 513, 1100])
+def test_weigh_chunks(n, shape, f16):
+    """Turns whose rows are summed in chunks, around whole blocks of keys, next to a shorter one."""
+    b = Batch(SHAPES[shape], f16, [n, n // 3 + 50], [n, n // 3], cap=n + 70, seed=n)
+    ref = b.expect()
+    w = torch.full((2, b.G, b.cap), 5.0, device="cuda")
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), stream=stream())
+    torch.cuda.synchronize()
+    b.check(b.out, ref)
+    used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+    assert bool((w[~used] == 5.0).all())
+    assert bool(((w.double() - ref[2]).abs() <= ref[3] + U * ref[2])[used].all())
+
+
+@pytest.mark.parametrize("low,high", [(-60, 60), (60, -60), (-100, 20), (0, 120)])
+@pytest.mark.parametrize("n", [192, 1])
+def test_attend_scales_far_apart(n, low, high):
+    """f32 caches: values of the first half of the keys 2^low, of the second 2^high; every output within the bound."""
+    b = Batch((32, 8, 128), False, [192], [n], prefix=320, cap=32768, seed=3)
+    b.pv.mul_(2.0 ** low)
+    b.v.mul_(2.0 ** high)
+    out = b.attend()
+    ref = b.expect()[0]
+    assert bool(out.isfinite().all())
+    p = kv_util.attend(b.q, b.k, torch.ones_like(b.v), b.lens_h, b.new_h, b.pk, torch.zeros_like(b.pv))[0]  # each row's weight on the second half
+    # 2^-20 of each half's part for products, sums and weights as in the plain bound; 2^-38 of the largest value for what falls below it
+    bound = 2.0 ** -20 * 8 * (p * 2.0 ** high + (1 - p) * 2.0 ** low) + 2.0 ** -38 * 8 * 2.0 ** max(low, high)
+    assert bool(((out.double() - ref).abs() <= bound).all())
