@@ -1305,6 +1305,12 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
       for (int v = 0; v < 16; ++v) sum[kw][v] = 0.0f;
+    if constexpr (KH) {  // (waited for here; in the loop that would be for the rows in flight too)
+#pragma unroll
+      for (int kw = 0; kw < KW; ++kw)
+#pragma unroll
+        for (int ks = 0; ks < DS; ++ks) asm volatile("" : "+v"(kh[kw][ks]));
+    }
     // Rows are loaded two steps ahead, and split for the next step while this one's products run.
     if (s_lo < s_hi) {
       load();
@@ -1319,16 +1325,24 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
       floatx16 s[KW];
 #pragma unroll
       for (int kw = 0; kw < KW; ++kw) s[kw] = floatx16{};
+      half8 q8[3][2];  // read two ahead
+      auto read = [&](int ks) {
+        const uint32_t off = k_at(r32, 2 * ks + h2);
+#pragma unroll
+        for (int p = 0; p < 2; ++p) q8[ks % 3][p] = *reinterpret_cast<const half8*>(&lds[buf][p * PLANE + off]);
+      };
+      read(0);
+      read(1);
 #pragma unroll
       for (int ks = 0; ks < DS; ++ks) {
-        const uint32_t off = k_at(r32, 2 * ks + h2);
-        const half8 qh = *reinterpret_cast<const half8*>(&lds[buf][off]), ql = *reinterpret_cast<const half8*>(&lds[buf][PLANE + off]);
+        if (ks + 2 < DS) read(ks + 2);
+        const half8 qh = q8[ks % 3][0], ql = q8[ks % 3][1];
 #pragma unroll
-        for (int kw = 0; kw < KW; ++kw) {
-          s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], qh, s[kw], 0, 0, 0);
-          s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
-          if constexpr (!KH) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[kw][ks], qh, s[kw], 0, 0, 0);
-        }
+        for (int kw = 0; kw < KW; ++kw) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], qh, s[kw], 0, 0, 0);
+#pragma unroll
+        for (int kw = 0; kw < KW; ++kw) s[kw] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[kw][ks], ql, s[kw], 0, 0, 0);
+        if constexpr (!KH) s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl[0][ks], qh, s[0], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (st + 1 < s_hi) {
         store(buf ^ 1u);
