@@ -46,6 +46,7 @@ struct KvSplit {
   float* ml;
   uint32_t tiles, splits;
   uint32_t least;  // key tiles per split, at least (kv_tile_kernel)
+  float up;        // o times this is the sum of weights with values (f32 caches)
 };
 
 // A step's scores, kept for the weights (nullable).

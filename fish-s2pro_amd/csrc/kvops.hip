@@ -147,12 +147,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 // their sum with the values; states over disjoint keys join by their m.
 
 // m follows a row's maximum only when it is SLACK behind: weights stay below
-// 2^SLACK and the o registers are hardly ever rescaled.  f16 parts of weights are
-// of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is exact to
-// 2^-25, 2^-31 of the largest.
-// Weights of f32 values are of 2^(s - m + F32_LIFT): 65536 of up to 2^SLACK sum up
-// to no more than 1, and o to no more than the largest value.
-constexpr float SLACK = 8.0f, F16_LIFT = 6.0f, F32_LIFT = -24.0f;
+// 2^SLACK and the o registers are hardly ever rescaled.  It is a whole number, so
+// that taking it off and the factors between states round nothing.  f16 parts of
+// weights are of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is
+// exact to 2^-25, 2^-31 of the largest.  The o of f32 values leave (and in
+// kv_step_kernel grow) times F32_DOWN: 65536 weights then add no more than the
+// largest value.
+constexpr float SLACK = 8.0f, F16_LIFT = 6.0f, F32_DOWN = 0x1p-30f, F32_UP = 0x1p30f;
 
 // max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48
 template <class Op>
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   constexpr int OT = HD / 16;                 // 16 x 16 output tiles
   constexpr int KL = HD * sizeof(T) / 64;     // 16-byte loads of a key row per lane
   constexpr int OP = HD + 4;                  // padded row of the joined states
-  constexpr float LIFT = KH ? F16_LIFT : F32_LIFT;
+  constexpr float LIFT = KH ? F16_LIFT : 0.0f;
   constexpr uint32_t VB = KT * HD * 2;        // bytes of a wave's value tile in LDS
   constexpr uint32_t JOIN = STEP_WAVES * 16 * OP * 4;
   constexpr uint32_t LDS = KH && STEP_WAVES * VB > JOIN ? STEP_WAVES * VB : JOIN;
@@ -486,17 +487,18 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
     for (int c = 1; c < NS; ++c) top = fmaxf(top, s[c]);
     const float mn = fmaxf(m, quarter_max(top));
     if (__any(mn > m + SLACK)) {
-      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - floorf(mn));
 #pragma unroll
       for (int c = 0; c < OT; ++c) o[c] *= f;
       l *= f;
-      m = mn;
+      m = floorf(mn);
     }
     const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
 #pragma unroll
     for (int c = 0; c < NS; ++c) {
       s[c] = __builtin_amdgcn_exp2f(s[c] - base);
       l += s[c];
+      if constexpr (!KH) s[c] *= F32_DOWN;
     }
     bool odd = false;  // a value that is no number, and rows that must not see it
     if constexpr (KH) {
@@ -620,7 +622,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
   if (last && !out_live) return;
   float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
-  const float inv = last ? (M_row == -INFINITY ? 0.0f : 1.0f / L_row) : 1.0f;
+  const float inv = last ? (M_row == -INFINITY ? 0.0f : (KH ? 1.0f : F32_UP) / L_row) : 1.0f;
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) {
     const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
@@ -921,11 +923,11 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       }
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
       if (__any(mn > m + SLACK)) {
-        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - floorf(mn));
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
         l *= f;
-        m = mn;
+        m = floorf(mn);
       }
       const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
       float ratio[4];
@@ -1046,9 +1048,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
-  // (a state of f32 values leaves with F32_LIFT)
-  const float down = KH || last ? 1.0f : __builtin_amdgcn_exp2f(F32_LIFT - LIFT);
-  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : down) * (KH ? 1.0f : __uint_as_float(unit));
+  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : KH ? 1.0f : F32_DOWN) * (KH ? 1.0f : __uint_as_float(unit));
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1057,8 +1057,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           floatx4{o[dt][4 * c] * f, o[dt][4 * c + 1] * f, o[dt][4 * c + 2] * f, o[dt][4 * c + 3] * f};
   if (h2 == 0 && (!last || stat)) {
     float* st = last ? stat + 2 * at_row : sp.ml + 2 * part;
-    st[0] = m - (KH || last ? LIFT : F32_LIFT);
-    st[1] = l * down;
+    st[0] = m - LIFT;
+    st[1] = l;
   }
 }
 
@@ -1133,7 +1133,7 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
     M = all;
   }
   if (done || !is_row || t >= checked(a.c, raw, nullptr).fresh) return;
-  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? 1.0f : 1.0f / L);
+  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? 1.0f : sp.up / L);
   if (stat && d == 0) {
     stat[2 * size_t(out)] = M;
     stat[2 * size_t(out) + 1] = L;
@@ -1806,6 +1806,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   KvSplit sp{};
   sp.o = w.part;
   sp.ml = w.part_ml;
+  sp.up = f16 ? 1.0f : F32_UP;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
   // Which kernel: by the scores to compute, over all heads and at most (capacities; lengths are on the device), for the
