@@ -68,9 +68,10 @@ using Elem = std::conditional_t<KH, _Float16, float>;
 // One block per token and run of heads (blockIdx.y, every gridDim.y-th 8 or 16):
 // the token's hd / 2 angles once (64-bit product with the position, whole turns
 // taken off in 64 bits, cos and sin of the rest in f32), then 4 elements (two
-// pairs) per thread.  Memory bound: 8 requests x 250 tokens of 32 + 8 + 8 heads
-// read and write 70 MB in 16 us; one step of 8 requests is all latency, so its
-// loads start together and its heads are spread over blocks.
+// pairs) per thread.  Memory bound: 8 requests x 250 tokens of 32 + 8 + 8 heads,
+// f16 caches, read and write 71 MB in 13.3 us (5.3 TB/s); one step of 8 requests
+// is all latency (3 us), so its loads start together and its heads are spread over
+// blocks.
 template <int HD, bool KH>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
   constexpr uint32_t LP = HD / 4;       // lanes per head
@@ -297,6 +298,12 @@ __device__ __forceinline__ Where<T> own_tile(const KvCaches& c, const Run& r, ui
 // not see in whole holds values that are no number (0 x NaN), they count as 0 in
 // the product, and a second product of marks, theirs with the keys each row
 // sees, says which outputs are no number.
+//   Bound by latency, then by memory: 8 requests over 1500 shared and 512 own
+// slots, f32, take 12.7 us, 6 of them start and end (3 to the requests' lengths
+// and the first keys, 3 the joining in LDS), the rest 39 MB; 16 over 24001 + 2000,
+// f16, 49 us: 200 MB from memory, 520 MB (10.7 TB/s) past the second-level cache,
+// for four row tiles read the prefix.  Two row tiles a wave, which halve that,
+// take 8 % off this call and put 10 to 60 % on shorter ones.
 constexpr int STEP_WAVES = 4;
 
 template <int HD, bool KH>
@@ -651,6 +658,11 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 // registers): three products, 2^-22 of each term, or 2^-39 of the largest value
 // of the run for terms far below it.  (The f32 matrix instructions do a
 // sixteenth of the f16 ones' work per cycle.)
+//   Bound by the matrix units: 8 requests x 250 tokens over 1500 + 250 slots, f16,
+// 104 us (0.85 PFLOP/s of hi + lo products), 2048 tokens over 6000 430 us (1.1, at
+// the 1.66 GHz that the clock falls to; a library's f16 product of 8192^3 reaches
+// 1.2 to 1.3).  f32, 3 x 37 over 1001 + 131: 26 us, of which a tile of 32 keys
+// takes 2.2, a third of it products: blocks are too few to hide the splitting.
 constexpr int TILE_ROWS = 128;
 constexpr float NO_STATE = -1.0f;  // in the place of l: no state here
 
@@ -1156,6 +1168,9 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp
 // sum has one order.  blockIdx.z = request, or R for the prefix with the rows of
 // all requests; with several row splits the sums go to the workspace and
 // kv_weights_join_kernel adds them.
+//   A prompt of 1500 tokens, f16: 37 us, 0.58 PFLOP/s of hi + lo products; vector
+// instructions (a step splits 32 rows and takes 64 exponentials a lane pair) take
+// as many cycles as the products.
 struct RowSteps {
   uint32_t base, begin, end, steps;
 };
@@ -1398,7 +1413,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // launch.  A block works out its rows' (m, l) from the splits itself, the more
 // lanes a row the fewer rows, then sums a key's weights per thread, or, of many
 // rows, per 16 lanes.  Against the scores computed once more, the whole call, us:
-// 8 requests of 1500 slots, f32, 24 : 40; 4 of 20000, f16, 74 : 95; 8 x 14 tokens
+// 8 requests of 1500 slots, f32, 23 : 40; 4 of 20000, f16, 70 : 95; 8 x 14 tokens
 // of 8 heads over 2 after 666 positions 32 : 23, 12 x 4 of 32 over 8 after 2900
 // 38 : 45.
 constexpr uint32_t KEPT_OWN_ROWS = 64, KEPT_ROWS = 512;  // rows of a request and, for the prefix, of all, at most
@@ -1591,9 +1606,8 @@ __device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, con
 //   The k-th largest score among the slots that compete (the safe ones all stay,
 // the others compete for the rest) by digits of 8 bits from the top, until all
 // scores that share them stay; of the slots that equal it in all four the lowest
-// stay.  Then the freed slots below m and the
-// kept ones from m on are counted off in slot order: the x-th of one takes the
-// x-th of the other.
+// stay.  Then the freed slots below m and the kept ones from m on are counted off
+// in slot order: the x-th of one takes the x-th of the other.
 //   MOVE: the block then moves the rows, its part blockIdx.y of them, 16 bytes a
 // thread; every part finds the same list (the scores are not written before all
 // have read them: in place, there is one part).  A cache's list takes about 10 us
@@ -1601,6 +1615,9 @@ __device__ __forceinline__ void move_rows(const KvEvictArgs& a, uint32_t sg, con
 // or more per CU one hides the other, and with fewer the parts share the rows
 // without a second launch.  Otherwise the list goes to the workspace for
 // kv_move_kernel.
+//   Bound by memory: 36 layers x 4 requests x 8 heads of 1999 slots cut to 777, f16,
+// 487 MB in 113 us (4.3 TB/s); 8 x 8 of 2560 to 1024, f32, 74 MB in 19 us, half of
+// them the list.
 struct KvMove {
   uint32_t max_moves, pieces;  // pieces: 16-byte pieces of a row
   uint32_t* moves;
@@ -1831,7 +1848,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   if (!many && most <= (a.w_out ? 20u : 24u * 128 / hd)) sp.splits = 1;
   if (many && lots > 256 && lots <= 448) {
     // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
-    // A prompt of 1500 tokens (376 row tiles) 81 : 65 us with the join; from 448 on the join costs what it saves.
+    // A prompt of 1500 tokens (376 row tiles) 80 : 68 us with the join, f32 134 : 98; from 448 on the join costs what it saves.
     sp.splits = 2;
     sp.least = 768 / kt;
   }
