@@ -14,6 +14,17 @@ from s2hip.kvops import ERR_F16_RANGE, ERR_LENS, ERR_POSITION
 
 pytestmark = pytest.mark.gpu
 U = kv_util.U
+
+
+@pytest.fixture(autouse=True)
+def float32_tensors():
+    """Whatever another module has made the default type."""
+    was = torch.get_default_dtype()
+    torch.set_default_dtype(torch.float32)
+    yield
+    torch.set_default_dtype(was)
+
+
 SHAPES = {"gqa4": (32, 8, 128), "tiny": (8, 2, 64), "mha": (4, 4, 64), "gqa3": (6, 2, 128), "gqa7": (14, 2, 128)}
 
 
