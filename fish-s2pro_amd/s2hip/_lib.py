@@ -103,6 +103,12 @@ def declared_functions():
     return sorted(set(re.findall(r"\b(s2hip_[a-z0-9_]+)\s*\(", text)))
 
 
+def hip_runtimes():
+    """Files of the HIP runtimes that are loaded."""
+    with open("/proc/self/maps") as f:
+        return sorted({line.split(None, 5)[5].strip() for line in f if "/libamdhip64.so" in line})
+
+
 def load():
     global _lib
     if _lib is not None:

@@ -9,11 +9,16 @@ launch on the given stream (e.g. torch.cuda.current_stream().cuda_stream; 0:
 the default stream) and return at once; the caller keeps the arrays alive and
 orders calls on one handle on the device.  Failures raise ``S2HipError``.
 There is no CPU fallback.
+
+torch brings a HIP runtime of its own, which s2hip shares if torch was imported
+before s2hip's library was loaded (the first handle does that); pointers and
+streams of torch's are no good to the other runtime otherwise, and KvOps refuses.
 """
 
 from __future__ import annotations
 
 import ctypes
+import sys
 
 from . import _lib
 from .engine import S2HipError
@@ -30,6 +35,9 @@ class KvOps:
         """max_requests, max_tokens: the most requests, and requests * n_tokens,
         of one call.  scale 0: 1 / sqrt(head_dim)."""
         L = _lib.load()
+        runtimes = _lib.hip_runtimes()
+        if "torch" in sys.modules and len(runtimes) > 1:
+            raise S2HipError("two HIP runtimes in this process (" + ", ".join(runtimes) + "): import torch before the first s2hip handle")
         cfg = _lib.KvConfig(device, heads, kv_heads, head_dim, int(kv_f16), max_requests, max_tokens, rope_base, eps,
                             scale)
         self._err = ctypes.create_string_buffer(_lib.ERR_CAP)
