@@ -483,7 +483,8 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * overlap q.
  *   Products and sums are f32 or better, except for calls of many tokens over
  * f32 caches: there each term is exact to 2^-22, or to 2^-39 of the largest
- * value among the keys that its block of rows reads. */
+ * value among the keys that its block of rows reads.  Values of f32 caches
+ * below 2^-80 may count as 0. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                         void* stream, char* err, size_t err_cap);
 /* s2hip_kv_attend, and for every slot s < lens[b] of every kv head g
