@@ -1415,13 +1415,19 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // rows, per 16 lanes.  Against the scores computed once more, the whole call, us:
 // 8 requests of 1500 slots, f32, 23 : 40; 4 of 20000, f16, 70 : 95; 8 x 14 tokens
 // of 8 heads over 2 after 666 positions 32 : 23, 12 x 4 of 32 over 8 after 2900
-// 38 : 45.
+// 33 : 45.
 constexpr uint32_t KEPT_OWN_ROWS = 64, KEPT_ROWS = 512;  // rows of a request and, for the prefix, of all, at most
 constexpr uint32_t KEPT_TEAM_ROWS = 32;                  // from here on 16 lanes a key: 3 x 3 tokens of 14 heads over 2 after 2800 positions, 17 : 23 us a call
-__host__ __device__ constexpr uint32_t kept_keys(uint32_t rows) { return rows >= KEPT_TEAM_ROWS ? 128 : 256; }  // per block
 struct KvKeptGrid {
-  uint32_t joins, prefix, own;  // blocks: of joins, per kv head of the prefix, per cache (a cache's walk over its keys)
+  uint32_t joins, prefix, own;     // blocks: of joins, per kv head of the prefix, per cache (a cache's walk over its keys)
+  uint32_t prefix_keys, own_keys;  // per block
 };
+// Keys per block of `rows` rows, of `keys` keys over all caches and heads: one per thread, or 16 lanes; of many rows
+// enough blocks that a block's walk is short (8 x 14 tokens of 8 heads over 2 after 666 positions 30 : 15 us a call).
+inline uint32_t kept_keys(uint32_t rows, size_t keys) {
+  if (rows < KEPT_TEAM_ROWS) return 256;
+  return uint32_t(min(size_t(128), max(size_t(16), (keys / 512 + 15) / 16 * 16)));
+}
 template <int HD>
 __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, KvSplit sp, const float* stat, KvScores keep, KvKeptGrid grid) {
   if (blockIdx.x < grid.joins) return join_rows<HD, 1024 / HD>(a, sp, nullptr);
@@ -1430,7 +1436,7 @@ __global__ __launch_bounds__(256) void kv_join_weights_kernel(KvAttendArgs a, Kv
   const bool prefix = i < grid.prefix * a.s.G;
   const uint32_t j = prefix ? i : i - grid.prefix * a.s.G, blocks = prefix ? grid.prefix : grid.own;
   const uint32_t kb0 = j % blocks, g = j / blocks % a.s.G, z = j / blocks / a.s.G;
-  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per, keys = kept_keys(n_rows);
+  const uint32_t per = a.c.n * a.s.rep, n_rows = prefix ? a.c.R * per : per, keys = prefix ? grid.prefix_keys : grid.own_keys;
   Request rq{a.c.P, a.c.n};
   if (!prefix) rq = request_of(a.c, z, nullptr);
   if (kb0 * keys >= rq.len) return;
@@ -1869,10 +1875,12 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     const uint32_t z = a.c.R + (a.pw_out ? 1 : 0), keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
     if (keep.own) {
-      KvKeptGrid grid{sp.splits > 1 ? out_rows : 0, 0, 0};
-      const uint32_t own_keys = kept_keys(a.c.n * a.s.rep), prefix_keys = kept_keys(rows);
-      grid.own = min(128u, (a.c.cap + own_keys - 1) / own_keys);
-      if (a.pw_out) grid.prefix = (a.c.P + prefix_keys - 1) / prefix_keys;
+      KvKeptGrid grid{};
+      grid.joins = sp.splits > 1 ? out_rows : 0;
+      grid.own_keys = kept_keys(a.c.n * a.s.rep, size_t(a.c.cap) * a.c.R * a.s.G);
+      grid.own = min(128u, (a.c.cap + grid.own_keys - 1) / grid.own_keys);
+      grid.prefix_keys = kept_keys(rows, size_t(a.c.P) * a.s.G);
+      if (a.pw_out) grid.prefix = (a.c.P + grid.prefix_keys - 1) / grid.prefix_keys;
       hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(grid.joins + a.s.G * (grid.prefix + grid.own * a.c.R)), dim3(256), 0, s, a, sp, stat, keep, grid);
       return hipGetLastError();
     }
