@@ -1414,10 +1414,12 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // lanes a row the fewer rows, then sums a key's weights per thread, or, of many
 // rows, per 16 lanes.  Against the scores computed once more, the whole call, us:
 // 8 requests of 1500 slots, f32, 23 : 40; 4 of 20000, f16, 70 : 95; 8 x 14 tokens
-// of 8 heads over 2 after 666 positions 32 : 23, 12 x 4 of 32 over 8 after 2900
-// 33 : 45.
-constexpr uint32_t KEPT_OWN_ROWS = 64, KEPT_ROWS = 512;  // rows of a request and, for the prefix, of all, at most
-constexpr uint32_t KEPT_TEAM_ROWS = 32;                  // from here on 16 lanes a key: 3 x 3 tokens of 14 heads over 2 after 2800 positions, 17 : 23 us a call
+// of 8 heads over 2 after 666 positions 15 : 23, 12 x 4 of 32 over 8 after 2900
+// 33 : 45, 1 x 139 18 : 23, 7 x 67 21 : 28; with shared positions 8 x 62 (1984 rows)
+// over 11 31 : 38, 4 x 100 of 8 over 2 (1600) over 1500 32 : 28, 8 x 83 (2656) over 3
+// 24 : 22.
+constexpr uint32_t KEPT_ROWS = 2048;     // of a request and, for the prefix, of all, at most
+constexpr uint32_t KEPT_TEAM_ROWS = 32;  // from here on 16 lanes a key: 3 x 3 tokens of 14 heads over 2 after 2800 positions, 17 : 23 us a call
 struct KvKeptGrid {
   uint32_t joins, prefix, own;     // blocks: of joins, per kv head of the prefix, per cache (a cache's walk over its keys)
   uint32_t prefix_keys, own_keys;  // per block
@@ -1863,7 +1865,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   // a step's scores are kept where there is room for them
   KvScores keep{};
   const size_t own_scores = size_t(rows) * a.s.G * a.c.cap, prefix_scores = a.pw_out ? size_t(rows) * a.s.G * a.c.P : 0;
-  if (a.w_out && !many && own_scores + prefix_scores <= w.cap_weights && a.c.n * a.s.rep <= KEPT_OWN_ROWS && (!a.pw_out || rows <= KEPT_ROWS)) {
+  if (a.w_out && !many && own_scores + prefix_scores <= w.cap_weights && a.c.n * a.s.rep <= KEPT_ROWS && (!a.pw_out || rows <= KEPT_ROWS)) {
     keep.own = w.weights;
     keep.prefix = a.pw_out ? w.weights + own_scores : nullptr;
   }

@@ -941,3 +941,21 @@ def test_attend_scales_far_apart(n, low, high):
     # 2^-20 of each half's part for products, sums and weights as in the plain bound; 2^-38 of the largest value for what falls below it
     bound = 2.0 ** -20 * 8 * (p * 2.0 ** high + (1 - p) * 2.0 ** low) + 2.0 ** -38 * 8 * 2.0 ** max(low, high)
     assert bool(((out.double() - ref).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("requests,n,heads,kv,prefix", [(8, 64, 8, 2, 20), (1, 683, 6, 2, 9), (1, 512, 8, 2, 0), (1, 513, 8, 2, 0), (9, 57, 8, 2, 33), (2, 1024, 2, 2, 5)])
+def test_weigh_rows_of_turns(requests, n, heads, kv, prefix, f16):
+    """Rows up to those whose scores are kept, and a few more."""
+    lens = [n + 3 * b for b in range(requests)]
+    new = [n - 7 * b for b in range(requests)]
+    b = Batch((heads, kv, 64), f16, lens, new, prefix=prefix, seed=n, rows=n)
+    ref = b.expect()
+    w, pw = torch.full((b.R, b.G, b.cap), 5.0, device="cuda"), torch.full((b.G, max(prefix, 1)), 5.0, device="cuda")
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), prefix_weights_out=ptr(pw) if prefix else 0, stream=stream())
+    torch.cuda.synchronize()
+    b.check(b.out, ref)
+    used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+    assert bool((w[~used] == 5.0).all())
+    assert bool(((w.double() - ref[2]).abs() <= ref[3] + U * ref[2])[used].all())
+    assert not prefix or bool(((pw.double() - ref[4]).abs() <= ref[5] + U * ref[4]).all())
