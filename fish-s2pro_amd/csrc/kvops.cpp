@@ -132,7 +132,7 @@ class KvOps {
     work_.cap_parts = 8192;
     work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
     work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
-    work_.cap_weights = size_t(1) << 24;
+    work_.cap_weights = size_t(1) << 25;
     work_.weights = alloc<float>(work_.cap_weights);
     work_.moves = alloc<uint32_t>(size_t(KV_LISTS) * KV_LIST);
     work_.counts = alloc<uint32_t>(2 * KV_LISTS);

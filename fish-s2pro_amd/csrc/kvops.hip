@@ -1834,14 +1834,19 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   sp.up = f16 ? 1.0f : F32_UP;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
-  // Which kernel: by the scores to compute, over all heads and at most (capacities; lengths are on the device), for the
-  // step kernel starts and ends quicker and the tile kernel multiplies quicker.  Both with their join, us, step : tile,
-  // 32 heads over 8: f16 4 requests x 64 tokens over 1500 positions (13M scores) 37 : 39, 8 x 64 over 300 (7M) 27 : 30,
-  // 1 x 130 over 4000 (18M) 80 : 44, 1 x 130 over 100 (1.2M) 12 : 21; f32 8 x 8 over 1500 (3.2M) 32 : 34, 8 x 16 (6.5M)
-  // 51 : 42, 3 x 37 over 1001 (4.2M) 39 : 37, 1 x 130 over 100 18 : 23; heads of 64 count half: 16 over 16, f16 8 x 96 over
-  // 838 (15M) 20 : 28, f32 8 over 2, 2 x 150 over 1500 (4.1M) 21 : 26, 3 x 436 over 1155 (17M) 55 : 38.  A request of fewer
-  // than 32 rows would leave most of a tile's waves idle in its own cache.
-  const bool many = a.c.n * a.s.rep >= 32 && size_t(a.s.G) * rows * (a.c.P + a.c.cap) * hd > (f16 ? 14000000u : 4000000u) * size_t(128);
+  // The scores of few enough rows can be kept, where there is room for them.
+  const size_t own_scores = size_t(rows) * a.s.G * a.c.cap, prefix_scores = a.pw_out ? size_t(rows) * a.s.G * a.c.P : 0;
+  const bool may_keep = a.w_out && own_scores + prefix_scores <= w.cap_weights && a.c.n * a.s.rep <= KEPT_ROWS && (!a.pw_out || rows <= KEPT_ROWS);
+  // Which kernel: by the scores to compute, over all heads and at most (capacities, of the turn's own slots half; lengths
+  // are on the device), for the step kernel starts and ends quicker and the tile kernel multiplies quicker; heads of 64
+  // count half.  Both with their join, us, step : tile, 32 heads over 8: f16 2 requests x 211 tokens over 110 + 452 slots
+  // (6M scores) 21 : 29, 5 x 35 over 1500 + 78 (6.6M) 34 : 33, 4 x 64 over 1500 (13M) 37 : 39, 2 x 517 over 146 + 624 (17M)
+  // 52 : 43; f32 8 x 12 over 728 + 235 (3M) 22 : 32, 3 x 37 over 1001 + 768 (6M) 33 : 32, 2 x 445 over 10 + 616 (11M) 66 : 46.
+  // Kept scores save the tile kernel's weights their products: f16 8 x 145 over 488 own slots (15M) 62 : 67, 8 x 174 (17M) 51 :
+  // 57, 4 x 142 of 24 over 1151 + 367 (20M) 80 : 66; f32 3 x 129 (3M) 24 : 43, 8 x 97 (8M) 39 : 47, 2 x 104 over 1500 + 239 (11M)
+  // 92 : 70.  A request of fewer than 32 rows would leave most of a tile's waves idle in its own cache.
+  const size_t scores = size_t(a.s.G) * rows * (a.c.P + a.c.cap - min(a.c.n, a.c.cap) / 2);
+  const bool many = a.c.n * a.s.rep >= 32 && scores * hd > (may_keep ? f16 ? 14000000u : 8000000u : f16 ? 10000000u : 4200000u) * size_t(128);
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
   // key tiles of a row tile, at most
   const uint32_t most = (a.c.P + kt - 1) / kt + (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));
@@ -1862,10 +1867,8 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   }
   if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   float* stat = a.w_out ? w.stat : nullptr;
-  // a step's scores are kept where there is room for them
   KvScores keep{};
-  const size_t own_scores = size_t(rows) * a.s.G * a.c.cap, prefix_scores = a.pw_out ? size_t(rows) * a.s.G * a.c.P : 0;
-  if (a.w_out && !many && own_scores + prefix_scores <= w.cap_weights && a.c.n * a.s.rep <= KEPT_ROWS && (!a.pw_out || rows <= KEPT_ROWS)) {
+  if (may_keep && !many) {
     keep.own = w.weights;
     keep.prefix = a.pw_out ? w.weights + own_scores : nullptr;
   }
