@@ -67,7 +67,8 @@ using Elem = std::conditional_t<KH, _Float16, float>;
 // ---------------------------------------------------------------------------
 // One block per token and run of heads (blockIdx.y, every gridDim.y-th 8 or 16):
 // the token's hd / 2 angles once (64-bit product with the position, whole turns
-// taken off in 64 bits, cos and sin of the rest in f32), then 4 elements (two
+// taken off in 64 bits, cos and sin of the rest in f32, turned by what its rounding
+// left), then 4 elements (two
 // pairs) per thread.  Memory bound: 8 requests x 250 tokens of 32 + 8 + 8 heads,
 // f16 caches, read and write 71 MB in 13.3 us (5.3 TB/s); one step of 8 requests
 // is all latency (3 us), so its loads start together and its heads are spread over
@@ -93,10 +94,11 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
   }
   if (tid < HD / 2) {
     const double angle = double(pos) * freq * 0.15915494309189535;  // in turns
-    const float rest = float(angle - rint(angle));
+    const double rest = angle - rint(angle);
+    const float part = float(rest), more = 6.2831853f * float(rest - double(part));  // (what f32 loses of the angle, in radians)
     float sn, cs;
-    sincospif(2.0f * rest, &sn, &cs);
-    turn[tid] = make_float2(cs, sn);
+    sincospif(2.0f * part, &sn, &cs);
+    turn[tid] = make_float2(fmaf(-sn, more, cs), fmaf(cs, more, sn));
   }
   __syncthreads();
   for (uint32_t h = h0; h < heads;) {  // whole rows of 16 lanes take part
@@ -107,7 +109,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
         float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w;
         ss = row_reduce(ss, [](float p, float q) { return p + q; });
         if constexpr (LP == 32) ss += __shfl_xor(ss, 16, 64);
-        const float f = rsqrtf(ss * (1.0f / HD) + a.s.eps);
+        const float mean = ss * (1.0f / HD) + a.s.eps, near = rsqrtf(mean), step = fmaf(-mean * near, near, 1.0f);
+        const float f = step == step ? fmaf(0.5f * near, step, near) : near;  // (mean 0 or infinite)
         const float4 gain = *reinterpret_cast<const float4*>((h < a.s.H ? a.q_norm : a.k_norm) + d);
         x = make_float4(x.x * f * gain.x, x.y * f * gain.y, x.z * f * gain.z, x.w * f * gain.w);
       }

@@ -959,3 +959,19 @@ def test_weigh_rows_of_turns(requests, n, heads, kv, prefix, f16):
     assert bool((w[~used] == 5.0).all())
     assert bool(((w.double() - ref[2]).abs() <= ref[3] + U * ref[2])[used].all())
     assert not prefix or bool(((pw.double() - ref[4]).abs() <= ref[5] + U * ref[4]).all())
+
+
+@pytest.mark.parametrize("size", [0.0, 1e-25, 1e25])
+def test_append_norm_of_extreme_rows(size):
+    """Rows of zeros, and ones whose squares leave f32: as y / sqrt(mean(y^2) + eps) gives them in f32."""
+    H, G, hd = 8, 2, 64
+    g = gen(21)
+    qkv = normal(g, 1, 3, H + 2 * G, hd) * size
+    k, v, q = torch.zeros(1, G, 4, hd, device="cuda"), torch.zeros(1, G, 4, hd, device="cuda"), torch.full((1, 3, H, hd), 7.0, device="cuda")
+    ones, pos, lens = torch.ones(hd, device="cuda"), torch.zeros(1, 3, dtype=torch.int32, device="cuda"), dev([3], torch.int32)
+    ops = KvOps(H, G, hd, max_requests=1, max_tokens=3)
+    ops.append(ops.view(ptr(k), ptr(v), ptr(lens), 1, 4), ptr(qkv), 3, ptr(pos), ptr(q), q_norm=ptr(ones), k_norm=ptr(ones), stream=stream())
+    torch.cuda.synchronize()
+    want = qkv * torch.rsqrt((qkv * qkv).mean(-1, keepdim=True) + 1e-6)
+    assert bool(((q - want[:, :, :H]).abs() <= 2.0**-20 * want[:, :, :H].abs()).all())
+    assert torch.equal(v[:, :, :3].transpose(1, 2), qkv[:, :, H + G :]) and ops.errors(stream()) == 0
