@@ -340,28 +340,33 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   // f32: K key r16, dims 16 j + 4 q4 ..; V key 4 q4 + i, dims 64 hh + 4 r16 ..
   // f16: K key 16 kt + r16, dims 32 j + 8 q4 ..; V 16-byte pieces lane + 64 i of the tile
   u32x4 kr[KH ? 2 : 1][KL], vr[KH ? HD / 16 : 4][KH ? 1 : HD / 64];
+  // (offsets in 32 bits from a uniform base: 64-bit products per row took a quarter of a tile's vector cycles)
   auto load_k = [&](const Where<T>& w) {
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(w.k);
+    const uint32_t stride = uint32_t(w.stride) * sizeof(T);
 #pragma unroll
     for (int kt = 0; kt < (KH ? 2 : 1); ++kt) {
-      const T* p = w.k + min(16u * kt + r16, w.keys - 1) * w.stride + (KH ? 8 : 4) * q4;
+      const uint32_t off = min(16u * kt + r16, w.keys - 1) * stride + 16 * q4;
 #pragma unroll
-      for (int j = 0; j < KL; ++j) kr[kt][j] = *reinterpret_cast<const u32x4*>(p + (KH ? 32 : 16) * j);
+      for (int j = 0; j < KL; ++j) kr[kt][j] = *reinterpret_cast<const u32x4*>(base + (off + 64 * j));
     }
   };
   auto load_v = [&](const Where<T>& w) {
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(w.v);
+    const uint32_t stride = uint32_t(w.stride) * sizeof(T);
     if constexpr (KH) {
       constexpr uint32_t PR = HD / 8;  // pieces per row
 #pragma unroll
       for (int i = 0; i < HD / 16; ++i) {
         const uint32_t p = lane + 64 * i;
-        vr[i][0] = *reinterpret_cast<const u32x4*>(w.v + min(p / PR, w.keys - 1) * w.stride + (p % PR) * 8);
+        vr[i][0] = *reinterpret_cast<const u32x4*>(base + (min(p / PR, w.keys - 1) * stride + (p % PR) * 16));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const T* p = w.v + min(4 * q4 + i, w.keys - 1) * w.stride + 4 * r16;
+        const uint32_t off = min(4 * q4 + i, w.keys - 1) * stride + 16 * r16;
 #pragma unroll
-        for (int hh = 0; hh < HD / 64; ++hh) vr[i][hh] = *reinterpret_cast<const u32x4*>(p + 64 * hh);
+        for (int hh = 0; hh < HD / 64; ++hh) vr[i][hh] = *reinterpret_cast<const u32x4*>(base + (off + 256 * hh));
       }
     }
   };
@@ -515,8 +520,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
       half8 ph, pl;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        ph[c] = _Float16(s[c]);
-        pl[c] = _Float16(s[c] - float(ph[c]));
+        const float hi = __uint_as_float(__float_as_uint(s[c]) & 0xffffe000u);  // the upper 11 bits, and the rest
+        ph[c] = _Float16(hi);
+        pl[c] = _Float16(s[c] - hi);
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       half8 v8[OT];
