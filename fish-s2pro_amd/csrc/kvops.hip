@@ -295,7 +295,7 @@ __device__ __forceinline__ Where<T> own_tile(const KvCaches& c, const Run& r, ui
 // operand registers by 16-byte loads in an order of dims of our own choosing.
 //   f16 caches: v_mfma_f32_16x16x32_f16, 32 keys a tile, q and the weights as
 // hi + lo f16 parts (2^-22 of a row's largest q, 2^-22 of a weight; weights are
-// scaled by 2^14 so that small ones keep their lo part); K from memory to
+// lifted by F16_LIFT so that small ones keep their lo part); K from memory to
 // registers, V through the wave's own 32 rows of LDS, read transposed.
 //   What a row must not see: scores by select; where a tile that some row does
 // not see in whole holds values that are no number (0 x NaN), they count as 0 in
