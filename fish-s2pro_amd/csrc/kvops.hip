@@ -39,6 +39,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int intx4 __attribute__((ext_vector_type(4)));
 
 // Sum over lanes 0 .. l of the wave (all 64 active): shifts by 1, 2, 4, 8 within
 // each 16 lanes, then their last lanes' sums to the rows behind them.
@@ -152,7 +153,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvAppendArgs a) {
 
 // m follows a row's maximum only when it is SLACK behind: weights stay below
 // 2^SLACK and the o registers are hardly ever rescaled.  It is a whole number, so
-// that taking it off and the factors between states round nothing.  f16 parts of
+// that taking it off and the factors between states round nothing, and each row's
+// goes by the keys that the row sees alone.  f16 parts of
 // weights are of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is
 // exact to 2^-25, 2^-31 of the largest.  The o of f32 values leave (and in
 // kv_step_kernel grow) times F32_DOWN: 65536 weights then add no more than the
@@ -501,12 +503,13 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 #pragma unroll
     for (int c = 1; c < NS; ++c) top = fmaxf(top, s[c]);
     const float mn = fmaxf(m, quarter_max(top));
-    if (__any(mn > m + SLACK)) {
-      const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - floorf(mn));
+    const bool up = mn > m + SLACK;
+    if (__any(up)) {
+      const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
 #pragma unroll
       for (int c = 0; c < OT; ++c) o[c] *= f;
       l *= f;
-      m = floorf(mn);
+      m = to;
     }
     const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
 #pragma unroll
@@ -663,9 +666,12 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 // holds one row (lane % 32).  q and the weights are hi + lo f16 parts, f16
 // caches as they are: two products each.
 //   f32 caches: keys and values are split into hi + lo f16 parts as they are
-// staged, scaled by a power of two per 8 keys (the 8 keys of four score
-// registers): three products, 2^-22 of each term, or 2^-39 of the largest value
-// of the run for terms far below it.  (The f32 matrix instructions do a
+// staged, each key's and each value's row scaled by a power of two of its own:
+// three products, 2^-22 of each term, or 2^-39 of the largest of its row.  A row
+// of o is in units of the largest value row that it has seen, so a term far below
+// is exact to 2^-39 of that.  No scale is shared with what a row does not see (one
+// for 8 keys, or for the rows of a wave, would let a later token's large value
+// take the low bits off the earlier ones').  (The f32 matrix instructions do a
 // sixteenth of the f16 ones' work per cycle.)
 //   Bound by the matrix units: 8 requests x 250 tokens over 1500 + 250 slots, f16,
 // 104 us (0.85 PFLOP/s of hi + lo products), 2048 tokens over 6000 430 us (1.1, at
@@ -674,6 +680,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 // takes 2.2, a third of it products: blocks are too few to hide the splitting.
 constexpr int TILE_ROWS = 128;
 constexpr float NO_STATE = -1.0f;  // in the place of l: no state here
+constexpr int NO_UNIT = -1000;     // of a row that has seen no value
 
 template <int HD, bool KH>
 __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit sp, float* stat) {
@@ -686,7 +693,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   constexpr uint32_t PR = HD * sizeof(T) / 16;            // 16-byte pieces of a row in memory
   constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
-  __shared__ float scales[2][2][4];  // f32: [buffer][K, V][8 keys]
+  __shared__ __align__(16) float k_scale[2][32];  // f32: [buffer][key], powers of two
+  __shared__ __align__(16) int v_exp[2][32];      // their exponents
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5;
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
@@ -703,10 +711,15 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
     for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
 
-  // f32: thread's pieces of a tile, of the wave's 8 keys: lane + 64 i
+  // f32: eight threads per key, 128 bytes of the row per load, in an order that keeps the writes to LDS of neighbouring
+  // keys in distinct banks
   u32x4 kr[KH ? 1 : LD], vr[KH ? 1 : LD];
-  auto key_of = [&](int i) { return 8 * wave + (lane + 64 * i) / PR; };
-  auto piece_of = [&](int i) { return (lane + 64 * i) % PR; };
+  const uint32_t key_f32 = 8 * wave + lane / 8;
+  auto piece_of = [&](int which, int i) {
+    uint32_t turn = HD == 128 ? (which ? 0u : key_f32 & 3u) : (which ? key_f32 : key_f32 ^ (key_f32 >> 1)) & 1u;
+    if (HD == 128 && !which) asm volatile("" : "+v"(turn));  // (worked out where it is used: addresses kept for the loop cost registers)
+    return lane % 8 + 8 * (uint32_t(i) ^ turn);
+  };
   // 16-byte piece p of row `key` stands at p ^ swz(key): keys' fragment reads take one piece of 8 rows in a row,
   // transposed value reads 64 bytes of 4 rows
   auto k_at = [](uint32_t key, uint32_t piece) { return key * RB + ((piece ^ (key & 7u)) << 4); };
@@ -724,11 +737,11 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       dma16(v, off + (v_at(key, x / 16 % PR) & (RB - 1)), lds0 + buf * BUF + PLANE + (wave * LD + i) * 1024);
     }
   };
-  auto load_f32 = [&](const Where<T>& w, const T* from, u32x4* r) {
+  auto load_f32 = [&](const Where<T>& w, const T* from, int which, u32x4* r) {
     const uint8_t* src = reinterpret_cast<const uint8_t*>(from);
-    const uint32_t stride = uint32_t(w.stride) * sizeof(T);
+    const uint32_t off = min(key_f32, w.keys - 1) * (uint32_t(w.stride) * uint32_t(sizeof(T)));
 #pragma unroll
-    for (int i = 0; i < LD; ++i) r[i] = *reinterpret_cast<const u32x4*>(src + (min(key_of(i), w.keys - 1) * stride + piece_of(i) * 16));
+    for (int i = 0; i < LD; ++i) r[i] = *reinterpret_cast<const u32x4*>(src + (off + piece_of(which, i) * 16));
   };
   auto store_f32 = [&](uint32_t buf, int which, const u32x4* r) {
     uint8_t* base = lds + buf * BUF;
@@ -739,8 +752,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
       for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]));
     }
-    big = wave_max(big);
-    if (!(big < INFINITY)) {  // the largest number, then
+    if (__any(!(big < INFINITY))) {  // the largest number, then
       big = 0.0f;
 #pragma unroll
       for (int i = 0; i < LD; ++i) {
@@ -748,17 +760,24 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
         for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[e]) < INFINITY ? fabsf(x[e]) : 0.0f);
       }
-      big = wave_max(big);
     }
+    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
+    big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
+    big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
     float scale, inv;
     pow2_scale(big, scale, inv);
-    if (lane == 0) scales[buf][which][wave] = scale;
+    if (lane % 8 == 0) {
+      if (which)
+        v_exp[buf][key_f32] = int(__float_as_uint(scale) >> 23) - 127;
+      else
+        k_scale[buf][key_f32] = scale;
+    }
 #pragma unroll
     for (int i = 0; i < LD; ++i) {
       const floatx4 x = __builtin_bit_cast(floatx4, r[i]) * inv;
       const half4 hi = __builtin_convertvector(x, half4);
       const half4 lo = __builtin_convertvector(x - __builtin_convertvector(hi, floatx4), half4);
-      const uint32_t p = piece_of(i), off = (which ? v_at(key_of(i), p / 2) : k_at(key_of(i), p / 2)) + 8 * (p % 2);
+      const uint32_t p = piece_of(which, i), off = (which ? v_at(key_f32, p / 2) : k_at(key_f32, p / 2)) + 8 * (p % 2);
       *reinterpret_cast<half4*>(base + 2 * which * PLANE + off) = hi;
       *reinterpret_cast<half4*>(base + (2 * which + 1) * PLANE + off) = lo;
       __builtin_amdgcn_sched_barrier(0);
@@ -768,8 +787,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     if constexpr (KH) {
       load(w, 0);
     } else {
-      load_f32(w, w.k, kr);
-      load_f32(w, w.v, vr);
+      load_f32(w, w.k, 0, kr);
+      load_f32(w, w.v, 1, vr);
     }
   };
 
@@ -833,8 +852,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
   for (int i = 0; i < DT; ++i) o[i] = floatx16{};
   float m = -INFINITY, l = 0.0f;
-  uint32_t unit = 0;  // f32: o is in units of this (its bits)
-  auto quotient = [](uint32_t p, uint32_t q) { return __uint_as_float(uint32_t(max(int(p - q + 0x3f800000u), 0))); };
+  int unit = NO_UNIT;  // f32: the row's o is in units of 2^unit
   uint32_t seg = 0;
   auto where = [&](uint32_t i) { return i < n_pre ? prefix_tile<T, KT>(a.c, g, p_lo + i) : own_tile<T, KT>(a.c, run, g, o_lo + (i - n_pre), seg); };
   Where<T> w{};
@@ -857,8 +875,8 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       if (more) load(next, buf ^ 1u);
     } else {
       if (more) {
-        load_f32(next, next.k, kr);
-        load_f32(next, next.v, vr);
+        load_f32(next, next.k, 0, kr);
+        load_f32(next, next.v, 1, vr);
       }
     }
     const int limit = !live ? -1 : w.seg < 0 ? int(a.c.P) - 1 : uint32_t(w.seg) == own_rows >> 16 ? int(own_rows & 0xffffu) : -1;
@@ -914,7 +932,14 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (!KH) s[0] += s_lo;
+        if constexpr (!KH) {  // (the scales with the query's own, all powers of two)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const floatx4 ks = *reinterpret_cast<const floatx4*>(&k_scale[buf][8 * c + 4 * h2]) * unscale;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0][4 * c + e] = (s[0][4 * c + e] + s_lo[4 * c + e]) * ks[e];
+          }
+        }
       }
       const bool whole = __all(limit >= int(w.key0) + KT - 1);
       if (!whole) {
@@ -924,7 +949,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           for (int v = 0; v < 16; ++v)
             if (int(w.key0) + int(32u * sub + 8u * (v / 4) + 4u * h2 + (v % 4)) > limit) s[sub][v] = -INFINITY;
       }
-      float factor[4], top = -INFINITY;  // factor: of the 8 keys of four scores
+      float top = -INFINITY;
       if constexpr (KH) {
         float top1 = -INFINITY;
 #pragma unroll
@@ -933,41 +958,42 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
           top1 = fmaxf(fmaxf(top1, s[NSUB - 1][v]), s[NSUB - 1][v + 1]);
         }
         top = fmaxf(top, top1) * unscale;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) factor[c] = unscale;
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          factor[c] = unscale * scales[buf][0][c];
-          top = fmaxf(top, fmaxf(fmaxf(s[0][4 * c], s[0][4 * c + 1]), fmaxf(s[0][4 * c + 2], s[0][4 * c + 3])) * factor[c]);
-        }
+        for (int v = 0; v < 16; v += 2) top = fmaxf(fmaxf(top, s[0][v]), s[0][v + 1]);
       }
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
-      if (__any(mn > m + SLACK)) {
-        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - floorf(mn));
+      const bool up = mn > m + SLACK;
+      if (__any(up)) {
+        const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
         l *= f;
-        m = floorf(mn);
+        m = to;
       }
       const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
-      float ratio[4];
       if constexpr (!KH) {
-        // (all powers of two, and quotients by their exponents: 0 below the normal numbers)
-        uint32_t vs[4], most = 0;
+        int most = NO_UNIT;
+        if (whole) {  // a key per lane
+          most = int(wave_reduce(uint32_t(v_exp[buf][r32]), [](uint32_t p, uint32_t q) { return uint32_t(max(int(p), int(q))); }));
+        } else {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          vs[c] = uniform(__float_as_uint(scales[buf][1][c]));
-          most = max(most, vs[c]);
+          for (int c = 0; c < 4; ++c) {
+            const intx4 ve = *reinterpret_cast<const intx4*>(&v_exp[buf][8 * c + 4 * h2]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) most = max(most, int(w.key0) + int(8u * c + 4u * h2 + e) <= limit ? ve[e] : NO_UNIT);
+          }
+          const auto both = __builtin_amdgcn_permlane32_swap(uint32_t(most), uint32_t(most), false, false);
+          most = max(int(both[0]), int(both[1]));
         }
-        if (most > unit) {
-          const float f = quotient(unit, most);
+        most = max(most, unit);
+        if (__any(most > unit)) {
+          const float f = __builtin_amdgcn_ldexpf(1.0f, unit - most);
 #pragma unroll
           for (int d = 0; d < DT; ++d) o[d] *= f;
           unit = most;
         }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) ratio[c] = quotient(vs[c], unit);
+        asm volatile("" ::: "memory");  // (the exponents are read again, not kept)
       }
       int odd = 0;  // a value that is no number, and rows that must not see it
       if (!whole && w.seg >= 0) {
@@ -986,12 +1012,14 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
       for (int sub = 0; sub < NSUB; ++sub) {
         half8 ph[2], pl[2];  // 16 keys each: the weights' upper 11 bits, and the rest
         float sum[2] = {0.0f, 0.0f};
+        intx4 ve;
 #pragma unroll
         for (int v = 0; v < 16; ++v) {
-          float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], factor[v / 4], bias));
+          if (!KH && v % 4 == 0) ve = *reinterpret_cast<const intx4*>(&v_exp[KH ? 0 : buf][8 * (v / 4) + 4 * h2]);
+          float p = __builtin_amdgcn_exp2f(KH ? fmaf(s[sub][v], unscale, bias) : s[sub][v] + bias);
           sum[v % 2] += p;
           s[sub][v] = p;
-          if constexpr (!KH) p *= ratio[v / 4];
+          if constexpr (!KH) p = __builtin_amdgcn_ldexpf(p, ve[v % 4] - unit);  // (0 of a key that the row does not see)
           const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
           ph[v / 8][v % 8] = _Float16(hi);
           pl[v / 8][v % 8] = _Float16(p - hi);
@@ -1000,7 +1028,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
         if constexpr (!KH) asm volatile("" : "+v"(l));  // (here, or the sums hold all the weights' registers to the end)
         int slow = __builtin_amdgcn_readfirstlane(odd);
         if (slow) {  // key by key, for the rows that see it
-          const float per_unit = KH ? 1.0f : quotient(0x3f800000u, unit);
+          const float per_unit = KH ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, -unit);
           for (int key = 0; key < 32 && 32 * sub + key < int(w.keys); ++key) {
             float p = 0.0f;
 #pragma unroll
@@ -1069,7 +1097,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
-  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : KH ? 1.0f : F32_DOWN) * (KH ? 1.0f : __uint_as_float(unit));
+  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : KH ? 1.0f : F32_DOWN) * (KH ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, unit));
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll

@@ -477,14 +477,16 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * 0 .. lens[b] - new_lens[b] + t; query head h reads kv head h / (heads /
  * kv_heads).  out like q; rows of tokens t >= new_lens[b] stay as they were.
  * What a token does not see (later slots, other requests, slots not in use)
- * never reaches its row, whatever bits stand there; an infinity or NaN that it
- * sees makes the elements of its row that it takes part in no number.  The
- * shared prefix is read once for several requests' queries.  out must not
- * overlap q.
+ * never reaches its row, whatever bits stand there (of numbers its row does not
+ * change a bit; where infinities or NaN stand, its last bits may be rounded
+ * another way); an infinity or NaN that it sees makes the elements of its row
+ * that it takes part in no number.  The shared prefix is read once for several
+ * requests' queries.  out must not overlap q.
  *   Products and sums are f32 or better, except for calls of many tokens over
  * f32 caches: there each term is exact to 2^-22, or to 2^-39 of the largest
- * value among the keys that its block of rows reads.  Values of f32 caches
- * below 2^-80 may count as 0. */
+ * element of the key, the value and the query that it comes from and of the
+ * values that its token sees.  Values of f32 caches below 2^-80 may count as
+ * 0. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                         void* stream, char* err, size_t err_cap);
 /* s2hip_kv_attend, and for every slot s < lens[b] of every kv head g

@@ -975,3 +975,43 @@ def test_append_norm_of_extreme_rows(size):
     want = qkv * torch.rsqrt((qkv * qkv).mean(-1, keepdim=True) + 1e-6)
     assert bool(((q - want[:, :, :H]).abs() <= 2.0**-20 * want[:, :, :H].abs()).all())
     assert torch.equal(v[:, :, :3].transpose(1, 2), qkv[:, :, H + G :]) and ops.errors(stream()) == 0
+
+
+def weigh(b, prefix=True):
+    """(weights, prefix weights) of the batch's call, from zero; out in b.out."""
+    w, pw = torch.zeros(b.R, b.G, b.cap, device="cuda"), torch.zeros(b.G, max(b.P, 1), device="cuda")
+    b.out.fill_(7.0)
+    b.ops.attend_weigh(b.view(), ptr(b.q), b.n, ptr(b.out), ptr(w), prefix_weights_out=ptr(pw) if prefix and b.P else 0, stream=stream())
+    torch.cuda.synchronize()
+    return w, pw
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("size", [2.0**20, 2.0**38, 1e30, 3e38])
+@pytest.mark.parametrize("hd,n", [(64, 1), (128, 1), (64, 40), (128, 40), (128, 150)])
+def test_attend_does_not_see_large_values(hd, n, size, f16, room):
+    """Finite keys and values far above the others in later tokens' slots, in
+    slots not in use and in other requests' caches: the rows that do not see
+    them keep their bits."""
+    size = min(size, 6e4) if f16 else size
+    b = Batch((8, 2, hd), f16, [n + 21, n, 30, n + 43], [n, n, 0, n], cap=room or n + 64, prefix=50, seed=n)
+    want = b.expect()
+    clean = b.attend().clone()
+    b.check(clean, want)
+    g = gen(99)
+    for r, used in enumerate(b.lens_h):
+        b.k[r, :, used:] = size
+        b.v[r, :, used:] = -size
+    b.k[2], b.v[2] = size, size
+    # the last tokens of requests 0 and 1 bring large keys and values, seen by their own rows alone
+    for r in (0, 1):
+        sign = torch.where(torch.rand(b.G, hd, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+        b.k[r, :, b.lens_h[r] - 1] = (sign * size).to(b.k.dtype)
+        b.v[r, :, b.lens_h[r] - 1] = (-sign * size).to(b.v.dtype)
+    b.out.fill_(7.0)
+    out = b.attend().clone()
+    for r in (0, 1):
+        out[r, n - 1] = clean[r, n - 1]
+    b.check(out, want)
+    assert torch.equal(out, clean)
