@@ -1247,7 +1247,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
     // the wave's keys: key 32 kw + r32, dims 16 ks + 8 h2 + e
     const uint32_t key0 = k0 + wave * 32 * KW;
     half8 kh[KW][DS], kl[KH ? 1 : KW][DS];
-    float key_scale[4] = {1.0f, 1.0f, 1.0f, 1.0f};  // f32: of 8 keys each
+    float key_scale[KH ? 1 : 16];  // f32: a power of two of each key's own (one for several would let a later key take the low bits off earlier ones)
 #pragma unroll
     for (int kw = 0; kw < KW; ++kw) {
       const size_t stride = prefix ? a.c.p_slot_stride : a.c.slot_stride;
@@ -1271,13 +1271,10 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
             }
           }
         big = half_reduce(big, [](float p, float q) { return fmaxf(p, q); });
-        big = fmaxf(big, dpp_f32<DPP_QUAD_XOR1>(big));
-        big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
-        big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
         float r, inv;
         pow2_scale(big, r, inv);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) key_scale[c] = lane_read_f32(r, 8 * c);
+        for (int v = 0; v < 16; ++v) key_scale[v] = __shfl(r, 8 * (v / 4) + 4 * int(h2) + v % 4, 64);
 #pragma unroll
         for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
@@ -1416,7 +1413,7 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
       for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], me.x * key_scale[v / 4], -me.y)), me.z, sum[kw][v]);
+          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], KH ? me.x : me.x * key_scale[v], -me.y)), me.z, sum[kw][v]);
       __syncthreads();
     }
 #pragma unroll

@@ -1015,3 +1015,29 @@ def test_attend_does_not_see_large_values(hd, n, size, f16, room):
         out[r, n - 1] = clean[r, n - 1]
     b.check(out, want)
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("size", [2.0**20, 2.0**38, 1e30])
+@pytest.mark.parametrize("hd,n", [(64, 1), (128, 3), (64, 50), (128, 50), (128, 150)])
+def test_weigh_does_not_see_large_keys(hd, n, size, f16, room):
+    """Large keys in the last tokens' slots, in slots not in use and in an idle
+    request's cache: the weights that the tokens before them give are those
+    without.  (The last tokens' queries are zeros, so that theirs are known.)"""
+    size = min(size, 6e4) if f16 else size
+    b = Batch((8, 2, hd), f16, [n + 21, n, 30, n + 43], [n, n, 0, n], cap=room or n + 64, prefix=50, seed=n)
+    g = gen(99)
+    for r in range(4):
+        b.q[r, n - 1] = 0
+        b.k[r, :, b.lens_h[r] :] = size
+        if r != 3:
+            sign = torch.where(torch.rand(b.G, hd, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+            b.k[r, :, b.lens_h[r] - 1] = (sign * size).to(b.k.dtype)
+    b.k[2] = size
+    want = b.expect()
+    w, pw = weigh(b)
+    b.check(b.out, want)
+    used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+    assert bool(((w.double() - want[2]).abs() <= want[3] + U * want[2])[used].all())
+    assert bool(((pw.double() - want[4]).abs() <= want[5] + U * want[4]).all())
