@@ -1149,8 +1149,9 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
         done |= s0 + i * TEAM == 0;
         continue;
       }
-      if (ml[i].x == -INFINITY) {  // no key, or none but of no number
+      if (ml[i].x == -INFINITY) {  // no key (zeros), or none but of no number
         x += y[i];
+        L += ml[i].y;
         continue;
       }
       const float mn = fmaxf(M, ml[i].x);

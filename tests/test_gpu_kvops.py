@@ -1041,3 +1041,22 @@ def test_weigh_does_not_see_large_keys(hd, n, size, f16, room):
     used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
     assert bool(((w.double() - want[2]).abs() <= want[3] + U * want[2])[used].all())
     assert bool(((pw.double() - want[4]).abs() <= want[5] + U * want[4]).all())
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 50, 130])
+def test_weigh_splits_of_no_number(n, f16, room):
+    """Keys of no number that fill whole splits of the work: the rows that see
+    them give no key a weight that is a number."""
+    b = Batch((8, 2, 128), f16, [n + 21, n], [n, n], cap=room or n + 64, prefix=2500, seed=n)
+    want = b.expect()
+    b.pk[0] = math.nan
+    w, pw = weigh(b)
+    half = b.H // b.G
+    assert bool(b.out[:, :, :half].isnan().all())
+    assert bool(w[0, 0, : n + 21].isnan().all()) and bool(w[1, 0, :n].isnan().all()) and bool(pw[0].isnan().all())
+    b.out[:, :, :half] = want[0][:, :, :half].float()
+    b.check(b.out, want)
+    assert bool(((w[:, 1].double() - want[2][:, 1]).abs() <= want[3][:, 1]).all())
+    assert bool(((pw[1].double() - want[4][1]).abs() <= want[5][1]).all())
