@@ -192,6 +192,20 @@ __device__ __forceinline__ void pow2_scale(float max, float& r, float& inv) {
   inv = __uint_as_float((254u - x) << 23);
 }
 
+// hi + lo parts of a query's element, below 2^14.  AWAY (f16 keys): hi is rounded away
+// from 0, so that lo has the other sign or is 0, and an infinity of a key gives
+// inf - inf or 0 x inf, no number, whichever its sign; lo, below 2^-10 then, is exact
+// to 2^-22 of the element instead of 2^-23.  (The lo part of an f32 key's infinity is
+// no number as it is.)
+struct Parts {
+  _Float16 hi, lo;
+};
+template <bool AWAY>
+__device__ __forceinline__ Parts split_query(float x) {
+  const float hi = AWAY ? __uint_as_float((__float_as_uint(x) + 0x1fffu) & 0xffffe000u) : float(_Float16(x));
+  return {_Float16(hi), _Float16(x - hi)};
+}
+
 // Eight halfs of a tile's transposed values: rows (keys) of `row_bytes` bytes in
 // LDS; lane i of 16 reads 8 bytes of row i / 4 and gets column i of four rows.
 typedef __attribute__((address_space(3))) uint8_t lds_byte;
@@ -419,9 +433,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
       for (int j = 0; j < HD / 32; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = x[2 * j + e / 4][e % 4] * inv;
-          qh[j][e] = _Float16(y);
-          ql[j][e] = _Float16(y - float(qh[j][e]));
+          const Parts y = split_query<true>(x[2 * j + e / 4][e % 4] * inv);
+          qh[j][e] = y.hi;
+          ql[j][e] = y.lo;
         }
     }
   }
@@ -466,8 +480,23 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
         x = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[2], qf[4 * j + 2], x, 0, 0, 0);
         y = __builtin_amdgcn_mfma_f32_16x16x4f32(k4[3], qf[4 * j + 3], y, 0, 0, 0);
       }
+      float z = 0.0f;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[c] = x[c] + y[c];
+      for (int c = 0; c < 4; ++c) {
+        s[c] = x[c] + y[c];
+        z = fmaf(s[c], 0.0f, z);
+      }
+      if (__any(!(z == 0.0f))) {  // keys that hold an infinity make theirs no number, whichever its sign (not so a sum beyond f32)
+        float big = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KL; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(__uint_as_float(kr[0][j][e])));
+        big = quarter_max(big);  // of key r16
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (__shfl(big, int(4 * q4) + c, 64) == INFINITY) s[c] = NAN;
+      }
     }
     if constexpr (KH) {  // the values go to LDS, their registers take the next tile's
       constexpr uint32_t PR = HD / 8;
@@ -641,7 +670,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
   const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
   if (last && !out_live) return;
   float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
-  const float inv = last ? (M_row == -INFINITY ? 0.0f : (KH ? 1.0f : F32_UP) / L_row) : 1.0f;
+  const float inv = last ? (M_row == -INFINITY ? NAN : (KH ? 1.0f : F32_UP) / L_row) : 1.0f;  // (it sees a key, its own)
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) {
     const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
@@ -842,9 +871,9 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float4 z = qx[ks][e / 4];
-        const float y = (e % 4 == 0 ? z.x : e % 4 == 1 ? z.y : e % 4 == 2 ? z.z : z.w) * inv;
-        qh[ks][e] = _Float16(y);
-        ql[ks][e] = _Float16(y - float(qh[ks][e]));
+        const Parts y = split_query<KH>((e % 4 == 0 ? z.x : e % 4 == 1 ? z.y : e % 4 == 2 ? z.z : z.w) * inv);
+        qh[ks][e] = y.hi;
+        ql[ks][e] = y.lo;
       }
   }
 
@@ -1097,7 +1126,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   if (at >= rows || (last && !live)) return;
   const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
-  const float f = (last ? (m == -INFINITY ? 0.0f : 1.0f / l) : KH ? 1.0f : F32_DOWN) * (KH ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, unit));
+  const float f = (last ? (m == -INFINITY ? NAN : 1.0f / l) : KH ? 1.0f : F32_DOWN) * (KH ? 1.0f : __builtin_amdgcn_ldexpf(1.0f, unit));
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -1183,7 +1212,7 @@ __device__ __forceinline__ void join_rows(const KvAttendArgs& a, const KvSplit& 
     M = all;
   }
   if (done || !is_row || t >= checked(a.c, raw, nullptr).fresh) return;
-  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? 1.0f : sp.up / L);
+  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? NAN : sp.up / L);
   if (stat && d == 0) {
     stat[2 * size_t(out)] = M;
     stat[2 * size_t(out) + 1] = L;

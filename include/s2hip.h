@@ -479,9 +479,10 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * What a token does not see (later slots, other requests, slots not in use)
  * never reaches its row, whatever bits stand there (of numbers its row does not
  * change a bit; where infinities or NaN stand, its last bits may be rounded
- * another way); an infinity or NaN that it sees makes the elements of its row
- * that it takes part in no number.  The shared prefix is read once for several
- * requests' queries.  out must not overlap q.
+ * another way).  An infinity or NaN in a value that it sees makes that element
+ * of its row no number, in a key all of them, with the weights that the row
+ * gives; so do scores that are all below the range of f32.  The shared prefix is
+ * read once for several requests' queries.  out must not overlap q.
  *   Products and sums are f32 or better, except for calls of many tokens over
  * f32 caches: there each term is exact to 2^-22, or to 2^-39 of the largest
  * element of the key, the value and the query that it comes from and of the

@@ -1060,3 +1060,47 @@ def test_weigh_splits_of_no_number(n, f16, room):
     b.check(b.out, want)
     assert bool(((w[:, 1].double() - want[2][:, 1]).abs() <= want[3][:, 1]).all())
     assert bool(((pw[1].double() - want[4][1]).abs() <= want[5][1]).all())
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+@pytest.mark.parametrize("n", [1, 3, 40, 150])
+def test_attend_sees_infinite_key(n, bad, f16, room):
+    """A key that holds an infinity makes the rows that see it no number, with
+    either sign of its score, and the weights of the keys that they see; no others."""
+    b = Batch((8, 2, 128), f16, [n + 21, n, 30, n + 40], [n, n, 0, n], cap=room or n + 64, prefix=50, seed=n)
+    want = b.expect()
+    b.k[0, 1, n + 20, 5] = bad  # request 0's last token alone sees it
+    b.k[3, 0, 7, 100] = bad  # all of request 3's rows
+    half = b.H // b.G
+    for weighed in (False, True):
+        b.out.fill_(7.0)
+        if weighed:
+            w, pw = weigh(b)
+        out = b.out.clone() if weighed else b.attend().clone()
+        assert bool(out[0, n - 1, half:].isnan().all()) and bool(out[3, :, :half].isnan().all())
+        out[0, n - 1, half:], out[3, :, :half] = want[0][0, n - 1, half:].float(), want[0][3, :, :half].float()
+        b.check(out, want)
+    assert bool(w[0, 1, : n + 21].isnan().all()) and bool(w[3, 0, : n + 40].isnan().all()) and bool(pw.isnan().all())
+    for r, j in ((0, 0), (1, 0), (1, 1), (3, 1)):
+        assert bool(((w[r, j].double() - want[2][r, j]).abs() <= want[3][r, j]).all())
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n", [1, 2, 33, 150])
+def test_attend_sees_infinite_keys_alone(n, f16, room):
+    """Rows all of whose scores are -infinity are no number, and so are the weights; the one-slot row among them."""
+    b = Batch((8, 2, 64), f16, [n, n], [n, n], cap=room, seed=n)
+    want = b.expect()
+    b.q[0].abs_()
+    b.k[0] = 0.0
+    b.k[0, :, :, 3] = -math.inf
+    out = b.attend().clone()
+    assert bool(out[0].isnan().all())
+    out[0] = want[0][0].float()
+    b.check(out, want)
+    w, _ = weigh(b)
+    assert bool(b.out[0].isnan().all()) and bool(w[0, :, :n].isnan().all())
+    assert bool(((w[1].double() - want[2][1]).abs() <= want[3][1]).all())
