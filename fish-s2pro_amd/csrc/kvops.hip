@@ -183,11 +183,13 @@ __device__ __forceinline__ float half_reduce(float x, Op op) {
   return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// a power of two r with max / r in [2^13, 2^14), and 1 / r; at least 2^-62, so
-// that the product of two is a normal number
+// a power of two r with max / r in [2^13, 2^14), and 1 / r; at least 2^LEAST.
+// (Queries and keys: what the product of two such scales loses is of scores below
+// 2^-80.  Values: times F32_DOWN and over a sum of weights it is a normal number.)
+template <int LEAST = -126>
 __device__ __forceinline__ void pow2_scale(float max, float& r, float& inv) {
   const int e = int((__float_as_uint(max) >> 23) & 255u) - 13;
-  const uint32_t x = uint32_t(e < 65 ? 65 : e);
+  const uint32_t x = uint32_t(e < LEAST + 127 ? LEAST + 127 : e);
   r = __uint_as_float(x << 23);
   inv = __uint_as_float((254u - x) << 23);
 }
@@ -794,7 +796,10 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
     big = fmaxf(big, dpp_f32<DPP_QUAD_XOR2>(big));
     big = fmaxf(big, dpp_f32<DPP_ROW_HALF_MIRROR>(big));
     float scale, inv;
-    pow2_scale(big, scale, inv);
+    if (which)
+      pow2_scale<-85>(big, scale, inv);
+    else
+      pow2_scale(big, scale, inv);
     if (lane % 8 == 0) {
       if (which)
         v_exp[buf][key_f32] = int(__float_as_uint(scale) >> 23) - 127;
@@ -1442,8 +1447,8 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 #pragma unroll
       for (int kw = 0; kw < KW; ++kw)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], KH ? me.x : me.x * key_scale[v], -me.y)), me.z, sum[kw][v]);
+        for (int v = 0; v < 16; ++v)  // (a factor of 0 would make the -infinity of a key that is not seen NaN)
+          sum[kw][v] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[kw][v], KH ? me.x : fmaxf(me.x * key_scale[v], 0x1p-126f), -me.y)), me.z, sum[kw][v]);
       __syncthreads();
     }
 #pragma unroll

@@ -1104,3 +1104,34 @@ def test_attend_sees_infinite_keys_alone(n, f16, room):
     w, _ = weigh(b)
     assert bool(b.out[0].isnan().all()) and bool(w[0, :, :n].isnan().all())
     assert bool(((w[1].double() - want[2][1]).abs() <= want[3][1]).all())
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("up", [-76, -100, 60, 100])
+@pytest.mark.parametrize("n", [1, 50, 150])
+def test_attend_small_keys_large_queries(n, up, room):
+    """f32 caches: queries times 2^up over keys times 2^-up, and values that small: as without."""
+    b = Batch((8, 2, 128), False, [n + 60, n + 5], [n, n], cap=room, prefix=150, seed=9)
+    clean = b.expect()
+    b.q.mul_(2.0**up)
+    b.k.mul_(2.0**-up)
+    b.pk.mul_(2.0**-up)
+    w, pw = weigh(b)
+    b.check(b.out, clean)
+    b.check(b.attend(), clean)
+    assert bool(((w.double() - clean[2]).abs() <= clean[3] + U * clean[2]).all())
+    assert bool(((pw.double() - clean[4]).abs() <= clean[5] + U * clean[4]).all())
+
+
+@pytest.mark.parametrize("room", ROOM)
+@pytest.mark.parametrize("up", [-74, -60, 100])
+@pytest.mark.parametrize("n", [1, 50, 150])
+def test_attend_values_of_any_size(n, up, room):
+    """f32 caches: values times 2^up give outputs times 2^up."""
+    b = Batch((8, 2, 128), False, [n + 60, n + 5], [n, n], cap=room, prefix=150, seed=9)
+    want = b.expect()
+    b.v.mul_(2.0**up)
+    b.pv.mul_(2.0**up)
+    out = b.attend()
+    live = torch.arange(n, device="cuda")[None] < b.new[:, None]
+    b.check(torch.where(live[:, :, None, None], out * 2.0**-up, out), want)
