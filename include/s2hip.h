@@ -462,7 +462,9 @@ int32_t s2hip_kv_errors(s2hip_kv* kv, void* stream, uint32_t* bits, char* err, s
  * [head_dim] (both or neither) each q and k head y becomes y / sqrt(mean(y^2)
  * + eps) * gain; then the pairs (2 i, 2 i + 1) turn by positions[b][t] *
  * rope_base^(-2 i / head_dim) (apply_rope_normal, attention.rs:172-206; angles
- * in 64 bits).  q_out [requests][n_tokens][heads head_dim]; token t's key and
+ * in 64 bits.  The engine and s2hip_op_qk_rope take the reference's f32 angles,
+ * off by up to 2^-23 of the angle: at far positions their keys differ from these,
+ * so a cache is filled by one of the two).  q_out [requests][n_tokens][heads head_dim]; token t's key and
  * value go to slot lens[b] - new_lens[b] + t.  scores and slot_positions
  * (nullable, [requests][kv_heads][capacity]): there the slot's score becomes 0
  * and its position the token's.  Positions need not be the slots: after an
@@ -483,11 +485,15 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * of its row no number, in a key all of them, with the weights that the row
  * gives; so do scores that are all below the range of f32.  The shared prefix is
  * read once for several requests' queries.  out must not overlap q.
- *   Products and sums are f32 or better, except for calls of many tokens over
- * f32 caches: there each term is exact to 2^-22, or to 2^-39 of the largest
- * element of the key, the value and the query that it comes from and of the
- * values that its token sees.  Values of f32 caches below 2^-80 may count as
- * 0. */
+ *   Products and sums are f32 or better, but for f32 caches where each request
+ * brings 32 rows or more to a kv head (n_tokens heads / kv_heads: one token of 32
+ * heads over one does) and the capacities make a call large, and for the weights
+ * of calls whose scores are too many to be kept (by rows and capacities; a step
+ * over large caches can be one): there each term is exact to 2^-22, or to 2^-39
+ * of the largest element of the key, the value and the query that it comes from
+ * and of the values that its token sees.  Values of f32 caches below 2^-80 may
+ * count as 0.  Which kernels run, and so the last bits, goes by the view's
+ * capacities and prefix_len, not only by the lengths in use. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                         void* stream, char* err, size_t err_cap);
 /* s2hip_kv_attend, and for every slot s < lens[b] of every kv head g

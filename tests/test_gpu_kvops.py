@@ -1135,3 +1135,30 @@ def test_attend_values_of_any_size(n, up, room):
     out = b.attend()
     live = torch.arange(n, device="cuda")[None] < b.new[:, None]
     b.check(torch.where(live[:, :, None, None], out * 2.0**-up, out), want)
+
+
+@pytest.mark.parametrize("cap", [130, 32768])
+@pytest.mark.parametrize("f16", [False, True])
+def test_one_token_of_many_heads(f16, cap):
+    """One token of 32 and of 64 heads over one: as many rows as a turn, in caches of the lengths' size and in large ones."""
+    for H, lens in (((64, 2, 64), [101, 1, 130]), ((64, 1, 128), [40, 77, 9])):
+        b = Batch(H, f16, lens, [1] * 3, cap=cap, prefix=300, seed=31)
+        want = b.expect()
+        b.check(b.attend(), want)
+        w, pw = weigh(b)
+        b.check(b.out, want)
+        used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+        assert bool(((w.double() - want[2]).abs() <= want[3] + U * want[2])[used].all())
+        assert bool(((pw.double() - want[4]).abs() <= want[5] + U * want[4]).all())
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_step_weights_computed_once_more(f16):
+    """A step in caches so large that its scores are not kept."""
+    b = Batch((32, 2, 64), f16, [1 + 9 * r for r in range(33)], [1] * 33, cap=32768, prefix=257, seed=32)
+    want = b.expect()
+    w, pw = weigh(b)
+    b.check(b.out, want)
+    used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
+    assert bool(((w.double() - want[2]).abs() <= want[3] + U * want[2])[used].all())
+    assert bool(((pw.double() - want[4]).abs() <= want[5] + U * want[4]).all())
