@@ -322,8 +322,9 @@ __device__ __forceinline__ Where<T> own_tile(const KvCaches& c, const Run& r, ui
 //   Bound by latency, then by memory: 8 requests over 1500 shared and 512 own
 // slots, f32, take 12.7 us, 6 of them start and end (3 to the requests' lengths
 // and the first keys, 3 the joining in LDS), the rest 39 MB; 16 over 24001 + 2000,
-// f16, 49 us: 200 MB from memory, 520 MB (10.7 TB/s) past the second-level cache,
-// for four row tiles read the prefix.  Two row tiles a wave, which halve that,
+// f16, 55 us (49 where the last-level cache still holds the keys): 200 MB from
+// memory, 520 MB (9.5 TB/s) past the second-level cache, for four row tiles read
+// the prefix.  Two row tiles a wave, which halve that,
 // take 8 % off this call and put 10 to 60 % on shorter ones.
 constexpr int STEP_WAVES = 4;
 
@@ -704,11 +705,15 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void kv_step_kernel(KvAttendArg
 // for 8 keys, or for the rows of a wave, would let a later token's large value
 // take the low bits off the earlier ones').  (The f32 matrix instructions do a
 // sixteenth of the f16 ones' work per cycle.)
-//   Bound by the matrix units: 8 requests x 250 tokens over 1500 + 250 slots, f16,
-// 104 us (0.85 PFLOP/s of hi + lo products), 2048 tokens over 6000 430 us (1.1, at
-// the 1.66 GHz that the clock falls to; a library's f16 product of 8192^3 reaches
-// 1.2 to 1.3).  f32, 3 x 37 over 1001 + 131: 26 us, of which a tile of 32 keys
-// takes 2.2, a third of it products: blocks are too few to hide the splitting.
+//   8 requests x 250 tokens over 1500 + 250 slots, f16, take 104 us (0.85 PFLOP/s of
+// hi + lo products), the matrix units busy for 34 % of it and the vector ones for
+// 26 %: a wave's products and its softmax follow one another, and the two blocks of a
+// CU do not fill each other's gaps.  2048 tokens over 6000, 430 us (1.1 PFLOP/s), keep
+// the matrix units busy for 61 % at the 1.66 GHz that the clock falls to; a library's
+// f16 product of 8192^3 reaches 1.2 to 1.3.  f32, 3 x 37 over 1001 + 131: 27 us, of
+// which a tile of 32 keys takes 2.2, a third of it products: blocks are too few to
+// hide the splitting.  A prompt of 1500 tokens, f32: 104 us, 34 % vector and 23 %
+// matrix cycles.
 constexpr int TILE_ROWS = 128;
 constexpr float NO_STATE = -1.0f;  // in the place of l: no state here
 constexpr int NO_UNIT = -1000;     // of a row that has seen no value
@@ -1240,7 +1245,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvAttendArgs a, KvSplit sp
 // sum has one order.  blockIdx.z = request, or R for the prefix with the rows of
 // all requests; with several row splits the sums go to the workspace and
 // kv_weights_join_kernel adds them.
-//   A prompt of 1500 tokens, f16: 37 us, 0.58 PFLOP/s of hi + lo products; vector
+//   A prompt of 1500 tokens, f16: 38 us, 0.57 PFLOP/s of hi + lo products; vector
 // instructions (a step splits 32 rows and takes 64 exponentials a lane pair) take
 // as many cycles as the products.
 struct RowSteps {
@@ -1485,8 +1490,9 @@ __global__ __launch_bounds__(256, 2) void kv_weigh_kernel(KvAttendArgs a, const 
 // 8 requests of 1500 slots, f32, 23 : 40; 4 of 20000, f16, 70 : 95; 8 x 14 tokens
 // of 8 heads over 2 after 666 positions 15 : 23, 12 x 4 of 32 over 8 after 2900
 // 33 : 45, 1 x 139 18 : 23, 7 x 67 21 : 28; with shared positions 8 x 62 (1984 rows)
-// over 11 31 : 38, 4 x 100 of 8 over 2 (1600) over 1500 32 : 28, 8 x 83 (2656) over 3
-// 24 : 22.
+// over 11 27 : 34, 4 x 100 of 8 over 2 (1600) over 1500 36 : 38, 1 x 400 over 6000 82 : 80.
+// Heads of 64, whose products are half as long, lose by it from about 1000 rows over
+// shared positions on (4 x 100 over 1500 32 : 28): the rule goes by rows alone.
 constexpr uint32_t KEPT_ROWS = 2048;     // of a request and, for the prefix, of all, at most
 constexpr uint32_t KEPT_TEAM_ROWS = 32;  // from here on 16 lanes a key: 3 x 3 tokens of 14 heads over 2 after 2800 positions, 17 : 23 us a call
 struct KvKeptGrid {
@@ -1910,10 +1916,10 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   // are on the device), for the step kernel starts and ends quicker and the tile kernel multiplies quicker; heads of 64
   // count half.  Both with their join, us, step : tile, 32 heads over 8: f16 2 requests x 211 tokens over 110 + 452 slots
   // (6M scores) 21 : 29, 5 x 35 over 1500 + 78 (6.6M) 34 : 33, 4 x 64 over 1500 (13M) 37 : 39, 2 x 517 over 146 + 624 (17M)
-  // 52 : 43; f32 8 x 12 over 728 + 235 (3M) 22 : 32, 3 x 37 over 1001 + 768 (6M) 33 : 32, 2 x 445 over 10 + 616 (11M) 66 : 46.
+  // 52 : 43; f32 8 x 12 over 728 + 235 (3M) 22 : 33, 3 x 37 over 1001 + 768 (6M) 34 : 34, 2 x 445 over 10 + 616 (11M) 62 : 48.
   // Kept scores save the tile kernel's weights their products: f16 8 x 145 over 488 own slots (15M) 62 : 67, 8 x 174 (17M) 51 :
-  // 57, 4 x 142 of 24 over 1151 + 367 (20M) 80 : 66; f32 3 x 129 (3M) 24 : 43, 8 x 97 (8M) 39 : 47, 2 x 104 over 1500 + 239 (11M)
-  // 92 : 70.  A request of fewer than 32 rows would leave most of a tile's waves idle in its own cache.
+  // 57, 4 x 142 of 24 over 1151 + 367 (20M) 80 : 66; f32 3 x 129 (3M) 24 : 44, 8 x 97 (8M) 34 : 46, 2 x 104 over 1500 + 239 (11M)
+  // 87 : 72.  A request of fewer than 32 rows would leave most of a tile's waves idle in its own cache.
   const size_t scores = size_t(a.s.G) * rows * (a.c.P + a.c.cap - min(a.c.n, a.c.cap) / 2);
   const bool many = a.c.n * a.s.rep >= 32 && scores * hd > (may_keep ? f16 ? 14000000u : 8000000u : f16 ? 10000000u : 4200000u) * size_t(128);
   const uint32_t lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles), kt = many ? (f16 ? 64 : 32) : (f16 ? 32 : 16);
@@ -1930,7 +1936,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
   if (!many && most <= (a.w_out ? 20u : 24u * 128 / hd)) sp.splits = 1;
   if (many && lots > 256 && lots <= 448) {
     // More than a block per CU and less than two: row tiles of many keys in two, so that no CU has the two longest.
-    // A prompt of 1500 tokens (376 row tiles) 80 : 68 us with the join, f32 134 : 98; from 448 on the join costs what it saves.
+    // A prompt of 1500 tokens (376 row tiles) 80 : 69 us with the join, f32 153 : 105; from 448 on the join costs what it saves.
     sp.splits = 2;
     sp.least = 768 / kt;
   }
