@@ -730,7 +730,7 @@ __global__ __launch_bounds__(256, 2) void kv_tile_kernel(KvAttendArgs a, KvSplit
   constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
   __shared__ __align__(16) float k_scale[2][32];  // f32: [buffer][key], powers of two
-  __shared__ __align__(16) int v_exp[2][32];      // their exponents
+  __shared__ __align__(16) int v_exp[2][32];      // f32: the values' scales, by their exponents
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5;
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
