@@ -5,77 +5,20 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
 #include <memory>
 #include <stdexcept>
 #include <string>
 #include <vector>
 
+#include "kv_host.h"
 #include "kvops.h"
 #include "s2hip.h"
 
 namespace s2 {
 namespace {
 
-struct KvFailure : std::runtime_error {
-  explicit KvFailure(const std::string& m) : std::runtime_error(m) {}
-};
-void hipc(hipError_t e, const char* what) {
-  if (e != hipSuccess) throw KvFailure(std::string(what) + ": " + hipGetErrorString(e));
-}
-#define CHK(expr) hipc((expr), #expr)
-[[noreturn]] void kfail(const char* fmt, ...) __attribute__((format(printf, 1, 2)));
-void kfail(const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof buf, fmt, ap);
-  va_end(ap);
-  throw KvFailure(buf);
-}
-
 constexpr uint32_t KV_MAX_SLOTS = 32768, KV_MAX_REQUESTS = 256, KV_MAX_TOKENS = 65536, KV_MAX_REP = 64,
                    KV_MAX_HEADS = 1024, KV_MAX_LAYERS = 1024;
-
-// The handle's device for the length of a call; the caller's afterwards.
-class DeviceScope {
- public:
-  explicit DeviceScope(int device) {
-    CHK(hipGetDevice(&was_));
-    if (was_ != device) {
-      CHK(hipSetDevice(device));
-      moved_ = true;
-    }
-  }
-  ~DeviceScope() {
-    if (moved_) (void)hipSetDevice(was_);
-  }
-  DeviceScope(const DeviceScope&) = delete;
-  DeviceScope& operator=(const DeviceScope&) = delete;
-
- private:
-  int was_ = 0;
-  bool moved_ = false;
-};
-
-void need(const void* p, const char* name, size_t align) {
-  if (!p) kfail("kv: %s is NULL", name);
-  if (reinterpret_cast<uintptr_t>(p) % align) kfail("kv: %s is not aligned to %zu bytes", name, align);
-}
-void may(const void* p, const char* name, size_t align) {
-  if (p) need(p, name, align);
-}
-
-// n words from p and m words from q have one in common.
-bool meet(const void* p, size_t n, const void* q, size_t m) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
-  return x < y + 4 * m && y < x + 4 * n;
-}
-// out is in itself, or shares no word of `words` with it.
-void same_or_apart(const void* in, const void* out, size_t words, const char* name) {
-  if (in != out && meet(in, words, out, words)) kfail("kv: %s_out overlaps %s without being it", name, name);
-}
 
 // A dimension of the caches' layout.
 struct Dim {
@@ -94,7 +37,7 @@ void check_apart(Dim (&dims)[N], uint64_t row) {
   }
 }
 
-class KvOps {
+class KvOps : DeviceArrays {
  public:
   explicit KvOps(const s2hip_kv_config& c) {
     if (c.kv_heads == 0 || c.heads == 0 || c.heads % c.kv_heads)
@@ -244,18 +187,6 @@ class KvOps {
   }
 
  private:
-  struct Free {
-    void operator()(void* p) const { (void)hipFree(p); }
-  };
-  template <class T>
-  T* alloc(size_t n) {
-    void* p = nullptr;
-    CHK(hipMalloc(&p, n * sizeof(T)));
-    std::unique_ptr<void, Free> own(p);
-    owned_.push_back(std::move(own));
-    return static_cast<T*>(p);
-  }
-
   void stride(uint64_t n, const char* name) const {
     const uint64_t unit = cfg_.kv_f16 ? 8 : 4;
     if (n % unit) kfail("kv: %s %llu is not a multiple of 16 bytes", name, (unsigned long long)n);
@@ -318,7 +249,6 @@ class KvOps {
   s2hip_kv_config cfg_{};
   KvShape shape_{};
   KvWorkspace work_{};
-  std::vector<std::unique_ptr<void, Free>> owned_;  // freed also where the constructor throws
 };
 
 }  // namespace
@@ -327,27 +257,6 @@ class KvOps {
 struct s2hip_kv {
   std::unique_ptr<s2::KvOps> ops;
 };
-
-namespace {
-template <class F>
-int32_t kv_guarded(char* err, size_t cap, F&& f) {
-  const char* what = "unknown error";
-  try {
-    f();
-    return 1;
-  } catch (const std::exception& ex) {
-    if (err && cap) snprintf(err, cap, "%s", ex.what());
-    return 0;
-  } catch (...) {
-  }
-  if (err && cap) snprintf(err, cap, "%s", what);
-  return 0;
-}
-void kv_args(const s2hip_kv* kv, const void* view) {
-  if (!kv || !view) throw std::runtime_error("NULL argument");
-}
-hipStream_t as_stream(void* s) { return static_cast<hipStream_t>(s); }
-}  // namespace
 
 extern "C" {
 
