@@ -1,0 +1,78 @@
+// pages.h -- launch interface of the paged 4-bit KV cache (pages.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "kvops.h"
+
+namespace s2 {
+
+// A pool of pages and the rows that hold them.
+struct PgPool {
+  uint8_t* pool;
+  const int32_t* table;  // [R][width]
+  uint32_t shift;        // log2(page_tokens)
+  uint32_t pages, width;
+  uint32_t chunk;        // bytes of a kv head's part of a page
+};
+
+struct PgRope {
+  const double* turns;  // [dims / 2]: angles per position, in turns
+  double gain;
+  uint32_t dims, half;
+};
+
+struct PgAppendArgs {
+  KvShape s;
+  KvCaches c;  // lens, new_lens, R, n and cap (tokens)
+  PgPool p;
+  PgRope rope;
+  const float* qkv;
+  const int32_t* positions;
+  const float* q_norm;  // nullable, with k_norm
+  const float* k_norm;
+  float* q_out;
+  float* k_held;  // nullable
+  float* v_held;  // nullable
+};
+
+struct PgAttendArgs {
+  KvAttendArgs a;  // shape, lens, new_lens, R, n, cap, q, out
+  PgPool p;
+};
+
+struct PgUpdateArgs {
+  PgPool p;
+  const int32_t* lens;
+  const int32_t* source;  // nullable
+  const int32_t* keep;    // nullable
+  const int32_t* add;     // nullable
+  const int32_t* refs;
+  int32_t* refs_out;
+  int32_t* table_out;
+  int32_t* lens_out;
+  int32_t* used_out;  // compact
+  int32_t* moved_to;  // compact, nullable
+  size_t layer_stride;
+  uint32_t layers, R;
+  uint32_t* err;
+};
+
+struct PgWorkspace {
+  float* part;     // [cap_parts][16][hd]: attention states
+  float* part_ml;  // [cap_parts][16][2]
+  size_t cap_parts;
+  int32_t* refs;   // [pages]
+  int32_t* list;   // [2][pages]: free pages; holes and movers
+  int32_t* table;  // [max_requests][width]
+  int32_t* moves;  // [256][2]: pages that are copied, from and to; [0]: their number (compact)
+};
+
+hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s);
+hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& a, const PgWorkspace& w, hipStream_t s);
+hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s);
+hipError_t launch_pg_compact(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s);
+
+}  // namespace s2

@@ -93,6 +93,18 @@ class KvView(ctypes.Structure):
         (n, ctypes.c_uint32) for n in ("requests", "capacity", "prefix_len", "prefix_capacity")]
 
 
+class PagesConfig(ctypes.Structure):
+    _fields_ = [("device", ctypes.c_int32)] + [
+        (n, ctypes.c_uint32) for n in ("heads", "kv_heads", "head_dim", "page_tokens", "pages", "table_pages",
+                                       "max_requests", "max_tokens", "rope_dims", "rope_half")] + [
+        ("rope_base", ctypes.c_double), ("rope_gain", ctypes.c_double), ("rope_freq", ctypes.c_void_p),
+        ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class PagesView(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pool", "table", "lens", "new_lens")] + [("requests", ctypes.c_uint32)]
+
+
 _lib = None
 
 
@@ -206,6 +218,23 @@ def load():
     L.s2hip_kv_attend_weigh.argtypes = [vp, view, vp, u32, vp, vp, vp, vp, vp, vp, cp, sz]
     L.s2hip_kv_evict.argtypes = [vp, view, u32, ctypes.c_uint64, u32, u32, u32, vp, vp, vp, vp, vp, vp, cp, sz]
     for name in ("s2hip_kv_errors", "s2hip_kv_append", "s2hip_kv_attend", "s2hip_kv_attend_weigh", "s2hip_kv_evict"):
+        getattr(L, name).restype = i32
+    f64, u64 = ctypes.c_double, ctypes.c_uint64
+    view = ctypes.POINTER(PagesView)
+    L.s2hip_rope_frequencies.argtypes = [u32, f64, u32, f64, f64, f64, f64, vp, ctypes.POINTER(f64), cp, sz]
+    L.s2hip_pages_open.argtypes = [ctypes.POINTER(PagesConfig), cp, sz]
+    L.s2hip_pages_open.restype = vp
+    L.s2hip_pages_close.argtypes = [vp]
+    L.s2hip_pages_close.restype = None
+    L.s2hip_pages_bytes.argtypes = [vp]
+    L.s2hip_pages_bytes.restype = u64
+    L.s2hip_pages_errors.argtypes = [vp, vp, ctypes.POINTER(u32), cp, sz]
+    L.s2hip_pages_append.argtypes = [vp, view, vp, u32, vp, vp, vp, vp, vp, vp, vp, cp, sz]
+    L.s2hip_pages_attend.argtypes = [vp, view, vp, u32, vp, vp, cp, sz]
+    L.s2hip_pages_update.argtypes = [vp, view, u32, u64, vp, vp, vp, vp, vp, vp, vp, vp, cp, sz]
+    L.s2hip_pages_compact.argtypes = [vp, view, u32, u64, vp, vp, vp, vp, vp, vp, cp, sz]
+    for name in ("s2hip_rope_frequencies", "s2hip_pages_errors", "s2hip_pages_append", "s2hip_pages_attend",
+                 "s2hip_pages_update", "s2hip_pages_compact"):
         getattr(L, name).restype = i32
     _lib = L
     return L

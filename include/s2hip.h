@@ -9,8 +9,8 @@
  * NUL-terminated) into a caller-provided err buffer of err_cap bytes.
  * No HIP, torch or device types cross this boundary: inputs are caller-owned
  * host pointers and outputs go to caller-provided host buffers, except where an
- * entry point says that it takes device memory (the KV-cache operators, the
- * codec's _device call).
+ * entry point says that it takes device memory (the KV-cache operators, dense and
+ * in pages, the codec's _device call).
  *
  * Threading: a handle is not thread-safe; the caller serialises calls on one
  * handle, as the reference serialises InferenceEngine behind a Mutex
@@ -525,6 +525,146 @@ int32_t s2hip_kv_evict(s2hip_kv* kv, const s2hip_kv_view* view, uint32_t layers,
                        uint32_t recent, uint32_t sinks, const float* scores, const int32_t* positions,
                        float* scores_out, int32_t* positions_out, int32_t* lens_out, void* stream, char* err,
                        size_t err_cap);
+
+/* ---------------------------------------------------------------------------
+ * A KV cache in pages, keys and values in 4 bits: for callers that serve more or
+ * longer sessions than dense f16 caches leave room for, or many that begin alike.
+ * No counterpart in the reference (one sequence, one f32 cache: slow_ar.rs:372-438).
+ *
+ * A page holds page_tokens tokens of all kv heads of one layer; a pool is `pages`
+ * of them, one pool per layer, in the caller's memory.  A request is a row of the
+ * table: the numbers of its pages in order (the same in every layer), with its
+ * tokens in lens.  Requests may have pages in common; refs counts the rows that
+ * hold a page (and what else the caller counts in), 0: the page is free.
+ * Pointers, streams, captured graphs and the handle's workspace: as for s2hip_kv_*
+ * above.  lens, new_lens, tables and the rest are read on the device.
+ *
+ * Layout of a page: kv_heads parts of s2hip_pages_bytes / kv_heads bytes, each
+ *   key codes    [page_tokens][4][hd / 32] words: word (i, j) holds dims 32 j + 8 i
+ *                + e, the even e = 2 f in bits 4 f .., the odd e = 2 f + 1 in 16 + 4 f
+ *   value codes  [page_tokens / 16][4][16][hd / 32][4] bytes: byte (u, i, m, j, t)
+ *                holds dims 32 j + 2 m (low half) and 32 j + 2 m + 1 of token 16 u + 4 i + t
+ *   key scales   [page_tokens][hd / 32] f16
+ *   value scales [page_tokens / 16][4][hd / 32][4] f16: (u, i, j, t) as above
+ * 32 elements of a head share a scale d, an element is d (code - 8): GGML's Q4_0
+ * values.  Of 32 numbers x, d is -1/8 of the one that is largest by size (the first
+ * of equals), rounded to 8 significant bits (so that every element is an f16
+ * number; at the bottom to multiples of 2^-24), and a code is the whole number
+ * nearest to x / d (the even one of two), from -8 to 7, plus 8; d 0: all elements 0.
+ * Where one of them is no number or not below 65408 by size, d is no number, and so
+ * are the 32 elements.
+ * ------------------------------------------------------------------------- */
+typedef struct s2hip_pages s2hip_pages;
+
+#define S2HIP_PAGES_ERR_LENS 1u     /* lens / new_lens (update: source, keep, add too) out of range */
+#define S2HIP_PAGES_ERR_POSITION 2u /* append: a negative position: the token was left out */
+#define S2HIP_PAGES_ERR_RANGE 4u    /* append: keys or values that 4 bits do not hold became no numbers */
+#define S2HIP_PAGES_ERR_PAGE 8u     /* a page of a token in use is not one of the pool */
+#define S2HIP_PAGES_ERR_FULL 16u    /* update: fewer free pages than the rows need */
+#define S2HIP_PAGES_ERR_REFS 32u    /* update, compact: refs below the rows that hold a page */
+
+typedef struct {
+  int32_t device;
+  uint32_t heads, kv_heads; /* heads: a multiple of kv_heads, at most 64 times it */
+  uint32_t head_dim;        /* 64 or 128 */
+  uint32_t page_tokens;     /* 16, 32, 64 or 128 */
+  uint32_t pages;           /* of a pool, 1..2^20 */
+  uint32_t table_pages;     /* of a table row; times page_tokens at most 2^20 */
+  uint32_t max_requests;    /* 1..256: rows per call */
+  uint32_t max_tokens;      /* 1..65536: requests * n_tokens per call */
+  uint32_t rope_dims;       /* the first dims of a head that are rotated: even; 0: all */
+  uint32_t rope_half;       /* 1: pairs (i, i + rope_dims / 2), rope_dims a multiple of 16; 0: pairs (2 i, 2 i + 1) */
+  double rope_base;         /* > 0; pair i turns by rope_base^(-2 i / rope_dims) a position */
+  double rope_gain;         /* what cos and sin are multiplied by; 0: 1 */
+  const double* rope_freq;  /* host, [rope_dims / 2], copied: angles per position in place of rope_base's; NULL: those */
+  float eps;                /* of the head norms, >= 0 */
+  float scale;              /* of the scores; 0: 1 / sqrt(head_dim) */
+} s2hip_pages_config;
+
+typedef struct {
+  void* pool;              /* [pages] pages (update, compact: of the first layer); 16-byte aligned */
+  const int32_t* table;    /* [requests][table_pages] */
+  const int32_t* lens;     /* [requests]: tokens in use, this call's new ones included */
+  const int32_t* new_lens; /* [requests]: this call's tokens, the last in use; NULL: n_tokens of each request, none where lens is 0 */
+  uint32_t requests;
+} s2hip_pages_view;
+
+/* Angles per position of dims / 2 pairs, base^(-2 i / dims), for s2hip_pages_config,
+ * and the gain that belongs to them; for contexts `factor` (>= 1) times as long as the
+ * `context` positions that a model was trained on:
+ *   S2HIP_ROPE_LINEAR   all over factor
+ *   S2HIP_ROPE_STRETCH  base times factor^(dims / (dims - 2)): the slowest over factor (dims >= 4)
+ *   S2HIP_ROPE_PARTS    pairs of `high` turns or more within `context` as they are, those
+ *                       of `low` or fewer over factor, between them in proportion to
+ *                       their turns (low < high); gain 1 + 0.1 ln(factor), else 1
+ * Host only: no device. */
+#define S2HIP_ROPE_PLAIN 0u
+#define S2HIP_ROPE_LINEAR 1u
+#define S2HIP_ROPE_STRETCH 2u
+#define S2HIP_ROPE_PARTS 3u
+int32_t s2hip_rope_frequencies(uint32_t dims, double base, uint32_t scaling, double factor, double context, double low,
+                               double high, double* freq, double* gain, char* err, size_t err_cap);
+
+s2hip_pages* s2hip_pages_open(const s2hip_pages_config* cfg, char* err, size_t err_cap);
+/* The handle's work has to be done (its streams synchronised). */
+void s2hip_pages_close(s2hip_pages* pages);
+/* Bytes of a page of one layer. */
+uint64_t s2hip_pages_bytes(const s2hip_pages* pages);
+/* The S2HIP_PAGES_ERR_* bits set since the last call, after the work on `stream`
+ * so far: waits for it.  Not for a stream that is being captured. */
+int32_t s2hip_pages_errors(s2hip_pages* pages, void* stream, uint32_t* bits, char* err, size_t err_cap);
+
+/* QK-norm, rotation and cache write of the new tokens: qkv [requests][n_tokens]
+ * [(heads + 2 kv_heads) head_dim] raw products, norms as s2hip_kv_append, rotation
+ * by positions[b][t] as the handle says (angles, norms and what is rounded to 4 bits
+ * in 64 bits).  q_out [requests][n_tokens][heads head_dim]; token t's key and value go
+ * to slot lens[b] - new_lens[b] + t of request b's pages, which have to be its alone
+ * (s2hip_pages_update sees to that).  k_held, v_held (nullable, [requests][n_tokens]
+ * [kv_heads head_dim]): the new keys and values as the cache holds them.  A request
+ * out of range is left out, so is a token whose page is not one of the pool, but for
+ * its query.  Rows of tokens t >= new_lens[b] stay as they were.  No output may
+ * overlap an input or another. */
+int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, const float* qkv, uint32_t n_tokens,
+                           const int32_t* positions, const float* q_norm, const float* k_norm, float* q_out,
+                           float* k_held, float* v_held, void* stream, char* err, size_t err_cap);
+/* Attention of the new tokens' queries q [requests][n_tokens][heads head_dim]:
+ * token t of request b sees its request's slots 0 .. lens[b] - new_lens[b] + t; query
+ * head h reads kv head h / (heads / kv_heads).  out like q; rows of tokens t >=
+ * new_lens[b] stay as they were, out must not overlap q.  What a token does not see
+ * never reaches its row, whatever bits stand there.  A value that it sees and that is
+ * no number makes that element of its row no number, a key all of them; so do a query
+ * of no number and scores that are all below the range of f32.  A page that is not one
+ * of the pool is not read: its tokens are not seen (a row that sees none is no
+ * number).  Pages that requests have in common are read once for several of them.
+ * Products and sums are f32 or better. */
+int32_t s2hip_pages_attend(s2hip_pages* pages, const s2hip_pages_view* view, const float* q, uint32_t n_tokens,
+                           float* out, void* stream, char* err, size_t err_cap);
+/* The rows made anew, all at once: row b becomes the first keep[b] tokens (all, where it
+ * has fewer) of what row source[b] was (-1: none), and add[b] new slots behind them.
+ * NULL: source b, keep all, add none.  So a row is freed (keep 0), cut back (keep),
+ * forked or reordered (source) and given room for its next tokens (add); what it grows
+ * into is its own: a last page that is not full and that others hold too gets a copy, in
+ * `layers` pools layer_stride bytes apart (0: one behind the other), for all but the
+ * last row that grows into it where only such rows hold it.
+ *   refs_out counts the new rows in place of the old.  Pages that no row holds any more
+ * are free at once; the lowest free ones go to the rows in order, a copy's before the
+ * slots behind it.  table_out [requests][table_pages] (-1 behind the pages in use),
+ * lens_out; each array out is its array in or shares nothing with it.  Where a value is
+ * out of range, refs do not fit, or too few pages are free, nothing changes (each array
+ * out is as its array in) and the error bits say why.  view->new_lens is not looked at. */
+int32_t s2hip_pages_update(s2hip_pages* pages, const s2hip_pages_view* view, uint32_t layers, uint64_t layer_stride,
+                           const int32_t* source, const int32_t* keep, const int32_t* add, const int32_t* refs,
+                           int32_t* refs_out, int32_t* table_out, int32_t* lens_out, void* stream, char* err,
+                           size_t err_cap);
+/* The U pages in use moved to the front of the pools: of those at U and behind, the i-th
+ * goes to the i-th free page below U, in every layer; other pages stay.  The table has
+ * to hold every row that refers to the pool; table_out's pages in use follow (other
+ * entries stay as they were), refs_out too, used_out[0] = U, moved_to (nullable,
+ * [pages]): each page's new number, -1 of a free one.  Arrays in place or apart and
+ * what is wrong on the device: as s2hip_pages_update. */
+int32_t s2hip_pages_compact(s2hip_pages* pages, const s2hip_pages_view* view, uint32_t layers, uint64_t layer_stride,
+                            const int32_t* refs, int32_t* refs_out, int32_t* table_out, int32_t* used_out,
+                            int32_t* moved_to, void* stream, char* err, size_t err_cap);
 
 #ifdef __cplusplus
 }
