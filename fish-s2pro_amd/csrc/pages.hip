@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       big = fmax(big, fabs(x[e]));
-      odd |= !(fabs(x[e]) < 65408.0);
+      odd |= !(fabs(x[e]) < 16384.0);
     }
     big = fmax(big, __shfl_xor(big, 1, 64));
     big = fmax(big, __shfl_xor(big, 2, 64));
@@ -158,63 +158,414 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
 // ---------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------
-// A wave per query row: 64 keys at a time, one per lane, then their values, two
-// elements per lane.
-template <int HD>
-__global__ __launch_bounds__(64) void pg_attend_kernel(PgAttendArgs pa) {
+// As for the dense caches: scores in powers of two, a kv head's query rows packed,
+// row (b n + t) rep + r, a row's softmax state (m, l, o); f16 parts of queries and
+// weights, whose keys and values are f16 numbers as they are.
+//   An element is d (c - 8).  Four bits c become the f16 number 16 + c by an or into
+// the upper mantissa bits, and one fma with d and -24 d takes them to the element,
+// exactly: -24 d has 8 + 2 significant bits, the element 8 + 3.
+
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
+__device__ __forceinline__ half2v both(_Float16 x) { return half2v{x, x}; }
+
+// The two elements whose codes are in bits 4 F .. of a word's halves.
+template <int F>
+__device__ __forceinline__ half2v elements(uint32_t w, half2v d, half2v c) {
+  const uint32_t x = F == 0 ? w << 6 : F == 1 ? w << 2 : F == 2 ? w >> 2 : w >> 6;
+  return __builtin_elementwise_fma(as_half2((x & 0x03c003c0u) | 0x4c004c00u), d, c);
+}
+// A key's eight elements of a word (dims in order).
+__device__ __forceinline__ half8 key8(uint32_t w, _Float16 d) {
+  const half2v dd = both(d), c = both(d * _Float16(-24.0f));
+  const half2v a = elements<0>(w, dd, c), b = elements<1>(w, dd, c), e = elements<2>(w, dd, c), f = elements<3>(w, dd, c);
+  return half8{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
+}
+// Scales of tokens t0 t1, t2 t3 as pairs t0 t2, t1 t3.
+__device__ __forceinline__ void token_pairs(u32x2 x, half2v& even, half2v& odd) {
+  even = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u));
+  odd = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u));
+}
+
+// Few rows over many keys (decode steps).  A wave owns 16 packed rows of a kv head
+// and a run of tiles of 32 keys; nothing is exchanged between waves before the end,
+// when the block's four join their states in LDS and, with several blocks per 16 rows,
+// leave them for the join kernel.
+//   S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_16x16x32_f16, so a lane holds one row
+// (lane % 16).  Keys lie in memory as the first product's lanes take them (lane % 16 =
+// key, 8 dims of each 32), values as the second's (lane % 16 = pair of dims, 4 tokens
+// of each 16, as the weights stand in the registers): both go from memory to operands
+// with no exchange.
+//   The run: first the tiles that all requests of the rows have in common (the same
+// pages at the head of their rows of the table, seen by all), read once for all; then
+// each request's own.  Page numbers stand one per lane, 64 at a time.
+constexpr int STEP_WAVES = 4;
+
+// The tiles of `n_rows` packed rows from row0 on.  Lane j holds request b_lo + j (at most 64 requests).
+struct PgRun {
+  uint32_t b_lo;
+  uint32_t common;    // keys that all have in common, a multiple of 32
+  uint32_t tiles;     // of the requests' own keys
+  Request rq;         // the lane's request
+  uint32_t seg_keys;  // keys that its rows see, at most (0: it has no row)
+  uint32_t seg_end;   // its last own tile + 1
+};
+
+template <int KT>
+__device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, uint32_t n_rows, RawRequest raw, uint32_t* err) {
   const KvAttendArgs& a = pa.a;
-  __shared__ float qs[HD], ps[64];
-  const uint32_t lane = threadIdx.x, h = blockIdx.x % a.s.H, bt = blockIdx.x / a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
-  const Request r = request_of(a.c, b, lane == 0 ? a.s.err : nullptr);
-  if (t >= r.fresh) return;
-  for (uint32_t d = lane; d < HD; d += 64) qs[d] = a.q[size_t(blockIdx.x) * HD + d] * a.s.scale2;
-  __syncthreads();
+  const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep, row1 = min(row0 + n_rows, a.c.R * per);
+  PgRun r{};
+  r.b_lo = row0 / per;
+  const uint32_t b = r.b_lo + lane;
+  if (b <= (row1 - 1) / per) {
+    r.rq = checked(a.c, raw, err);
+    const uint32_t first = max(row0, b * per) - b * per, last = min(row1, (b + 1) * per) - 1 - b * per;
+    if (first / a.s.rep < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(last / a.s.rep, r.rq.fresh - 1) + 1;
+  }
+  // what every row with a token sees, as far as the tables agree
+  const uint64_t has = __ballot(r.seg_keys != 0);
+  if (__popcll(has) > 1) {
+    const uint32_t lead = uint32_t(__ffsll((unsigned long long)has)) - 1;
+    uint32_t least = r.seg_keys ? r.rq.len - r.rq.fresh + 1 : 0xffffffffu;
+    least = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+    const uint32_t pages = least >> pa.p.shift;
+    uint32_t same = 0;
+    for (; same < pages;) {
+      const uint32_t i = min(same + lane, pages - 1);
+      const int32_t mine = pa.p.table[size_t(r.b_lo + lead) * pa.p.width + i];
+      bool differs = false;
+      for (uint64_t rest = has & (has - 1); rest; rest &= rest - 1)
+        differs |= pa.p.table[size_t(r.b_lo + uint32_t(__ffsll((unsigned long long)rest)) - 1) * pa.p.width + i] != mine;
+      const uint64_t out = __ballot(differs);
+      if (out) {
+        same += uint32_t(__ffsll((unsigned long long)out)) - 1;
+        break;
+      }
+      same = min(same + 64, pages);
+    }
+    r.common = (same << pa.p.shift) / KT * KT;
+  }
+  r.seg_end = wave_scan(r.seg_keys > r.common ? (r.seg_keys - r.common + KT - 1) / KT : 0u);
+  r.tiles = lane_read_u32(r.seg_end, 63);
+  return r;
+}
+
+// 64 page numbers of a request, one per lane.
+struct PageWindow {
+  uint32_t b = 0xffffffffu, first = 0;
+  int32_t page = 0;
+  __device__ __forceinline__ uint32_t get(const PgPool& p, uint32_t req, uint32_t i) {
+    if (req != b || i - first >= 64u) {
+      b = req;
+      first = i;
+      page = p.table[size_t(req) * p.width + min(i + (threadIdx.x & 63u), p.width - 1)];
+    }
+    return lane_read_u32(uint32_t(page), int(i - first));
+  }
+};
+
+// A tile of 32 keys in two halves of 16, which may lie in different pages.
+struct PgTile {
+  uint32_t req, key0, keys;  // request, first key; keys of it that are there
+  int seg;                   // -1: in common; else request b_lo + seg
+  const uint8_t* part[2];    // the kv head's part of the page, of each half
+  uint32_t slot[2];          // its first slot there
+  uint32_t gone;             // bit h: half h lies in no page of the pool
+};
+
+template <int HD>
+__global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArgs pa, KvSplit sp) {
+  constexpr int KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
+  constexpr int OP = HD + 4;                          // padded row of the joined states
+  constexpr float LIFT = F16_LIFT;
+  __shared__ __align__(16) float os_all[STEP_WAVES * 16 * OP];
+  __shared__ float ml[STEP_WAVES][16][2];
+  const KvAttendArgs& a = pa.a;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
+  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
+  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
   const Chunk<HD> at{pa.p.shift};
-  const uint32_t keys = r.len - r.fresh + t + 1, mask = (1u << pa.p.shift) - 1u;
-  auto page_of = [&](uint32_t key) { return uint32_t(pa.p.table[size_t(b) * pa.p.width + (key >> pa.p.shift)]); };
-  float m = -INFINITY, l = 0.0f, o[2] = {0.0f, 0.0f};
-  for (uint32_t k0 = 0; k0 < keys; k0 += 64) {
-    const uint32_t key = k0 + lane;
-    float s = -INFINITY;
-    if (key < keys) {
-      const uint32_t page = page_of(key), slot = key & mask;
-      if (page < pa.p.pages) {
-        const uint8_t* part = pa.p.pool + (size_t(page) * a.s.G + g) * pa.p.chunk;
-        s = 0.0f;
-        for (uint32_t j = 0; j < HD / 32; ++j) {
-          const float d = float(*reinterpret_cast<const _Float16*>(part + at.ks() + (slot * (HD / 32) + j) * 2));
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t word = *reinterpret_cast<const uint32_t*>(part + ((slot * 4 + i) * (HD / 32) + j) * 4);
-            for (int e = 0; e < 8; ++e) s = fmaf(d * float(int((word >> (e / 2 * 4 + e % 2 * 16)) & 15u) - 8), qs[32 * j + 8 * i + e], s);
-          }
-        }
+
+  const RawRequest raw = load_request(a.c, min(tile * 16 / per + lane, a.c.R - 1));
+  const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
+  float4 qx[HD / 16];  // dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
+#pragma unroll
+  for (int j = 0; j < HD / 16; ++j) qx[j] = *reinterpret_cast<const float4*>(a.q + q_at + 32 * (j / 2) + 8 * q4 + 4 * (j % 2));
+  const PgRun run = pg_run<KT>(pa, tile * 16, 16, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint32_t b_lo = run.b_lo, lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
+  const uint32_t c_tiles = run.common / KT, c_lo = c_tiles * lot / lots, n_com = c_tiles * (lot + 1) / lots - c_lo;
+  // (the own tiles the other way round: the waves with one more in common get one fewer)
+  const uint32_t o_lo = run.tiles * (lots - 1 - lot) / lots, n_tiles = n_com + run.tiles * (lots - lot) / lots - o_lo;
+
+  uint32_t seg = 0;
+  PageWindow window;
+  auto where = [&](uint32_t i) {
+    PgTile w;
+    if (i < n_com) {
+      w.seg = -1;
+      w.req = b_lo + uint32_t(__ffsll((unsigned long long)__ballot(run.seg_keys != 0))) - 1;
+      w.key0 = (c_lo + i) * KT;
+      w.keys = KT;
+    } else {
+      const uint32_t x = o_lo + (i - n_com);
+      while (x >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+      const uint32_t begin = seg ? lane_read_u32(run.seg_end, int(seg) - 1) : 0u;
+      w.seg = int(seg);
+      w.req = b_lo + seg;
+      w.key0 = run.common + (x - begin) * KT;
+      w.keys = min(uint32_t(KT), lane_read_u32(run.seg_keys, int(seg)) - w.key0);
+    }
+    w.gone = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t key = w.key0 + (h && w.keys > 16 ? 16 : 0);
+      const uint32_t page = window.get(pa.p, w.req, key >> pa.p.shift);
+      const bool in = page < pa.p.pages;
+      w.gone |= in ? 0u : 1u << h;
+      w.part[h] = pa.p.pool + (size_t(in ? page : 0u) * a.s.G + g) * pa.p.chunk;
+      w.slot[h] = key & ((1u << pa.p.shift) - 1u);
+    }
+    if (w.gone && lane == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
+    return w;
+  };
+  // Of each half: codes of key r16, dims 32 j + 8 q4 ..; its scales; codes of dims 32 j + 2 r16 .. of tokens 4 q4 ..; their scales
+  uint32_t kc[2][GR], vc[2][GR], ks[2][GR / 2];
+  u32x2 vs[2][GR];
+  auto load_k = [&](const PgTile& w) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t* p = w.part[h] + w.slot[h] * (HD / 2);
+      if constexpr (HD == 128) {
+        *reinterpret_cast<u32x4*>(kc[h]) = *reinterpret_cast<const u32x4*>(p + r16 * (HD / 2) + q4 * (HD / 8));
+        *reinterpret_cast<u32x2*>(ks[h]) = *reinterpret_cast<const u32x2*>(w.part[h] + at.ks() + w.slot[h] * (HD / 16) + r16 * (HD / 16));
       } else {
-        atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
+        *reinterpret_cast<u32x2*>(kc[h]) = *reinterpret_cast<const u32x2*>(p + r16 * (HD / 2) + q4 * (HD / 8));
+        ks[h][0] = *reinterpret_cast<const uint32_t*>(w.part[h] + at.ks() + w.slot[h] * (HD / 16) + r16 * (HD / 16));
       }
     }
-    const float mn = fmaxf(m, wave_max(s));
-    const float base = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f((m == -INFINITY ? base : m) - base);
-    const float p = __builtin_amdgcn_exp2f(s - base);
-    l = l * f + wave_sum(p);
-    m = mn;
-    ps[lane] = p;
-    __syncthreads();
-    o[0] *= f;
-    o[1] *= f;
-    for (uint32_t k = k0; k < min(keys, k0 + 64) && lane < HD / 2; ++k) {
-      const uint32_t page = page_of(k), slot = k & mask;
-      if (page >= pa.p.pages) continue;
-      const uint8_t* part = pa.p.pool + (size_t(page) * a.s.G + g) * pa.p.chunk;
-      const uint32_t quad = slot / 4, one = slot % 4, j = lane / 16;
-      const uint32_t c = part[at.v() + ((quad * 16 + lane % 16) * (HD / 32) + j) * 4 + one];
-      const float d = float(*reinterpret_cast<const _Float16*>(part + at.vs() + ((quad * (HD / 32) + j) * 4 + one) * 2));
-      o[0] = fmaf(ps[k - k0], d * float(int(c & 15u) - 8), o[0]);
-      o[1] = fmaf(ps[k - k0], d * float(int(c >> 4) - 8), o[1]);
+  };
+  auto load_v = [&](const PgTile& w) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint8_t *p = w.part[h] + at.v() + w.slot[h] * (HD / 2) + lane * (HD / 8), *d = w.part[h] + at.vs() + w.slot[h] * (HD / 16) + q4 * (HD / 4);
+      if constexpr (HD == 128) {
+        *reinterpret_cast<u32x4*>(vc[h]) = *reinterpret_cast<const u32x4*>(p);
+        *reinterpret_cast<u32x4*>(&vs[h][0]) = *reinterpret_cast<const u32x4*>(d);
+        *reinterpret_cast<u32x4*>(&vs[h][2]) = *reinterpret_cast<const u32x4*>(d + 16);
+      } else {
+        *reinterpret_cast<u32x2*>(vc[h]) = *reinterpret_cast<const u32x2*>(p);
+        *reinterpret_cast<u32x4*>(&vs[h][0]) = *reinterpret_cast<const u32x4*>(d);
+      }
     }
-    __syncthreads();
+  };
+  PgTile w{};
+  if (n_tiles) {
+    w = where(0);
+    load_k(w);
+    load_v(w);
   }
-  const float inv = m == -INFINITY ? NAN : 1.0f / l;
-  if (lane < HD / 2) *reinterpret_cast<float2*>(a.out + size_t(blockIdx.x) * HD + 2 * lane) = make_float2(o[0] * inv, o[1] * inv);
+
+  // this lane's row
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
+  const bool live = tile * 16 + r16 < rows && t_row < fresh_row;
+  // (a row of no token may see anything: nobody reads it)
+  const int own_limit = live ? int(len_row - fresh_row + t_row) : 0x7fffffff, own_seg = live ? int(b_row - b_lo) : -2;
+  half8 qh[GR], ql[GR];  // dims 32 j + 8 q4 + e
+  float unscale = 1.0f;
+  {
+    const float s2 = live ? a.s.scale2 : 0.0f;
+    float x[HD / 16][4], big = 0.0f;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+      x[j][0] = live ? qx[j].x * s2 : 0.0f;  // (a query of no token may hold anything)
+      x[j][1] = live ? qx[j].y * s2 : 0.0f;
+      x[j][2] = live ? qx[j].z * s2 : 0.0f;
+      x[j][3] = live ? qx[j].w * s2 : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[j][e]));
+    }
+    float inv;
+    pow2_scale(quarter_max(big), unscale, inv);
+#pragma unroll
+    for (int j = 0; j < GR; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const Parts y = split_query<false>(x[2 * j + e / 4][e % 4] * inv);
+        qh[j][e] = y.hi;
+        ql[j][e] = y.lo;
+      }
+  }
+
+  floatx4 o[OT];  // o[2 c + h][i]: dim 32 c + 8 q4 + 2 i + h
+#pragma unroll
+  for (int i = 0; i < OT; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.0f;
+
+  for (uint32_t i = 0; i < n_tiles; ++i) {
+    const bool more = i + 1 < n_tiles;
+    PgTile next = w;
+    if (more) next = where(i + 1);
+    float s[8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      floatx4 hi = floatx4{0.f, 0.f, 0.f, 0.f}, lo = hi;
+#pragma unroll
+      for (int j = 0; j < GR; ++j) {
+        const half8 k8 = key8(kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
+        hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], hi, 0, 0, 0);
+        lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], lo, 0, 0, 0);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[4 * h + c] = (hi[c] + lo[c]) * unscale;
+    }
+    load_k(next);
+    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : own_seg == w.seg ? own_limit : -1;
+    // rows that see the whole tile: nothing to mask
+    const bool whole = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;
+    if (!whole) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
+        if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c] = -INFINITY;
+      }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int c = 1; c < 8; ++c) top = fmaxf(top, s[c]);
+    const float mn = fmaxf(m, quarter_max(top));
+    const bool up = mn > m + SLACK;
+    if (__any(up)) {
+      const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+#pragma unroll
+      for (int c = 0; c < OT; ++c) o[c] *= f;
+      l *= f;
+      m = to;
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
+    half8 ph, pl;  // tokens 0 2 1 3 of the lane's four in each half
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      s[c] = __builtin_amdgcn_exp2f(s[c] - base);
+      l += s[c];
+      const float hi = __uint_as_float(__float_as_uint(s[c]) & 0xffffe000u);  // the upper 11 bits, and the rest
+      const int to = (c & 4) + (c % 4 == 1 ? 2 : c % 4 == 2 ? 1 : c % 4);
+      ph[to] = _Float16(hi);
+      pl[to] = _Float16(s[c] - hi);
+    }
+    if (!whole) {
+      if (w.keys < KT || w.gone) {  // scales of tokens that no row sees may hold anything: 0
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int there = (w.gone >> h) & 1u ? 0 : int(w.keys) - int(16u * h + 4u * q4);  // of the lane's four
+          const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
+#pragma unroll
+          for (int c = 0; c < GR; ++c) vs[h][c] = u32x2{vs[h][c][0] & low, vs[h][c][1] & high};
+        }
+      }
+      // of no number, and not seen by some: 0 too, and a product of marks says which outputs are no number
+      half2v z = half2v{};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < GR; ++c)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[h][c][x]), half2v{}, z);
+      const bool odd = !(z[0] == _Float16(0)) || !(z[1] == _Float16(0));
+      if (__any(odd)) {
+        half8 seen;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) seen[c] = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4)) <= limit ? _Float16(1) : _Float16(0);
+#pragma unroll
+        for (int c = 0; c < GR; ++c) {
+          half8 marks;
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            uint32_t& pair = reinterpret_cast<uint32_t*>(&vs[x / 4][c])[x % 4 / 2];
+            const bool bad = ((pair >> (16 * (x % 2))) & 0x7c00u) == 0x7c00u;
+            marks[x] = bad ? _Float16(1) : _Float16(0);
+            if (bad) pair &= ~(0xffffu << (16 * (x % 2)));
+          }
+          const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, seen, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (hits[x] > 0.0f) o[2 * c][x] = o[2 * c + 1][x] = NAN;
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < GR; ++c) {
+      half2v v[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        half2v de, dd;
+        token_pairs(vs[h][c], de, dd);
+        const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
+        v[h][0] = elements<0>(vc[h][c], de, ce);
+        v[h][1] = elements<1>(vc[h][c], de, ce);
+        v[h][2] = elements<2>(vc[h][c], dd, cd);
+        v[h][3] = elements<3>(vc[h][c], dd, cd);
+      }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const half8 v8 = {v[0][x][0], v[0][x][1], v[0][2 + x][0], v[0][2 + x][1], v[1][x][0], v[1][x][1], v[1][2 + x][0], v[1][2 + x][1]};
+        o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[2 * c + x], 0, 0, 0);
+        o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[2 * c + x], 0, 0, 0);
+      }
+    }
+    load_v(next);
+    w = next;
+  }
+
+  // the block's four states as one
+  l = quarter_sum(l);
+  if (q4 == 0) {
+    ml[wave][r16][0] = m;
+    ml[wave][r16][1] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i) M = fmaxf(M, ml[i][r16][0]);
+  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+  float* os = os_all + (wave * 16 + r16) * OP;
+#pragma unroll
+  for (int c = 0; c < GR; ++c)
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      *reinterpret_cast<floatx4*>(os + 32 * c + 8 * q4 + 4 * x) =
+          floatx4{o[2 * c][2 * x] * f, o[2 * c + 1][2 * x] * f, o[2 * c][2 * x + 1] * f, o[2 * c + 1][2 * x + 1] * f};
+  __syncthreads();
+  const uint32_t jr = tid / 16, d0 = tid % 16 * 4;  // a row per 16 threads
+  const uint32_t out_row = tile * 16 + jr;
+  float M_row = -INFINITY, L_row = 0.0f;
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i) M_row = fmaxf(M_row, ml[i][jr][0]);
+  const float M_base = M_row == -INFINITY ? 0.0f : M_row;  // (then every l is 0, or no number)
+#pragma unroll
+  for (int i = 0; i < STEP_WAVES; ++i) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_base), L_row);
+  const size_t part = ((size_t(g) * sp.tiles + tile) * sp.splits + split) * 16 + jr;
+  const bool last = sp.splits == 1;
+  const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
+  const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
+  if (last && !out_live) return;
+  float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
+  const float inv = last ? (M_row == -INFINITY ? NAN : 1.0f / L_row) : 1.0f;  // (it sees a key, its own)
+#pragma unroll
+  for (int c = 0; c < HD / 64; ++c) {
+    const float* src = os_all + jr * OP + d0 + 64 * c;
+    floatx4 x = *reinterpret_cast<const floatx4*>(src);
+#pragma unroll
+    for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * 16 * OP);
+    *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
+  }
+  if (tid % 16 == 0 && !last) {
+    sp.ml[2 * part] = M_row - LIFT;
+    sp.ml[2 * part + 1] = L_row;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -483,10 +834,21 @@ hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s) {
   });
 }
 
-hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& a, const PgWorkspace&, hipStream_t s) {
+hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspace& w, hipStream_t s) {
+  const KvAttendArgs& a = pa.a;
+  KvSplit sp{};
+  sp.o = w.part;
+  sp.ml = w.part_ml;
+  sp.up = 1.0f;
+  const uint32_t rows = a.c.R * a.c.n * a.s.rep;
+  sp.tiles = (rows + 15) / 16;
+  const uint32_t lots = a.s.G * sp.tiles, most = (a.c.cap + 31) / 32 * min(a.c.R, 15 / (a.c.n * a.s.rep) + 1);  // key tiles of a row tile, at most
+  sp.splits = max(1u, min(512 / lots, (most + STEP_WAVES - 1) / STEP_WAVES));
+  if (most <= 24u * 128 / hd) sp.splits = 1;
+  if (size_t(lots) * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / lots));
   return by_dim(hd, [&](auto HD) {
-    hipLaunchKernelGGL(pg_attend_kernel<HD()>, dim3(a.a.c.R * a.a.c.n * a.a.s.H), dim3(64), 0, s, a);
-    return hipGetLastError();
+    hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+    return sp.splits > 1 ? launch_kv_join(hd, a, sp, s) : hipGetLastError();
   });
 }
 

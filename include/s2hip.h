@@ -551,7 +551,7 @@ int32_t s2hip_kv_evict(s2hip_kv* kv, const s2hip_kv_view* view, uint32_t layers,
  * of equals), rounded to 8 significant bits (so that every element is an f16
  * number; at the bottom to multiples of 2^-24), and a code is the whole number
  * nearest to x / d (the even one of two), from -8 to 7, plus 8; d 0: all elements 0.
- * Where one of them is no number or not below 65408 by size, d is no number, and so
+ * Where one of them is no number or not below 16384 by size, d is no number, and so
  * are the 32 elements.
  * ------------------------------------------------------------------------- */
 typedef struct s2hip_pages s2hip_pages;

@@ -21,7 +21,7 @@ def quantised(x):
     y = x.reshape(-1, 32)
     size = np.abs(y)
     with np.errstate(invalid="ignore"):
-        bad = ~(size < 65408.0).all(1)
+        bad = ~(size < 16384.0).all(1)
     at = np.where(np.isnan(size), -1.0, size).argmax(1)  # (the first of equals)
     d = np.array([math.nan if b else d8(float(v)) for v, b in zip(y[np.arange(len(y)), at] / -8, bad)])
     with np.errstate(invalid="ignore", divide="ignore"):

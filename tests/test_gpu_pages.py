@@ -321,7 +321,7 @@ def test_attend_request_out_of_range_is_left_out(bad):
     assert p.ops.errors(stream()) == ERR_LENS
 
 
-@pytest.mark.parametrize("scale", [2.0**-20, 2.0**-12, 2.0**4, 8160.0])
+@pytest.mark.parametrize("scale", [2.0**-20, 2.0**-12, 2.0**4, 2040.0])
 def test_attend_scales(scale):
     """Values as small and as large as 4 bits hold; the scores' scale undone by the queries."""
     p = Pool((8, 2, 128), 32, [77, 33], [1, 1], seed=6)
@@ -490,16 +490,16 @@ def test_append_equals_and_ties():
 
 def test_append_small_and_large():
     r = np.random.default_rng(5)
-    x = (r.standard_normal((40, 32)) * 2.0 ** r.integers(-30, 14, (40, 1))).astype(np.float32)
-    x[0] *= 65407.0 / np.abs(x[0]).max()
-    x = np.clip(x, -65407, 65407)
+    x = (r.standard_normal((40, 32)) * 2.0 ** r.integers(-30, 12, (40, 1))).astype(np.float32)
+    x[0] *= 16383.0 / np.abs(x[0]).max()
+    x = np.clip(x, -16383, 16383)
     a, held = _values(x)
     for got, y in zip(held, x):
         assert np.array_equal(got, pages_util.quantised(y)[2])
     assert a.pool.ops.errors(stream()) == 0
 
 
-@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 65408.0, -1e30])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 16384.0, -1e30])
 def test_append_beyond_the_range(bad):
     x = np.ones((3, 32))
     x[1, 20] = bad
