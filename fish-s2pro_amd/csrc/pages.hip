@@ -189,6 +189,20 @@ __device__ __forceinline__ void token_pairs(u32x2 x, half2v& even, half2v& odd) 
   odd = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u));
 }
 
+// Of pair x of scales those of no number become 0; the first of them, or a large number.
+template <class Pairs>
+__device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
+  uint32_t first = 1000, pair = pairs[x];
+#pragma unroll
+  for (int i = 1; i >= 0; --i)
+    if (((pair >> (16 * i)) & 0x7c00u) == 0x7c00u) {
+      pair &= ~(0xffffu << (16 * i));
+      first = i;
+    }
+  pairs[x] = pair;
+  return first;
+}
+
 // Few rows over many keys (decode steps).  A wave owns 16 packed rows of a kv head
 // and a run of tiles of 32 keys; nothing is exchanged between waves before the end,
 // when the block's four join their states in LDS and, with several blocks per 16 rows,
@@ -466,7 +480,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
           for (int c = 0; c < GR; ++c) vs[h][c] = u32x2{vs[h][c][0] & low, vs[h][c][1] & high};
         }
       }
-      // of no number, and not seen by some: 0 too, and a product of marks says which outputs are no number
+      // of no number, and not seen by some: 0 too; the outputs of rows that see the first of them are no number
       half2v z = half2v{};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -476,23 +490,15 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
           for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[h][c][x]), half2v{}, z);
       const bool odd = !(z[0] == _Float16(0)) || !(z[1] == _Float16(0));
       if (__any(odd)) {
-        half8 seen;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) seen[c] = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4)) <= limit ? _Float16(1) : _Float16(0);
 #pragma unroll
         for (int c = 0; c < GR; ++c) {
-          half8 marks;
+          uint32_t first = KT;
 #pragma unroll
-          for (int x = 0; x < 8; ++x) {
-            uint32_t& pair = reinterpret_cast<uint32_t*>(&vs[x / 4][c])[x % 4 / 2];
-            const bool bad = ((pair >> (16 * (x % 2))) & 0x7c00u) == 0x7c00u;
-            marks[x] = bad ? _Float16(1) : _Float16(0);
-            if (bad) pair &= ~(0xffffu << (16 * (x % 2)));
-          }
-          const floatx4 hits = __builtin_amdgcn_mfma_f32_16x16x32_f16(marks, seen, floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (hits[x] > 0.0f) o[2 * c][x] = o[2 * c + 1][x] = NAN;
+            for (int x = 0; x < 2; ++x) first = min(first, take_odd_scales(vs[h][c], x) + 16 * h + 4 * q4 + 2 * x);
+          first = wave_reduce(first, [](uint32_t x, uint32_t y) { return min(x, y); });
+          if (first < KT && limit >= int(w.key0 + first)) o[2 * c] = o[2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
         }
       }
     }
@@ -565,6 +571,320 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
   if (tid % 16 == 0 && !last) {
     sp.ml[2 * part] = M_row - LIFT;
     sp.ml[2 * part + 1] = L_row;
+  }
+}
+
+// Many rows (turns, prompts).  A block of four waves owns 128 packed rows of a kv
+// head, 32 per wave, and walks the run of tiles of 64 keys.  Each wave takes 16 of a
+// tile's keys and values from 4 bits to f16, once for the block, and leaves them in
+// LDS, the next tile's while this one's products run; codes are loaded another tile
+// ahead.
+//   v_mfma_f32_32x32x16_f16, S^T = K Q^T and O^T += V^T P^T, a lane holds one row
+// (lane % 32).  Values stand transposed, a row of 64 tokens per dim, each 16 bytes the
+// 8 tokens that a lane's 8 weights belong to.
+constexpr int TILE_ROWS = 128;
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSplit sp) {
+  constexpr int KT = 64, GR = HD / 32, DS = HD / 16, DT = HD / 32;
+  constexpr uint32_t RB = HD * 2, PLANE = KT * RB, BUF = 2 * PLANE;  // bytes of a key's row, of the keys (and of the values), of both
+  constexpr float LIFT = F16_LIFT;
+  __shared__ __align__(16) uint8_t lds[2 * BUF];
+  // of tiles i, i + 1 and the one behind: bit w: the 16 keys of wave w lie in no page; a group's first value of no number
+  __shared__ uint32_t gone_tile[3], odd_tile[3][GR];
+  const KvAttendArgs& a = pa.a;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5, r16 = lane & 15u, q4 = lane >> 4;
+  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
+  const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
+  const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
+  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const Chunk<HD> at{pa.p.shift};
+
+  const RawRequest raw = load_request(a.c, min(tile * TILE_ROWS / per + lane, a.c.R - 1));
+  const uint32_t my_row = tile * TILE_ROWS + wave * 32 + r32, row = min(my_row, rows - 1);
+  const uint32_t b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
+  float4 qx[DS][2];  // dims 16 ks + 8 h2 ..
+#pragma unroll
+  for (int ks = 0; ks < DS; ++ks)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
+  const PgRun run = pg_run<KT>(pa, tile * TILE_ROWS, TILE_ROWS, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const uint64_t has = __ballot(run.seg_keys != 0);
+  if (!has) return;  // no row of a token
+  const uint32_t c_all = run.common / KT, c_lo = c_all * split / sp.splits, n_com = c_all * (split + 1) / sp.splits - c_lo;
+  const uint32_t o_lo = run.tiles * (sp.splits - 1 - split) / sp.splits, n_tiles = n_com + run.tiles * (sp.splits - split) / sp.splits - o_lo;
+
+  uint32_t seg = 0;
+  PageWindow window;
+  // a tile, and where the wave's 16 keys of it are
+  struct Tile {
+    uint32_t key0, keys;
+    int seg;
+    const uint8_t* part;
+    uint32_t slot;
+    bool gone;
+  };
+  auto where = [&](uint32_t i) {
+    Tile w;
+    uint32_t req;
+    if (i < n_com) {
+      w.seg = -1;
+      req = run.b_lo + uint32_t(__ffsll((unsigned long long)has)) - 1;
+      w.key0 = (c_lo + i) * KT;
+      w.keys = KT;
+    } else {
+      const uint32_t x = o_lo + (i - n_com);
+      while (x >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+      const uint32_t begin = seg ? lane_read_u32(run.seg_end, int(seg) - 1) : 0u;
+      w.seg = int(seg);
+      req = run.b_lo + seg;
+      w.key0 = run.common + (x - begin) * KT;
+      w.keys = min(uint32_t(KT), lane_read_u32(run.seg_keys, int(seg)) - w.key0);
+    }
+    const uint32_t key = w.key0 + (16 * wave < w.keys ? 16 * wave : 0u);
+    const uint32_t page = window.get(pa.p, req, key >> pa.p.shift);
+    w.gone = page >= pa.p.pages;
+    w.part = pa.p.pool + (size_t(w.gone ? 0u : page) * a.s.G + g) * pa.p.chunk;
+    w.slot = key & ((1u << pa.p.shift) - 1u);
+    if (w.gone && lane == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
+    return w;
+  };
+  // codes of key lane / 4, dims 32 j + 8 (lane % 4) ..; its scales; codes of dims 32 j + 2 r16 .. of tokens 4 q4 ..; their scales
+  uint32_t kc[GR], vc[GR], ks[GR / 2];
+  u32x2 vs[GR];
+  auto load = [&](const Tile& w) {
+    const uint8_t *k = w.part + w.slot * (HD / 2) + lane * (HD / 8), *d = w.part + at.ks() + w.slot * (HD / 16) + lane / 4 * (HD / 16);
+    const uint8_t *v = w.part + at.v() + w.slot * (HD / 2) + lane * (HD / 8), *e = w.part + at.vs() + w.slot * (HD / 16) + q4 * (HD / 4);
+    if constexpr (HD == 128) {
+      *reinterpret_cast<u32x4*>(kc) = *reinterpret_cast<const u32x4*>(k);
+      *reinterpret_cast<u32x2*>(ks) = *reinterpret_cast<const u32x2*>(d);
+      *reinterpret_cast<u32x4*>(vc) = *reinterpret_cast<const u32x4*>(v);
+      *reinterpret_cast<u32x4*>(&vs[0]) = *reinterpret_cast<const u32x4*>(e);
+      *reinterpret_cast<u32x4*>(&vs[2]) = *reinterpret_cast<const u32x4*>(e + 16);
+    } else {
+      *reinterpret_cast<u32x2*>(kc) = *reinterpret_cast<const u32x2*>(k);
+      ks[0] = *reinterpret_cast<const uint32_t*>(d);
+      *reinterpret_cast<u32x2*>(vc) = *reinterpret_cast<const u32x2*>(v);
+      *reinterpret_cast<u32x4*>(&vs[0]) = *reinterpret_cast<const u32x4*>(e);
+    }
+  };
+  // 16-byte piece p of key's row stands at p ^ k_swz(key), piece p of a dim's row of values at p ^ (dim / 2 % 8): 16 lanes'
+  // reads of one piece (16 keys, or dims) and 16 lanes' writes (4 keys x 4 pieces; 16 pairs of dims: half as many) are apart.
+  // A lane's addresses differ by an exclusive or with constants; they are worked out where they are used, for kept ones cost
+  // registers.
+  auto k_at = [](uint32_t key, uint32_t piece) {
+    const uint32_t swz = HD == 128 ? 4 * (key & 3u) + ((key >> 2) & 3u) : 4 * ((key >> 1) & 1u) + ((key >> 2) & 3u);
+    return key * RB + ((piece ^ swz) << 4);
+  };
+  auto v_at = [](uint32_t dim, uint32_t piece) { return PLANE + dim * (KT * 2) + ((piece ^ ((dim >> 1) & 7u)) << 4); };
+  lds_byte* const lds0 = (lds_byte*)lds;
+  typedef __attribute__((address_space(3))) half4 lds_half4;
+  auto store = [&](const Tile& w, uint32_t buf, uint32_t flag) {
+    uint32_t k_to = buf * BUF + k_at(16 * wave + lane / 4, lane % 4), v_to = buf * BUF + v_at(2 * r16, 2 * wave + (q4 & 1u)) + 8 * (q4 >> 1);
+    asm volatile("" : "+v"(k_to), "+v"(v_to));
+#pragma unroll
+    for (int j = 0; j < GR; ++j) *reinterpret_cast<lds_half8*>(lds0 + (k_to ^ (64u * j))) = key8(kc[j], as_half2(ks[j / 2])[j % 2]);
+    // scales of tokens that are not there may hold anything: 0
+    const int there = w.gone ? 0 : int(w.keys) - int(16u * wave + 4u * q4);  // of the lane's four
+    const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
+    half2v z = half2v{};
+#pragma unroll
+    for (int c = 0; c < GR; ++c) {
+      vs[c] = u32x2{vs[c][0] & low, vs[c][1] & high};
+#pragma unroll
+      for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[c][x]), half2v{}, z);
+    }
+    if (__any(!(z[0] == _Float16(0)) || !(z[1] == _Float16(0)))) {  // of no number: 0 too, and noted
+#pragma unroll
+      for (int c = 0; c < GR; ++c)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t first = take_odd_scales(vs[c], x) + 16 * wave + 4 * q4 + 2 * x;
+          if (first < KT) atomicMin(&odd_tile[flag][c], first);
+        }
+    }
+    if (w.gone && lane == 0) atomicOr(&gone_tile[flag], 1u << wave);
+#pragma unroll
+    for (int c = 0; c < GR; ++c) {
+      half2v de, dd;
+      token_pairs(vs[c], de, dd);
+      const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
+      const half2v v[4] = {elements<0>(vc[c], de, ce), elements<1>(vc[c], de, ce), elements<2>(vc[c], dd, cd), elements<3>(vc[c], dd, cd)};
+#pragma unroll
+      for (int x = 0; x < 2; ++x)  // tokens 0 2 1 3 of the four, the first or second half of a piece
+        *reinterpret_cast<lds_half4*>(lds0 + (v_to + (32 * c + x) * (KT * 2))) = half4{v[x][0], v[x][1], v[2 + x][0], v[2 + x][1]};
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // this lane's row
+  const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
+  const bool live = my_row < rows && t_row < fresh_row;
+  const int own_seg = int(b_row - run.b_lo), own_limit = int(len_row - fresh_row + t_row);
+  half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
+  float unscale;
+  {
+    float big = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DS; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float4& y = qx[c][e];
+        y = live ? make_float4(y.x * a.s.scale2, y.y * a.s.scale2, y.z * a.s.scale2, y.w * a.s.scale2) : make_float4(0.f, 0.f, 0.f, 0.f);
+        big = fmaxf(big, fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w))));
+      }
+    float inv;
+    pow2_scale(half_reduce(big, [](float p, float q) { return fmaxf(p, q); }), unscale, inv);
+#pragma unroll
+    for (int c = 0; c < DS; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float4 z = qx[c][e / 4];
+        const Parts y = split_query<false>((e % 4 == 0 ? z.x : e % 4 == 1 ? z.y : e % 4 == 2 ? z.z : z.w) * inv);
+        qh[c][e] = y.hi;
+        ql[c][e] = y.lo;
+      }
+  }
+
+  floatx16 o[DT];  // dim 32 dt + 8 (v / 4) + 4 h2 + v % 4
+#pragma unroll
+  for (int i = 0; i < DT; ++i) o[i] = floatx16{};
+  float m = -INFINITY, l = 0.0f;
+  if (tid < 3 * GR) (&odd_tile[0][0])[tid] = KT;
+  if (tid < 3) gone_tile[tid] = 0;
+  Tile w{}, next{};
+  __syncthreads();
+  if (n_tiles) {
+    w = where(0);
+    load(w);
+    store(w, 0, 0);
+    if (n_tiles > 1) {
+      next = where(1);
+      load(next);
+    }
+  }
+  __syncthreads();
+  uint32_t flag = 0;
+  for (uint32_t i = 0; i < n_tiles; ++i) {
+    const uint32_t buf = i & 1u, flag1 = flag == 2 ? 0 : flag + 1, flag2 = flag1 == 2 ? 0 : flag1 + 1;
+    const Tile cur = w;
+    if (tid < GR) odd_tile[flag2][tid] = KT;  // (last looked at a tile ago)
+    if (tid == 0) gone_tile[flag2] = 0;
+    if (i + 1 < n_tiles) {
+      store(next, buf ^ 1u, flag1);
+      w = next;
+      if (i + 2 < n_tiles) {
+        next = where(i + 2);
+        load(next);
+      }
+    }
+    const uint32_t gone = uniform(gone_tile[flag]);
+    const int limit = !live ? -1 : cur.seg < 0 ? 0x7fffffff : cur.seg == own_seg ? own_limit : -1;
+    if (__any(limit >= int(cur.key0))) {  // else nothing of it is for this wave's rows
+      uint32_t k_from = buf * BUF + k_at(r32, h2), v_from = buf * BUF + v_at(r32, h2);
+      asm volatile("" : "+v"(k_from), "+v"(v_from));
+      auto value8 = [&](int sub, int st, int dt) { return *reinterpret_cast<const lds_half8*>(lds0 + ((v_from ^ (64u * sub + 32u * st)) + 32 * dt * (KT * 2))); };
+      // Fragments are read two products ahead; the barriers keep the compiler from reading all of them first.
+      floatx16 s[2] = {};
+      {
+        half8 k8[3][2];
+        auto read = [&](int c) {
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub) k8[c % 3][sub] = *reinterpret_cast<const lds_half8*>(lds0 + ((k_from ^ (32u * c)) + 32 * sub * RB));
+        };
+        read(0);
+        read(1);
+#pragma unroll
+        for (int c = 0; c < DS; ++c) {
+          if (c + 2 < DS) read(c + 2);
+          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], qh[c], s[0], 0, 0, 0);
+          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], qh[c], s[1], 0, 0, 0);
+          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], ql[c], s[0], 0, 0, 0);
+          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], ql[c], s[1], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      const bool whole = __all(!live || limit >= int(cur.key0) + KT - 1) && !gone;
+      if (!whole) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (int(cur.key0) + int(32u * sub + 8u * (v / 4) + 4u * h2 + (v % 4)) > limit || ((gone >> (2 * sub + v / 8)) & 1u)) s[sub][v] = -INFINITY;
+      }
+      float top = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < 16; v += 2) {
+        top = fmaxf(fmaxf(top, s[0][v]), s[0][v + 1]);
+        top1 = fmaxf(fmaxf(top1, s[1][v]), s[1][v + 1]);
+      }
+      top = fmaxf(top, top1) * unscale;
+      const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
+      const bool up = mn > m + SLACK;
+      if (__any(up)) {
+        const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+        l *= f;
+        m = to;
+      }
+      const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const uint32_t first = uniform(odd_tile[flag][dt]);
+        if (first < KT && limit >= int(cur.key0 + first)) o[dt] = floatx16{} + NAN;
+      }
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        half8 ph[2], pl[2];  // 16 keys each, tokens 0 2 1 3 of each four: the weights' upper 11 bits, and the rest
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias));
+          sum[v % 2] += p;
+          const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
+          const int to = (v & 4) + (v % 4 == 1 ? 2 : v % 4 == 2 ? 1 : v % 4);
+          ph[v / 8][to] = _Float16(hi);
+          pl[v / 8][to] = _Float16(p - hi);
+        }
+        l += sum[0] + sum[1];
+        {
+          // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind the first
+          constexpr int BL = 2 * DT;
+          half8 v8[4];
+          auto read = [&](int c) { v8[c % 4] = value8(sub, c / DT, c % DT); };
+          read(0);
+          read(1);
+#pragma unroll
+          for (int c = 0; c <= BL; ++c) {
+            if (c + 2 < BL) read(c + 2);
+            if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[c / DT], o[c % DT], 0, 0, 0);
+            if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    flag = flag1;
+  }
+
+  l = half_reduce(l, [](float p, float q) { return p + q; });
+  const bool last = sp.splits == 1;
+  if (my_row >= rows || (last && !live)) return;
+  const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
+  float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
+  const float f = last ? (m == -INFINITY ? NAN : 1.0f / l) : 1.0f;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      *reinterpret_cast<floatx4*>(dst + 32 * dt + 8 * c + 4 * h2) =
+          floatx4{o[dt][4 * c] * f, o[dt][4 * c + 1] * f, o[dt][4 * c + 2] * f, o[dt][4 * c + 3] * f};
+  if (h2 == 0 && !last) {
+    sp.ml[2 * part] = m - LIFT;
+    sp.ml[2 * part + 1] = l;
   }
 }
 
@@ -842,12 +1162,18 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
   sp.up = 1.0f;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
-  const uint32_t lots = a.s.G * sp.tiles, most = (a.c.cap + 31) / 32 * min(a.c.R, 15 / (a.c.n * a.s.rep) + 1);  // key tiles of a row tile, at most
-  sp.splits = max(1u, min(512 / lots, (most + STEP_WAVES - 1) / STEP_WAVES));
-  if (most <= 24u * 128 / hd) sp.splits = 1;
-  if (size_t(lots) * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / lots));
+  const size_t scores = size_t(a.s.G) * rows * (a.c.cap - min(a.c.n, a.c.cap) / 2);
+  const bool many = a.c.n * a.s.rep >= 32 && scores * hd > 10000000u * size_t(128);
+  const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles);
+  const uint32_t most = (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));  // key tiles of a row tile, at most
+  sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
+  if (!many && most <= 24u * 128 / hd) sp.splits = 1;
+  if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   return by_dim(hd, [&](auto HD) {
-    hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+    if (many)
+      hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * sp.splits), dim3(256), 0, s, pa, sp);
+    else
+      hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, pa, sp);
     return sp.splits > 1 ? launch_kv_join(hd, a, sp, s) : hipGetLastError();
   });
 }

@@ -164,21 +164,35 @@ def test_attend_rows_all_the_same(page):
     p.check_all()
 
 
+# Rows of the table as long as the lengths need, and so long that a call counts as much work (it is launched by them)
+ROOM = [None, 32768]
+
+
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("page", [16, 64])
 @pytest.mark.parametrize("n", [2, 3, 4, 5, 7, 8, 9, 16, 31, 32, 33, 64, 65, 130])
-def test_attend_several_tokens(n, page):
+def test_attend_several_tokens(n, page, room):
     """Causal within the new tokens; ragged; an idle request between others."""
     new = [n, max(1, n // 2), 0, 1, n]
     lens = [n, n // 2 + 40, 9, 1, n + 77]
-    Pool((8, 2, 128), page, lens, new, seed=n).check_all()
+    Pool((8, 2, 128), page, lens, new, seed=n, width=room and room // page).check_all()
 
 
+@pytest.mark.parametrize("room", ROOM)
 @pytest.mark.parametrize("shape,requests,n,length,shared", [
     ((32, 8, 128), 2, 200, 63, 0), ((32, 8, 128), 1, 500, 0, 0), ((32, 8, 128), 2, 130, 1000, 15), ((8, 2, 64), 3, 300, 700, 10), ((16, 16, 64), 2, 257, 100, 0),
     ((14, 2, 128), 2, 150, 300, 4), ((32, 8, 128), 5, 40, 800, 12), ((64, 1, 64), 2, 40, 300, 2), ((6, 2, 128), 9, 33, 129, 2)])
-def test_attend_turns(shape, requests, n, length, shared):
+def test_attend_turns(shape, requests, n, length, shared, room):
     new = [max(1, n - 13 * b) for b in range(requests)]
-    Pool(shape, 64, [length + x for x in new], new, shared=shared, seed=n).check_all()
+    Pool(shape, 64, [length + x for x in new], new, shared=shared, seed=n, width=room and room // 64).check_all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("extra", [0, 1, 14, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 127, 128, 129])
+def test_attend_turn_borders(extra, hd, page):
+    """Turns that begin and end around the borders of tiles and pages."""
+    Pool((8, 2, hd), page, [32 + extra, 64 + extra, 33], [32, 9, 33], seed=extra, width=32768 // page).check_all()
 
 
 def test_attend_many_requests():
@@ -195,7 +209,7 @@ def test_attend_long(shape):
 def test_attend_drawn():
     """Sizes, pages and lengths at random, many of them."""
     g = random.Random(77)
-    for i in range(40):
+    for i in range(60):
         shape = g.choice(list(SHAPES.values()))
         requests = g.randint(1, 9)
         n = g.choice([1, 1, 1, 2, 3, 5, 17, 60, 100])
@@ -203,8 +217,9 @@ def test_attend_drawn():
         shared = g.choice([0, 0, g.randint(1, 6)])
         page = g.choice([16, 32, 64, 128])
         lens = [shared * page + x + g.choice([0, 1, g.randint(0, 40), g.randint(0, 400)]) if x else 0 for x in new]
-        print(i, shape, page, shared, lens, new, flush=True)
-        Pool(shape, page, lens, new, shared=shared, rows=n, seed=i).check_all()
+        width = g.choice([None, 40000 // page])
+        print(i, shape, page, shared, lens, new, width, flush=True)
+        Pool(shape, page, lens, new, shared=shared, rows=n, seed=i, width=width).check_all()
 
 
 def test_attend_without_new_lens():
@@ -215,12 +230,13 @@ def test_attend_without_new_lens():
     assert p.ops.errors(stream()) == 0
 
 
+@pytest.mark.parametrize("room", [None, 1000])
 @pytest.mark.parametrize("n", [1, 3, 40])
 @pytest.mark.parametrize("hd", [64, 128])
-def test_attend_never_sees_the_rest(n, hd):
+def test_attend_never_sees_the_rest(n, hd, room):
     """Slots behind the last token, pages of no row and table entries behind a row may hold anything: no bit changes."""
     lens = [n + 21, n, n + 90]
-    p = Pool((8, 2, hd), 32, lens, [n, n, max(1, n - 1)], seed=n, width=7)
+    p = Pool((8, 2, hd), 32, lens, [n, n, max(1, n - 1)], seed=n, width=room or 7)
     want = p.attend().clone()
     p.check(want)
     for fill in (0xFF, 0x7C, 0x00):
@@ -240,11 +256,12 @@ def test_attend_never_sees_the_rest(n, hd):
 
 
 @pytest.mark.parametrize("part", ["key", "value"])
+@pytest.mark.parametrize("room", [None, 2000])
 @pytest.mark.parametrize("n", [1, 5, 40])
-def test_attend_no_number_reaches_who_sees_it(part, n):
+def test_attend_no_number_reaches_who_sees_it(part, n, room):
     """A block of no numbers in one slot: rows that see it, and no others."""
     length = n + 30
-    p = Pool((8, 2, 128), 16, [length, length], [n, n], seed=n)
+    p = Pool((8, 2, 128), 16, [length, length], [n, n], seed=n, width=room)
     slot, g, group = length - max(1, n // 2), 1, 2  # of request 1
     clean = p.attend().clone()
     p.check(clean)
@@ -271,32 +288,33 @@ def _without(p, pool):
     return k, v
 
 
-def test_attend_query_of_no_number():
-    p = Pool((8, 2, 128), 16, [50, 50], [3, 3], seed=9)
+@pytest.mark.parametrize("n", [3, 40])
+def test_attend_query_of_no_number(n):
+    p = Pool((8, 2, 128), 16, [50, 50], [n, n], seed=9, width=2000)
     clean = p.attend().clone()
     p.q[1, 1, 5, 17] = math.nan
     p.q[0, 2, 0, 3] = math.inf
     p.out.fill_(7.0)
     out = p.attend()
     assert bool(out[1, 1, 5].isnan().all()) and bool(out[0, 2, 0].isnan().all())
-    rest = torch.ones(2, 3, 8, dtype=torch.bool, device="cuda")
+    rest = torch.ones(2, n, 8, dtype=torch.bool, device="cuda")
     rest[1, 1, 5] = rest[0, 2, 0] = False
     assert torch.equal(out[rest], clean[rest])
 
 
+@pytest.mark.parametrize("room", [None, 2000])
 @pytest.mark.parametrize("n", [1, 40])
-def test_attend_page_outside_the_pool(n):
+def test_attend_page_outside_the_pool(n, room):
     """Its tokens are not seen; rows that see nothing else are no number."""
-    p = Pool((8, 2, 128), 16, [n + 40, n + 1, 7], [n, n, 0], seed=n)
+    p = Pool((8, 2, 128), 16, [n + 40, n + 1, 7], [n, n, 0], seed=n, width=room)
     for b, i, to in ((0, 1, 1 << 20), (1, 0, -1)):
         p.table_h[b][i] = to
     p.table.copy_(dev(p.table_h))
     out = p.attend()
     assert p.ops.errors(stream()) == ERR_PAGE and p.ops.errors(stream()) == 0
     # request 0 without slots 16 .. 31: the same as a row whose second page is left out
-    keep = [x for i, x in enumerate(p.table_h[0]) if i != 1]
-    table = [keep + [-1], p.table_h[1], p.table_h[2]]
-    q = Pool((8, 2, 128), 16, [n + 40, n + 1, 7], [n, n, 0], seed=n)
+    table = [[x for i, x in enumerate(p.table_h[0]) if i != 1] + [-1], p.table_h[1], p.table_h[2]]
+    q = Pool((8, 2, 128), 16, [n + 40, n + 1, 7], [n, n, 0], seed=n, width=room)
     q.table.copy_(dev(table))
     q.lens.copy_(dev([n + 24, 0, 7]))
     q.new.copy_(dev([n, 0, 0]))
@@ -321,10 +339,11 @@ def test_attend_request_out_of_range_is_left_out(bad):
     assert p.ops.errors(stream()) == ERR_LENS
 
 
+@pytest.mark.parametrize("n", [1, 40])
 @pytest.mark.parametrize("scale", [2.0**-20, 2.0**-12, 2.0**4, 2040.0])
-def test_attend_scales(scale):
+def test_attend_scales(scale, n):
     """Values as small and as large as 4 bits hold; the scores' scale undone by the queries."""
-    p = Pool((8, 2, 128), 32, [77, 33], [1, 1], seed=6)
+    p = Pool((8, 2, 128), 32, [77, 43], [n, n], seed=6, width=1000)
     pool = p.pool_h.copy()
     d = np.sign(np.random.default_rng(1).standard_normal(pool[:, :, 32 * 128 :].shape[:-1] + (2 * 32 * 4,))) * scale
     pool[:, :, 32 * 128 :] = d.astype(np.float16).view(np.uint8).reshape(pool.shape[0], 2, -1)
