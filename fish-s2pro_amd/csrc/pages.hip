@@ -30,109 +30,158 @@ __device__ __forceinline__ double rounded8(double x) {
   return ldexp(rint(ldexp(x, -e)), e);
 }
 
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t v = uint64_t(__double_as_longlong(x));
+  return __longlong_as_double((long long)(uint64_t(dpp_u32<CTRL>(uint32_t(v >> 32))) << 32 | dpp_u32<CTRL>(uint32_t(v))));
+}
+
 // One block per token and run of heads (blockIdx.y, every gridDim.y-th 16 or 32), 8
 // elements per thread.  Norms, angles, rotation and what is rounded to 4 bits are in
-// 64 bits: a rounding of f32 in front would move a code across a border now and then,
-// and the value by a sixteenth of its block's range.
-template <int HD>
+// 64 bits, whose instructions cost what those of 32 bits do here: a rounding of f32 in
+// front would move a code across a border now and then, and the element by a sixteenth
+// of its block's range.
+template <int HD, bool HALF>
 __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
   constexpr uint32_t LP = HD / 8;     // lanes per head
   constexpr uint32_t HPB = 256 / LP;  // heads per step of the block
+  constexpr int PAIRS = HALF ? 8 : 4;
   __shared__ double2 turn[HD / 2];
   const uint32_t tid = threadIdx.x, b = blockIdx.x / a.c.n, t = blockIdx.x % a.c.n;
-  const Request r = request_of(a.c, b, tid == 0 && t == 0 && blockIdx.y == 0 ? a.s.err : nullptr);
-  if (t >= r.fresh) return;
+  const RawRequest raw = load_request(a.c, b);
   const int32_t pos = a.positions[size_t(b) * a.c.n + t];
+  const uint32_t heads = a.s.H + 2 * a.s.G, l = tid % LP, d0 = 8 * l, half = a.rope.dims / 2, h0 = blockIdx.y * HPB + tid / LP;
+  const float* src = a.qkv + (size_t(b) * a.c.n + t) * heads * HD;
+  // in halves: the other half's elements, 8 dims of it
+  const bool turns = d0 < a.rope.dims, second = HALF && d0 >= half;
+  const uint32_t o0 = HALF && turns ? (second ? d0 - half : d0 + half) : d0;
+  float x[8], z[HALF ? 8 : 1];
+  auto load = [&](uint32_t h) {
+    const float* row = src + size_t(min(h, heads - 1)) * HD;
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row + d0);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(row + d0 + 4);
+    if constexpr (HALF) {
+      *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(row + o0);
+      *reinterpret_cast<float4*>(z + 4) = *reinterpret_cast<const float4*>(row + o0 + 4);
+    }
+  };
+  load(h0);
+  const double per_token = tid < half ? a.rope.turns[tid] : 0.0;
+  const Request r = checked(a.c, raw, tid == 0 && t == 0 && blockIdx.y == 0 ? a.s.err : nullptr);
+  if (t >= r.fresh) return;
   if (pos < 0) {
     if (tid == 0 && blockIdx.y == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_POSITION);
     return;
   }
-  const uint32_t slot = r.len - r.fresh + t, half = a.rope.dims / 2;
+  const uint32_t slot = r.len - r.fresh + t;
   const uint32_t page = uint32_t(a.p.table[size_t(b) * a.p.width + (slot >> a.p.shift)]);
   const bool there = page < a.p.pages;
   if (!there && tid == 0 && blockIdx.y == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
-  if (tid < half) {
-    const double angle = double(pos) * a.rope.turns[tid];
+  if (tid < HD / 2) {
+    const double angle = double(pos) * per_token;
     double sn, cs;
     sincospi(2.0 * (angle - rint(angle)), &sn, &cs);
-    turn[tid] = make_double2(cs * a.rope.gain, sn * a.rope.gain);
+    turn[tid] = tid < half ? make_double2(cs * a.rope.gain, sn * a.rope.gain) : make_double2(1.0, 0.0);
   }
   __syncthreads();
-  const uint32_t heads = a.s.H + 2 * a.s.G, l = tid % LP, d0 = 8 * l;
-  const float* src = a.qkv + (size_t(b) * a.c.n + t) * heads * HD;
-  for (uint32_t h = blockIdx.y * HPB + tid / LP; h < heads; h += HPB * gridDim.y) {  // whole rows of LP lanes take part
-    const float* row = src + size_t(h) * HD;
-    double x[8];
+  double2 cs[PAIRS];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = row[d0 + e];
+  for (int i = 0; i < PAIRS; ++i) {
+    cs[i] = turn[HALF ? (second ? d0 - half + i : d0 + i) % (HD / 2) : d0 / 2 + i];
+    if (HALF && !turns) cs[i] = make_double2(1.0, 0.0);
+    if (second) cs[i].y = -cs[i].y;  // the second of a pair takes the first's times sin, the first the second's times -sin
+  }
+  for (uint32_t h = h0; h < heads;) {  // whole rows of LP lanes take part
     const bool value = h >= a.s.H + a.s.G;
+    double y[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = x[e];
     if (!value) {
       double f = 1.0;
       const float* gain = h < a.s.H ? a.q_norm : a.k_norm;
+      double w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = HALF ? z[e] : 0.0f;
       if (gain) {
         double ss = 0.0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fma(x[e], x[e], ss);
-#pragma unroll
-        for (uint32_t m = 1; m < LP; m *= 2) ss += __shfl_xor(ss, int(m), 64);
+        for (int e = 0; e < 8; ++e) ss = fma(y[e], y[e], ss);
+        ss += dpp_f64<DPP_QUAD_XOR1>(ss);
+        ss += dpp_f64<DPP_QUAD_XOR2>(ss);
+        ss += dpp_f64<DPP_ROW_HALF_MIRROR>(ss);
+        if constexpr (LP == 16) ss += dpp_f64<DPP_ROW_MIRROR>(ss);
         f = 1.0 / sqrt(ss * (1.0 / HD) + double(a.s.eps));
-      }
-      auto normed = [&](uint32_t d) { return gain ? double(row[d]) * f * double(gain[d]) : double(row[d]); };
-      double y[8];
+        float gs[8], go[8];
+        *reinterpret_cast<float4*>(gs) = *reinterpret_cast<const float4*>(gain + d0);
+        *reinterpret_cast<float4*>(gs + 4) = *reinterpret_cast<const float4*>(gain + d0 + 4);
+        if constexpr (HALF) {
+          *reinterpret_cast<float4*>(go) = *reinterpret_cast<const float4*>(gain + o0);
+          *reinterpret_cast<float4*>(go + 4) = *reinterpret_cast<const float4*>(gain + o0 + 4);
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t d = d0 + e;
-        y[e] = normed(d);
-        if (d < a.rope.dims) {
-          const uint32_t i = a.rope.half ? (d < half ? d : d - half) : d / 2;
-          const bool second = a.rope.half ? d >= half : d % 2;
-          const double other = normed(a.rope.half ? (second ? d - half : d + half) : d ^ 1u);
-          const double2 cs = turn[i];
-          y[e] = second ? other * cs.y + y[e] * cs.x : y[e] * cs.x - other * cs.y;
+        for (int e = 0; e < 8; ++e) {
+          y[e] *= double(gs[e]);
+          if constexpr (HALF) w[e] *= double(go[e]);
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = y[e];
+      for (int e = 0; e < (HALF ? 8 : 4); ++e) {
+        if constexpr (HALF) {
+          y[e] = (y[e] * cs[e].x - w[e] * cs[e].y) * f;
+        } else {
+          const double p = y[2 * e], q = y[2 * e + 1];
+          y[2 * e] = (p * cs[e].x - q * cs[e].y) * f;
+          y[2 * e + 1] = (p * cs[e].y + q * cs[e].x) * f;
+        }
+      }
     }
-    if (h < a.s.H) {
-      float* dst = a.q_out + ((size_t(b) * a.c.n + t) * a.s.H + h) * HD + d0;
-      *reinterpret_cast<float4*>(dst) = make_float4(float(x[0]), float(x[1]), float(x[2]), float(x[3]));
-      *reinterpret_cast<float4*>(dst + 4) = make_float4(float(x[4]), float(x[5]), float(x[6]), float(x[7]));
+    const uint32_t now = h;
+    h += HPB * gridDim.y;
+    load(h);
+    if (now < a.s.H) {
+      float* dst = a.q_out + ((size_t(b) * a.c.n + t) * a.s.H + now) * HD + d0;
+      *reinterpret_cast<float4*>(dst) = make_float4(float(y[0]), float(y[1]), float(y[2]), float(y[3]));
+      *reinterpret_cast<float4*>(dst + 4) = make_float4(float(y[4]), float(y[5]), float(y[6]), float(y[7]));
       continue;
     }
     // the group's largest by size (4 lanes), the first of equals
     double big = 0.0;
-    bool odd = false;
+    uint32_t odd = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      big = fmax(big, fabs(x[e]));
-      odd |= !(fabs(x[e]) < 16384.0);
+      big = fmax(big, fabs(y[e]));
+      odd |= !(fabs(y[e]) < 16384.0);
     }
-    big = fmax(big, __shfl_xor(big, 1, 64));
-    big = fmax(big, __shfl_xor(big, 2, 64));
-    int first = 1 << 20;  // place in the group, doubled, + 1 of a negative one
+    big = fmax(big, dpp_f64<DPP_QUAD_XOR1>(big));
+    big = fmax(big, dpp_f64<DPP_QUAD_XOR2>(big));
+    uint32_t first = 1000;  // place in the group, doubled, + 1 of a negative one
 #pragma unroll
     for (int e = 7; e >= 0; --e)
-      if (fabs(x[e]) == big) first = 2 * int(8 * (l % 4) + e) + (x[e] < 0.0 ? 1 : 0);
-    int any = odd;
-#pragma unroll
-    for (int m = 1; m < 4; m *= 2) {
-      first = min(first, __shfl_xor(first, m, 64));
-      any |= __shfl_xor(any, m, 64);
-    }
-    odd = any != 0;
+      if (fabs(y[e]) == big) first = 2 * (8 * (l % 4) + e) + (y[e] < 0.0 ? 1 : 0);
+    first = min(first, dpp_u32<DPP_QUAD_XOR1>(first));
+    first = min(first, dpp_u32<DPP_QUAD_XOR2>(first));
+    odd |= dpp_u32<DPP_QUAD_XOR1>(odd);
+    odd |= dpp_u32<DPP_QUAD_XOR2>(odd);
     double d = rounded8(big * 0.125);
     if (!(first & 1)) d = -d;
+    const double inv = odd || d == 0.0 ? 0.0 : 1.0 / d;
+    // y / d is y inv but for 2^-52 of it.  It is at most 8 2^9 / (2^9 - 1): taken to a multiple of 2^-40 first, one that is
+    // halfway between whole numbers is so again (no other quotient of a value's 24 bits by 8 comes so near).
     uint32_t code[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = odd || d == 0.0 ? 8u : uint32_t(int(fmin(fmax(rint(x[e] / d), -8.0), 7.0)) + 8);
+    for (int e = 0; e < 8; ++e) {
+      const double near = (odd ? 0.0 : y[e]) * inv + 0x1.8p12;
+      code[e] = uint32_t(min(max(int(rint(near - 0x1.8p12)), -8), 7) + 8);
+    }
     const float scale = odd ? NAN : float(d);
-    const uint32_t g = value ? h - a.s.H - a.s.G : h - a.s.H, j = l / 4;
+    const uint32_t g = value ? now - a.s.H - a.s.G : now - a.s.H, j = l / 4;
     float* held = value ? a.v_held : a.k_held;
     if (held) {
       held += ((size_t(b) * a.c.n + t) * a.s.G + g) * HD + d0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) held[e] = scale * float(int(code[e]) - 8);
+      for (int e = 0; e < 8; e += 4)
+        *reinterpret_cast<float4*>(held + e) = make_float4(scale * float(int(code[e]) - 8), scale * float(int(code[e + 1]) - 8),
+                                                           scale * float(int(code[e + 2]) - 8), scale * float(int(code[e + 3]) - 8));
     }
     if (!there) continue;
     if (odd) atomicOr(a.s.err, S2HIP_PAGES_ERR_RANGE);
@@ -1149,7 +1198,11 @@ hipError_t by_dim(uint32_t hd, F&& f) {
 hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s) {
   return by_dim(hd, [&](auto HD) {
     const uint32_t tokens = a.c.R * a.c.n, steps = (a.s.H + 2 * a.s.G + 2048 / HD() - 1) / (2048 / HD());
-    hipLaunchKernelGGL(pg_append_kernel<HD()>, dim3(tokens, min(steps, max(1u, 512 / tokens))), dim3(256), 0, s, a);
+    const dim3 grid(tokens, min(steps, max(1u, 512 / tokens)));
+    if (a.rope.half)
+      hipLaunchKernelGGL((pg_append_kernel<HD(), true>), grid, dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((pg_append_kernel<HD(), false>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
   });
 }
