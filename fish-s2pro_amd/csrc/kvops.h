@@ -98,8 +98,6 @@ struct KvEvictArgs {
 
 hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStream_t s);
 hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const KvWorkspace& w, hipStream_t s);
-// The splits' states of every row of the output joined.
-hipError_t launch_kv_join(uint32_t hd, const KvAttendArgs& a, const KvSplit& sp, hipStream_t s);
 hipError_t launch_kv_evict(const KvEvictArgs& a, const KvWorkspace& w, uint32_t hd, hipStream_t s);
 hipError_t launch_kv_take_errors(uint32_t* err, uint32_t* taken, hipStream_t s);
 

@@ -1757,22 +1757,6 @@ hipError_t by_shape(uint32_t hd, bool f16, F&& f) {
 
 }  // namespace
 
-template <int HD>
-static void join_launch(const KvAttendArgs& a, const KvSplit& sp, float* stat, hipStream_t s) {
-  const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD / 4);
-  if (out_rows <= 2048)
-    hipLaunchKernelGGL((kv_join_kernel<HD, 1024 / HD>), dim3(out_rows), dim3(256), 0, s, a, sp, stat);
-  else
-    hipLaunchKernelGGL((kv_join_kernel<HD, 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
-}
-
-hipError_t launch_kv_join(uint32_t hd, const KvAttendArgs& a, const KvSplit& sp, hipStream_t s) {
-  return by_shape(hd, true, [&](auto HD, auto) {
-    join_launch<HD()>(a, sp, nullptr, s);
-    return hipGetLastError();
-  });
-}
-
 hipError_t launch_kv_append(uint32_t hd, bool f16, const KvAppendArgs& a, hipStream_t s) {
   return by_shape(hd, f16, [&](auto HD, auto KH) {
     const uint32_t tokens = a.c.R * a.c.n, steps = (a.s.H + 2 * a.s.G + 1024 / HD() - 1) / (1024 / HD());
@@ -1831,7 +1815,7 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_tile_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(256), 0, s, a, sp, stat);
     else
       hipLaunchKernelGGL((kv_step_kernel<HD(), KH()>), dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, a, sp, stat, keep);
-    const uint32_t out_rows = a.c.R * a.c.n * a.s.H;
+    const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     const uint32_t z = a.c.R + (a.pw_out ? 1 : 0), keys = a.pw_out ? max(a.c.P, a.c.cap) : a.c.cap;
     if (keep.own) {
       KvKeptGrid grid{};
@@ -1843,7 +1827,10 @@ hipError_t launch_kv_attend(uint32_t hd, bool f16, const KvAttendArgs& a, const 
       hipLaunchKernelGGL((kv_join_weights_kernel<HD()>), dim3(grid.joins + a.s.G * (grid.prefix + grid.own * a.c.R)), dim3(256), 0, s, a, sp, stat, keep, grid);
       return hipGetLastError();
     }
-    if (sp.splits > 1) join_launch<HD()>(a, sp, stat, s);
+    if (sp.splits > 1 && out_rows <= 2048)
+      hipLaunchKernelGGL((kv_join_kernel<HD(), 1024 / HD()>), dim3(out_rows), dim3(256), 0, s, a, sp, stat);
+    else if (sp.splits > 1)
+      hipLaunchKernelGGL((kv_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp, stat);
     if (a.w_out) {
       const uint32_t kb = KH() ? 256 : 128;
       // Steps of 32 rows.  Lengths are on the device: chunks are made for a cache of no more than the turn, whose key block i

@@ -90,6 +90,7 @@ class Pages : DeviceArrays {
     work_.cap_parts = 8192;
     work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
     work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
+    work_.ranges = alloc<uint2>(64);
     work_.refs = alloc<int32_t>(c.pages);
     work_.list = alloc<int32_t>(size_t(c.pages) * 2);
     work_.table = alloc<int32_t>(size_t(c.max_requests) * c.table_pages);

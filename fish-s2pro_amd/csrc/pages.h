@@ -64,6 +64,7 @@ struct PgWorkspace {
   float* part;     // [cap_parts][16][hd]: attention states
   float* part_ml;  // [cap_parts][16][2]
   size_t cap_parts;
+  uint2* ranges;   // [64]: a row tile's states
   int32_t* refs;   // [pages]
   int32_t* list;   // [2][pages]: free pages; holes and movers
   int32_t* table;  // [max_requests][width]

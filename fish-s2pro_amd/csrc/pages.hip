@@ -220,16 +220,27 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ half2v as_half2(uint32_t x) { return __builtin_bit_cast(half2v, x); }
 __device__ __forceinline__ half2v both(_Float16 x) { return half2v{x, x}; }
 
+// The mask of the codes and the bits of 16, in registers: as literals they would take an and and an or apart (an
+// instruction of three operands has no literal, and one scalar register).
+struct Bits {
+  uint32_t mask, sixteen;
+};
+__device__ __forceinline__ Bits code_bits() {
+  Bits b{0x03c003c0u, 0x4c004c00u};
+  asm("" : "+s"(b.mask));
+  asm("" : "+v"(b.sixteen));
+  return b;
+}
 // The two elements whose codes are in bits 4 F .. of a word's halves.
 template <int F>
-__device__ __forceinline__ half2v elements(uint32_t w, half2v d, half2v c) {
+__device__ __forceinline__ half2v elements(Bits bits, uint32_t w, half2v d, half2v c) {
   const uint32_t x = F == 0 ? w << 6 : F == 1 ? w << 2 : F == 2 ? w >> 2 : w >> 6;
-  return __builtin_elementwise_fma(as_half2((x & 0x03c003c0u) | 0x4c004c00u), d, c);
+  return __builtin_elementwise_fma(as_half2((x & bits.mask) | bits.sixteen), d, c);
 }
 // A key's eight elements of a word (dims in order).
-__device__ __forceinline__ half8 key8(uint32_t w, _Float16 d) {
+__device__ __forceinline__ half8 key8(Bits bits, uint32_t w, _Float16 d) {
   const half2v dd = both(d), c = both(d * _Float16(-24.0f));
-  const half2v a = elements<0>(w, dd, c), b = elements<1>(w, dd, c), e = elements<2>(w, dd, c), f = elements<3>(w, dd, c);
+  const half2v a = elements<0>(bits, w, dd, c), b = elements<1>(bits, w, dd, c), e = elements<2>(bits, w, dd, c), f = elements<3>(bits, w, dd, c);
   return half8{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
 }
 // Scales of tokens t0 t1, t2 t3 as pairs t0 t2, t1 t3.
@@ -330,6 +341,37 @@ struct PageWindow {
   }
 };
 
+// The blocks of a kv head, `blocks` of them, and its states [kv heads][blocks][16 rows].
+struct PgShare {
+  float* o;
+  float* ml;
+  uint2* ranges;  // [row tiles]: first block and number of them; NULL: blocks / tiles each
+  uint32_t tiles, blocks;
+};
+// The row tile of block x, its first block and how many it has: one at least, and the rest by the keys in its
+// requests' caches, so that no block has much more than another.
+struct Share {
+  uint32_t tile, first, count;
+};
+__device__ __forceinline__ Share share_of(const KvAttendArgs& a, const PgShare& sp, uint32_t x) {
+  if (!sp.ranges) {
+    const uint32_t count = sp.blocks / sp.tiles;
+    return {x / count, x / count * count, count};
+  }
+  const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep;  // (at most 64 row tiles)
+  uint32_t keys = 0;
+  if (lane < sp.tiles)
+    for (uint32_t b = lane * 16 / per; b <= min((lane * 16 + 15) / per, a.c.R - 1); ++b) {
+      const int32_t len = a.c.lens[b];
+      keys += len > 0 && len <= int32_t(a.c.cap) ? uint32_t(len) / 32 + 1 : 0u;
+    }
+  const uint32_t upto = wave_scan(keys), all = max(1u, lane_read_u32(upto, 63));
+  const uint32_t first = lane < sp.tiles ? lane + uint32_t(uint64_t(sp.blocks - sp.tiles) * (upto - keys) / all) : sp.blocks;
+  const uint32_t tile = uint32_t(__popcll(__ballot(first <= x))) - 1;  // (first goes up with the lane)
+  const uint32_t begin = lane_read_u32(first, int(tile)), end = tile == 63 ? sp.blocks : lane_read_u32(first, int(tile) + 1);
+  return {tile, begin, end - begin};
+}
+
 // A tile of 32 keys in two halves of 16, which may lie in different pages.
 struct PgTile {
   uint32_t req, key0, keys;  // request, first key; keys of it that are there
@@ -340,7 +382,7 @@ struct PgTile {
 };
 
 template <int HD>
-__global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArgs pa, KvSplit sp) {
+__global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArgs pa, PgShare sp) {
   constexpr int KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
   constexpr int OP = HD + 4;                          // padded row of the joined states
   constexpr float LIFT = F16_LIFT;
@@ -348,9 +390,12 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
   __shared__ float ml[STEP_WAVES][16][2];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
-  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G, tile = rest % sp.tiles, split = rest / sp.tiles;
+  const uint32_t g = blockIdx.x % a.s.G, block = blockIdx.x / a.s.G;
+  const Share share = share_of(a, sp, block);
+  const uint32_t tile = share.tile, split = block - share.first;
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
   const Chunk<HD> at{pa.p.shift};
+  const Bits bits = code_bits();
 
   const RawRequest raw = load_request(a.c, min(tile * 16 / per + lane, a.c.R - 1));
   const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
@@ -359,7 +404,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
 #pragma unroll
   for (int j = 0; j < HD / 16; ++j) qx[j] = *reinterpret_cast<const float4*>(a.q + q_at + 32 * (j / 2) + 8 * q4 + 4 * (j % 2));
   const PgRun run = pg_run<KT>(pa, tile * 16, 16, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-  const uint32_t b_lo = run.b_lo, lots = sp.splits * STEP_WAVES, lot = split * STEP_WAVES + wave;
+  const uint32_t b_lo = run.b_lo, lots = share.count * STEP_WAVES, lot = split * STEP_WAVES + wave;
   const uint32_t c_tiles = run.common / KT, c_lo = c_tiles * lot / lots, n_com = c_tiles * (lot + 1) / lots - c_lo;
   // (the own tiles the other way round: the waves with one more in common get one fewer)
   const uint32_t o_lo = run.tiles * (lots - 1 - lot) / lots, n_tiles = n_com + run.tiles * (lots - lot) / lots - o_lo;
@@ -478,7 +523,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
       floatx4 hi = floatx4{0.f, 0.f, 0.f, 0.f}, lo = hi;
 #pragma unroll
       for (int j = 0; j < GR; ++j) {
-        const half8 k8 = key8(kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
+        const half8 k8 = key8(bits, kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
         hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], hi, 0, 0, 0);
         lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], lo, 0, 0, 0);
       }
@@ -559,10 +604,10 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
         half2v de, dd;
         token_pairs(vs[h][c], de, dd);
         const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
-        v[h][0] = elements<0>(vc[h][c], de, ce);
-        v[h][1] = elements<1>(vc[h][c], de, ce);
-        v[h][2] = elements<2>(vc[h][c], dd, cd);
-        v[h][3] = elements<3>(vc[h][c], dd, cd);
+        v[h][0] = elements<0>(bits, vc[h][c], de, ce);
+        v[h][1] = elements<1>(bits, vc[h][c], de, ce);
+        v[h][2] = elements<2>(bits, vc[h][c], dd, cd);
+        v[h][3] = elements<3>(bits, vc[h][c], dd, cd);
       }
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -602,8 +647,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
   const float M_base = M_row == -INFINITY ? 0.0f : M_row;  // (then every l is 0, or no number)
 #pragma unroll
   for (int i = 0; i < STEP_WAVES; ++i) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_base), L_row);
-  const size_t part = ((size_t(g) * sp.tiles + tile) * sp.splits + split) * 16 + jr;
-  const bool last = sp.splits == 1;
+  const size_t part = (size_t(g) * sp.blocks + block) * 16 + jr;
+  const bool last = sp.blocks == sp.tiles;
+  if (sp.ranges && g == 0 && split == 0 && tid == 0) sp.ranges[tile] = make_uint2(share.first, share.count);
   const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
   const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
   if (last && !out_live) return;
@@ -634,7 +680,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 2) void pg_step_kernel(PgAttendArg
 constexpr int TILE_ROWS = 128;
 
 template <int HD>
-__global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSplit sp) {
+__global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShare sp) {
   constexpr int KT = 64, GR = HD / 32, DS = HD / 16, DT = HD / 32;
   constexpr uint32_t RB = HD * 2, PLANE = KT * RB, BUF = 2 * PLANE;  // bytes of a key's row, of the keys (and of the values), of both
   constexpr float LIFT = F16_LIFT;
@@ -646,8 +692,9 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
   const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
   const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
-  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const uint32_t splits = sp.blocks / sp.tiles, per = a.c.n * a.s.rep, rows = a.c.R * per;
   const Chunk<HD> at{pa.p.shift};
+  const Bits bits = code_bits();
 
   const RawRequest raw = load_request(a.c, min(tile * TILE_ROWS / per + lane, a.c.R - 1));
   const uint32_t my_row = tile * TILE_ROWS + wave * 32 + r32, row = min(my_row, rows - 1);
@@ -661,8 +708,8 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
   const PgRun run = pg_run<KT>(pa, tile * TILE_ROWS, TILE_ROWS, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint64_t has = __ballot(run.seg_keys != 0);
   if (!has) return;  // no row of a token
-  const uint32_t c_all = run.common / KT, c_lo = c_all * split / sp.splits, n_com = c_all * (split + 1) / sp.splits - c_lo;
-  const uint32_t o_lo = run.tiles * (sp.splits - 1 - split) / sp.splits, n_tiles = n_com + run.tiles * (sp.splits - split) / sp.splits - o_lo;
+  const uint32_t c_all = run.common / KT, c_lo = c_all * split / splits, n_com = c_all * (split + 1) / splits - c_lo;
+  const uint32_t o_lo = run.tiles * (splits - 1 - split) / splits, n_tiles = n_com + run.tiles * (splits - split) / splits - o_lo;
 
   uint32_t seg = 0;
   PageWindow window;
@@ -733,7 +780,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
     uint32_t k_to = buf * BUF + k_at(16 * wave + lane / 4, lane % 4), v_to = buf * BUF + v_at(2 * r16, 2 * wave + (q4 & 1u)) + 8 * (q4 >> 1);
     asm volatile("" : "+v"(k_to), "+v"(v_to));
 #pragma unroll
-    for (int j = 0; j < GR; ++j) *reinterpret_cast<lds_half8*>(lds0 + (k_to ^ (64u * j))) = key8(kc[j], as_half2(ks[j / 2])[j % 2]);
+    for (int j = 0; j < GR; ++j) *reinterpret_cast<lds_half8*>(lds0 + (k_to ^ (64u * j))) = key8(bits, kc[j], as_half2(ks[j / 2])[j % 2]);
     // scales of tokens that are not there may hold anything: 0
     const int there = w.gone ? 0 : int(w.keys) - int(16u * wave + 4u * q4);  // of the lane's four
     const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
@@ -759,7 +806,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
       half2v de, dd;
       token_pairs(vs[c], de, dd);
       const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
-      const half2v v[4] = {elements<0>(vc[c], de, ce), elements<1>(vc[c], de, ce), elements<2>(vc[c], dd, cd), elements<3>(vc[c], dd, cd)};
+      const half2v v[4] = {elements<0>(bits, vc[c], de, ce), elements<1>(bits, vc[c], de, ce), elements<2>(bits, vc[c], dd, cd), elements<3>(bits, vc[c], dd, cd)};
 #pragma unroll
       for (int x = 0; x < 2; ++x)  // tokens 0 2 1 3 of the four, the first or second half of a piece
         *reinterpret_cast<lds_half4*>(lds0 + (v_to + (32 * c + x) * (KT * 2))) = half4{v[x][0], v[x][1], v[2 + x][0], v[2 + x][1]};
@@ -920,9 +967,9 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
   }
 
   l = half_reduce(l, [](float p, float q) { return p + q; });
-  const bool last = sp.splits == 1;
+  const bool last = splits == 1;
   if (my_row >= rows || (last && !live)) return;
-  const size_t part = ((size_t(g) * sp.tiles + row / 16) * sp.splits + split) * 16 + row % 16;
+  const size_t part = ((size_t(g) * sp.tiles + row / 16) * splits + split) * 16 + row % 16;
   float* dst = last ? a.out + at_row * HD : sp.o + part * HD;
   const float f = last ? (m == -INFINITY ? NAN : 1.0f / l) : 1.0f;
 #pragma unroll
@@ -935,6 +982,72 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, KvSpli
     sp.ml[2 * part] = m - LIFT;
     sp.ml[2 * part + 1] = l;
   }
+}
+
+// The blocks' states of the rows of the output joined: HD / 4 threads per row and TEAM teams of them per row, each
+// with every TEAM-th state.
+template <int HD, int TEAM>
+__global__ __launch_bounds__(256) void pg_join_kernel(KvAttendArgs a, PgShare sp) {
+  constexpr uint32_t LP = HD / 4, ROWS = 256 / LP / TEAM;
+  __shared__ floatx4 os[TEAM == 1 ? 1 : TEAM][LP];
+  __shared__ float ms[TEAM], ls[TEAM];
+  const uint32_t tid = threadIdx.x, team = tid / LP % TEAM, d = tid % LP;
+  const uint32_t at = blockIdx.x * ROWS + tid / LP / TEAM;
+  const bool is_row = at < a.c.R * a.c.n * a.s.H;
+  const uint32_t out = is_row ? at : 0u, bt = out / a.s.H, h = out % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
+  const RawRequest raw = load_request(a.c, b);
+  const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16, even = sp.blocks / sp.tiles;
+  const uint2 range = sp.ranges ? sp.ranges[tile] : make_uint2(tile * even, even);
+  const size_t part = (size_t(g) * sp.blocks + range.x) * 16 + row % 16;
+  float M = -INFINITY, L = 0.0f;
+  floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t s0 = team; s0 < range.y; s0 += 4 * TEAM) {
+    floatx4 y[4];
+    float2 ml[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t s = min(s0 + i * TEAM, range.y - 1);
+      ml[i] = *reinterpret_cast<const float2*>(sp.ml + 2 * (part + 16 * s));
+      if (TEAM > 1 || s0 + i < range.y) y[i] = *reinterpret_cast<const floatx4*>(sp.o + (part + 16 * s) * HD + 4 * d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (s0 + i * TEAM >= range.y) continue;
+      if (ml[i].x == -INFINITY) {  // no key (zeros), or none but of no number
+        x += y[i];
+        L += ml[i].y;
+        continue;
+      }
+      const float mn = fmaxf(M, ml[i].x);
+      const float f0 = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(ml[i].x - mn);
+      L = L * f0 + ml[i].y * f1;
+      x = x * f0 + y[i] * f1;
+      M = mn;
+    }
+  }
+  if constexpr (TEAM > 1) {
+    os[team][d] = x;
+    if (d == 0) {
+      ms[team] = M;
+      ls[team] = L;
+    }
+    __syncthreads();
+    if (team) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) all = fmaxf(all, ms[i]);
+    x = floatx4{0.f, 0.f, 0.f, 0.f};
+    L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) {
+      const float f = ms[i] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[i] - all);
+      x += os[i][d] * f;
+      L = fmaf(ls[i], f, L);
+    }
+    M = all;
+  }
+  if (!is_row || t >= checked(a.c, raw, nullptr).fresh) return;
+  *reinterpret_cast<floatx4*>(a.out + size_t(out) * HD + 4 * d) = x * (M == -INFINITY ? NAN : 1.0f / L);
 }
 
 // ---------------------------------------------------------------------------
@@ -1209,25 +1322,32 @@ hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s) {
 
 hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspace& w, hipStream_t s) {
   const KvAttendArgs& a = pa.a;
-  KvSplit sp{};
+  PgShare sp{};
   sp.o = w.part;
   sp.ml = w.part_ml;
-  sp.up = 1.0f;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
   const size_t scores = size_t(a.s.G) * rows * (a.c.cap - min(a.c.n, a.c.cap) / 2);
   const bool many = a.c.n * a.s.rep >= 32 && scores * hd > 10000000u * size_t(128);
   const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles);
   const uint32_t most = (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));  // key tiles of a row tile, at most
-  sp.splits = max(1u, min(512 / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
-  if (!many && most <= 24u * 128 / hd) sp.splits = 1;
-  if (size_t(a.s.G) * sp.tiles * sp.splits > w.cap_parts) sp.splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
+  const uint32_t fill = many ? 512 : 768;
+  uint32_t splits = max(1u, min(fill / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
+  if (!many && most <= 24u * 128 / hd) splits = 1;
+  if (size_t(a.s.G) * sp.tiles * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
+  sp.blocks = sp.tiles * splits;
+  if (!many && splits > 1 && sp.tiles > 1 && sp.tiles <= 64) sp.ranges = w.ranges;
   return by_dim(hd, [&](auto HD) {
     if (many)
-      hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * sp.splits), dim3(256), 0, s, pa, sp);
+      hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * splits), dim3(256), 0, s, pa, sp);
     else
-      hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(lots * sp.splits), dim3(64 * STEP_WAVES), 0, s, pa, sp);
-    return sp.splits > 1 ? launch_kv_join(hd, a, sp, s) : hipGetLastError();
+      hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+    const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
+    if (splits > 1 && out_rows <= 2048)
+      hipLaunchKernelGGL((pg_join_kernel<HD(), 1024 / HD()>), dim3(out_rows), dim3(256), 0, s, a, sp);
+    else if (splits > 1)
+      hipLaunchKernelGGL((pg_join_kernel<HD(), 1>), dim3((out_rows + teams - 1) / teams), dim3(256), 0, s, a, sp);
+    return hipGetLastError();
   });
 }
 
