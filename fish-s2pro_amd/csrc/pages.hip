@@ -287,8 +287,21 @@ struct PgRun {
   uint32_t seg_end;   // its last own tile + 1
 };
 
+// The first 64 page numbers of a row tile's first FEW requests, one per lane: loaded before anything is known of the requests.
+constexpr int FEW = 4;
+struct Pages64 {
+  int32_t of[FEW];
+};
+__device__ __forceinline__ Pages64 load_pages(const PgAttendArgs& pa, uint32_t b_lo) {
+  Pages64 p;
+  const uint32_t i = min(threadIdx.x & 63u, pa.p.width - 1);
+#pragma unroll
+  for (int j = 0; j < FEW; ++j) p.of[j] = pa.p.table[size_t(min(b_lo + j, pa.a.c.R - 1)) * pa.p.width + i];
+  return p;
+}
+
 template <int KT>
-__device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, uint32_t n_rows, RawRequest raw, uint32_t* err) {
+__device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, uint32_t n_rows, RawRequest raw, const Pages64& early, uint32_t* err) {
   const KvAttendArgs& a = pa.a;
   const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep, row1 = min(row0 + n_rows, a.c.R * per);
   PgRun r{};
@@ -302,17 +315,30 @@ __device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, u
   // what every row with a token sees, as far as the tables agree
   const uint64_t has = __ballot(r.seg_keys != 0);
   if (__popcll(has) > 1) {
-    const uint32_t lead = uint32_t(__ffsll((unsigned long long)has)) - 1;
     uint32_t least = r.seg_keys ? r.rq.len - r.rq.fresh + 1 : 0xffffffffu;
     least = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
     const uint32_t pages = least >> pa.p.shift;
     uint32_t same = 0;
     for (; same < pages;) {
-      const uint32_t i = min(same + lane, pages - 1);
-      const int32_t mine = pa.p.table[size_t(r.b_lo + lead) * pa.p.width + i];
-      bool differs = false;
-      for (uint64_t rest = has & (has - 1); rest; rest &= rest - 1)
-        differs |= pa.p.table[size_t(r.b_lo + uint32_t(__ffsll((unsigned long long)rest)) - 1) * pa.p.width + i] != mine;
+      const uint32_t i = min(same + lane, pages - 1);  // (of the first pages, lane i's: what is behind is looked at twice or not)
+      int32_t first = 0;
+      bool differs = false, led = false;
+      auto look = [&](int32_t page) {
+        differs |= led && page != first;
+        if (!led) first = page;
+        led = true;
+      };
+      if (same == 0) {
+#pragma unroll
+        for (int j = 0; j < FEW; ++j)
+          if ((has >> j) & 1u) look(early.of[j]);
+        for (uint64_t rest = has >> FEW << FEW; rest; rest &= rest - 1)
+          look(pa.p.table[size_t(r.b_lo + uint32_t(__ffsll((unsigned long long)rest)) - 1) * pa.p.width + min(lane, pa.p.width - 1)]);
+        differs = differs && lane < pages;
+      } else {
+        for (uint64_t rest = has; rest; rest &= rest - 1)
+          look(pa.p.table[size_t(r.b_lo + uint32_t(__ffsll((unsigned long long)rest)) - 1) * pa.p.width + i]);
+      }
       const uint64_t out = __ballot(differs);
       if (out) {
         same += uint32_t(__ffsll((unsigned long long)out)) - 1;
@@ -331,6 +357,13 @@ __device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, u
 struct PageWindow {
   uint32_t b = 0xffffffffu, first = 0;
   int32_t page = 0;
+  __device__ __forceinline__ void begin(const Pages64& early, uint32_t b_lo, uint32_t req) {  // (where req is one of the few)
+    if (req - b_lo >= uint32_t(FEW)) return;
+    b = req;
+#pragma unroll
+    for (int j = 0; j < FEW; ++j)
+      if (req - b_lo == uint32_t(j)) page = early.of[j];
+  }
   __device__ __forceinline__ uint32_t get(const PgPool& p, uint32_t req, uint32_t i) {
     if (req != b || i - first >= 64u) {
       b = req;
@@ -398,24 +431,29 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   const Bits bits = code_bits();
 
   const RawRequest raw = load_request(a.c, min(tile * 16 / per + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, tile * 16 / per);
   const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
   const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
   float4 qx[HD / 16];  // dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
 #pragma unroll
   for (int j = 0; j < HD / 16; ++j) qx[j] = *reinterpret_cast<const float4*>(a.q + q_at + 32 * (j / 2) + 8 * q4 + 4 * (j % 2));
-  const PgRun run = pg_run<KT>(pa, tile * 16, 16, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const PgRun run = pg_run<KT>(pa, tile * 16, 16, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint32_t b_lo = run.b_lo, lots = share.count * STEP_WAVES, lot = split * STEP_WAVES + wave;
   const uint32_t c_tiles = run.common / KT, c_lo = c_tiles * lot / lots, n_com = c_tiles * (lot + 1) / lots - c_lo;
   // (the own tiles the other way round: the waves with one more in common get one fewer)
   const uint32_t o_lo = run.tiles * (lots - 1 - lot) / lots, n_tiles = n_com + run.tiles * (lots - lot) / lots - o_lo;
 
   uint32_t seg = 0;
+  const uint32_t lead = uint32_t(__ffsll((unsigned long long)__ballot(run.seg_keys != 0))) - 1;  // (with the others' pages in common)
   PageWindow window;
+  if (n_com == 0)
+    while (seg < 63 && o_lo >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+  window.begin(early, b_lo, b_lo + (n_com ? lead : seg));
   auto where = [&](uint32_t i) {
     PgTile w;
     if (i < n_com) {
       w.seg = -1;
-      w.req = b_lo + uint32_t(__ffsll((unsigned long long)__ballot(run.seg_keys != 0))) - 1;
+      w.req = b_lo + lead;
       w.key0 = (c_lo + i) * KT;
       w.keys = KT;
     } else {
@@ -697,6 +735,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   const Bits bits = code_bits();
 
   const RawRequest raw = load_request(a.c, min(tile * TILE_ROWS / per + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, tile * TILE_ROWS / per);
   const uint32_t my_row = tile * TILE_ROWS + wave * 32 + r32, row = min(my_row, rows - 1);
   const uint32_t b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
   const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
@@ -705,14 +744,18 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
     for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
-  const PgRun run = pg_run<KT>(pa, tile * TILE_ROWS, TILE_ROWS, raw, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const PgRun run = pg_run<KT>(pa, tile * TILE_ROWS, TILE_ROWS, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint64_t has = __ballot(run.seg_keys != 0);
   if (!has) return;  // no row of a token
   const uint32_t c_all = run.common / KT, c_lo = c_all * split / splits, n_com = c_all * (split + 1) / splits - c_lo;
   const uint32_t o_lo = run.tiles * (splits - 1 - split) / splits, n_tiles = n_com + run.tiles * (splits - split) / splits - o_lo;
 
   uint32_t seg = 0;
+  const uint32_t lead = uint32_t(__ffsll((unsigned long long)has)) - 1;  // (with the others' pages in common)
   PageWindow window;
+  if (n_com == 0)
+    while (seg < 63 && o_lo >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+  window.begin(early, run.b_lo, run.b_lo + (n_com ? lead : seg));
   // a tile, and where the wave's 16 keys of it are
   struct Tile {
     uint32_t key0, keys;
@@ -726,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
     uint32_t req;
     if (i < n_com) {
       w.seg = -1;
-      req = run.b_lo + uint32_t(__ffsll((unsigned long long)has)) - 1;
+      req = run.b_lo + lead;
       w.key0 = (c_lo + i) * KT;
       w.keys = KT;
     } else {
@@ -1331,12 +1374,19 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
   const bool many = a.c.n * a.s.rep >= 32 && scores * hd > 10000000u * size_t(128);
   const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles);
   const uint32_t most = (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));  // key tiles of a row tile, at most
-  const uint32_t fill = many ? 512 : 768;
+  // Blocks of the step kernel, by the key tiles that a wave of 256 would walk at most: short runs end sooner with fewer
+  // states to join, long ones want more waves to take turns.  256 : 512 : 768 blocks, us: 8 x 1 over 1500 + 512 (4 tiles) 13 :
+  // 17 : 21, 16 x 1 over 1000 (5) 17 : 18 : 21, 1 x 1 over 30000 (7) 21 : 20 : 22, 16 x 1 over 6000 (24) 44 : 35 : 34, over
+  // 32001 (126) 202 : 127 : 120.
+  const size_t walk = size_t(lots) * most / 1024;
+  const uint32_t fill = many || (walk >= 6 && walk < 24) ? 512 : walk < 6 ? 256 : 768;
   uint32_t splits = max(1u, min(fill / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
   if (!many && most <= 24u * 128 / hd) splits = 1;
   if (size_t(a.s.G) * sp.tiles * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   sp.blocks = sp.tiles * splits;
-  if (!many && splits > 1 && sp.tiles > 1 && sp.tiles <= 64) sp.ranges = w.ranges;
+  // Shares by length where runs are long (1 of 16 over 32001, the others over 500: 30 us, equal shares 39): they take up to a
+  // microsecond to work out.
+  if (!many && splits > 1 && walk >= 6 && sp.tiles > 1 && sp.tiles <= 64) sp.ranges = w.ranges;
   return by_dim(hd, [&](auto HD) {
     if (many)
       hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * splits), dim3(256), 0, s, pa, sp);
