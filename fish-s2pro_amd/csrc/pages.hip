@@ -723,7 +723,8 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   constexpr uint32_t RB = HD * 2, PLANE = KT * RB, BUF = 2 * PLANE;  // bytes of a key's row, of the keys (and of the values), of both
   constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
-  // of tiles i, i + 1 and the one behind: bit w: the 16 keys of wave w lie in no page; a group's first value of no number
+  // of tiles i, i + 1 and the one behind: bit w: the 16 keys of wave w lie in no page, bit 8: there are values of no number; a
+  // group's first
   __shared__ uint32_t gone_tile[3], odd_tile[3][GR];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5, r16 = lane & 15u, q4 = lane >> 4;
@@ -842,6 +843,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
           const uint32_t first = take_odd_scales(vs[c], x) + 16 * wave + 4 * q4 + 2 * x;
           if (first < KT) atomicMin(&odd_tile[flag][c], first);
         }
+      if (lane == 0) atomicOr(&gone_tile[flag], 256u);
     }
     if (w.gone && lane == 0) atomicOr(&gone_tile[flag], 1u << wave);
 #pragma unroll
@@ -918,7 +920,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
         load(next);
       }
     }
-    const uint32_t gone = uniform(gone_tile[flag]);
+    const uint32_t gone = uniform(gone_tile[flag]);  // (and bit 8)
     const int limit = !live ? -1 : cur.seg < 0 ? 0x7fffffff : cur.seg == own_seg ? own_limit : -1;
     if (__any(limit >= int(cur.key0))) {  // else nothing of it is for this wave's rows
       uint32_t k_from = buf * BUF + k_at(r32, h2), v_from = buf * BUF + v_at(r32, h2);
@@ -944,8 +946,9 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      const bool whole = __all(!live || limit >= int(cur.key0) + KT - 1) && !gone;
+      const bool whole = __all(!live || limit >= int(cur.key0) + KT - 1) && !(gone & 15u);
       if (!whole) {
+        asm volatile("");  // (a branch: selects for every tile would cost as much as a fifth of its other vector work)
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
@@ -969,10 +972,13 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
         m = to;
       }
       const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
+      if (gone >> 8) {  // values of no number
+        asm volatile("");
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const uint32_t first = uniform(odd_tile[flag][dt]);
-        if (first < KT && limit >= int(cur.key0 + first)) o[dt] = floatx16{} + NAN;
+        for (int dt = 0; dt < DT; ++dt) {
+          const uint32_t first = uniform(odd_tile[flag][dt]);
+          if (first < KT && limit >= int(cur.key0 + first)) o[dt] = floatx16{} + NAN;
+        }
       }
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
