@@ -820,21 +820,28 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   auto v_at = [](uint32_t dim, uint32_t piece) { return PLANE + dim * (KT * 2) + ((piece ^ ((dim >> 1) & 7u)) << 4); };
   lds_byte* const lds0 = (lds_byte*)lds;
   typedef __attribute__((address_space(3))) half4 lds_half4;
-  auto store = [&](const Tile& w, uint32_t buf, uint32_t flag) {
-    uint32_t k_to = buf * BUF + k_at(16 * wave + lane / 4, lane % 4), v_to = buf * BUF + v_at(2 * r16, 2 * wave + (q4 & 1u)) + 8 * (q4 >> 1);
+  // The wave's 16 keys and values from registers to LDS, in pieces: 0 .. GR - 1 a key's words, from GR on a group of the
+  // values, before which their scales are looked over.
+  uint32_t k_to = 0, v_to = 0;
+  auto store_begin = [&](uint32_t buf) {
+    k_to = buf * BUF + k_at(16 * wave + lane / 4, lane % 4);
+    v_to = buf * BUF + v_at(2 * r16, 2 * wave + (q4 & 1u)) + 8 * (q4 >> 1);
     asm volatile("" : "+v"(k_to), "+v"(v_to));
+  };
+  auto store_key = [&](int j) { *reinterpret_cast<lds_half8*>(lds0 + (k_to ^ (64u * j))) = key8(bits, kc[j], as_half2(ks[j / 2])[j % 2]); };
+  auto store_scales = [&](const Tile& w, uint32_t flag) {
+    if (w.gone || w.keys < KT) {  // scales of tokens that are not there may hold anything: 0
+      asm volatile("");
+      const int there = w.gone ? 0 : int(w.keys) - int(16u * wave + 4u * q4);  // of the lane's four
+      const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
 #pragma unroll
-    for (int j = 0; j < GR; ++j) *reinterpret_cast<lds_half8*>(lds0 + (k_to ^ (64u * j))) = key8(bits, kc[j], as_half2(ks[j / 2])[j % 2]);
-    // scales of tokens that are not there may hold anything: 0
-    const int there = w.gone ? 0 : int(w.keys) - int(16u * wave + 4u * q4);  // of the lane's four
-    const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
+      for (int c = 0; c < GR; ++c) vs[c] = u32x2{vs[c][0] & low, vs[c][1] & high};
+    }
     half2v z = half2v{};
 #pragma unroll
-    for (int c = 0; c < GR; ++c) {
-      vs[c] = u32x2{vs[c][0] & low, vs[c][1] & high};
+    for (int c = 0; c < GR; ++c)
 #pragma unroll
       for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[c][x]), half2v{}, z);
-    }
     if (__any(!(z[0] == _Float16(0)) || !(z[1] == _Float16(0)))) {  // of no number: 0 too, and noted
 #pragma unroll
       for (int c = 0; c < GR; ++c)
@@ -846,15 +853,28 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       if (lane == 0) atomicOr(&gone_tile[flag], 256u);
     }
     if (w.gone && lane == 0) atomicOr(&gone_tile[flag], 1u << wave);
+  };
+  auto store_value = [&](int c) {
+    half2v de, dd;
+    token_pairs(vs[c], de, dd);
+    const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
+    const half2v v[4] = {elements<0>(bits, vc[c], de, ce), elements<1>(bits, vc[c], de, ce), elements<2>(bits, vc[c], dd, cd), elements<3>(bits, vc[c], dd, cd)};
 #pragma unroll
-    for (int c = 0; c < GR; ++c) {
-      half2v de, dd;
-      token_pairs(vs[c], de, dd);
-      const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
-      const half2v v[4] = {elements<0>(bits, vc[c], de, ce), elements<1>(bits, vc[c], de, ce), elements<2>(bits, vc[c], dd, cd), elements<3>(bits, vc[c], dd, cd)};
+    for (int x = 0; x < 2; ++x)  // tokens 0 2 1 3 of the four, the first or second half of a piece
+      *reinterpret_cast<lds_half4*>(lds0 + (v_to + (32 * c + x) * (KT * 2))) = half4{v[x][0], v[x][1], v[2 + x][0], v[2 + x][1]};
+  };
+  auto store_piece = [&](int c) {
+    if (c < GR)
+      store_key(c);
+    else
+      store_value(c - GR);
+  };
+  auto store = [&](const Tile& w, uint32_t buf, uint32_t flag) {
+    store_begin(buf);
+    store_scales(w, flag);
 #pragma unroll
-      for (int x = 0; x < 2; ++x)  // tokens 0 2 1 3 of the four, the first or second half of a piece
-        *reinterpret_cast<lds_half4*>(lds0 + (v_to + (32 * c + x) * (KT * 2))) = half4{v[x][0], v[x][1], v[2 + x][0], v[2 + x][1]};
+    for (int c = 0; c < 2 * GR; ++c) {
+      store_piece(c);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -912,40 +932,52 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
     const Tile cur = w;
     if (tid < GR) odd_tile[flag2][tid] = KT;  // (last looked at a tile ago)
     if (tid == 0) gone_tile[flag2] = 0;
-    if (i + 1 < n_tiles) {
-      store(next, buf ^ 1u, flag1);
+    const uint32_t gone = uniform(gone_tile[flag]);  // (and bit 8)
+    const bool more = i + 1 < n_tiles;
+    const int limit = !live ? -1 : cur.seg < 0 ? 0x7fffffff : cur.seg == own_seg ? own_limit : -1;
+    const bool sees = __any(limit >= int(cur.key0));  // else nothing of it is for this wave's rows
+    if (more && !sees) store(next, buf ^ 1u, flag1);
+    uint32_t k_from = buf * BUF + k_at(r32, h2), v_from = buf * BUF + v_at(r32, h2);
+    asm volatile("" : "+v"(k_from), "+v"(v_from));
+    auto value8 = [&](int sub, int st, int dt) { return *reinterpret_cast<const lds_half8*>(lds0 + ((v_from ^ (64u * sub + 32u * st)) + 32 * dt * (KT * 2))); };
+    floatx16 s[2] = {};
+    if (sees) {
+      // A step: 16 dims of all scores, and a piece of the next tile (of what the registers hold, where there is none: it
+      // goes where nobody reads).  Fragments are read a step ahead; the barriers keep the compiler from reading all of
+      // them first, the groups have it put other work between the products, which take as long as eight of it each.
+      store_begin(buf ^ 1u);
+      if (more) store_scales(next, flag1);
+      half8 k8[2][2];
+      auto read = [&](int c) {
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) k8[c % 2][sub] = *reinterpret_cast<const lds_half8*>(lds0 + ((k_from ^ (32u * c)) + 32 * sub * RB));
+      };
+      read(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < DS; ++c) {
+        if (c + 1 < DS) read(c + 1);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][0], qh[c], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][1], qh[c], s[1], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][0], ql[c], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][1], ql[c], s[1], 0, 0, 0);
+        store_piece(c);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+          __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // vector instructions
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (more) {
       w = next;
       if (i + 2 < n_tiles) {
         next = where(i + 2);
         load(next);
       }
     }
-    const uint32_t gone = uniform(gone_tile[flag]);  // (and bit 8)
-    const int limit = !live ? -1 : cur.seg < 0 ? 0x7fffffff : cur.seg == own_seg ? own_limit : -1;
-    if (__any(limit >= int(cur.key0))) {  // else nothing of it is for this wave's rows
-      uint32_t k_from = buf * BUF + k_at(r32, h2), v_from = buf * BUF + v_at(r32, h2);
-      asm volatile("" : "+v"(k_from), "+v"(v_from));
-      auto value8 = [&](int sub, int st, int dt) { return *reinterpret_cast<const lds_half8*>(lds0 + ((v_from ^ (64u * sub + 32u * st)) + 32 * dt * (KT * 2))); };
-      // Fragments are read two products ahead; the barriers keep the compiler from reading all of them first.
-      floatx16 s[2] = {};
-      {
-        half8 k8[3][2];
-        auto read = [&](int c) {
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub) k8[c % 3][sub] = *reinterpret_cast<const lds_half8*>(lds0 + ((k_from ^ (32u * c)) + 32 * sub * RB));
-        };
-        read(0);
-        read(1);
-#pragma unroll
-        for (int c = 0; c < DS; ++c) {
-          if (c + 2 < DS) read(c + 2);
-          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], qh[c], s[0], 0, 0, 0);
-          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], qh[c], s[1], 0, 0, 0);
-          s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], ql[c], s[0], 0, 0, 0);
-          s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], ql[c], s[1], 0, 0, 0);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
+    if (sees) {
       const bool whole = __all(!live || limit >= int(cur.key0) + KT - 1) && !(gone & 15u);
       if (!whole) {
         asm volatile("");  // (a branch: selects for every tile would cost as much as a fifth of its other vector work)
@@ -980,36 +1012,46 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
           if (first < KT && limit >= int(cur.key0 + first)) o[dt] = floatx16{} + NAN;
         }
       }
+      // 16 keys each, tokens 0 2 1 3 of each four: the weights' upper 11 bits, and the rest
+      half8 ph[2][2], pl[2][2];
+      float sum[2] = {0.0f, 0.0f};
+      auto weight = [&](int sub, int v) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias));
+        sum[v % 2] += p;
+        const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
+        const int to = (v & 4) + (v % 4 == 1 ? 2 : v % 4 == 2 ? 1 : v % 4);
+        ph[sub][v / 8][to] = _Float16(hi);
+        pl[sub][v / 8][to] = _Float16(p - hi);
+      };
+#pragma unroll
+      for (int v = 0; v < 16; ++v) weight(0, v);
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
-        half8 ph[2], pl[2];  // 16 keys each, tokens 0 2 1 3 of each four: the weights' upper 11 bits, and the rest
-        float sum[2] = {0.0f, 0.0f};
+        // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind the first.  The
+        // second half's weights are worked out between the first's products.
+        constexpr int BL = 2 * DT, EACH = 16 / BL;
+        half8 v8[4];
+        auto read = [&](int c) { v8[c % 4] = value8(sub, c / DT, c % DT); };
+        read(0);
+        read(1);
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias));
-          sum[v % 2] += p;
-          const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
-          const int to = (v & 4) + (v % 4 == 1 ? 2 : v % 4 == 2 ? 1 : v % 4);
-          ph[v / 8][to] = _Float16(hi);
-          pl[v / 8][to] = _Float16(p - hi);
-        }
-        l += sum[0] + sum[1];
-        {
-          // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind the first
-          constexpr int BL = 2 * DT;
-          half8 v8[4];
-          auto read = [&](int c) { v8[c % 4] = value8(sub, c / DT, c % DT); };
-          read(0);
-          read(1);
+        for (int c = 0; c <= BL; ++c) {
+          if (c + 2 < BL) read(c + 2);
+          if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[sub][c / DT], o[c % DT], 0, 0, 0);
+          if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[sub][(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
+          if (sub == 0 && c < BL) {
 #pragma unroll
-          for (int c = 0; c <= BL; ++c) {
-            if (c + 2 < BL) read(c + 2);
-            if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[c / DT], o[c % DT], 0, 0, 0);
-            if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int v = 0; v < EACH; ++v) weight(1, EACH * c + v);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+            }
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
+      l += sum[0] + sum[1];
     }
     __syncthreads();
     flag = flag1;
