@@ -243,6 +243,20 @@ __device__ __forceinline__ half8 key8(Bits bits, uint32_t w, _Float16 d) {
   const half2v a = elements<0>(bits, w, dd, c), b = elements<1>(bits, w, dd, c), e = elements<2>(bits, w, dd, c), f = elements<3>(bits, w, dd, c);
   return half8{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
 }
+// Two weights' f16 parts and what those leave of them (f16 too: 2^-22 of the weight), both in one register each.
+struct WeightParts {
+  half2v hi, lo;
+};
+__device__ __forceinline__ WeightParts split_weights(float p, float q) {
+  typedef float float2v __attribute__((ext_vector_type(2)));
+  WeightParts w;
+  w.hi = __builtin_convertvector((float2v{p, q}), half2v);
+  uint32_t lo;  // p - hi in f32, rounded once
+  asm("v_fma_mixlo_f16 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(lo) : "v"(w.hi), "v"(p));
+  asm("v_fma_mixhi_f16 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(lo) : "v"(w.hi), "v"(q));
+  w.lo = as_half2(lo);
+  return w;
+}
 // Scales of tokens t0 t1, t2 t3 as pairs t0 t2, t1 t3.
 __device__ __forceinline__ void token_pairs(u32x2 x, half2v& even, half2v& odd) {
   even = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u));
@@ -555,34 +569,41 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
     const bool more = i + 1 < n_tiles;
     PgTile next = w;
     if (more) next = where(i + 1);
-    float s[8];
+    floatx4 s[2] = {};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      floatx4 hi = floatx4{0.f, 0.f, 0.f, 0.f}, lo = hi;
+    for (int j = 0; j < GR; ++j) {
+      half8 k8[2];
 #pragma unroll
-      for (int j = 0; j < GR; ++j) {
-        const half8 k8 = key8(bits, kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
-        hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, qh[j], hi, 0, 0, 0);
-        lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8, ql[j], lo, 0, 0, 0);
+      for (int h = 0; h < 2; ++h) {
+        k8[h] = key8(bits, kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
+        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], ql[j], s[h], 0, 0, 0);
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s[4 * h + c] = (hi[c] + lo[c]) * unscale;
+      for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], qh[j], s[h], 0, 0, 0);
+    }
+    const bool mine = w.seg < 0 || own_seg == -2 || own_seg == w.seg;
+    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : mine ? own_limit : -1;
+    const bool all_see = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;  // every row, the whole tile: nothing to keep off
+    if (!all_see) {
+      half2v z = half2v{};  // (0 x what is no number)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < GR / 2; ++c) z = __builtin_elementwise_fma(as_half2(ks[h][c]), half2v{}, z);
+      // Where the rows of its request see all of it and its keys are numbers, the other rows' weights are 0 by their bias.
+      if (w.gone || !__all((!mine || limit >= int(w.key0 + KT - 1)) && z[0] == _Float16(0) && z[1] == _Float16(0))) {
+        asm volatile("");
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
+          if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c / 4][c % 4] = -INFINITY;
+        }
+      }
     }
     load_k(next);
-    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : own_seg == w.seg ? own_limit : -1;
-    // rows that see the whole tile: nothing to mask
-    const bool whole = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;
-    if (!whole) {
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
-        if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c] = -INFINITY;
-      }
-    }
-    float top = s[0];
-#pragma unroll
-    for (int c = 1; c < 8; ++c) top = fmaxf(top, s[c]);
-    const float mn = fmaxf(m, quarter_max(top));
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]), top1 = fmaxf(fmaxf(s[1][0], s[1][1]), s[1][2]);
+    top = fmaxf(fmaxf(top, s[0][3]), fmaxf(top1, s[1][3]));
+    const float mn = mine ? fmaxf(m, quarter_max(top) * unscale) : m;
     const bool up = mn > m + SLACK;
     if (__any(up)) {
       const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
@@ -591,18 +612,25 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
       l *= f;
       m = to;
     }
-    const float base = (m == -INFINITY ? 0.0f : m) - LIFT;
+    // (a weight of a row that is not of the request: 2^-infinity)
+    const float bias = mine ? LIFT - (m == -INFINITY ? 0.0f : m) : -INFINITY;
     half8 ph, pl;  // tokens 0 2 1 3 of the lane's four in each half
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      s[c] = __builtin_amdgcn_exp2f(s[c] - base);
-      l += s[c];
-      const float hi = __uint_as_float(__float_as_uint(s[c]) & 0xffffe000u);  // the upper 11 bits, and the rest
-      const int to = (c & 4) + (c % 4 == 1 ? 2 : c % 4 == 2 ? 1 : c % 4);
-      ph[to] = _Float16(hi);
-      pl[to] = _Float16(s[c] - hi);
+    for (int i = 0; i < 4; ++i) {  // weights v and v + 2 of a half: neighbours where they go
+      const int h = i / 2, v = i % 2;
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[h][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[h][v + 2], unscale, bias));
+      sum[0] += p;
+      sum[1] += q;
+      const WeightParts w2 = split_weights(p, q);
+      ph[4 * h + 2 * v] = w2.hi[0];
+      ph[4 * h + 2 * v + 1] = w2.hi[1];
+      pl[4 * h + 2 * v] = w2.lo[0];
+      pl[4 * h + 2 * v + 1] = w2.lo[1];
     }
-    if (!whole) {
+    l += sum[0] + sum[1];
+    if (!all_see) {
+      asm volatile("");
       if (w.keys < KT || w.gone) {  // scales of tokens that no row sees may hold anything: 0
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -612,7 +640,6 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
           for (int c = 0; c < GR; ++c) vs[h][c] = u32x2{vs[h][c][0] & low, vs[h][c][1] & high};
         }
       }
-      // of no number, and not seen by some: 0 too; the outputs of rows that see the first of them are no number
       half2v z = half2v{};
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -620,8 +647,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
         for (int c = 0; c < GR; ++c)
 #pragma unroll
           for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[h][c][x]), half2v{}, z);
-      const bool odd = !(z[0] == _Float16(0)) || !(z[1] == _Float16(0));
-      if (__any(odd)) {
+      if (!__all(z[0] == _Float16(0) && z[1] == _Float16(0))) {  // of no number: 0 too; outputs of rows that see the first are no number
 #pragma unroll
         for (int c = 0; c < GR; ++c) {
           uint32_t first = KT;
@@ -954,6 +980,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       };
       read(0);
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int c = 0; c < DS; ++c) {
         if (c + 1 < DS) read(c + 1);
@@ -978,6 +1005,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       }
     }
     if (sees) {
+      __builtin_amdgcn_s_setprio(0);
       const bool whole = __all(!live || limit >= int(cur.key0) + KT - 1) && !(gone & 15u);
       if (!whole) {
         asm volatile("");  // (a branch: selects for every tile would cost as much as a fifth of its other vector work)
@@ -1015,21 +1043,25 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       // 16 keys each, tokens 0 2 1 3 of each four: the weights' upper 11 bits, and the rest
       half8 ph[2][2], pl[2][2];
       float sum[2] = {0.0f, 0.0f};
-      auto weight = [&](int sub, int v) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias));
-        sum[v % 2] += p;
-        const float hi = __uint_as_float(__float_as_uint(p) & 0xffffe000u);
-        const int to = (v & 4) + (v % 4 == 1 ? 2 : v % 4 == 2 ? 1 : v % 4);
-        ph[sub][v / 8][to] = _Float16(hi);
-        pl[sub][v / 8][to] = _Float16(p - hi);
+      auto weigh = [&](int sub, int v) {  // weights v and v + 2: neighbours where they go
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[sub][v + 2], unscale, bias));
+        sum[0] += p;
+        sum[1] += q;
+        const WeightParts w2 = split_weights(p, q);
+        const int to = (v & 4) + 2 * (v % 2);
+        ph[sub][v / 8][to] = w2.hi[0];
+        ph[sub][v / 8][to + 1] = w2.hi[1];
+        pl[sub][v / 8][to] = w2.lo[0];
+        pl[sub][v / 8][to + 1] = w2.lo[1];
       };
+      auto weigh_pair = [&](int sub, int i) { weigh(sub, 4 * (i / 2) + i % 2); };  // i: 0 .. 7
 #pragma unroll
-      for (int v = 0; v < 16; ++v) weight(0, v);
+      for (int i = 0; i < 8; ++i) weigh_pair(0, i);
 #pragma unroll
       for (int sub = 0; sub < 2; ++sub) {
         // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind the first.  The
         // second half's weights are worked out between the first's products.
-        constexpr int BL = 2 * DT, EACH = 16 / BL;
+        constexpr int BL = 2 * DT, EACH = 8 / BL;
         half8 v8[4];
         auto read = [&](int c) { v8[c % 4] = value8(sub, c / DT, c % DT); };
         read(0);
@@ -1041,7 +1073,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
           if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[sub][(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
           if (sub == 0 && c < BL) {
 #pragma unroll
-            for (int v = 0; v < EACH; ++v) weight(1, EACH * c + v);
+            for (int i = 0; i < EACH; ++i) weigh_pair(1, EACH * c + i);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
