@@ -3,6 +3,7 @@
 // over the requests' pages; the rows of pages made anew; a pool compacted.
 
 #include "kv_dev.h"
+#include "lds_dma.h"
 #include "pages.h"
 
 namespace s2 {
@@ -257,12 +258,16 @@ __device__ __forceinline__ WeightParts split_weights(float p, float q) {
   w.lo = as_half2(lo);
   return w;
 }
-// Scales of tokens t0 t1, t2 t3 as pairs t0 t2, t1 t3.
-__device__ __forceinline__ void token_pairs(u32x2 x, half2v& even, half2v& odd) {
-  even = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u));
-  odd = as_half2(__builtin_amdgcn_perm(x[1], x[0], 0x07060302u));
+// Four tokens' values of two dims (a byte each, dim 2 m below) as pairs of neighbours: v[x]: tokens 0 1 of dim 2 m + x,
+// v[2 + x]: tokens 2 3.  d: the tokens' scales.
+__device__ __forceinline__ void values8(Bits bits, uint32_t w, u32x2 d, half2v (&v)[4]) {
+  w = __builtin_amdgcn_perm(w, w, 0x03010200u);  // bytes 0 2 1 3
+  const half2v d0 = as_half2(d[0]), d1 = as_half2(d[1]), c0 = d0 * both(_Float16(-24.0f)), c1 = d1 * both(_Float16(-24.0f));
+  v[0] = elements<0>(bits, w, d0, c0);
+  v[1] = elements<1>(bits, w, d0, c0);
+  v[2] = elements<2>(bits, w, d1, c1);
+  v[3] = elements<3>(bits, w, d1, c1);
 }
-
 // Of pair x of scales those of no number become 0; the first of them, or a large number.
 template <class Pairs>
 __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
@@ -367,6 +372,11 @@ __device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, u
   return r;
 }
 
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  return reinterpret_cast<const uint8_t*>(uint64_t(uniform(uint32_t(x >> 32))) << 32 | uniform(uint32_t(x)));
+}
+
 // 64 page numbers of a request, one per lane.
 struct PageWindow {
   uint32_t b = 0xffffffffu, first = 0;
@@ -419,21 +429,28 @@ __device__ __forceinline__ Share share_of(const KvAttendArgs& a, const PgShare& 
   return {tile, begin, end - begin};
 }
 
-// A tile of 32 keys in two halves of 16, which may lie in different pages.
+// A tile of 32 keys in halves of 16, which lie in one page or (TWO) may lie in two.
+template <bool TWO>
 struct PgTile {
-  uint32_t req, key0, keys;  // request, first key; keys of it that are there
-  int seg;                   // -1: in common; else request b_lo + seg
-  const uint8_t* part[2];    // the kv head's part of the page, of each half
-  uint32_t slot[2];          // its first slot there
-  uint32_t gone;             // bit h: half h lies in no page of the pool
+  uint32_t req, key0, keys;      // request, first key; keys of it that are there
+  uint32_t left, seg_keys;       // further tiles of the same request (or in common), and its keys
+  int seg;                       // -1: in common; else request b_lo + seg
+  const uint8_t* part[1 + TWO];  // the kv head's part of the page
+  uint32_t slot[1 + TWO];        // the first slot there
+  uint32_t gone;                 // bit h: half h lies in no page of the pool
 };
 
-template <int HD>
+template <int HD, bool TWO>
 __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArgs pa, PgShare sp) {
   constexpr int KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
   constexpr int OP = HD + 4;                          // padded row of the joined states
   constexpr float LIFT = F16_LIFT;
-  __shared__ __align__(16) float os_all[STEP_WAVES * 16 * OP];
+  // A tile: key codes, value codes, key scales, value scales (and what the load of those leaves behind them); a wave's two, and in their place its
+  // state in the end.
+  constexpr uint32_t TILE = KT * HD + 1024, STAGE = 2 * TILE, K_AT = 0, V_AT = KT * HD / 2, KS_AT = KT * HD, VS_AT = KT * (HD + HD / 16);
+  constexpr int LOADS = HD == 128 ? 5 : 3;
+  static_assert(16 * OP * 4 <= STAGE, "a state fits");
+  __shared__ __align__(16) uint8_t lds[STEP_WAVES * STAGE];
   __shared__ float ml[STEP_WAVES][16][2];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
@@ -463,13 +480,28 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   if (n_com == 0)
     while (seg < 63 && o_lo >= lane_read_u32(run.seg_end, int(seg))) ++seg;
   window.begin(early, b_lo, b_lo + (n_com ? lead : seg));
+  using Tile = PgTile<TWO>;
+  auto turn_page = [&](Tile& w) {
+    w.gone = 0;
+#pragma unroll
+    for (int h = 0; h < 1 + TWO; ++h) {
+      const uint32_t key = w.key0 + (h && w.keys > 16 ? 16 : 0);
+      const uint32_t page = window.get(pa.p, w.req, key >> pa.p.shift);
+      const bool in = page < pa.p.pages;
+      w.gone |= in ? 0u : TWO ? 1u << h : 3u;
+      w.part[h] = pa.p.pool + (size_t(in ? page : 0u) * a.s.G + g) * pa.p.chunk;
+      w.slot[h] = key & ((1u << pa.p.shift) - 1u);
+    }
+    if (w.gone && lane == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
+  };
   auto where = [&](uint32_t i) {
-    PgTile w;
+    Tile w;
     if (i < n_com) {
       w.seg = -1;
       w.req = b_lo + lead;
       w.key0 = (c_lo + i) * KT;
-      w.keys = KT;
+      w.left = n_com - 1 - i;
+      w.seg_keys = run.common;
     } else {
       const uint32_t x = o_lo + (i - n_com);
       while (x >= lane_read_u32(run.seg_end, int(seg))) ++seg;
@@ -477,56 +509,93 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
       w.seg = int(seg);
       w.req = b_lo + seg;
       w.key0 = run.common + (x - begin) * KT;
-      w.keys = min(uint32_t(KT), lane_read_u32(run.seg_keys, int(seg)) - w.key0);
+      w.left = lane_read_u32(run.seg_end, int(seg)) - 1 - x;
+      w.seg_keys = lane_read_u32(run.seg_keys, int(seg));
     }
-    w.gone = 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t key = w.key0 + (h && w.keys > 16 ? 16 : 0);
-      const uint32_t page = window.get(pa.p, w.req, key >> pa.p.shift);
-      const bool in = page < pa.p.pages;
-      w.gone |= in ? 0u : 1u << h;
-      w.part[h] = pa.p.pool + (size_t(in ? page : 0u) * a.s.G + g) * pa.p.chunk;
-      w.slot[h] = key & ((1u << pa.p.shift) - 1u);
-    }
-    if (w.gone && lane == 0) atomicOr(a.s.err, S2HIP_PAGES_ERR_PAGE);
+    w.keys = min(uint32_t(KT), w.seg_keys - w.key0);
+    turn_page(w);
     return w;
   };
-  // Of each half: codes of key r16, dims 32 j + 8 q4 ..; its scales; codes of dims 32 j + 2 r16 .. of tokens 4 q4 ..; their scales
-  uint32_t kc[2][GR], vc[2][GR], ks[2][GR / 2];
-  u32x2 vs[2][GR];
-  auto load_k = [&](const PgTile& w) {
+  // the tile behind w, the i-th
+  auto behind = [&](const Tile& was, uint32_t i) {
+    if (was.left == 0) return where(i);
+    Tile w = was;
+    --w.left;
+    w.key0 += KT;
+    w.keys = min(uint32_t(KT), w.seg_keys - w.key0);
+    w.slot[0] += KT;
+    if (TWO || w.slot[0] >> pa.p.shift) turn_page(w);
+    return w;
+  };
+  // Tiles go straight to LDS, two ahead of their use: in registers one more tile would cost a fourth wave per SIMD.
+  lds_byte* const stage = (lds_byte*)lds + wave * STAGE;
+  const uint32_t stage_at = uint32_t(uintptr_t(stage));
+  const uint32_t k_lane = r16 * (HD / 2) + q4 * 16, s_lane = (lane & 16u ? at.vs() - at.ks() : 0u) + r16 * 16;
+  auto fetch = [&](const Tile& w, uint32_t slot) {
+    const uint32_t to = uniform(stage_at + slot * TILE);
+    if constexpr (!TWO) {
+      const uint8_t* part = uniform(w.part[0]);
+      const uint32_t first = uniform(w.slot[0]);
+      const uint8_t *k = part + first * (HD / 2), *v = k + at.v(), *d = part + at.ks() + first * (HD / 16);
+      if constexpr (HD == 128) {
+        dma16(k, k_lane, to + K_AT);
+        dma16(k, k_lane + 1024, to + K_AT + 1024);
+        dma16(v, lane * 16, to + V_AT);
+        dma16(v, lane * 16 + 1024, to + V_AT + 1024);
+        dma16(d, s_lane, to + KS_AT);  // 16 lanes each: key scales, value scales, and both again behind the tile
+      } else {
+        dma16(k, lane * 16, to + K_AT);
+        dma16(v, lane * 16, to + V_AT);
+        dma16(d, (lane & 8u ? at.vs() - at.ks() : 0u) + (lane & 7u) * 16, to + KS_AT);  // 8 lanes each
+      }
+    } else {
+      const bool second = lane >= 32;
+      const uint8_t* mine = second ? w.part[TWO] : w.part[0];
+      const uint32_t at_slot = second ? w.slot[TWO] : w.slot[0], l32 = lane & 31u;
+      if constexpr (HD == 128) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          dma16(w.part[h] + w.slot[h] * (HD / 2), k_lane, to + K_AT + 1024 * h);
+          dma16(w.part[h] + at.v() + w.slot[h] * (HD / 2), lane * 16, to + V_AT + 1024 * h);
+        }
+      } else {
+        dma_lane<16>(mine + at_slot * (HD / 2) + l32 * 16, to + K_AT);
+        dma_lane<16>(mine + at.v() + at_slot * (HD / 2) + l32 * 16, to + V_AT);
+      }
+      // pieces of 16 bytes: key scales of both halves, value scales of both, and all again
+      constexpr uint32_t PH = HD / 16;  // of a half
+      const uint32_t piece = lane % (4 * PH);
+      const bool odd = (piece / PH) & 1u;
+      const uint8_t* from = odd ? w.part[TWO] : w.part[0];
+      dma_lane<16>(from + (piece >= 2 * PH ? at.vs() : at.ks()) + (odd ? w.slot[TWO] : w.slot[0]) * (HD / 16) + piece % PH * 16, to + KS_AT);
+    }
+  };
+  // codes of key r16, dims 32 j + 8 q4 ..; its scales; codes of dims 32 j + 2 r16 .. of tokens 4 q4 ..; their scales
+  typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+  typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+  typedef __attribute__((address_space(3))) uint32_t lds_u32;
+  uint32_t kc[2][GR], ks[2][GR / 2];
+  auto take_k = [&](uint32_t slot) {
+    lds_byte* p = stage + slot * TILE;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint8_t* p = w.part[h] + w.slot[h] * (HD / 2);
       if constexpr (HD == 128) {
-        *reinterpret_cast<u32x4*>(kc[h]) = *reinterpret_cast<const u32x4*>(p + r16 * (HD / 2) + q4 * (HD / 8));
-        *reinterpret_cast<u32x2*>(ks[h]) = *reinterpret_cast<const u32x2*>(w.part[h] + at.ks() + w.slot[h] * (HD / 16) + r16 * (HD / 16));
+        *reinterpret_cast<u32x4*>(kc[h]) = *reinterpret_cast<lds_u32x4*>(p + K_AT + 1024 * h + lane * 16);
+        *reinterpret_cast<u32x2*>(ks[h]) = *reinterpret_cast<lds_u32x2*>(p + KS_AT + 128 * h + r16 * 8);
       } else {
-        *reinterpret_cast<u32x2*>(kc[h]) = *reinterpret_cast<const u32x2*>(p + r16 * (HD / 2) + q4 * (HD / 8));
-        ks[h][0] = *reinterpret_cast<const uint32_t*>(w.part[h] + at.ks() + w.slot[h] * (HD / 16) + r16 * (HD / 16));
+        *reinterpret_cast<u32x2*>(kc[h]) = *reinterpret_cast<lds_u32x2*>(p + K_AT + 512 * h + r16 * 32 + q4 * 8);
+        ks[h][0] = *reinterpret_cast<lds_u32*>(p + KS_AT + 64 * h + r16 * 4);
       }
     }
   };
-  auto load_v = [&](const PgTile& w) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t *p = w.part[h] + at.v() + w.slot[h] * (HD / 2) + lane * (HD / 8), *d = w.part[h] + at.vs() + w.slot[h] * (HD / 16) + q4 * (HD / 4);
-      if constexpr (HD == 128) {
-        *reinterpret_cast<u32x4*>(vc[h]) = *reinterpret_cast<const u32x4*>(p);
-        *reinterpret_cast<u32x4*>(&vs[h][0]) = *reinterpret_cast<const u32x4*>(d);
-        *reinterpret_cast<u32x4*>(&vs[h][2]) = *reinterpret_cast<const u32x4*>(d + 16);
-      } else {
-        *reinterpret_cast<u32x2*>(vc[h]) = *reinterpret_cast<const u32x2*>(p);
-        *reinterpret_cast<u32x4*>(&vs[h][0]) = *reinterpret_cast<const u32x4*>(d);
-      }
-    }
-  };
-  PgTile w{};
+  Tile w{}, next{};
   if (n_tiles) {
     w = where(0);
-    load_k(w);
-    load_v(w);
+    fetch(w, 0);
+  }
+  if (n_tiles > 1) {
+    next = behind(w, 1);
+    fetch(next, 1);
   }
 
   // this lane's row
@@ -566,9 +635,43 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   float m = -INFINITY, l = 0.0f;
 
   for (uint32_t i = 0; i < n_tiles; ++i) {
-    const bool more = i + 1 < n_tiles;
-    PgTile next = w;
-    if (more) next = where(i + 1);
+    const uint32_t slot = i & 1u;
+    if (i + 1 < n_tiles)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // (all but the next tile's)
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const bool mine = w.seg < 0 || own_seg == -2 || own_seg == w.seg;
+    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : mine ? own_limit : -1;
+    const bool all_see = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;  // every row, the whole tile: nothing to keep off
+    bool masks = false;
+    if (!all_see) {
+      // A pair of scales per lane: keys' of dims .., values' of tokens 16 h + 4 i + 2 x and the next.
+      constexpr uint32_t PAIRS = 16 * GR;
+      lds_u32* const kp = reinterpret_cast<lds_u32*>(stage + slot * TILE + KS_AT) + lane % PAIRS;
+      lds_u32* const vp = reinterpret_cast<lds_u32*>(stage + slot * TILE + VS_AT) + lane % PAIRS;
+      const uint32_t quad = lane % PAIRS / (2 * GR), first_token = 4 * quad + 2 * (lane & 1u);
+      auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
+      uint32_t pair = *vp;
+      if (w.keys < KT || w.gone) {  // scales of tokens that no row sees may hold anything: 0
+        const int there = (w.gone >> (quad / 4)) & 1u ? 0 : int(w.keys) - int(first_token);
+        pair &= there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u;
+        *vp = pair;
+      }
+      // Where the rows of its request see all of it and its keys are numbers, the other rows' weights are 0 by their bias.
+      masks = w.gone || !__all((!mine || limit >= int(w.key0 + KT - 1)) && !odd(*kp));
+      if (__any(odd(pair))) {  // values of no number: 0 too; outputs of rows that see the first of them are no number
+        const uint32_t at_token = (pair & 0x7c00u) == 0x7c00u ? first_token : odd(pair) ? first_token + 1 : 1000u;
+        if ((pair & 0x7c00u) == 0x7c00u) pair &= 0xffff0000u;
+        if ((pair & 0x7c000000u) == 0x7c000000u) pair &= 0xffffu;
+        *vp = pair;
+#pragma unroll
+        for (int c = 0; c < GR; ++c) {
+          const uint32_t first = wave_reduce(int(lane / 2 % GR) == c ? at_token : 1000u, [](uint32_t x, uint32_t y) { return min(x, y); });
+          if (first < KT && limit >= int(w.key0 + first)) o[2 * c] = o[2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
+        }
+      }
+    }
+    take_k(slot);
     floatx4 s[2] = {};
 #pragma unroll
     for (int j = 0; j < GR; ++j) {
@@ -581,26 +684,14 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
 #pragma unroll
       for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], qh[j], s[h], 0, 0, 0);
     }
-    const bool mine = w.seg < 0 || own_seg == -2 || own_seg == w.seg;
-    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : mine ? own_limit : -1;
-    const bool all_see = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;  // every row, the whole tile: nothing to keep off
-    if (!all_see) {
-      half2v z = half2v{};  // (0 x what is no number)
+    if (masks) {
+      asm volatile("");
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < GR / 2; ++c) z = __builtin_elementwise_fma(as_half2(ks[h][c]), half2v{}, z);
-      // Where the rows of its request see all of it and its keys are numbers, the other rows' weights are 0 by their bias.
-      if (w.gone || !__all((!mine || limit >= int(w.key0 + KT - 1)) && z[0] == _Float16(0) && z[1] == _Float16(0))) {
-        asm volatile("");
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
-          if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c / 4][c % 4] = -INFINITY;
-        }
+      for (int c = 0; c < 8; ++c) {
+        const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
+        if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c / 4][c % 4] = -INFINITY;
       }
     }
-    load_k(next);
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]), top1 = fmaxf(fmaxf(s[1][0], s[1][1]), s[1][2]);
     top = fmaxf(fmaxf(top, s[0][3]), fmaxf(top1, s[1][3]));
     const float mn = mine ? fmaxf(m, quarter_max(top) * unscale) : m;
@@ -614,74 +705,54 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
     }
     // (a weight of a row that is not of the request: 2^-infinity)
     const float bias = mine ? LIFT - (m == -INFINITY ? 0.0f : m) : -INFINITY;
-    half8 ph, pl;  // tokens 0 2 1 3 of the lane's four in each half
+    half8 ph, pl;  // the lane's four tokens of each half
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // weights v and v + 2 of a half: neighbours where they go
-      const int h = i / 2, v = i % 2;
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[h][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[h][v + 2], unscale, bias));
+    for (int i = 0; i < 4; ++i) {
+      const int v = 2 * (i % 2);
+      const float p = __builtin_amdgcn_exp2f(fmaf(s[i / 2][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[i / 2][v + 1], unscale, bias));
       sum[0] += p;
       sum[1] += q;
       const WeightParts w2 = split_weights(p, q);
-      ph[4 * h + 2 * v] = w2.hi[0];
-      ph[4 * h + 2 * v + 1] = w2.hi[1];
-      pl[4 * h + 2 * v] = w2.lo[0];
-      pl[4 * h + 2 * v + 1] = w2.lo[1];
+      ph[2 * i] = w2.hi[0];
+      ph[2 * i + 1] = w2.hi[1];
+      pl[2 * i] = w2.lo[0];
+      pl[2 * i + 1] = w2.lo[1];
     }
     l += sum[0] + sum[1];
-    if (!all_see) {
-      asm volatile("");
-      if (w.keys < KT || w.gone) {  // scales of tokens that no row sees may hold anything: 0
+    lds_byte* const values = stage + slot * TILE;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int there = (w.gone >> h) & 1u ? 0 : int(w.keys) - int(16u * h + 4u * q4);  // of the lane's four
-          const uint32_t low = there >= 2 ? 0xffffffffu : there == 1 ? 0xffffu : 0u, high = there >= 4 ? 0xffffffffu : there == 3 ? 0xffffu : 0u;
-#pragma unroll
-          for (int c = 0; c < GR; ++c) vs[h][c] = u32x2{vs[h][c][0] & low, vs[h][c][1] & high};
-        }
-      }
-      half2v z = half2v{};
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < GR; ++c)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[h][c][x]), half2v{}, z);
-      if (!__all(z[0] == _Float16(0) && z[1] == _Float16(0))) {  // of no number: 0 too; outputs of rows that see the first are no number
-#pragma unroll
-        for (int c = 0; c < GR; ++c) {
-          uint32_t first = KT;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) first = min(first, take_odd_scales(vs[h][c], x) + 16 * h + 4 * q4 + 2 * x);
-          first = wave_reduce(first, [](uint32_t x, uint32_t y) { return min(x, y); });
-          if (first < KT && limit >= int(w.key0 + first)) o[2 * c] = o[2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
-        }
-      }
-    }
-#pragma unroll
-    for (int c = 0; c < GR; ++c) {
-      half2v v[2][4];
+    for (int half_c = 0; half_c < GR / 2; ++half_c) {  // two groups of 32 dims
+      uint32_t vc[2][2];
+      u32x2 vs[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        half2v de, dd;
-        token_pairs(vs[h][c], de, dd);
-        const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
-        v[h][0] = elements<0>(bits, vc[h][c], de, ce);
-        v[h][1] = elements<1>(bits, vc[h][c], de, ce);
-        v[h][2] = elements<2>(bits, vc[h][c], dd, cd);
-        v[h][3] = elements<3>(bits, vc[h][c], dd, cd);
+        if constexpr (HD == 128)
+          *reinterpret_cast<u32x2*>(vc[h]) = *reinterpret_cast<lds_u32x2*>(values + V_AT + 1024 * h + lane * 16 + 8 * half_c);
+        else
+          *reinterpret_cast<u32x2*>(vc[h]) = *reinterpret_cast<lds_u32x2*>(values + V_AT + 512 * h + lane * 8);
+        *reinterpret_cast<u32x4*>(vs[h]) = *reinterpret_cast<lds_u32x4*>(values + VS_AT + HD * h + q4 * (HD / 4) + 16 * half_c);
       }
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const half8 v8 = {v[0][x][0], v[0][x][1], v[0][2 + x][0], v[0][2 + x][1], v[1][x][0], v[1][x][1], v[1][2 + x][0], v[1][2 + x][1]};
-        o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[2 * c + x], 0, 0, 0);
-        o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[2 * c + x], 0, 0, 0);
+      for (int cc = 0; cc < 2; ++cc) {
+        const int c = 2 * half_c + cc;
+        half2v v[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) values8(bits, vc[h][cc], vs[h][cc], v[h]);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const half8 v8 = {v[0][x][0], v[0][x][1], v[0][2 + x][0], v[0][2 + x][1], v[1][x][0], v[1][x][1], v[1][2 + x][0], v[1][2 + x][1]};
+          o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[2 * c + x], 0, 0, 0);
+          o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[2 * c + x], 0, 0, 0);
+        }
       }
     }
-    load_v(next);
     w = next;
+    if (i + 2 < n_tiles) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the tile is in registers)
+      next = behind(next, i + 2);
+      fetch(next, slot);
+    }
   }
 
   // the block's four states as one
@@ -695,7 +766,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
 #pragma unroll
   for (int i = 0; i < STEP_WAVES; ++i) M = fmaxf(M, ml[i][r16][0]);
   const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-  float* os = os_all + (wave * 16 + r16) * OP;
+  float* os = reinterpret_cast<float*>(lds + wave * STAGE) + r16 * OP;
 #pragma unroll
   for (int c = 0; c < GR; ++c)
 #pragma unroll
@@ -721,10 +792,10 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   const float inv = last ? (M_row == -INFINITY ? NAN : 1.0f / L_row) : 1.0f;  // (it sees a key, its own)
 #pragma unroll
   for (int c = 0; c < HD / 64; ++c) {
-    const float* src = os_all + jr * OP + d0 + 64 * c;
+    const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
     floatx4 x = *reinterpret_cast<const floatx4*>(src);
 #pragma unroll
-    for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * 16 * OP);
+    for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * (STAGE / 4));
     *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
   }
   if (tid % 16 == 0 && !last) {
@@ -881,12 +952,10 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
     if (w.gone && lane == 0) atomicOr(&gone_tile[flag], 1u << wave);
   };
   auto store_value = [&](int c) {
-    half2v de, dd;
-    token_pairs(vs[c], de, dd);
-    const half2v ce = de * both(_Float16(-24.0f)), cd = dd * both(_Float16(-24.0f));
-    const half2v v[4] = {elements<0>(bits, vc[c], de, ce), elements<1>(bits, vc[c], de, ce), elements<2>(bits, vc[c], dd, cd), elements<3>(bits, vc[c], dd, cd)};
+    half2v v[4];
+    values8(bits, vc[c], vs[c], v);
 #pragma unroll
-    for (int x = 0; x < 2; ++x)  // tokens 0 2 1 3 of the four, the first or second half of a piece
+    for (int x = 0; x < 2; ++x)  // the first or second half of a piece
       *reinterpret_cast<lds_half4*>(lds0 + (v_to + (32 * c + x) * (KT * 2))) = half4{v[x][0], v[x][1], v[2 + x][0], v[2 + x][1]};
   };
   auto store_piece = [&](int c) {
@@ -1040,21 +1109,20 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
           if (first < KT && limit >= int(cur.key0 + first)) o[dt] = floatx16{} + NAN;
         }
       }
-      // 16 keys each, tokens 0 2 1 3 of each four: the weights' upper 11 bits, and the rest
+      // 16 keys each: the weights' f16 parts, and the rest
       half8 ph[2][2], pl[2][2];
       float sum[2] = {0.0f, 0.0f};
-      auto weigh = [&](int sub, int v) {  // weights v and v + 2: neighbours where they go
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[sub][v + 2], unscale, bias));
+      auto weigh_pair = [&](int sub, int i) {
+        const int v = 2 * i, to = v % 8;
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[sub][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[sub][v + 1], unscale, bias));
         sum[0] += p;
         sum[1] += q;
         const WeightParts w2 = split_weights(p, q);
-        const int to = (v & 4) + 2 * (v % 2);
         ph[sub][v / 8][to] = w2.hi[0];
         ph[sub][v / 8][to + 1] = w2.hi[1];
         pl[sub][v / 8][to] = w2.lo[0];
         pl[sub][v / 8][to + 1] = w2.lo[1];
       };
-      auto weigh_pair = [&](int sub, int i) { weigh(sub, 4 * (i / 2) + i % 2); };  // i: 0 .. 7
 #pragma unroll
       for (int i = 0; i < 8; ++i) weigh_pair(0, i);
 #pragma unroll
@@ -1470,8 +1538,10 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
   return by_dim(hd, [&](auto HD) {
     if (many)
       hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * splits), dim3(256), 0, s, pa, sp);
+    else if (pa.p.shift == 4)  // a tile takes two pages
+      hipLaunchKernelGGL((pg_step_kernel<HD(), true>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
     else
-      hipLaunchKernelGGL(pg_step_kernel<HD()>, dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+      hipLaunchKernelGGL((pg_step_kernel<HD(), false>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     if (splits > 1 && out_rows <= 2048)
       hipLaunchKernelGGL((pg_join_kernel<HD(), 1024 / HD()>), dim3(out_rows), dim3(256), 0, s, a, sp);
