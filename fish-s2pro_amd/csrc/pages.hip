@@ -1038,25 +1038,26 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
     floatx16 s[2] = {};
     if (sees) {
       // A step: 16 dims of all scores, and a piece of the next tile (of what the registers hold, where there is none: it
-      // goes where nobody reads).  Fragments are read a step ahead; the barriers keep the compiler from reading all of
+      // goes where nobody reads).  Fragments are read two steps ahead; the barriers keep the compiler from reading all of
       // them first, the groups have it put other work between the products, which take as long as eight of it each.
       store_begin(buf ^ 1u);
       if (more) store_scales(next, flag1);
-      half8 k8[2][2];
+      half8 k8[3][2];
       auto read = [&](int c) {
 #pragma unroll
-        for (int sub = 0; sub < 2; ++sub) k8[c % 2][sub] = *reinterpret_cast<const lds_half8*>(lds0 + ((k_from ^ (32u * c)) + 32 * sub * RB));
+        for (int sub = 0; sub < 2; ++sub) k8[c % 3][sub] = *reinterpret_cast<const lds_half8*>(lds0 + ((k_from ^ (32u * c)) + 32 * sub * RB));
       };
-      read(0);
+      if (0 < DS) read(0);
+      if (1 < DS) read(1);
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int c = 0; c < DS; ++c) {
-        if (c + 1 < DS) read(c + 1);
-        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][0], qh[c], s[0], 0, 0, 0);
-        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][1], qh[c], s[1], 0, 0, 0);
-        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][0], ql[c], s[0], 0, 0, 0);
-        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 2][1], ql[c], s[1], 0, 0, 0);
+        if (c + 2 < DS) read(c + 2);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], qh[c], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], qh[c], s[1], 0, 0, 0);
+        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][0], ql[c], s[0], 0, 0, 0);
+        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k8[c % 3][1], ql[c], s[1], 0, 0, 0);
         store_piece(c);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -1130,15 +1131,18 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
         // block c: 16 keys (st = c / DT) of 32 dims; its second term comes a block later, not right behind the first.  The
         // second half's weights are worked out between the first's products.
         constexpr int BL = 2 * DT, EACH = 8 / BL;
-        half8 v8[4];
-        auto read = [&](int c) { v8[c % 4] = value8(sub, c / DT, c % DT); };
-        read(0);
-        read(1);
+        half8 v8[6];
+        auto read = [&](int c) { v8[c % 6] = value8(sub, c / DT, c % DT); };
+        if (0 < BL) read(0);
+        if (1 < BL) read(1);
+        if (2 < BL) read(2);
+        if (3 < BL) read(3);
+
 #pragma unroll
         for (int c = 0; c <= BL; ++c) {
-          if (c + 2 < BL) read(c + 2);
-          if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 4], ph[sub][c / DT], o[c % DT], 0, 0, 0);
-          if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 4], pl[sub][(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
+          if (c + 4 < BL) read(c + 4);
+          if (c < BL) o[c % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[c % 6], ph[sub][c / DT], o[c % DT], 0, 0, 0);
+          if (c >= 1) o[(c - 1) % DT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[(c - 1) % 6], pl[sub][(c - 1) / DT], o[(c - 1) % DT], 0, 0, 0);
           if (sub == 0 && c < BL) {
 #pragma unroll
             for (int i = 0; i < EACH; ++i) weigh_pair(1, EACH * c + i);
