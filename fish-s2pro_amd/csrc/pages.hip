@@ -3,6 +3,7 @@
 // over the requests' pages; the rows of pages made anew; a pool compacted.
 
 #include "kv_dev.h"
+#include "launch.h"
 #include "lds_dma.h"
 #include "pages.h"
 
@@ -1293,20 +1294,42 @@ __device__ __forceinline__ void copy_rows(const PgUpdateArgs& a) {
   if (a.lens_out && a.lens_out != a.lens && tid < a.R) a.lens_out[tid] = a.lens[tid];
 }
 
-// One block.  References are counted in the workspace: what rows let go of is taken
-// off, what they take added; the rest of a row that stays its own is not looked at
-// twice.  Of w rows that write to a page of r references, the first r - 1 write to
-// copies: the last writes in place if no one else holds it.
+// One block, a wave per row at a time.  References are counted apart: what rows let go of is taken off, what they take
+// added; the rest of a row that stays its own counts as it is.  Of w rows that write to a page of r references, the
+// first r - 1 write to copies: the last writes in place if no one else holds it.
+//   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores.  FITS:
+// counts, free pages and new rows are in LDS (64 rows of 104 pages: 21 us -> 7 against the workspace, where each turn is
+// a trip to the second-level cache); else in the workspace.
+constexpr uint32_t ROWS_LDS = 150 * 1024;  // bytes: counts, free pages, rows
+
+template <bool FITS>
 __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a, PgWorkspace w) {
+  extern __shared__ int32_t dyn[];
   __shared__ int32_t source[MAX_ROWS], lens[MAX_ROWS], kept[MAX_ROWS], total[MAX_ROWS], last[MAX_ROWS];
   __shared__ uint32_t first[MAX_ROWS], offset[MAX_ROWS], bad;
-  const uint32_t tid = threadIdx.x, width = a.p.width, page_up = (1u << a.p.shift) - 1u;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), width = a.p.width, page_up = (1u << a.p.shift) - 1u;
   const int64_t cap = int64_t(width) << a.p.shift;
+  auto refs = [&](uint32_t p) -> int32_t* {
+    if constexpr (FITS) return dyn + p;
+    return w.refs + p;
+  };
+  auto list = [&](uint32_t i) -> int32_t* {
+    if constexpr (FITS) return dyn + a.p.pages + i;
+    return w.list + i;
+  };
+  auto rows = [&](uint32_t x) -> int32_t* {
+    if constexpr (FITS) return dyn + 2 * a.p.pages + x;
+    return w.table + x;
+  };
+  auto count = [&](uint32_t p) {  // now, with what others have added
+    if constexpr (FITS) return *refs(p);
+    return load_now(refs(p));
+  };
   auto pages_of = [&](int32_t n) { return (uint32_t(n) + page_up) >> a.p.shift; };
   auto report = [&](uint32_t bits) { atomicOr(&bad, bits); };
   if (tid == 0) bad = 0;
-  __syncthreads();
   int32_t keep = 0, add = 0;
+  __syncthreads();
   if (tid < a.R) {
     source[tid] = a.source ? a.source[tid] : int32_t(tid);
     lens[tid] = a.lens[tid];
@@ -1315,7 +1338,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     w.moves[2 * tid] = -1;
     if (lens[tid] < 0 || lens[tid] > cap || source[tid] < -1 || source[tid] >= int32_t(a.R) || keep < 0 || add < 0) report(S2HIP_PAGES_ERR_LENS);
   }
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) w.refs[p] = a.refs[p];
+  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) *refs(p) = a.refs[p];
   auto stops = [&] {
     const uint32_t why = settled(bad);
     if (why) copy_rows(a);
@@ -1329,69 +1352,70 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     total[tid] = int32_t(uint32_t(kept[tid]) + uint32_t(add));
   }
   if (stops()) return;
-  for (uint32_t x = tid; x < a.R * width; x += ROWS_THREADS) {
-    const uint32_t b = x / width, i = x % width;
+  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
     const int32_t s = source[b];
-    const bool old = i < pages_of(lens[b]), base = i < pages_of(kept[b]);
-    const int32_t e = old ? a.p.table[x] : -1, v = !base ? -1 : s == int32_t(b) ? e : a.p.table[size_t(s) * width + i];
-    const bool e_in = uint32_t(e) < a.p.pages, v_in = uint32_t(v) < a.p.pages;
-    if ((old && !e_in) || (base && !v_in)) report(S2HIP_PAGES_ERR_PAGE);
-    if (s != int32_t(b) || !base) {
-      if (old && e_in) atomicSub(&w.refs[e], 1);
-      if (base && v_in) atomicAdd(&w.refs[v], 1);
+    const uint32_t n_old = pages_of(lens[b]), n_base = pages_of(kept[b]);
+    const int32_t *old_row = a.p.table + size_t(b) * width, *base_row = a.p.table + size_t(max(s, 0)) * width;
+    for (uint32_t i = lane; i < max(n_old, n_base); i += 64) {
+      const bool old = i < n_old, base = i < n_base;
+      const int32_t e = old ? old_row[i] : -1, v = !base ? -1 : s == int32_t(b) ? e : base_row[i];
+      const bool e_in = uint32_t(e) < a.p.pages, v_in = uint32_t(v) < a.p.pages;
+      if ((old && !e_in) || (base && !v_in)) report(S2HIP_PAGES_ERR_PAGE);
+      if (s != int32_t(b) || !base) {
+        if (old && e_in) atomicSub(refs(uint32_t(e)), 1);
+        if (base && v_in) atomicAdd(refs(uint32_t(v)), 1);
+      }
+      if (base) *rows(b * width + i) = v;
     }
-    w.table[x] = v;
   }
   if (stops()) return;
-  for (uint32_t x = tid; x < a.R * width; x += ROWS_THREADS) {
-    const uint32_t b = x / width, i = x % width;
-    if (i < pages_of(kept[b]) && load_now(&w.refs[w.table[x]]) < 1) report(S2HIP_PAGES_ERR_REFS);
-    if (i < pages_of(lens[b]) && load_now(&w.refs[a.p.table[x]]) < 0) report(S2HIP_PAGES_ERR_REFS);
-  }
+  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64)
+    for (uint32_t i = lane; i < pages_of(kept[b]); i += 64)
+      if (count(uint32_t(*rows(b * width + i))) < 1) report(S2HIP_PAGES_ERR_REFS);
   const bool grows = tid < a.R && add > 0 && (uint32_t(kept[tid]) & page_up) != 0;
-  if (tid < a.R) last[tid] = grows ? w.table[size_t(tid) * width + (uint32_t(kept[tid]) >> a.p.shift)] : -1;
+  if (tid < a.R) last[tid] = grows ? *rows(tid * width + (uint32_t(kept[tid]) >> a.p.shift)) : -1;
   __syncthreads();
   uint32_t needs = 0, copies = 0;
   if (tid < a.R) {
     if (grows) {
       int32_t before = 0;
       for (uint32_t b = 0; b < tid; ++b) before += last[b] == last[tid];
-      copies = before < load_now(&w.refs[last[tid]]) - 1;
+      copies = before < count(uint32_t(last[tid])) - 1;
     }
     first[tid] = pages_of(kept[tid]) - copies;
     needs = pages_of(total[tid]) - first[tid];
   }
-  uint32_t all, found = 0;
+  uint32_t all, found;
   const uint32_t begin = block_scan(needs, all);
   if (tid < a.R) offset[tid] = begin;
-  for (uint32_t p0 = 0; p0 < a.p.pages && found < all; p0 += ROWS_THREADS) {
-    const bool free = p0 + tid < a.p.pages && load_now(&w.refs[p0 + tid]) == 0;
-    uint32_t more;
-    const uint32_t rank = found + block_scan(free, more);
-    if (free && rank < all) w.list[rank] = int32_t(p0 + tid);
-    found += more;
+  // the free pages: each thread counts those of a run of pages, then says which they are
+  const uint32_t run = (a.p.pages + ROWS_THREADS - 1) / ROWS_THREADS, p_lo = min(tid * run, a.p.pages), p_hi = min(p_lo + run, a.p.pages);
+  uint32_t mine = 0;
+  for (uint32_t p = p_lo; p < p_hi; ++p) {
+    const int32_t r = count(p);
+    mine += r == 0;
+    if (r < 0) report(S2HIP_PAGES_ERR_REFS);
   }
+  uint32_t rank = block_scan(mine, found);
+  for (uint32_t p = p_lo; p < p_hi && mine && rank < all; ++p)
+    if (count(p) == 0) *list(rank++) = int32_t(p);
   if (found < all && tid == 0) report(S2HIP_PAGES_ERR_FULL);
   if (stops()) return;
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = load_now(&w.refs[p]);
-  settled();
-  for (uint32_t x = tid; x < a.R * width; x += ROWS_THREADS) {
-    const uint32_t b = x / width, i = x % width;
-    int32_t v = w.table[x];
-    if (i >= first[b] && i < pages_of(total[b])) {
-      v = w.list[offset[b] + i - first[b]];
-      a.refs_out[v] = 1;
-    }
-    a.table_out[x] = v;
-  }
+  for (uint32_t i = tid; i < all; i += ROWS_THREADS) *refs(uint32_t(*list(i))) = 1;
   if (tid < a.R) {
     a.lens_out[tid] = total[tid];
     if (copies) {
       w.moves[2 * tid] = last[tid];
-      w.moves[2 * tid + 1] = w.list[offset[tid]];
-      atomicSub(&a.refs_out[last[tid]], 1);
+      w.moves[2 * tid + 1] = *list(offset[tid]);
+      atomicSub(refs(uint32_t(last[tid])), 1);
     }
   }
+  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
+    const uint32_t n = pages_of(total[b]), from = first[b], at = offset[b];
+    for (uint32_t i = lane; i < width; i += 64) a.table_out[size_t(b) * width + i] = i < from ? *rows(b * width + i) : i < n ? *list(at + i - from) : -1;
+  }
+  settled();
+  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = count(p);
 }
 
 __device__ __forceinline__ void copy_page(const PgUpdateArgs& a, uint32_t layer, int32_t from, int32_t to, uint32_t bytes, uint32_t i0, uint32_t step) {
@@ -1556,7 +1580,15 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
 }
 
 hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
-  hipLaunchKernelGGL(pg_update_kernel, dim3(1), dim3(ROWS_THREADS), 0, s, a, w);
+  const size_t lds = (2 * size_t(a.p.pages) + size_t(a.R) * a.p.width) * 4;
+  if (lds <= ROWS_LDS) {
+    static std::atomic<uint64_t> devices{0};
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(pg_update_kernel<true>), ROWS_LDS, devices);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(pg_update_kernel<true>, dim3(1), dim3(ROWS_THREADS), lds, s, a, w);
+  } else {
+    hipLaunchKernelGGL(pg_update_kernel<false>, dim3(1), dim3(ROWS_THREADS), 0, s, a, w);
+  }
   hipLaunchKernelGGL(pg_copy_kernel, dim3((page_bytes + 16383) / 16384, a.R, a.layers), dim3(256), 0, s, a, w.moves, page_bytes);
   return hipGetLastError();
 }

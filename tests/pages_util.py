@@ -105,9 +105,8 @@ def update(table, lens, refs, source, keep, add, page, width):
         for i in range(pages_of(kept[b])):
             new[b][i] = table[source[b]][i]
             refs[new[b][i]] += 1
-    for b in range(rows):
-        if any(refs[p] < 1 for p in new[b][: pages_of(kept[b])]) or any(refs[p] < 0 for p in table[b][: pages_of(lens[b])]):
-            return None
+    if any(r < 0 for r in refs) or any(refs[p] < 1 for b in range(rows) for p in new[b][: pages_of(kept[b])]):
+        return None
     free = [p for p in range(len(refs)) if refs[p] == 0]
     copies = {}
     for b in range(rows):

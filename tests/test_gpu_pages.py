@@ -640,12 +640,13 @@ def test_update_a_session(in_place):
 
 
 @pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("pages", [7, 20000])  # spare ones: few, and so many that the counts do not fit a block's LDS
 @pytest.mark.parametrize("seed", range(6))
-def test_update_and_compact_at_random(seed, in_place):
+def test_update_and_compact_at_random(seed, pages, in_place):
     g = random.Random(seed)
-    rows, page = g.choice([1, 2, 5, 17, 64]), g.choice([16, 32, 64, 128])
+    rows, page = g.choice([1, 2, 5, 17, 64]), g.choice([16, 32, 64, 128]) if pages < 100 else 16
     width = g.choice([1, 3, 12])
-    k = Book(rows, width, rows * width + 7, page=page, layers=g.choice([1, 2]), seed=seed)
+    k = Book(rows, width, rows * width + pages, page=page, layers=g.choice([1, 2]) if pages < 100 else 1, seed=seed)
     for i in range(25):
         if i % 6 == 5:
             k.compact(in_place)
@@ -683,8 +684,15 @@ def test_update_refused(in_place):
     k.table[1][0] = was
     k.d["table"].copy_(dev(k.table))
     full, k.refs[was] = k.refs[was], 1
+    assert full > 1
     k.d["refs"].copy_(dev(k.refs))
-    k.update(source=[-1, -1, -1], errors=ERR_REFS if full > 1 else 0, in_place=in_place)
+    k.update(source=[-1, -1, -1], errors=ERR_REFS, in_place=in_place)
+    k.refs[was], k.refs[8] = 0, 0
+    k.d["refs"].copy_(dev(k.refs))
+    k.update(add=[1, 0, 0], errors=ERR_REFS, in_place=in_place)  # a page that a row keeps, counted by none
+    k.refs[was], k.refs[8] = full, -1
+    k.d["refs"].copy_(dev(k.refs))
+    k.update(errors=ERR_REFS, in_place=in_place)
 
 
 def test_update_full_to_the_last_page():
