@@ -1294,19 +1294,47 @@ __device__ __forceinline__ void copy_rows(const PgUpdateArgs& a) {
   if (a.lens_out && a.lens_out != a.lens && tid < a.R) a.lens_out[tid] = a.lens[tid];
 }
 
+__device__ __forceinline__ void copy_page(const PgUpdateArgs& a, uint32_t layer, int32_t from, int32_t to, uint32_t bytes, uint32_t i0, uint32_t step) {
+  uint8_t* pool = a.p.pool + layer * a.layer_stride;
+  const u32x4* src = reinterpret_cast<const u32x4*>(pool + size_t(from) * bytes);
+  u32x4* dst = reinterpret_cast<u32x4*>(pool + size_t(to) * bytes);
+  for (uint32_t i = i0; i < bytes / 16; i += step) dst[i] = src[i];
+}
+
+// n pages, from[i] to to[i], in every layer, by all of the grid's blocks: 16 KB a turn.
+__device__ __forceinline__ void copy_pages(const PgUpdateArgs& a, const int32_t* from, const int32_t* to, uint32_t n, uint32_t bytes) {
+  constexpr uint32_t TURN = 16 * ROWS_THREADS;
+  const uint32_t parts = (bytes + TURN - 1) / TURN, per_layer = n * parts, all = per_layer * a.layers;
+  u32x4* to_now = nullptr;  // a turn's loads before the stores of the one before
+  u32x4 now{};
+  for (uint32_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const uint32_t layer = i / per_layer, page = i % per_layer / parts, at = i % parts * TURN + threadIdx.x * 16;
+    if (at >= bytes) continue;
+    uint8_t* pool = a.p.pool + layer * a.layer_stride + at;
+    const u32x4 next = *reinterpret_cast<const u32x4*>(pool + size_t(from[page]) * bytes);
+    if (to_now) *to_now = now;
+    to_now = reinterpret_cast<u32x4*>(pool + size_t(to[page]) * bytes);
+    now = next;
+  }
+  if (to_now) *to_now = now;
+}
+
 // One block, a wave per row at a time.  References are counted apart: what rows let go of is taken off, what they take
 // added; the rest of a row that stays its own counts as it is.  Of w rows that write to a page of r references, the
 // first r - 1 write to copies: the last writes in place if no one else holds it.
 //   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores.  FITS:
 // counts, free pages and new rows are in LDS (64 rows of 104 pages: 21 us -> 7 against the workspace, where each turn is
 // a trip to the second-level cache); else in the workspace.
+//   MOVES (arrays out apart from those in): every block works it all out for itself, the first writes it down, and all of
+// them copy pages: one launch, where the caller's own time per launch is what small calls take.
 constexpr uint32_t ROWS_LDS = 150 * 1024;  // bytes: counts, free pages, rows
 
-template <bool FITS>
-__global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a, PgWorkspace w) {
+template <bool FITS, bool MOVES>
+__global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a, PgWorkspace w, uint32_t bytes) {
   extern __shared__ int32_t dyn[];
   __shared__ int32_t source[MAX_ROWS], lens[MAX_ROWS], kept[MAX_ROWS], total[MAX_ROWS], last[MAX_ROWS];
   __shared__ uint32_t first[MAX_ROWS], offset[MAX_ROWS], bad;
+  const bool writes = !MOVES || blockIdx.x == 0;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), width = a.p.width, page_up = (1u << a.p.shift) - 1u;
   const int64_t cap = int64_t(width) << a.p.shift;
   auto refs = [&](uint32_t p) -> int32_t* {
@@ -1335,14 +1363,14 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     lens[tid] = a.lens[tid];
     keep = a.keep ? a.keep[tid] : 0x7fffffff;
     add = a.add ? a.add[tid] : 0;
-    w.moves[2 * tid] = -1;
+    if (!MOVES) w.moves[2 * tid] = -1;
     if (lens[tid] < 0 || lens[tid] > cap || source[tid] < -1 || source[tid] >= int32_t(a.R) || keep < 0 || add < 0) report(S2HIP_PAGES_ERR_LENS);
   }
   for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) *refs(p) = a.refs[p];
   auto stops = [&] {
     const uint32_t why = settled(bad);
-    if (why) copy_rows(a);
-    if (why && tid == 0) atomicOr(a.err, why);
+    if (why && writes) copy_rows(a);
+    if (why && writes && tid == 0) atomicOr(a.err, why);
     return why != 0;
   };
   if (stops()) return;
@@ -1401,12 +1429,26 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     if (count(p) == 0) *list(rank++) = int32_t(p);
   if (found < all && tid == 0) report(S2HIP_PAGES_ERR_FULL);
   if (stops()) return;
+  if constexpr (MOVES) {
+    uint32_t n;
+    const uint32_t at = block_scan(copies, n);
+    if (copies) {
+      source[at] = last[tid];
+      kept[at] = *list(offset[tid]);
+    }
+    __syncthreads();
+    copy_pages(a, source, kept, n, bytes);
+    if (!writes) return;
+  }
   for (uint32_t i = tid; i < all; i += ROWS_THREADS) *refs(uint32_t(*list(i))) = 1;
+  settled();
   if (tid < a.R) {
     a.lens_out[tid] = total[tid];
     if (copies) {
-      w.moves[2 * tid] = last[tid];
-      w.moves[2 * tid + 1] = *list(offset[tid]);
+      if (!MOVES) {
+        w.moves[2 * tid] = last[tid];
+        w.moves[2 * tid + 1] = *list(offset[tid]);
+      }
       atomicSub(refs(uint32_t(last[tid])), 1);
     }
   }
@@ -1418,38 +1460,44 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
   for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = count(p);
 }
 
-__device__ __forceinline__ void copy_page(const PgUpdateArgs& a, uint32_t layer, int32_t from, int32_t to, uint32_t bytes, uint32_t i0, uint32_t step) {
-  uint8_t* pool = a.p.pool + layer * a.layer_stride;
-  const u32x4* src = reinterpret_cast<const u32x4*>(pool + size_t(from) * bytes);
-  u32x4* dst = reinterpret_cast<u32x4*>(pool + size_t(to) * bytes);
-  for (uint32_t i = i0; i < bytes / 16; i += step) dst[i] = src[i];
-}
-
 // blockIdx.y = row, z = layer
 __global__ __launch_bounds__(256) void pg_copy_kernel(PgUpdateArgs a, const int32_t* moves, uint32_t bytes) {
   const int32_t from = moves[2 * blockIdx.y];
   if (from >= 0) copy_page(a, blockIdx.z, from, moves[2 * blockIdx.y + 1], bytes, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
-// One block: the pages in use, the lists of holes and movers, refs.
-__global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, PgWorkspace w) {
+// The pages in use, the lists of holes and movers, refs.  MOVES (arrays out apart from those in, and few enough pages):
+// every block works them out in its LDS, and all of them move pages and rewrite the table; else one block leaves the
+// lists in the workspace.
+template <bool MOVES>
+__global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, PgWorkspace w, uint32_t bytes) {
+  extern __shared__ int32_t dyn[];  // MOVES: holes, movers, where each page goes
   __shared__ uint32_t bad;
-  const uint32_t tid = threadIdx.x, width = a.p.width, page_up = (1u << a.p.shift) - 1u;
+  const bool writes = !MOVES || blockIdx.x == 0;
+  const uint32_t tid = threadIdx.x, width = a.p.width, page_up = (1u << a.p.shift) - 1u, pages = a.p.pages;
+  int32_t* const holes = MOVES ? dyn : w.list;
+  int32_t* const movers = MOVES ? dyn + pages : w.list + pages;
+  int32_t* const moved = MOVES ? dyn + 2 * pages : w.refs;
+  auto pages_of = [&](int32_t n) { return (uint32_t(n) + page_up) >> a.p.shift; };
   if (tid == 0) bad = 0;
   __syncthreads();
+  // each thread looks at a run of pages
+  const uint32_t run = (pages + ROWS_THREADS - 1) / ROWS_THREADS, p_lo = min(tid * run, pages), p_hi = min(p_lo + run, pages);
   uint32_t mine = 0, used;
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) {
+  for (uint32_t p = p_lo; p < p_hi; ++p) {
     const int32_t r = a.refs[p];
     mine += r > 0;
     if (r < 0) atomicOr(&bad, S2HIP_PAGES_ERR_REFS);
   }
-  for (uint32_t x = tid; x < a.R * width; x += ROWS_THREADS) {
-    const int32_t len = a.lens[x / width];
+  for (uint32_t b = tid >> 6; b < a.R; b += ROWS_THREADS / 64) {
+    const int32_t len = a.lens[b];
     if (len < 0 || int64_t(len) > int64_t(width) << a.p.shift) {
       atomicOr(&bad, S2HIP_PAGES_ERR_LENS);
-    } else if (x % width < (uint32_t(len) + page_up) >> a.p.shift) {
-      const int32_t e = a.p.table[x];
-      if (uint32_t(e) >= a.p.pages)
+      continue;
+    }
+    for (uint32_t i = tid & 63u; i < pages_of(len); i += 64) {
+      const int32_t e = a.p.table[size_t(b) * width + i];
+      if (uint32_t(e) >= pages)
         atomicOr(&bad, S2HIP_PAGES_ERR_PAGE);
       else if (a.refs[e] < 1)
         atomicOr(&bad, S2HIP_PAGES_ERR_REFS);
@@ -1457,47 +1505,58 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, P
   }
   block_scan(mine, used);
   const uint32_t why = settled(bad);
-  if (tid == 0) a.used_out[0] = int32_t(used);
+  if (writes && tid == 0) a.used_out[0] = int32_t(used);
   if (why) {
+    if (!writes) return;
     if (tid == 0) {
       w.moves[0] = 0;
       w.moves[1] = 0x7fffffff;  // no entry follows
       atomicOr(a.err, why);
     }
     if (a.refs_out != a.refs)
-      for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = a.refs[p];
+      for (uint32_t p = tid; p < pages; p += ROWS_THREADS) a.refs_out[p] = a.refs[p];
     if (a.moved_to)
-      for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.moved_to[p] = a.refs[p] > 0 ? int32_t(p) : -1;
+      for (uint32_t p = tid; p < pages; p += ROWS_THREADS) a.moved_to[p] = a.refs[p] > 0 ? int32_t(p) : -1;
+    if (MOVES)
+      for (uint32_t i = tid; i < a.R * width; i += ROWS_THREADS) a.table_out[i] = a.p.table[i];
     return;
   }
-  uint32_t holes = 0, movers = 0;
-  for (uint32_t p0 = 0; p0 < a.p.pages; p0 += ROWS_THREADS) {
-    const uint32_t p = p0 + tid;
-    const int32_t r = p < a.p.pages ? a.refs[p] : 0;
-    const bool hole = p < used && r == 0, mover = p >= used && r > 0;
-    uint32_t all;
-    const uint32_t rank = block_scan(uint32_t(hole) | uint32_t(mover) << 16, all);
-    if (hole) w.list[holes + (rank & 0xffffu)] = int32_t(p);
-    if (mover) w.list[a.p.pages + movers + (rank >> 16)] = int32_t(p);
-    holes += all & 0xffffu;
-    movers += all >> 16;
-  }
-  settled();
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) {
+  uint32_t here[2] = {0, 0}, n_holes, n_movers;
+  for (uint32_t p = p_lo; p < p_hi; ++p) {
     const int32_t r = a.refs[p];
-    if (a.refs_out != a.refs) a.refs_out[p] = p < used ? r : 0;
-    if (a.moved_to) a.moved_to[p] = r > 0 ? int32_t(p) : -1;
+    here[0] += p < used && r == 0;
+    here[1] += p >= used && r > 0;
+  }
+  uint32_t h = block_scan(here[0], n_holes), m = block_scan(here[1], n_movers);  // (as many of one as of the other)
+  for (uint32_t p = p_lo; p < p_hi; ++p) {
+    const int32_t r = a.refs[p];
+    if (p < used && r == 0) holes[h++] = int32_t(p);
+    if (p >= used && r > 0) movers[m++] = int32_t(p);
   }
   settled();
-  for (uint32_t i = tid; i < movers; i += ROWS_THREADS) {
-    const int32_t from = w.list[a.p.pages + i], to = w.list[i], r = a.refs[from];
-    a.refs_out[to] = r;
-    a.refs_out[from] = 0;
-    w.refs[from] = to;
-    if (a.moved_to) a.moved_to[from] = to;
-  }
-  if (tid == 0) {
-    w.moves[0] = int32_t(movers);
+  for (uint32_t i = tid; i < n_movers; i += ROWS_THREADS) moved[movers[i]] = holes[i];
+  if (writes)
+    for (uint32_t p = tid; p < pages; p += ROWS_THREADS) {
+      const int32_t r = a.refs[p];
+      if (a.refs_out != a.refs) a.refs_out[p] = p < used ? r : 0;
+      if (a.moved_to) a.moved_to[p] = r > 0 ? int32_t(p) : -1;
+    }
+  settled();
+  if (writes)
+    for (uint32_t i = tid; i < n_movers; i += ROWS_THREADS) {
+      const int32_t from = movers[i], to = holes[i], r = a.refs[from];
+      a.refs_out[to] = r;
+      a.refs_out[from] = 0;
+      if (a.moved_to) a.moved_to[from] = to;
+    }
+  if constexpr (MOVES) {
+    for (uint32_t x = blockIdx.x * ROWS_THREADS + tid; x < a.R * width; x += gridDim.x * ROWS_THREADS) {
+      const int32_t e = a.p.table[x];
+      if (x % width < pages_of(a.lens[x / width])) a.table_out[x] = uint32_t(e) >= used ? moved[e] : e;
+    }
+    copy_pages(a, movers, holes, n_movers, bytes);
+  } else if (tid == 0) {
+    w.moves[0] = int32_t(n_movers);
     w.moves[1] = int32_t(used);
   }
 }
@@ -1579,22 +1638,42 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
   });
 }
 
-hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
-  const size_t lds = (2 * size_t(a.p.pages) + size_t(a.R) * a.p.width) * 4;
-  if (lds <= ROWS_LDS) {
-    static std::atomic<uint64_t> devices{0};
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(pg_update_kernel<true>), ROWS_LDS, devices);
+// n ints from p, from q: any in common?
+static bool meets(const void* p, const void* q, size_t n) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q);
+  return x < y + 4 * n && y < x + 4 * n;
+}
+
+// A kernel of one block (or several that do the same) with `lds` bytes of LDS.
+template <class K>
+static hipError_t launch_rows(K kernel, std::atomic<uint64_t>& devices, uint32_t blocks, size_t lds, hipStream_t s, const PgUpdateArgs& a, const PgWorkspace& w, uint32_t bytes) {
+  if (lds) {
+    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), ROWS_LDS, devices);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(pg_update_kernel<true>, dim3(1), dim3(ROWS_THREADS), lds, s, a, w);
-  } else {
-    hipLaunchKernelGGL(pg_update_kernel<false>, dim3(1), dim3(ROWS_THREADS), 0, s, a, w);
   }
+  hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ROWS_THREADS), lds, s, a, w, bytes);
+  return hipGetLastError();
+}
+
+hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
+  const size_t words = size_t(a.R) * a.p.width, lds = (2 * size_t(a.p.pages) + words) * 4;
+  const bool fits = lds <= ROWS_LDS, in_place = meets(a.refs, a.refs_out, a.p.pages) || meets(a.p.table, a.table_out, words) || meets(a.lens, a.lens_out, a.R);
+  static std::atomic<uint64_t> both{0}, one{0};
+  if (fits && !in_place) return launch_rows(pg_update_kernel<true, true>, both, 256, lds, s, a, w, page_bytes);
+  const hipError_t e = fits ? launch_rows(pg_update_kernel<true, false>, one, 1, lds, s, a, w, page_bytes)
+                            : launch_rows(pg_update_kernel<false, false>, one, 1, 0, s, a, w, page_bytes);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pg_copy_kernel, dim3((page_bytes + 16383) / 16384, a.R, a.layers), dim3(256), 0, s, a, w.moves, page_bytes);
   return hipGetLastError();
 }
 
 hipError_t launch_pg_compact(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
-  hipLaunchKernelGGL(pg_pack_kernel, dim3(1), dim3(ROWS_THREADS), 0, s, a, w);
+  const size_t words = size_t(a.R) * a.p.width, lds = 3 * size_t(a.p.pages) * 4;
+  static std::atomic<uint64_t> both{0}, one{0};
+  if (lds <= ROWS_LDS && !meets(a.refs, a.refs_out, a.p.pages) && !meets(a.p.table, a.table_out, words))
+    return launch_rows(pg_pack_kernel<true>, both, 256, lds, s, a, w, page_bytes);
+  const hipError_t e = launch_rows(pg_pack_kernel<false>, one, 1, 0, s, a, w, page_bytes);
+  if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pg_move_kernel, dim3(2048), dim3(256), 0, s, a, w, page_bytes);
   return hipGetLastError();
 }
