@@ -49,6 +49,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
   constexpr uint32_t HPB = 256 / LP;  // heads per step of the block
   constexpr int PAIRS = HALF ? 8 : 4;
   __shared__ double2 turn[HD / 2];
+  __shared__ __align__(16) float gains[2][HD];  // of queries, of keys
   const uint32_t tid = threadIdx.x, b = blockIdx.x / a.c.n, t = blockIdx.x % a.c.n;
   const RawRequest raw = load_request(a.c, b);
   const int32_t pos = a.positions[size_t(b) * a.c.n + t];
@@ -62,13 +63,16 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     const float* row = src + size_t(min(h, heads - 1)) * HD;
     *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(row + d0);
     *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(row + d0 + 4);
-    if constexpr (HALF) {
+    if constexpr (HALF) {  // (loaded once more: exchanged between lanes they cost 5 % of a turn)
       *reinterpret_cast<float4*>(z) = *reinterpret_cast<const float4*>(row + o0);
       *reinterpret_cast<float4*>(z + 4) = *reinterpret_cast<const float4*>(row + o0 + 4);
     }
   };
   load(h0);
   const double per_token = tid < half ? a.rope.turns[tid] : 0.0;
+  float4 gain4{};
+  const bool brings = a.q_norm && tid < HD / 2;  // 4 of the gains each
+  if (brings) gain4 = *reinterpret_cast<const float4*>((tid < HD / 4 ? a.q_norm : a.k_norm) + 4 * (tid % (HD / 4)));
   const Request r = checked(a.c, raw, tid == 0 && t == 0 && blockIdx.y == 0 ? a.s.err : nullptr);
   if (t >= r.fresh) return;
   if (pos < 0) {
@@ -85,6 +89,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     sincospi(2.0 * (angle - rint(angle)), &sn, &cs);
     turn[tid] = tid < half ? make_double2(cs * a.rope.gain, sn * a.rope.gain) : make_double2(1.0, 0.0);
   }
+  if (brings) *reinterpret_cast<float4*>(&gains[0][4 * tid]) = gain4;
   __syncthreads();
   double2 cs[PAIRS];
 #pragma unroll
@@ -100,11 +105,11 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     for (int e = 0; e < 8; ++e) y[e] = x[e];
     if (!value) {
       double f = 1.0;
-      const float* gain = h < a.s.H ? a.q_norm : a.k_norm;
+      const float* gain = gains[h < a.s.H ? 0 : 1];
       double w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = HALF ? z[e] : 0.0f;
-      if (gain) {
+      if (a.q_norm) {
         double ss = 0.0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fma(y[e], y[e], ss);
@@ -146,34 +151,43 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
       *reinterpret_cast<float4*>(dst + 4) = make_float4(float(y[4]), float(y[5]), float(y[6]), float(y[7]));
       continue;
     }
-    // the group's largest by size (4 lanes), the first of equals
-    double big = 0.0;
-    uint32_t odd = 0;
+    // the group's ends (4 lanes), and whether all are numbers (0 x what is none)
+    double most = y[0], least = y[0], zero = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      big = fmax(big, fabs(y[e]));
-      odd |= !(fabs(y[e]) < 16384.0);
+      if (e) most = fmax(most, y[e]);
+      if (e) least = fmin(least, y[e]);
+      zero = fma(y[e], 0.0, zero);
     }
-    big = fmax(big, dpp_f64<DPP_QUAD_XOR1>(big));
-    big = fmax(big, dpp_f64<DPP_QUAD_XOR2>(big));
-    uint32_t first = 1000;  // place in the group, doubled, + 1 of a negative one
+    most = fmax(most, dpp_f64<DPP_QUAD_XOR1>(most));
+    least = fmin(least, dpp_f64<DPP_QUAD_XOR1>(least));
+    zero += dpp_f64<DPP_QUAD_XOR1>(zero);
+    most = fmax(most, dpp_f64<DPP_QUAD_XOR2>(most));
+    least = fmin(least, dpp_f64<DPP_QUAD_XOR2>(least));
+    zero += dpp_f64<DPP_QUAD_XOR2>(zero);
+    const double big = fmax(most, -least);
+    const bool odd = !(zero == 0.0) || big >= 16384.0;
+    bool negative = -least > most;  // the largest by size is
+    if (__any(most == -least && most != 0.0)) {  // two are, one of either sign: the first of them
+      uint32_t first = 1000;  // place in the group, doubled, + 1 of a negative one
 #pragma unroll
-    for (int e = 7; e >= 0; --e)
-      if (fabs(y[e]) == big) first = 2 * (8 * (l % 4) + e) + (y[e] < 0.0 ? 1 : 0);
-    first = min(first, dpp_u32<DPP_QUAD_XOR1>(first));
-    first = min(first, dpp_u32<DPP_QUAD_XOR2>(first));
-    odd |= dpp_u32<DPP_QUAD_XOR1>(odd);
-    odd |= dpp_u32<DPP_QUAD_XOR2>(odd);
-    double d = rounded8(big * 0.125);
-    if (!(first & 1)) d = -d;
-    const double inv = odd || d == 0.0 ? 0.0 : 1.0 / d;
+      for (int e = 7; e >= 0; --e)
+        if (fabs(y[e]) == big) first = 2 * (8 * (l % 4) + e) + (y[e] < 0.0 ? 1 : 0);
+      first = min(first, dpp_u32<DPP_QUAD_XOR1>(first));
+      first = min(first, dpp_u32<DPP_QUAD_XOR2>(first));
+      if (most == -least) negative = first & 1u;
+    }
+    const double size = rounded8(big * 0.125), d = negative ? size : -size;
+    const double inv = odd || size == 0.0 ? 0.0 : 1.0 / d;
     // y / d is y inv but for 2^-52 of it.  It is at most 8 2^9 / (2^9 - 1): taken to a multiple of 2^-40 first, one that is
-    // halfway between whole numbers is so again (no other quotient of a value's 24 bits by 8 comes so near).
-    uint32_t code[8];
+    // halfway between whole numbers is so again (no other quotient of a value's 24 bits by 8 comes so near).  Then to a whole
+    // number, ties to even, which stands in the low bits of the sum with 1.5 2^52.
+    int code[8];  // less 8
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const double near = (odd ? 0.0 : y[e]) * inv + 0x1.8p12;
-      code[e] = uint32_t(min(max(int(rint(near - 0x1.8p12)), -8), 7) + 8);
+      const double near = fma(y[e], inv, 0x1.8p12);
+      const int whole = int(uint32_t(uint64_t(__double_as_longlong(near + (0x1.8p52 - 0x1.8p12)))));
+      code[e] = odd ? 0 : min(max(whole, -8), 7);
     }
     const float scale = odd ? NAN : float(d);
     const uint32_t g = value ? now - a.s.H - a.s.G : now - a.s.H, j = l / 4;
@@ -182,8 +196,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
       held += ((size_t(b) * a.c.n + t) * a.s.G + g) * HD + d0;
 #pragma unroll
       for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<float4*>(held + e) = make_float4(scale * float(int(code[e]) - 8), scale * float(int(code[e + 1]) - 8),
-                                                           scale * float(int(code[e + 2]) - 8), scale * float(int(code[e + 3]) - 8));
+        *reinterpret_cast<float4*>(held + e) = make_float4(scale * float(code[e]), scale * float(code[e + 1]), scale * float(code[e + 2]), scale * float(code[e + 3]));
     }
     if (!there) continue;
     if (odd) atomicOr(a.s.err, S2HIP_PAGES_ERR_RANGE);
@@ -191,16 +204,16 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     uint8_t* part = a.p.pool + (size_t(page) * a.s.G + g) * a.p.chunk;
     const uint32_t s = slot & ((1u << a.p.shift) - 1u);
     if (!value) {
-      uint32_t word = 0;
+      uint32_t word = 0x88888888u;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) word |= code[e] << (e / 2 * 4 + e % 2 * 16);
+      for (int e = 0; e < 8; ++e) word += uint32_t(code[e]) << (e / 2 * 4 + e % 2 * 16);
       *reinterpret_cast<uint32_t*>(part + ((s * 4 + l % 4) * (HD / 32) + j) * 4) = word;
       if (l % 4 == 0) *reinterpret_cast<_Float16*>(part + at.ks() + (s * (HD / 32) + j) * 2) = _Float16(scale);
     } else {
       const uint32_t quad = s / 4, one = s % 4;  // (16 u + 4 i = 4 quad)
 #pragma unroll
       for (uint32_t m = 0; m < 4; ++m)
-        part[at.v() + ((quad * 16 + 4 * (l % 4) + m) * (HD / 32) + j) * 4 + one] = uint8_t(code[2 * m] | code[2 * m + 1] << 4);
+        part[at.v() + ((quad * 16 + 4 * (l % 4) + m) * (HD / 32) + j) * 4 + one] = uint8_t(0x88u + uint32_t(code[2 * m]) + (uint32_t(code[2 * m + 1]) << 4));
       if (l % 4 == 0) *reinterpret_cast<_Float16*>(part + at.vs() + ((quad * (HD / 32) + j) * 4 + one) * 2) = _Float16(scale);
     }
   }
@@ -1588,12 +1601,13 @@ hipError_t by_dim(uint32_t hd, F&& f) {
 
 hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s) {
   return by_dim(hd, [&](auto HD) {
-    const uint32_t tokens = a.c.R * a.c.n, steps = (a.s.H + 2 * a.s.G + 2048 / HD() - 1) / (2048 / HD());
+    const uint32_t tokens = a.c.R * a.c.n, steps = ((a.s.H + 2 * a.s.G) * HD() + 2047) / 2048;
     const dim3 grid(tokens, min(steps, max(1u, 512 / tokens)));
+    auto go = [&](auto HALF) { hipLaunchKernelGGL((pg_append_kernel<HD(), HALF()>), grid, dim3(256), 0, s, a); };
     if (a.rope.half)
-      hipLaunchKernelGGL((pg_append_kernel<HD(), true>), grid, dim3(256), 0, s, a);
+      go(std::true_type());
     else
-      hipLaunchKernelGGL((pg_append_kernel<HD(), false>), grid, dim3(256), 0, s, a);
+      go(std::false_type());
     return hipGetLastError();
   });
 }
