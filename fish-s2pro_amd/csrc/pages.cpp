@@ -95,6 +95,7 @@ class Pages : DeviceArrays {
     work_.list = alloc<int32_t>(size_t(c.pages) * 2);
     work_.table = alloc<int32_t>(size_t(c.max_requests) * c.table_pages);
     work_.moves = alloc<int32_t>(2 * PG_MAX_REQUESTS);
+    CHK(prepare_pg());
     CHK(hipDeviceSynchronize());
   }
   uint64_t bytes() const { return uint64_t(chunk_) * cfg_.kv_heads; }

@@ -71,6 +71,7 @@ struct PgWorkspace {
   int32_t* moves;  // [256][2]: pages that are copied, from and to; [0]: their number (compact)
 };
 
+hipError_t prepare_pg();  // of the current device, before the others
 hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s);
 hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& a, const PgWorkspace& w, hipStream_t s);
 hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s);

@@ -684,6 +684,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
           if (first < KT && limit >= int(w.key0 + first)) o[2 * c] = o[2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
         }
       }
+      asm volatile("" ::: "memory");  // (what is read below in other types is what was written here)
     }
     take_k(slot);
     floatx4 s[2] = {};
@@ -1345,7 +1346,7 @@ constexpr uint32_t ROWS_LDS = 150 * 1024;  // bytes: counts, free pages, rows
 template <bool FITS, bool MOVES>
 __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a, PgWorkspace w, uint32_t bytes) {
   extern __shared__ int32_t dyn[];
-  __shared__ int32_t source[MAX_ROWS], lens[MAX_ROWS], kept[MAX_ROWS], total[MAX_ROWS], last[MAX_ROWS];
+  __shared__ int32_t source[MAX_ROWS], lens[MAX_ROWS], kept[MAX_ROWS], total[MAX_ROWS], last[MAX_ROWS], before[MAX_ROWS];
   __shared__ uint32_t first[MAX_ROWS], offset[MAX_ROWS], bad;
   const bool writes = !MOVES || blockIdx.x == 0;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), width = a.p.width, page_up = (1u << a.p.shift) - 1u;
@@ -1380,8 +1381,16 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     if (lens[tid] < 0 || lens[tid] > cap || source[tid] < -1 || source[tid] >= int32_t(a.R) || keep < 0 || add < 0) report(S2HIP_PAGES_ERR_LENS);
   }
   for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) *refs(p) = a.refs[p];
+  auto turn_over = [&] {
+    if constexpr (FITS)
+      __syncthreads();
+    else
+      settled();
+  };
   auto stops = [&] {
-    const uint32_t why = settled(bad);
+    turn_over();
+    const uint32_t why = *const_cast<const volatile uint32_t*>(&bad);
+    __syncthreads();
     if (why && writes) copy_rows(a);
     if (why && writes && tid == 0) atomicOr(a.err, why);
     return why != 0;
@@ -1393,36 +1402,51 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     total[tid] = int32_t(uint32_t(kept[tid]) + uint32_t(add));
   }
   if (stops()) return;
+  // (what is the same for a row's lanes in scalar registers: the block's sixteen waves share four vector units)
   for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
-    const int32_t s = source[b];
-    const uint32_t n_old = pages_of(lens[b]), n_base = pages_of(kept[b]);
-    const int32_t *old_row = a.p.table + size_t(b) * width, *base_row = a.p.table + size_t(max(s, 0)) * width;
-    for (uint32_t i = lane; i < max(n_old, n_base); i += 64) {
-      const bool old = i < n_old, base = i < n_base;
-      const int32_t e = old ? old_row[i] : -1, v = !base ? -1 : s == int32_t(b) ? e : base_row[i];
-      const bool e_in = uint32_t(e) < a.p.pages, v_in = uint32_t(v) < a.p.pages;
-      if ((old && !e_in) || (base && !v_in)) report(S2HIP_PAGES_ERR_PAGE);
-      if (s != int32_t(b) || !base) {
-        if (old && e_in) atomicSub(refs(uint32_t(e)), 1);
-        if (base && v_in) atomicAdd(refs(uint32_t(v)), 1);
+    const uint32_t n_old = uniform(pages_of(lens[b])), n_base = uniform(pages_of(kept[b])), s = uniform(uint32_t(source[b]));
+    const int32_t *old_row = a.p.table + size_t(b) * width, *base_row = a.p.table + size_t(s == 0xffffffffu ? 0 : s) * width;
+    const bool same = s == b;
+    for (uint32_t i0 = 0; i0 < max(n_old, n_base); i0 += 128) {  // two entries a lane, their loads together
+      int32_t e[2], v[2];
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t i = i0 + 64 * k + lane;
+        e[k] = i < n_old ? old_row[i] : 0;
+        v[k] = same ? e[k] : i < n_base ? base_row[i] : 0;
       }
-      if (base) *rows(b * width + i) = v;
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        const uint32_t i = i0 + 64 * k + lane;
+        const bool in = uint32_t(e[k]) < a.p.pages && uint32_t(v[k]) < a.p.pages;
+        if (!in) report(S2HIP_PAGES_ERR_PAGE);
+        if (in && i < n_old && (!same || i >= n_base)) atomicSub(refs(uint32_t(e[k])), 1);
+        if (in && i < n_base && !same) atomicAdd(refs(uint32_t(v[k])), 1);
+        if (i < n_base) *rows(b * width + i) = v[k];
+      }
     }
   }
   if (stops()) return;
-  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64)
-    for (uint32_t i = lane; i < pages_of(kept[b]); i += 64)
-      if (count(uint32_t(*rows(b * width + i))) < 1) report(S2HIP_PAGES_ERR_REFS);
+  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
+    const uint32_t n = uniform(pages_of(kept[b]));
+    for (uint32_t i0 = 0; i0 < n; i0 += 128) {
+      const uint32_t i = i0 + lane;
+      const int32_t x = i < n ? count(uint32_t(*rows(b * width + i))) : 1, y = i + 64 < n ? count(uint32_t(*rows(b * width + i + 64))) : 1;
+      if (min(x, y) < 1) report(S2HIP_PAGES_ERR_REFS);
+    }
+  }
   const bool grows = tid < a.R && add > 0 && (uint32_t(kept[tid]) & page_up) != 0;
   if (tid < a.R) last[tid] = grows ? *rows(tid * width + (uint32_t(kept[tid]) >> a.p.shift)) : -1;
   __syncthreads();
+  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {  // earlier rows that grow into the same page
+    uint32_t n = 0;
+    for (uint32_t i = lane; i < (b + 63) / 64 * 64; i += 64) n += uint32_t(__popcll(__ballot(i < b && last[i] == last[b])));
+    if (lane == 0) before[b] = int32_t(n);
+  }
+  __syncthreads();
   uint32_t needs = 0, copies = 0;
   if (tid < a.R) {
-    if (grows) {
-      int32_t before = 0;
-      for (uint32_t b = 0; b < tid; ++b) before += last[b] == last[tid];
-      copies = before < count(uint32_t(last[tid])) - 1;
-    }
+    if (grows) copies = before[tid] < count(uint32_t(last[tid])) - 1;
     first[tid] = pages_of(kept[tid]) - copies;
     needs = pages_of(total[tid]) - first[tid];
   }
@@ -1454,7 +1478,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     if (!writes) return;
   }
   for (uint32_t i = tid; i < all; i += ROWS_THREADS) *refs(uint32_t(*list(i))) = 1;
-  settled();
+  turn_over();
   if (tid < a.R) {
     a.lens_out[tid] = total[tid];
     if (copies) {
@@ -1466,10 +1490,10 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     }
   }
   for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
-    const uint32_t n = pages_of(total[b]), from = first[b], at = offset[b];
+    const uint32_t n = uniform(pages_of(total[b])), from = uniform(first[b]), at = uniform(offset[b]);
     for (uint32_t i = lane; i < width; i += 64) a.table_out[size_t(b) * width + i] = i < from ? *rows(b * width + i) : i < n ? *list(at + i - from) : -1;
   }
-  settled();
+  turn_over();
   for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = count(p);
 }
 
@@ -1658,13 +1682,21 @@ static bool meets(const void* p, const void* q, size_t n) {
   return x < y + 4 * n && y < x + 4 * n;
 }
 
-// A kernel of one block (or several that do the same) with `lds` bytes of LDS.
-template <class K>
-static hipError_t launch_rows(K kernel, std::atomic<uint64_t>& devices, uint32_t blocks, size_t lds, hipStream_t s, const PgUpdateArgs& a, const PgWorkspace& w, uint32_t bytes) {
-  if (lds) {
-    const hipError_t e = allow_lds(reinterpret_cast<const void*>(kernel), ROWS_LDS, devices);
+// Once per device, before the launches there.
+hipError_t prepare_pg() {
+  static std::atomic<uint64_t> devices[3];
+  const void* kernels[3] = {reinterpret_cast<const void*>(pg_update_kernel<true, true>), reinterpret_cast<const void*>(pg_update_kernel<true, false>),
+                            reinterpret_cast<const void*>(pg_pack_kernel<true>)};
+  for (int i = 0; i < 3; ++i) {
+    const hipError_t e = allow_lds(kernels[i], ROWS_LDS, devices[i]);
     if (e != hipSuccess) return e;
   }
+  return hipSuccess;
+}
+
+// A kernel of one block (or several that do the same) with `lds` bytes of LDS.
+template <class K>
+static hipError_t launch_rows(K kernel, uint32_t blocks, size_t lds, hipStream_t s, const PgUpdateArgs& a, const PgWorkspace& w, uint32_t bytes) {
   hipLaunchKernelGGL(kernel, dim3(blocks), dim3(ROWS_THREADS), lds, s, a, w, bytes);
   return hipGetLastError();
 }
@@ -1672,10 +1704,9 @@ static hipError_t launch_rows(K kernel, std::atomic<uint64_t>& devices, uint32_t
 hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
   const size_t words = size_t(a.R) * a.p.width, lds = (2 * size_t(a.p.pages) + words) * 4;
   const bool fits = lds <= ROWS_LDS, in_place = meets(a.refs, a.refs_out, a.p.pages) || meets(a.p.table, a.table_out, words) || meets(a.lens, a.lens_out, a.R);
-  static std::atomic<uint64_t> both{0}, one{0};
-  if (fits && !in_place) return launch_rows(pg_update_kernel<true, true>, both, 256, lds, s, a, w, page_bytes);
-  const hipError_t e = fits ? launch_rows(pg_update_kernel<true, false>, one, 1, lds, s, a, w, page_bytes)
-                            : launch_rows(pg_update_kernel<false, false>, one, 1, 0, s, a, w, page_bytes);
+  if (fits && !in_place) return launch_rows(pg_update_kernel<true, true>, 256, lds, s, a, w, page_bytes);
+  const hipError_t e = fits ? launch_rows(pg_update_kernel<true, false>, 1, lds, s, a, w, page_bytes)
+                            : launch_rows(pg_update_kernel<false, false>, 1, 0, s, a, w, page_bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pg_copy_kernel, dim3((page_bytes + 16383) / 16384, a.R, a.layers), dim3(256), 0, s, a, w.moves, page_bytes);
   return hipGetLastError();
@@ -1683,10 +1714,9 @@ hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_
 
 hipError_t launch_pg_compact(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
   const size_t words = size_t(a.R) * a.p.width, lds = 3 * size_t(a.p.pages) * 4;
-  static std::atomic<uint64_t> both{0}, one{0};
   if (lds <= ROWS_LDS && !meets(a.refs, a.refs_out, a.p.pages) && !meets(a.p.table, a.table_out, words))
-    return launch_rows(pg_pack_kernel<true>, both, 256, lds, s, a, w, page_bytes);
-  const hipError_t e = launch_rows(pg_pack_kernel<false>, one, 1, 0, s, a, w, page_bytes);
+    return launch_rows(pg_pack_kernel<true>, 256, lds, s, a, w, page_bytes);
+  const hipError_t e = launch_rows(pg_pack_kernel<false>, 1, 0, s, a, w, page_bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pg_move_kernel, dim3(2048), dim3(256), 0, s, a, w, page_bytes);
   return hipGetLastError();

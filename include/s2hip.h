@@ -621,9 +621,9 @@ int32_t s2hip_pages_errors(s2hip_pages* pages, void* stream, uint32_t* bits, cha
  * to slot lens[b] - new_lens[b] + t of request b's pages, which have to be its alone
  * (s2hip_pages_update sees to that).  k_held, v_held (nullable, [requests][n_tokens]
  * [kv_heads head_dim]): the new keys and values as the cache holds them.  A request
- * out of range is left out, so is a token whose page is not one of the pool, but for
- * its query.  Rows of tokens t >= new_lens[b] stay as they were.  No output may
- * overlap an input or another. */
+ * out of range is left out; of a token whose page is not one of the pool only the
+ * outputs are written.  Rows of tokens t >= new_lens[b] stay as they were.  No output
+ * may overlap an input or another. */
 int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, const float* qkv, uint32_t n_tokens,
                            const int32_t* positions, const float* q_norm, const float* k_norm, float* q_out,
                            float* k_held, float* v_held, void* stream, char* err, size_t err_cap);
