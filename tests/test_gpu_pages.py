@@ -730,6 +730,31 @@ def test_rows_of_large_tables():
     k.compact(in_place=False)
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+def test_update_most_rows(in_place):
+    """256 rows: all fork one, grow into its last page, and are sorted anew."""
+    k = Book(256, 3, 700, page=16, layers=1)
+    k.update(add=[20] + [0] * 255, in_place=in_place)
+    k.update(source=[0] * 256, add=[b % 3 for b in range(256)], in_place=in_place)
+    k.update(source=list(range(255, -1, -1)), add=[1] * 256, in_place=in_place)
+    k.update(source=[b // 2 for b in range(256)], keep=[21 + b % 3 for b in range(256)], in_place=in_place)
+    k.compact(in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_update_what_else_holds_pages(in_place):
+    """Counts that no row of the table stands for: a page with one is neither free nor any row's alone."""
+    k = Book(3, 4, 12)
+    k.update(add=[20, 16, 5], in_place=in_place)
+    for p in (k.table[0][1], k.table[2][0], 9):
+        k.refs[p] += 1
+    k.d["refs"].copy_(dev(k.refs))
+    k.update(add=[1, 1, 0], in_place=in_place)  # row 0 grows into a copy
+    k.update(keep=[0, 17, 0], in_place=in_place)
+    assert [p for p, n in enumerate(k.refs) if n] and k.refs[9] == 1
+    k.update(add=[64, 0, 0], in_place=in_place)
+
+
 def test_layers_apart():
     k = Book(3, 4, 8, layers=2)
     gap = torch.full((2, 8 * k.ops.page_bytes + 64), 3, dtype=torch.uint8, device="cuda")
@@ -844,6 +869,102 @@ def test_sessions_in_a_graph():
             assert torch.equal(getattr(a, x), getattr(b, x)), x
         assert torch.equal(a.out[live], b.out[live])
         a.check()
+
+
+def other_arrays(p):
+    """The pool's arrays at addresses of 16 bytes and no more, as parts of larger ones."""
+    def moved(x, to):
+        y = torch.zeros(x.numel() * x.element_size() + 4096, dtype=torch.uint8, device="cuda")[to : to + x.numel() * x.element_size()]
+        y = y.view(x.dtype).view(x.shape)
+        assert y.data_ptr() % 256 == to % 256
+        return y.copy_(x)
+
+    p.pool, p.q, p.out = moved(p.pool, 16), moved(p.q, 48), moved(p.out, 80)
+    p.table, p.lens, p.new = moved(p.table, 4), moved(p.lens, 12), moved(p.new, 20)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attend_addresses(hd, n, page):
+    p = Pool((8, 2, hd), page, [333, 40 + n], [n, n], shared=1, seed=40, width=None if n == 1 else 4000 // page)
+    other_arrays(p)
+    p.check_all()
+
+
+def test_graphs_on_one_handle_from_its_first_calls():
+    """Attention of one token, of a turn and of a prompt, captured by a handle that has run nothing, two graphs of one
+    workspace; replayed in turn, with eager calls, new lengths, tables and queries in between."""
+    for n, width in ((1, 40000 // 64), (40, 20000 // 64)):
+        p = Pool((32, 8, 128), 64, [5000, 300, 64 + n], [n, n, n], shared=1, seed=50 + n, width=width)
+        side = torch.cuda.Stream()
+        outs = [torch.full_like(p.out, 7.0) for _ in range(2)]
+        queries = [p.q.clone(), p.q.flip(0).contiguous()]
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        torch.cuda.synchronize()
+        for graph, q, out in zip(graphs, queries, outs):
+            with torch.cuda.graph(graph, stream=side):
+                p.ops.attend(p.view(), ptr(q), n, ptr(out), stream=torch.cuda.current_stream().cuda_stream)
+        for turn in range(4):
+            p.lens_h = [5000 - 700 * turn, 300 - turn, 64 + n]
+            p.new_h = [n, n if turn % 2 else 0, n]
+            p.lens.copy_(dev(p.lens_h))
+            p.new.copy_(dev(p.new_h))
+            p.table_h[0][1], p.table_h[0][2] = p.table_h[0][2], p.table_h[0][1]
+            p.table.copy_(dev(p.table_h))
+            for graph, q, out in zip(graphs, queries, outs):
+                q.add_(0.01 * turn)
+                out.fill_(7.0)
+                graph.replay()
+                p.q = q
+                p.out = torch.full_like(out, 7.0)
+                want = p.expect()
+                p.check(p.attend(), want)
+                p.check(out, want)
+                assert torch.equal(out, p.out)
+        assert p.ops.errors(stream()) == 0
+
+
+def test_rows_in_a_graph_apart():
+    """Update and compact of arrays apart (one launch each), captured as a handle's first calls; replayed there and back."""
+    rows, page, pages, width = 5, 16, 40, 6
+    ops = PagedKv(4, 1, 64, page, pages, width, max_requests=rows, max_tokens=64)
+    lay = [dict(table=torch.full((rows, width), -1, dtype=torch.int32, device="cuda"), lens=dev([0] * rows), refs=dev([0] * pages)) for _ in range(3)]
+    pool = torch.arange(pages * ops.page_bytes // 4, dtype=torch.int32, device="cuda").view(pages, -1)
+    source, keep, add, used = dev(list(range(rows))), dev([1 << 30] * rows), dev([0] * rows), dev([0])
+    host = pool.cpu().numpy().copy()
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    a, b, c = lay
+    with torch.cuda.graph(graph, stream=side):
+        at = torch.cuda.current_stream().cuda_stream
+        ops.update(ops.view(ptr(pool), ptr(a["table"]), ptr(a["lens"]), rows), ptr(a["refs"]), ptr(b["refs"]), ptr(b["table"]), ptr(b["lens"]),
+                   source=ptr(source), keep=ptr(keep), add=ptr(add), stream=at)
+        ops.compact(ops.view(ptr(pool), ptr(b["table"]), ptr(b["lens"]), rows), ptr(b["refs"]), ptr(c["refs"]), ptr(c["table"]), ptr(used), stream=at)
+    table, lens, refs = [[-1] * width for _ in range(rows)], [0] * rows, [0] * pages
+    g = random.Random(3)
+    for turn in range(8):
+        src = [g.randrange(rows) for _ in range(rows)]
+        kp = [g.randint(0, 60) for _ in range(rows)]
+        ad = [g.randint(0, 30) for _ in range(rows)]
+        source.copy_(dev(src)), keep.copy_(dev(kp)), add.copy_(dev(ad))
+        c["table"].fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        table, lens, refs, copies = pages_util.update(table, lens, refs, src, kp, ad, page, width)
+        old = host.copy()
+        for to, at in copies.items():
+            host[to] = old[at]
+        table, refs, to, n = pages_util.compact(table, lens, refs, page)
+        old = host.copy()
+        for x, y in to.items():
+            host[y] = old[x]
+        assert b["lens"].tolist() == lens and c["refs"].tolist() == refs and int(used) == n
+        for row, got, length in zip(table, c["table"].tolist(), lens):
+            assert got[: -(-length // page)] == row[: -(-length // page)]
+        assert np.array_equal(pool.cpu().numpy(), host)
+        a["table"].copy_(c["table"]), a["lens"].copy_(b["lens"]), a["refs"].copy_(c["refs"])
+        assert ops.errors(stream()) == 0
 
 
 def test_two_handles_side_by_side():
