@@ -38,9 +38,23 @@ struct PgAppendArgs {
   float* v_held;  // nullable
 };
 
+// n / d for n below 2^31: m is above 2^(31 + s) / d by less than 2^s / d, where 2^s is at least d, so 2 n m is above
+// 2^(32 + s) n / d by less than 2^(32 + s) / d.  (A division of the compiler's is 35 instructions, and a step's kernel begins
+// with ten of them one behind the other.)
+struct Div {
+  uint32_t m, s;
+  static Div by(uint32_t d) {
+    uint32_t s = 0;
+    while ((uint64_t(1) << s) < d) ++s;
+    return {uint32_t((uint64_t(1) << (31 + s)) / d + 1), s};
+  }
+  __host__ __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return uint32_t((uint64_t(n + n) * m) >> 32) >> s; }
+};
+
 struct PgAttendArgs {
   KvAttendArgs a;  // shape, lens, new_lens, R, n, cap, q, out
   PgPool p;
+  Div by_rows, by_rep, by_groups;  // n rep (a request's packed rows), rep, G
 };
 
 struct PgUpdateArgs {
@@ -73,7 +87,7 @@ struct PgWorkspace {
 
 hipError_t prepare_pg();  // of the current device, before the others
 hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s);
-hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& a, const PgWorkspace& w, hipStream_t s);
+hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs a, const PgWorkspace& w, hipStream_t s);
 hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s);
 hipError_t launch_pg_compact(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s);
 

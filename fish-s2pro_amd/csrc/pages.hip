@@ -310,7 +310,7 @@ __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
 // each request's own.  Page numbers stand one per lane, 64 at a time.
 constexpr int STEP_WAVES = 4;
 
-// The tiles of `n_rows` packed rows from row0 on.  Lane j holds request b_lo + j (at most 64 requests).
+// The tiles of `n_rows` packed rows from row0 on.  Lane j holds request b_lo + j (at most 16 requests).
 struct PgRun {
   uint32_t b_lo;
   uint32_t common;    // keys that all have in common, a multiple of 32
@@ -333,23 +333,32 @@ __device__ __forceinline__ Pages64 load_pages(const PgAttendArgs& pa, uint32_t b
   return p;
 }
 
+// Sum over lanes 0 .. l of 16.
+__device__ __forceinline__ uint32_t row_scan(uint32_t x) {
+  x += dpp_or_0<0x111, 0xF>(x);
+  x += dpp_or_0<0x112, 0xF>(x);
+  x += dpp_or_0<0x114, 0xF>(x);
+  x += dpp_or_0<0x118, 0xF>(x);
+  return x;
+}
+
 template <int KT>
 __device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, uint32_t n_rows, RawRequest raw, const Pages64& early, uint32_t* err) {
   const KvAttendArgs& a = pa.a;
   const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep, row1 = min(row0 + n_rows, a.c.R * per);
   PgRun r{};
-  r.b_lo = row0 / per;
+  r.b_lo = pa.by_rows(row0);
   const uint32_t b = r.b_lo + lane;
-  if (b <= (row1 - 1) / per) {
+  if (b <= pa.by_rows(row1 - 1)) {
     r.rq = checked(a.c, raw, err);
     const uint32_t first = max(row0, b * per) - b * per, last = min(row1, (b + 1) * per) - 1 - b * per;
-    if (first / a.s.rep < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(last / a.s.rep, r.rq.fresh - 1) + 1;
+    if (pa.by_rep(first) < r.rq.fresh) r.seg_keys = r.rq.len - r.rq.fresh + min(pa.by_rep(last), r.rq.fresh - 1) + 1;
   }
   // what every row with a token sees, as far as the tables agree
   const uint64_t has = __ballot(r.seg_keys != 0);
   if (__popcll(has) > 1) {
     uint32_t least = r.seg_keys ? r.rq.len - r.rq.fresh + 1 : 0xffffffffu;
-    least = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+    least = lane_read_u32(row_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); }), 0);
     const uint32_t pages = least >> pa.p.shift;
     uint32_t same = 0;
     for (; same < pages;) {
@@ -381,9 +390,13 @@ __device__ __forceinline__ PgRun pg_run(const PgAttendArgs& pa, uint32_t row0, u
     }
     r.common = (same << pa.p.shift) / KT * KT;
   }
-  r.seg_end = wave_scan(r.seg_keys > r.common ? (r.seg_keys - r.common + KT - 1) / KT : 0u);
-  r.tiles = lane_read_u32(r.seg_end, 63);
+  r.seg_end = row_scan(r.seg_keys > r.common ? (r.seg_keys - r.common + KT - 1) / KT : 0u);
+  r.tiles = lane_read_u32(r.seg_end, 15);
   return r;
+}
+// The request of own tile x, less b_lo: how many end before it.
+__device__ __forceinline__ uint32_t owner(const PgRun& r, uint32_t x) {
+  return min(15u, uint32_t(__popcll(__ballot(r.seg_end <= x) & 0xffffu)));
 }
 
 __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
@@ -416,23 +429,25 @@ struct PageWindow {
 struct PgShare {
   float* o;
   float* ml;
-  uint2* ranges;  // [row tiles]: first block and number of them; NULL: blocks / tiles each
-  uint32_t tiles, blocks;
+  uint2* ranges;  // [row tiles]: first block and number of them; NULL: each
+  uint32_t tiles, blocks, each;
+  Div by_each;
 };
 // The row tile of block x, its first block and how many it has: one at least, and the rest by the keys in its
 // requests' caches, so that no block has much more than another.
 struct Share {
   uint32_t tile, first, count;
 };
-__device__ __forceinline__ Share share_of(const KvAttendArgs& a, const PgShare& sp, uint32_t x) {
+__device__ __forceinline__ Share share_of(const PgAttendArgs& pa, const PgShare& sp, uint32_t x) {
   if (!sp.ranges) {
-    const uint32_t count = sp.blocks / sp.tiles;
-    return {x / count, x / count * count, count};
+    const uint32_t tile = sp.by_each(x);
+    return {tile, tile * sp.each, sp.each};
   }
-  const uint32_t lane = threadIdx.x & 63u, per = a.c.n * a.s.rep;  // (at most 64 row tiles)
+  const KvAttendArgs& a = pa.a;
+  const uint32_t lane = threadIdx.x & 63u;  // (at most 64 row tiles)
   uint32_t keys = 0;
   if (lane < sp.tiles)
-    for (uint32_t b = lane * 16 / per; b <= min((lane * 16 + 15) / per, a.c.R - 1); ++b) {
+    for (uint32_t b = pa.by_rows(lane * 16); b <= min(pa.by_rows(lane * 16 + 15), a.c.R - 1); ++b) {
       const int32_t len = a.c.lens[b];
       keys += len > 0 && len <= int32_t(a.c.cap) ? uint32_t(len) / 32 + 1 : 0u;
     }
@@ -468,16 +483,17 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   __shared__ float ml[STEP_WAVES][16][2];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
-  const uint32_t g = blockIdx.x % a.s.G, block = blockIdx.x / a.s.G;
-  const Share share = share_of(a, sp, block);
+  const uint32_t block = pa.by_groups(blockIdx.x), g = blockIdx.x - block * a.s.G;
+  const Share share = share_of(pa, sp, block);
   const uint32_t tile = share.tile, split = block - share.first;
   const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
-  const RawRequest raw = load_request(a.c, min(tile * 16 / per + lane, a.c.R - 1));
-  const Pages64 early = load_pages(pa, tile * 16 / per);
-  const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const RawRequest raw = load_request(a.c, min(pa.by_rows(tile * 16) + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, pa.by_rows(tile * 16));
+  const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = pa.by_rows(row), t_row = pa.by_rep(row - b_row * per);
+  const uint32_t h_row = g * a.s.rep + row - (b_row * a.c.n + t_row) * a.s.rep;
   const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
   float4 qx[HD / 16];  // dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
 #pragma unroll
@@ -491,8 +507,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   uint32_t seg = 0;
   const uint32_t lead = uint32_t(__ffsll((unsigned long long)__ballot(run.seg_keys != 0))) - 1;  // (with the others' pages in common)
   PageWindow window;
-  if (n_com == 0)
-    while (seg < 63 && o_lo >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+  if (n_com == 0) seg = owner(run, o_lo);
   window.begin(early, b_lo, b_lo + (n_com ? lead : seg));
   using Tile = PgTile<TWO>;
   auto turn_page = [&](Tile& w) {
@@ -518,7 +533,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
       w.seg_keys = run.common;
     } else {
       const uint32_t x = o_lo + (i - n_com);
-      while (x >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+      seg = owner(run, x);
       const uint32_t begin = seg ? lane_read_u32(run.seg_end, int(seg) - 1) : 0u;
       w.seg = int(seg);
       w.req = b_lo + seg;
@@ -800,7 +815,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   const size_t part = (size_t(g) * sp.blocks + block) * 16 + jr;
   const bool last = sp.blocks == sp.tiles;
   if (sp.ranges && g == 0 && split == 0 && tid == 0) sp.ranges[tile] = make_uint2(share.first, share.count);
-  const uint32_t ob = out_row / per, ot = out_row / a.s.rep % a.c.n, oh = g * a.s.rep + out_row % a.s.rep;
+  const uint32_t ob = pa.by_rows(out_row), ot = pa.by_rep(out_row - ob * per), oh = g * a.s.rep + out_row - (ob * a.c.n + ot) * a.s.rep;
   const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
   if (last && !out_live) return;
   float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
@@ -840,17 +855,17 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   __shared__ uint32_t gone_tile[3], odd_tile[3][GR];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5, r16 = lane & 15u, q4 = lane >> 4;
-  const uint32_t g = blockIdx.x % a.s.G, rest = blockIdx.x / a.s.G;
+  const uint32_t rest = pa.by_groups(blockIdx.x), g = blockIdx.x - rest * a.s.G;
   const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
   const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
-  const uint32_t splits = sp.blocks / sp.tiles, per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const uint32_t splits = sp.each, per = a.c.n * a.s.rep, rows = a.c.R * per;
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
-  const RawRequest raw = load_request(a.c, min(tile * TILE_ROWS / per + lane, a.c.R - 1));
-  const Pages64 early = load_pages(pa, tile * TILE_ROWS / per);
+  const RawRequest raw = load_request(a.c, min(pa.by_rows(tile * TILE_ROWS) + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, pa.by_rows(tile * TILE_ROWS));
   const uint32_t my_row = tile * TILE_ROWS + wave * 32 + r32, row = min(my_row, rows - 1);
-  const uint32_t b_row = row / per, t_row = row / a.s.rep % a.c.n, h_row = g * a.s.rep + row % a.s.rep;
+  const uint32_t b_row = pa.by_rows(row), t_row = pa.by_rep(row - b_row * per), h_row = g * a.s.rep + row - (b_row * a.c.n + t_row) * a.s.rep;
   const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
   float4 qx[DS][2];  // dims 16 ks + 8 h2 ..
 #pragma unroll
@@ -866,8 +881,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   uint32_t seg = 0;
   const uint32_t lead = uint32_t(__ffsll((unsigned long long)has)) - 1;  // (with the others' pages in common)
   PageWindow window;
-  if (n_com == 0)
-    while (seg < 63 && o_lo >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+  if (n_com == 0) seg = owner(run, o_lo);
   window.begin(early, run.b_lo, run.b_lo + (n_com ? lead : seg));
   // a tile, and where the wave's 16 keys of it are
   struct Tile {
@@ -887,7 +901,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       w.keys = KT;
     } else {
       const uint32_t x = o_lo + (i - n_com);
-      while (x >= lane_read_u32(run.seg_end, int(seg))) ++seg;
+      seg = owner(run, x);
       const uint32_t begin = seg ? lane_read_u32(run.seg_end, int(seg) - 1) : 0u;
       w.seg = int(seg);
       req = run.b_lo + seg;
@@ -1206,8 +1220,8 @@ __global__ __launch_bounds__(256) void pg_join_kernel(KvAttendArgs a, PgShare sp
   const bool is_row = at < a.c.R * a.c.n * a.s.H;
   const uint32_t out = is_row ? at : 0u, bt = out / a.s.H, h = out % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
   const RawRequest raw = load_request(a.c, b);
-  const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16, even = sp.blocks / sp.tiles;
-  const uint2 range = sp.ranges ? sp.ranges[tile] : make_uint2(tile * even, even);
+  const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
+  const uint2 range = sp.ranges ? sp.ranges[tile] : make_uint2(tile * sp.each, sp.each);
   const size_t part = (size_t(g) * sp.blocks + range.x) * 16 + row % 16;
   float M = -INFINITY, L = 0.0f;
   floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -1636,8 +1650,11 @@ hipError_t launch_pg_append(uint32_t hd, const PgAppendArgs& a, hipStream_t s) {
   });
 }
 
-hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspace& w, hipStream_t s) {
+hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, hipStream_t s) {
   const KvAttendArgs& a = pa.a;
+  pa.by_rows = Div::by(a.c.n * a.s.rep);
+  pa.by_rep = Div::by(a.s.rep);
+  pa.by_groups = Div::by(a.s.G);
   PgShare sp{};
   sp.o = w.part;
   sp.ml = w.part_ml;
@@ -1657,6 +1674,8 @@ hipError_t launch_pg_attend(uint32_t hd, const PgAttendArgs& pa, const PgWorkspa
   if (!many && most <= 24u * 128 / hd) splits = 1;
   if (size_t(a.s.G) * sp.tiles * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   sp.blocks = sp.tiles * splits;
+  sp.each = splits;
+  sp.by_each = Div::by(splits);
   // Shares by length where runs are long (1 of 16 over 32001, the others over 500: 30 us, equal shares 39): they take up to a
   // microsecond to work out.
   if (!many && splits > 1 && walk >= 6 && sp.tiles > 1 && sp.tiles <= 64) sp.ranges = w.ranges;
