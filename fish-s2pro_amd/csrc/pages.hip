@@ -1312,6 +1312,61 @@ __device__ __forceinline__ uint32_t settled(const uint32_t& bad) {
   return x;
 }
 
+// Neighbouring counts of a pool's pages (4-byte addresses will do).
+template <int N>
+struct Counts {
+  int32_t of[N];
+};
+template <int N>
+__device__ __forceinline__ Counts<N> load_counts(const int32_t* from) {
+  Counts<N> x;
+  __builtin_memcpy(&x, from, sizeof x);
+  return x;
+}
+template <int N>
+__device__ __forceinline__ void store_counts(int32_t* to, Counts<N> x) {
+  __builtin_memcpy(to, &x, sizeof x);
+}
+// f(p, counts from p on) for all pages, by the block's threads: of many pages four at a time, two such loads together.  (One
+// block, so what is in flight is what there is of bandwidth; a turn that a small pool does not need is a jump.)
+template <class F>
+__device__ __forceinline__ void each_page(const int32_t* refs, uint32_t pages, F&& f) {
+  constexpr uint32_t T = ROWS_THREADS;
+  const uint32_t tid = threadIdx.x;
+  uint32_t p0 = 0;
+  for (; p0 + 8 * T <= pages; p0 += 8 * T) {
+    const uint32_t p = p0 + 4 * tid;
+    const Counts<4> x = load_counts<4>(refs + p), y = load_counts<4>(refs + p + 4 * T);
+    f(p, x);
+    f(p + 4 * T, y);
+  }
+  for (; p0 < pages; p0 += T)
+    if (p0 + tid < pages) f(p0 + tid, load_counts<1>(refs + p0 + tid));
+}
+// f(p, count) where order counts: each wave has a run of pages, 64 at a time, and all its lanes take part (`rest` behind the pages).
+template <class F>
+__device__ __forceinline__ void by_waves(const int32_t* refs, uint32_t pages, int32_t rest, F&& f) {
+  constexpr uint32_t WAVES = ROWS_THREADS / 64;
+  const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), per = ((pages + WAVES - 1) / WAVES + 63) / 64 * 64;
+  const uint32_t lo = min(wave * per, pages), hi = min(lo + per, pages);
+  uint32_t p0 = lo;
+  for (; p0 + 256 <= hi; p0 += 256) {
+    int32_t x[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) x[k] = refs[p0 + 64 * k + lane];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) f(p0 + 64 * k + lane, x[k]);
+  }
+  for (; p0 < hi; p0 += 64) f(p0 + lane, p0 + lane < hi ? refs[p0 + lane] : rest);
+}
+__device__ __forceinline__ uint32_t lanes_below(uint64_t of) {
+  return __builtin_amdgcn_mbcnt_hi(uint32_t(of >> 32), __builtin_amdgcn_mbcnt_lo(uint32_t(of), 0));
+}
+// The block's sum of what its waves have, each the same in all lanes, and that of the waves before.
+__device__ __forceinline__ uint32_t wave_offsets(uint32_t x, uint32_t& all) {
+  return uniform(block_scan((threadIdx.x & 63u) == 0 ? x : 0u, all));
+}
+
 // Nothing changes: arrays out become as those in.
 __device__ __forceinline__ void copy_rows(const PgUpdateArgs& a) {
   const uint32_t tid = threadIdx.x;
@@ -1394,7 +1449,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     if (!MOVES) w.moves[2 * tid] = -1;
     if (lens[tid] < 0 || lens[tid] > cap || source[tid] < -1 || source[tid] >= int32_t(a.R) || keep < 0 || add < 0) report(S2HIP_PAGES_ERR_LENS);
   }
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) *refs(p) = a.refs[p];
+  each_page(a.refs, a.p.pages, [&](uint32_t p, auto x) { store_counts(refs(p), x); });
   auto turn_over = [&] {
     if constexpr (FITS)
       __syncthreads();
@@ -1467,17 +1522,23 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
   uint32_t all, found;
   const uint32_t begin = block_scan(needs, all);
   if (tid < a.R) offset[tid] = begin;
-  // the free pages: each thread counts those of a run of pages, then says which they are
-  const uint32_t run = (a.p.pages + ROWS_THREADS - 1) / ROWS_THREADS, p_lo = min(tid * run, a.p.pages), p_hi = min(p_lo + run, a.p.pages);
+  // the free pages: each wave counts those of a run of pages, then says which they are
+  if constexpr (!FITS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (plain loads of what atomics have changed)
   uint32_t mine = 0;
-  for (uint32_t p = p_lo; p < p_hi; ++p) {
-    const int32_t r = count(p);
-    mine += r == 0;
-    if (r < 0) report(S2HIP_PAGES_ERR_REFS);
-  }
-  uint32_t rank = block_scan(mine, found);
-  for (uint32_t p = p_lo; p < p_hi && mine && rank < all; ++p)
-    if (count(p) == 0) *list(rank++) = int32_t(p);
+  bool below = false;
+  by_waves(refs(0), a.p.pages, 1, [&](uint32_t, int32_t r) {
+    mine += uint32_t(__popcll(__ballot(r == 0)));
+    below |= r < 0;
+  });
+  if (below) report(S2HIP_PAGES_ERR_REFS);
+  uint32_t rank = wave_offsets(mine, found);
+  if (mine && rank < all)
+    by_waves(refs(0), a.p.pages, 1, [&](uint32_t p, int32_t r) {
+      const uint64_t free = __ballot(r == 0);
+      const uint32_t to = rank + lanes_below(free);
+      if (r == 0 && to < all) *list(to) = int32_t(p);
+      rank += uint32_t(__popcll(free));
+    });
   if (found < all && tid == 0) report(S2HIP_PAGES_ERR_FULL);
   if (stops()) return;
   if constexpr (MOVES) {
@@ -1508,7 +1569,8 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     for (uint32_t i = lane; i < width; i += 64) a.table_out[size_t(b) * width + i] = i < from ? *rows(b * width + i) : i < n ? *list(at + i - from) : -1;
   }
   turn_over();
-  for (uint32_t p = tid; p < a.p.pages; p += ROWS_THREADS) a.refs_out[p] = count(p);
+  if constexpr (!FITS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  each_page(refs(0), a.p.pages, [&](uint32_t p, auto x) { store_counts(a.refs_out + p, x); });
 }
 
 // blockIdx.y = row, z = layer
@@ -1532,21 +1594,22 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, P
   auto pages_of = [&](int32_t n) { return (uint32_t(n) + page_up) >> a.p.shift; };
   if (tid == 0) bad = 0;
   __syncthreads();
-  // each thread looks at a run of pages
-  const uint32_t run = (pages + ROWS_THREADS - 1) / ROWS_THREADS, p_lo = min(tid * run, pages), p_hi = min(p_lo + run, pages);
+  // each wave looks at a run of pages
+  const uint32_t lane = tid & 63u;
   uint32_t mine = 0, used;
-  for (uint32_t p = p_lo; p < p_hi; ++p) {
-    const int32_t r = a.refs[p];
-    mine += r > 0;
-    if (r < 0) atomicOr(&bad, S2HIP_PAGES_ERR_REFS);
-  }
+  bool below = false;
+  by_waves(a.refs, pages, 0, [&](uint32_t, int32_t r) {
+    mine += uint32_t(__popcll(__ballot(r > 0)));
+    below |= r < 0;
+  });
+  if (below) atomicOr(&bad, S2HIP_PAGES_ERR_REFS);
   for (uint32_t b = tid >> 6; b < a.R; b += ROWS_THREADS / 64) {
     const int32_t len = a.lens[b];
     if (len < 0 || int64_t(len) > int64_t(width) << a.p.shift) {
       atomicOr(&bad, S2HIP_PAGES_ERR_LENS);
       continue;
     }
-    for (uint32_t i = tid & 63u; i < pages_of(len); i += 64) {
+    for (uint32_t i = lane; i < pages_of(len); i += 64) {
       const int32_t e = a.p.table[size_t(b) * width + i];
       if (uint32_t(e) >= pages)
         atomicOr(&bad, S2HIP_PAGES_ERR_PAGE);
@@ -1554,7 +1617,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, P
         atomicOr(&bad, S2HIP_PAGES_ERR_REFS);
     }
   }
-  block_scan(mine, used);
+  wave_offsets(mine, used);
   const uint32_t why = settled(bad);
   if (writes && tid == 0) a.used_out[0] = int32_t(used);
   if (why) {
@@ -1573,25 +1636,33 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_pack_kernel(PgUpdateArgs a, P
     return;
   }
   uint32_t here[2] = {0, 0}, n_holes, n_movers;
-  for (uint32_t p = p_lo; p < p_hi; ++p) {
-    const int32_t r = a.refs[p];
-    here[0] += p < used && r == 0;
-    here[1] += p >= used && r > 0;
-  }
-  uint32_t h = block_scan(here[0], n_holes), m = block_scan(here[1], n_movers);  // (as many of one as of the other)
-  for (uint32_t p = p_lo; p < p_hi; ++p) {
-    const int32_t r = a.refs[p];
-    if (p < used && r == 0) holes[h++] = int32_t(p);
-    if (p >= used && r > 0) movers[m++] = int32_t(p);
-  }
+  by_waves(a.refs, pages, -1, [&](uint32_t p, int32_t r) {
+    here[0] += uint32_t(__popcll(__ballot(p < used && r == 0)));
+    here[1] += uint32_t(__popcll(__ballot(p >= used && r > 0)));
+  });
+  uint32_t h = wave_offsets(here[0], n_holes), m = wave_offsets(here[1], n_movers);  // (as many of one as of the other)
+  if (here[0] || here[1])
+    by_waves(a.refs, pages, -1, [&](uint32_t p, int32_t r) {
+      const bool hole = p < used && r == 0, mover = p >= used && r > 0;
+      const uint64_t hs = __ballot(hole), ms = __ballot(mover);
+      if (hole) holes[h + lanes_below(hs)] = int32_t(p);
+      if (mover) movers[m + lanes_below(ms)] = int32_t(p);
+      h += uint32_t(__popcll(hs));
+      m += uint32_t(__popcll(ms));
+    });
   settled();
   for (uint32_t i = tid; i < n_movers; i += ROWS_THREADS) moved[movers[i]] = holes[i];
-  if (writes)
-    for (uint32_t p = tid; p < pages; p += ROWS_THREADS) {
-      const int32_t r = a.refs[p];
-      if (a.refs_out != a.refs) a.refs_out[p] = p < used ? r : 0;
-      if (a.moved_to) a.moved_to[p] = r > 0 ? int32_t(p) : -1;
-    }
+  if (writes && (a.refs_out != a.refs || a.moved_to))
+    each_page(a.refs, pages, [&](uint32_t p, auto x) {
+      auto out = x, to = x;
+#pragma unroll
+      for (uint32_t i = 0; i < sizeof x / 4; ++i) {
+        out.of[i] = p + i < used ? x.of[i] : 0;
+        to.of[i] = x.of[i] > 0 ? int32_t(p + i) : -1;
+      }
+      if (a.refs_out != a.refs) store_counts(a.refs_out + p, out);
+      if (a.moved_to) store_counts(a.moved_to + p, to);
+    });
   settled();
   if (writes)
     for (uint32_t i = tid; i < n_movers; i += ROWS_THREADS) {
