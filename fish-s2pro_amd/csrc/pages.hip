@@ -43,6 +43,9 @@ __device__ __forceinline__ double dpp_f64(double x) {
 // 64 bits, whose instructions cost what those of 32 bits do here: a rounding of f32 in
 // front would move a code across a border now and then, and the element by a sixteenth
 // of its block's range.
+//   Memory bounds a turn: 8 x 250 tokens of 32 + 2 x 8 heads of 128, 78 MB, 20.4 us (3.9
+// TB/s), vector units 28 % busy.  A step's token is split over blocks by runs of heads
+// (up to 512 blocks; 8 x 1 tokens in 3.9 us, all of it latency).
 template <int HD, bool HALF>
 __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
   constexpr uint32_t LP = HD / 8;     // lanes per head
@@ -305,6 +308,11 @@ __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
 // key, 8 dims of each 32), values as the second's (lane % 16 = pair of dims, 4 tokens
 // of each 16, as the weights stand in the registers): both go from memory to operands
 // with no exchange.
+//   Vector instructions bound it: 4 bits become f16 numbers, and a weight two of them, at one
+// issue of four units (16 x 1 over 32001 slots: 105 us for 450 MB, 4.3 TB/s, vector units 60 %
+// busy, matrix units 19 %; its loads alone take 97).  Short runs are latency: of 10 us of 8 x 1
+// over 1500 + 512, 2.5 go before the first load of a page (lengths, tables, queries), 1 in it, 1 to
+// a tile (a wave alone on its unit issues every fifth cycle), 1 at the end, and 3.5 in the join.
 //   The run: first the tiles that all requests of the rows have in common (the same
 // pages at the head of their rows of the table, seen by all), read once for all; then
 // each request's own.  Page numbers stand one per lane, 64 at a time.
@@ -432,6 +440,7 @@ struct PgShare {
   uint2* ranges;  // [row tiles]: first block and number of them; NULL: each
   uint32_t tiles, blocks, each;
   Div by_each;
+  uint32_t row_tiles, of_request;  // pg_tile_kernel: row tiles of 128 in all; of a request, where none has rows of two (0: they may)
 };
 // The row tile of block x, its first block and how many it has: one at least, and the rest by the keys in its
 // requests' caches, so that no block has much more than another.
@@ -834,11 +843,14 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   }
 }
 
-// Many rows (turns, prompts).  A block of four waves owns 128 packed rows of a kv
+// Many rows (turns, prompts).  A block of four waves owns up to 128 packed rows of a kv
 // head, 32 per wave, and walks the run of tiles of 64 keys.  Each wave takes 16 of a
 // tile's keys and values from 4 bits to f16, once for the block, and leaves them in
 // LDS, the next tile's while this one's products run; codes are loaded another tile
 // ahead.
+//   Its products bound it (two for a term: hi and lo): a prompt of 3999 takes 254 us, the products
+// alone, at the rate that the card's power allows, 226; matrix units 48 % busy by cycles, vector units 42.
+// Of 8 x 250 tokens over 1500 + 250 (97 us) 380 blocks have rows: a second one on half of the CUs.
 //   v_mfma_f32_32x32x16_f16, S^T = K Q^T and O^T += V^T P^T, a lane holds one row
 // (lane % 32).  Values stand transposed, a row of 64 tokens per dim, each 16 bytes the
 // 8 tokens that a lane's 8 weights belong to.
@@ -856,15 +868,16 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5, r16 = lane & 15u, q4 = lane >> 4;
   const uint32_t rest = pa.by_groups(blockIdx.x), g = blockIdx.x - rest * a.s.G;
-  const uint32_t blocks = (a.c.R * a.c.n * a.s.rep + TILE_ROWS - 1) / TILE_ROWS;
-  const uint32_t tile = blocks - 1 - rest % blocks, split = rest / blocks;  // later rows see more keys: they go first
-  const uint32_t splits = sp.each, per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const uint32_t split = rest / sp.row_tiles, tile = sp.row_tiles - 1 - (rest - split * sp.row_tiles);  // later rows see more keys: they go first
+  const uint32_t splits = sp.each, per = a.c.n * a.s.rep, whose = sp.of_request ? tile / sp.of_request : 0u;
+  const uint32_t row0 = sp.of_request ? whose * per + (tile - whose * sp.of_request) * TILE_ROWS : tile * TILE_ROWS;
+  const uint32_t rows = sp.of_request ? (whose + 1) * per : a.c.R * per, n_rows = min(uint32_t(TILE_ROWS), rows - row0);
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
-  const RawRequest raw = load_request(a.c, min(pa.by_rows(tile * TILE_ROWS) + lane, a.c.R - 1));
-  const Pages64 early = load_pages(pa, pa.by_rows(tile * TILE_ROWS));
-  const uint32_t my_row = tile * TILE_ROWS + wave * 32 + r32, row = min(my_row, rows - 1);
+  const RawRequest raw = load_request(a.c, min(pa.by_rows(row0) + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, pa.by_rows(row0));
+  const uint32_t my_row = row0 + wave * 32 + r32, row = min(my_row, rows - 1);
   const uint32_t b_row = pa.by_rows(row), t_row = pa.by_rep(row - b_row * per), h_row = g * a.s.rep + row - (b_row * a.c.n + t_row) * a.s.rep;
   const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
   float4 qx[DS][2];  // dims 16 ks + 8 h2 ..
@@ -872,7 +885,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
     for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
-  const PgRun run = pg_run<KT>(pa, tile * TILE_ROWS, TILE_ROWS, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  const PgRun run = pg_run<KT>(pa, row0, n_rows, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint64_t has = __ballot(run.seg_keys != 0);
   if (!has) return;  // no row of a token
   const uint32_t c_all = run.common / KT, c_lo = c_all * split / splits, n_com = c_all * (split + 1) / splits - c_lo;
@@ -1405,11 +1418,13 @@ __device__ __forceinline__ void copy_pages(const PgUpdateArgs& a, const int32_t*
 // One block, a wave per row at a time.  References are counted apart: what rows let go of is taken off, what they take
 // added; the rest of a row that stays its own counts as it is.  Of w rows that write to a page of r references, the
 // first r - 1 write to copies: the last writes in place if no one else holds it.
-//   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores.  FITS:
-// counts, free pages and new rows are in LDS (64 rows of 104 pages: 21 us -> 7 against the workspace, where each turn is
-// a trip to the second-level cache); else in the workspace.
+//   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores; sixteen
+// waves share four vector units, so each instruction of a turn counts (64 rows of 102 pages 13 us, 16 of 32 pages 8, of a
+// pool of 7000).  FITS: counts, free pages and new rows are in LDS; else in the workspace, where each turn is a trip to the
+// second-level cache (64 rows of 102 pages of a pool of 15800, which fits, 14.5 us; of 15900, which does not, 21).
 //   MOVES (arrays out apart from those in): every block works it all out for itself, the first writes it down, and all of
-// them copy pages: one launch, where the caller's own time per launch is what small calls take.
+// them copy pages: one launch (16 rows 8.5 us; in place, with a second launch that copies, 9.3, and the caller's own 2.7 for
+// it).  64 rows that each copy a page in 36 layers: 31 us, 122 MB in 18 of them.
 constexpr uint32_t ROWS_LDS = 150 * 1024;  // bytes: counts, free pages, rows
 
 template <bool FITS, bool MOVES>
@@ -1579,7 +1594,8 @@ __global__ __launch_bounds__(256) void pg_copy_kernel(PgUpdateArgs a, const int3
   if (from >= 0) copy_page(a, blockIdx.z, from, moves[2 * blockIdx.y + 1], bytes, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
-// The pages in use, the lists of holes and movers, refs.  MOVES (arrays out apart from those in, and few enough pages):
+// The pages in use, the lists of holes and movers, refs.  A short call is three trips over refs (1 layer of a few hundred
+// pages 6 us), a long one memory (36 layers, 12 x 3500 tokens, half of the pages moved: 270 to 280 us, 1.36 GB: 4.9 TB/s).  MOVES (arrays out apart from those in, and few enough pages):
 // every block works them out in its LDS, and all of them move pages and rewrite the table; else one block leaves the
 // lists in the workspace.
 template <bool MOVES>
@@ -1731,9 +1747,19 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   sp.ml = w.part_ml;
   const uint32_t rows = a.c.R * a.c.n * a.s.rep;
   sp.tiles = (rows + 15) / 16;
+  const uint32_t per = a.c.n * a.s.rep, of_request = (per + TILE_ROWS - 1) / TILE_ROWS;
+  // The tile kernel takes half as long for a score but 10 us more (128 rows' states), and where a request has few rows it
+  // does several requests' keys for all of them.  Step : tile kernel, us, heads 32 over 8 of 128: 1 x 1000 tokens over 1000
+  // (16 M scores) 50 : 55, 1 x 1200 over 1200 (23) 67 : 56, 2 x 100 over 4000 (25) 58 : 50, 8 x 40 over 2000 (20) 43 : 48; of
+  // 32 rows 8 x 8 over 6000 shared + 500 (13) 40 : 42, over 20000 + 500 (42) 86 : 64, over 16000 of their own (33) 64 : 99.
   const size_t scores = size_t(a.s.G) * rows * (a.c.cap - min(a.c.n, a.c.cap) / 2);
-  const bool many = a.c.n * a.s.rep >= 32 && scores * hd > 10000000u * size_t(128);
-  const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? (rows + TILE_ROWS - 1) / TILE_ROWS : sp.tiles);
+  const bool many = per >= 32 && scores / 64 * min(per, 64u) > 18000000u * size_t(128) / hd;
+  // A row tile with rows of two requests walks both's keys, twice as long as its neighbours; tiles of one request each have
+  // up to a third of their rows empty.  Tiles of two : of one, us: 8 x 500 over 4000 467 : 329, 8 x 100 (400 rows) over 4000
+  // 188 : 112, over 1500 shared + 500 79 : 70; 8 x 40 (160 rows, 96 of 256 empty) over 3500 + 500 60 : 69.
+  if (many && of_request * TILE_ROWS <= per + per / 3) sp.of_request = of_request;
+  sp.row_tiles = sp.of_request ? a.c.R * of_request : (rows + TILE_ROWS - 1) / TILE_ROWS;
+  const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? sp.row_tiles : sp.tiles);
   const uint32_t most = (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));  // key tiles of a row tile, at most
   // Blocks of the step kernel, by the key tiles that a wave of 256 would walk at most: short runs end sooner with fewer
   // states to join, long ones want more waves to take turns.  256 : 512 : 768 blocks, us: 8 x 1 over 1500 + 512 (4 tiles) 13 :
@@ -1742,7 +1768,9 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   const size_t walk = size_t(lots) * most / 1024;
   const uint32_t fill = many || (walk >= 6 && walk < 24) ? 512 : walk < 6 ? 256 : 768;
   uint32_t splits = max(1u, min(fill / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
-  if (!many && most <= 24u * 128 / hd) splits = 1;
+  // One block, and no join, for short runs (in a graph, one : several, us: 1 x 1, table of 14 tiles 8.9 : 9.1, of 18 10.1 : 9.2;
+  // heads of 64, 18 8.3 : 8.4, 26 10.1 : 8.4).
+  if (!many && most <= (hd == 64 ? 24u : 16u)) splits = 1;
   if (size_t(a.s.G) * sp.tiles * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
   sp.blocks = sp.tiles * splits;
   sp.each = splits;
@@ -1757,6 +1785,7 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
       hipLaunchKernelGGL((pg_step_kernel<HD(), true>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
     else
       hipLaunchKernelGGL((pg_step_kernel<HD(), false>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+    // (several teams a row : one, us: 8 x 1 over 2000 16.7 : 18.6, 16 x 1 over 8000 40.3 : 44.7, 64 x 1 over 2000 43.0 : 42.6)
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     if (splits > 1 && out_rows <= 2048)
       hipLaunchKernelGGL((pg_join_kernel<HD(), 1024 / HD()>), dim3(out_rows), dim3(256), 0, s, a, sp);

@@ -165,7 +165,7 @@ def test_attend_rows_all_the_same(page):
 
 
 # Rows of the table as long as the lengths need, and so long that a call counts as much work (it is launched by them)
-ROOM = [None, 32768]
+ROOM = [None, 32768, 131072]
 
 
 @pytest.mark.parametrize("room", ROOM)
@@ -187,12 +187,23 @@ def test_attend_turns(shape, requests, n, length, shared, room):
     Pool(shape, 64, [length + x for x in new], new, shared=shared, seed=n, width=room and room // 64).check_all()
 
 
+@pytest.mark.parametrize("room", ROOM[1:])
 @pytest.mark.parametrize("page", [16, 32, 128])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("extra", [0, 1, 14, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 127, 128, 129])
-def test_attend_turn_borders(extra, hd, page):
+def test_attend_turn_borders(extra, hd, page, room):
     """Turns that begin and end around the borders of tiles and pages."""
-    Pool((8, 2, hd), page, [32 + extra, 64 + extra, 33], [32, 9, 33], seed=extra, width=32768 // page).check_all()
+    Pool((8, 2, hd), page, [32 + extra, 64 + extra, 33], [32, 9, 33], seed=extra, width=room // page).check_all()
+
+
+@pytest.mark.parametrize("shared", [0, 5])
+@pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65, 95, 96, 97])
+def test_attend_row_tiles(n, shared):
+    """Tiles of 128 rows: of one request each, or of several, by how many rows a request has; idle ones among them."""
+    new = [n, 1, 0, n, n - 1, n // 2, n]
+    Pool((8, 2, 64), 32, [shared * 32 + x + 10 * i if x else 0 for i, x in enumerate(new)], new, shared=shared, seed=n, width=4096).check_all()
+    new = [n // 2, n // 2, 0, 1, n // 4, n // 2, n // 2, n // 2, n // 2]
+    Pool((4, 2, 128), 64, [shared * 64 + x + 10 * i if x else 0 for i, x in enumerate(new)], new, shared=shared, seed=n, width=4096).check_all()
 
 
 def test_attend_many_requests():
@@ -230,7 +241,7 @@ def test_attend_without_new_lens():
     assert p.ops.errors(stream()) == 0
 
 
-@pytest.mark.parametrize("room", [None, 1000])
+@pytest.mark.parametrize("room", [None, 1000, 4000])
 @pytest.mark.parametrize("n", [1, 3, 40])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attend_never_sees_the_rest(n, hd, room):
