@@ -389,6 +389,21 @@ def test_attend_offsets_beyond_32_bits():
     assert ops.errors(stream()) == 0
 
 
+def test_attend_most_tokens():
+    """The most tokens of a call, 4 M packed rows; a few of them against 64 bits."""
+    n, page, hd = 32768, 128, 64
+    lens = [n + 5, n + 1]
+    p = Pool((64, 1, hd), page, lens, [n, n], seed=12)
+    p.attend()
+    k, v = p.dense()
+    for b in range(2):
+        for t in (0, 1, 16383, 16384, n - 1):
+            seen = lens[b] - n + t + 1
+            want, tol = kv_util.attend(p.q[b : b + 1, t : t + 1], k[b : b + 1], v[b : b + 1], [seen], [1])[:2]
+            assert bool(((p.out[b : b + 1, t : t + 1].double() - want).abs() <= tol).all()), (b, t)
+    assert p.ops.errors(stream()) == 0 and not bool((p.out == 7.0).all(-1).any())
+
+
 # --------------------------------------------------------------------------
 # append
 # --------------------------------------------------------------------------
@@ -764,6 +779,43 @@ def test_update_what_else_holds_pages(in_place):
     k.update(keep=[0, 17, 0], in_place=in_place)
     assert [p for p, n in enumerate(k.refs) if n] and k.refs[9] == 1
     k.update(add=[64, 0, 0], in_place=in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_largest_pool(in_place):
+    """2^20 pages, many of them held by others: the rows grow into free ones, then the pool is compacted."""
+    pages, page, width, rows = 1 << 20, 16, 40, 3
+    ops = PagedKv(4, 1, 64, page, pages, width, max_requests=rows, max_tokens=64)
+    pool = torch.zeros(pages, ops.page_bytes // 4, dtype=torch.int32, device="cuda")
+    pool[:, 0] = pool[:, -1] = torch.arange(pages, device="cuda")
+    r = np.random.default_rng(3)
+    held = np.where(r.random(pages) < 0.999, r.integers(1, 4, pages), 0)
+    held[-50000:] = 0
+    table, lens, refs = [[-1] * width for _ in range(rows)], [0] * rows, held.tolist()
+    d = [dev(x) for x in (table, lens, refs)]
+    for source, keep, add in (([0, 1, 2], [0, 0, 0], [600, 333, 0]), ([0, 0, 1], [599, 100, 333], [41, 1, 64])):
+        out = d if in_place else [torch.full_like(x, 99) for x in d]
+        args = [dev(x) for x in (source, keep, add)]
+        ops.update(ops.view(ptr(pool), ptr(d[0]), ptr(d[1]), rows), ptr(d[2]), ptr(out[2]), ptr(out[0]), ptr(out[1]), source=ptr(args[0]), keep=ptr(args[1]), add=ptr(args[2]), stream=stream())
+        table, lens, refs, copies = pages_util.update(table, lens, refs, source, keep, add, page, width)
+        d = out
+        assert [x.tolist() for x in d] == [table, lens, refs]
+        for to, at in copies.items():
+            assert pool[to, 0] == at and pool[to, -1] == at
+            pool[to, 0] = pool[to, -1] = to
+    used, moved = dev([-1]), torch.full((pages,), 99, dtype=torch.int32, device="cuda")
+    out = d if in_place else [d[0].clone(), d[1], torch.full_like(d[2], 99)]
+    ops.compact(ops.view(ptr(pool), ptr(d[0]), ptr(d[1]), rows), ptr(d[2]), ptr(out[2]), ptr(out[0]), ptr(used), moved_to=ptr(moved), stream=stream())
+    was = np.array(refs)
+    table, refs, to, n = pages_util.compact(table, lens, refs, page)
+    assert ops.errors(stream()) == 0 and len(to) > 0 and int(used) == n
+    assert out[0].tolist() == table and out[2].tolist() == refs
+    want = np.where(was > 0, np.arange(pages), -1)
+    want[list(to)] = list(to.values())
+    assert np.array_equal(moved.cpu().numpy(), want)
+    at = moved[moved >= 0].long()
+    names = torch.arange(pages, device="cuda")[moved >= 0].int()
+    assert torch.equal(pool[at, 0], names) and torch.equal(pool[at, -1], names)
 
 
 def test_layers_apart():
