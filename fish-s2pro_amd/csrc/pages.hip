@@ -299,10 +299,10 @@ __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
   return first;
 }
 
-// Few rows over many keys (decode steps).  A wave owns 16 packed rows of a kv head
-// and a run of tiles of 32 keys; nothing is exchanged between waves before the end,
-// when the block's four join their states in LDS and, with several blocks per 16 rows,
-// leave them for the join kernel.
+// Few rows over many keys (decode steps, short turns).  A wave owns RG groups of 16
+// packed rows of a kv head and a run of tiles of 32 keys; nothing is exchanged between
+// waves before the end, when the block's four join their states in LDS and, with several
+// blocks per row tile, leave them for the join kernel.
 //   S^T = K Q^T and O^T += V^T P^T by v_mfma_f32_16x16x32_f16, so a lane holds one row
 // (lane % 16).  Keys lie in memory as the first product's lanes take them (lane % 16 =
 // key, 8 dims of each 32), values as the second's (lane % 16 = pair of dims, 4 tokens
@@ -433,20 +433,24 @@ struct PageWindow {
   }
 };
 
-// The blocks of a kv head, `blocks` of them, and its states [kv heads][blocks][16 rows].
+// The blocks of a kv head, `blocks` of them, and its states [kv heads][blocks][1 << shift rows] (of the tile kernel, whose
+// splits are the same for all: each 16 rows' as if a block did no more).
 struct PgShare {
   float* o;
   float* ml;
   uint2* ranges;  // [row tiles]: first block and number of them; NULL: each
   uint32_t tiles, blocks, each;
   Div by_each;
-  uint32_t row_tiles, of_request;  // pg_tile_kernel: row tiles of 128 in all; of a request, where none has rows of two (0: they may)
+  uint32_t row_tiles, of_request;  // the kernel's row tiles; those of a request, where none has rows of two (0: they may)
+  Div by_of;
+  uint32_t shift;
 };
 // The row tile of block x, its first block and how many it has: one at least, and the rest by the keys in its
 // requests' caches, so that no block has much more than another.
 struct Share {
   uint32_t tile, first, count;
 };
+template <int ROWS>
 __device__ __forceinline__ Share share_of(const PgAttendArgs& pa, const PgShare& sp, uint32_t x) {
   if (!sp.ranges) {
     const uint32_t tile = sp.by_each(x);
@@ -456,7 +460,7 @@ __device__ __forceinline__ Share share_of(const PgAttendArgs& pa, const PgShare&
   const uint32_t lane = threadIdx.x & 63u;  // (at most 64 row tiles)
   uint32_t keys = 0;
   if (lane < sp.tiles)
-    for (uint32_t b = pa.by_rows(lane * 16); b <= min(pa.by_rows(lane * 16 + 15), a.c.R - 1); ++b) {
+    for (uint32_t b = sp.of_request ? sp.by_of(lane) : pa.by_rows(lane * ROWS), end = sp.of_request ? b : min(pa.by_rows((lane + 1) * ROWS - 1), a.c.R - 1); b <= end; ++b) {
       const int32_t len = a.c.lens[b];
       keys += len > 0 && len <= int32_t(a.c.cap) ? uint32_t(len) / 32 + 1 : 0u;
     }
@@ -478,9 +482,9 @@ struct PgTile {
   uint32_t gone;                 // bit h: half h lies in no page of the pool
 };
 
-template <int HD, bool TWO>
-__global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArgs pa, PgShare sp) {
-  constexpr int KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
+template <int HD, bool TWO, int RG>
+__global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kernel(PgAttendArgs pa, PgShare sp) {
+  constexpr int ROWS = 16 * RG, KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
   constexpr int OP = HD + 4;                          // padded row of the joined states
   constexpr float LIFT = F16_LIFT;
   // A tile: key codes, value codes, key scales, value scales (and what the load of those leaves behind them); a wave's two, and in their place its
@@ -489,25 +493,32 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
   constexpr int LOADS = HD == 128 ? 5 : 3;
   static_assert(16 * OP * 4 <= STAGE, "a state fits");
   __shared__ __align__(16) uint8_t lds[STEP_WAVES * STAGE];
-  __shared__ float ml[STEP_WAVES][16][2];
+  __shared__ float ml[STEP_WAVES][ROWS][2];
   const KvAttendArgs& a = pa.a;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r16 = lane & 15u, q4 = lane >> 4;
   const uint32_t block = pa.by_groups(blockIdx.x), g = blockIdx.x - block * a.s.G;
-  const Share share = share_of(pa, sp, block);
+  const Share share = share_of<ROWS>(pa, sp, block);
   const uint32_t tile = share.tile, split = block - share.first;
-  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
+  const uint32_t per = a.c.n * a.s.rep, whose = sp.by_of(tile), row0 = sp.of_request ? whose * per + (tile - whose * sp.of_request) * ROWS : tile * ROWS;
+  const uint32_t n_rows = min(uint32_t(ROWS), (sp.of_request ? whose + 1 : a.c.R) * per - row0);
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
-  const RawRequest raw = load_request(a.c, min(pa.by_rows(tile * 16) + lane, a.c.R - 1));
-  const Pages64 early = load_pages(pa, pa.by_rows(tile * 16));
-  const uint32_t row = min(tile * 16 + r16, rows - 1), b_row = pa.by_rows(row), t_row = pa.by_rep(row - b_row * per);
-  const uint32_t h_row = g * a.s.rep + row - (b_row * a.c.n + t_row) * a.s.rep;
-  const size_t q_at = ((size_t(b_row) * a.c.n + t_row) * a.s.H + h_row) * HD;
-  float4 qx[HD / 16];  // dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
+  const RawRequest raw = load_request(a.c, min(pa.by_rows(row0) + lane, a.c.R - 1));
+  const Pages64 early = load_pages(pa, pa.by_rows(row0));
+  uint32_t b_row[RG], t_row[RG];
+  float4 qx[RG][HD / 16];  // dims 32 (j / 2) + 8 q4 + 4 (j % 2) ..
 #pragma unroll
-  for (int j = 0; j < HD / 16; ++j) qx[j] = *reinterpret_cast<const float4*>(a.q + q_at + 32 * (j / 2) + 8 * q4 + 4 * (j % 2));
-  const PgRun run = pg_run<KT>(pa, tile * 16, 16, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
+  for (int r = 0; r < RG; ++r) {
+    const uint32_t row = row0 + min(16 * r + r16, n_rows - 1);
+    b_row[r] = pa.by_rows(row);
+    t_row[r] = pa.by_rep(row - b_row[r] * per);
+    const uint32_t h_row = g * a.s.rep + row - (b_row[r] * a.c.n + t_row[r]) * a.s.rep;
+    const size_t q_at = ((size_t(b_row[r]) * a.c.n + t_row[r]) * a.s.H + h_row) * HD;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) qx[r][j] = *reinterpret_cast<const float4*>(a.q + q_at + 32 * (j / 2) + 8 * q4 + 4 * (j % 2));
+  }
+  const PgRun run = pg_run<KT>(pa, row0, n_rows, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
   const uint32_t b_lo = run.b_lo, lots = share.count * STEP_WAVES, lot = split * STEP_WAVES + wave;
   const uint32_t c_tiles = run.common / KT, c_lo = c_tiles * lot / lots, n_com = c_tiles * (lot + 1) / lots - c_lo;
   // (the own tiles the other way round: the waves with one more in common get one fewer)
@@ -636,41 +647,50 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
     fetch(next, 1);
   }
 
-  // this lane's row
-  const uint32_t len_row = __shfl(run.rq.len, int(b_row - b_lo) & 15, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - b_lo) & 15, 64);
-  const bool live = tile * 16 + r16 < rows && t_row < fresh_row;
-  // (a row of no token may see anything: nobody reads it)
-  const int own_limit = live ? int(len_row - fresh_row + t_row) : 0x7fffffff, own_seg = live ? int(b_row - b_lo) : -2;
-  half8 qh[GR], ql[GR];  // dims 32 j + 8 q4 + e
-  float unscale = 1.0f;
-  {
+  // this lane's rows
+  int own_limit[RG], own_seg[RG];
+  half8 qh[RG][GR], ql[RG][GR];  // dims 32 j + 8 q4 + e
+  float unscale[RG];
+#pragma unroll
+  for (int r = 0; r < RG; ++r) {
+    const int mine = int(b_row[r] - b_lo);
+    const uint32_t len_row = __shfl(run.rq.len, mine & 15, 64), fresh_row = __shfl(run.rq.fresh, mine & 15, 64);
+    const bool live = 16 * r + r16 < n_rows && t_row[r] < fresh_row;
+    // (a row of no token may see anything: nobody reads it)
+    own_limit[r] = live ? int(len_row - fresh_row + t_row[r]) : 0x7fffffff;
+    own_seg[r] = live ? mine : -2;
     const float s2 = live ? a.s.scale2 : 0.0f;
     float x[HD / 16][4], big = 0.0f;
 #pragma unroll
     for (int j = 0; j < HD / 16; ++j) {
-      x[j][0] = live ? qx[j].x * s2 : 0.0f;  // (a query of no token may hold anything)
-      x[j][1] = live ? qx[j].y * s2 : 0.0f;
-      x[j][2] = live ? qx[j].z * s2 : 0.0f;
-      x[j][3] = live ? qx[j].w * s2 : 0.0f;
+      x[j][0] = live ? qx[r][j].x * s2 : 0.0f;  // (a query of no token may hold anything)
+      x[j][1] = live ? qx[r][j].y * s2 : 0.0f;
+      x[j][2] = live ? qx[r][j].z * s2 : 0.0f;
+      x[j][3] = live ? qx[r][j].w * s2 : 0.0f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) big = fmaxf(big, fabsf(x[j][e]));
     }
     float inv;
-    pow2_scale(quarter_max(big), unscale, inv);
+    pow2_scale(quarter_max(big), unscale[r], inv);
 #pragma unroll
     for (int j = 0; j < GR; ++j)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const Parts y = split_query<false>(x[2 * j + e / 4][e % 4] * inv);
-        qh[j][e] = y.hi;
-        ql[j][e] = y.lo;
+        qh[r][j][e] = y.hi;
+        ql[r][j][e] = y.lo;
       }
   }
 
-  floatx4 o[OT];  // o[2 c + h][i]: dim 32 c + 8 q4 + 2 i + h
+  floatx4 o[RG][OT];  // o[][2 c + h][i]: dim 32 c + 8 q4 + 2 i + h
+  float m[RG], l[RG];
 #pragma unroll
-  for (int i = 0; i < OT; ++i) o[i] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.0f;
+  for (int r = 0; r < RG; ++r) {
+#pragma unroll
+    for (int i = 0; i < OT; ++i) o[r][i] = floatx4{0.f, 0.f, 0.f, 0.f};
+    m[r] = -INFINITY;
+    l[r] = 0.0f;
+  }
 
   for (uint32_t i = 0; i < n_tiles; ++i) {
     const uint32_t slot = i & 1u;
@@ -678,9 +698,16 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
       asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");  // (all but the next tile's)
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    const bool mine = w.seg < 0 || own_seg == -2 || own_seg == w.seg;
-    const int limit = w.seg < 0 || own_seg == -2 ? 0x7fffffff : mine ? own_limit : -1;
-    const bool all_see = __all(limit >= int(w.key0 + KT - 1)) && !w.gone;  // every row, the whole tile: nothing to keep off
+    bool mine[RG], sees = true, fits = true;
+    int limit[RG];
+#pragma unroll
+    for (int r = 0; r < RG; ++r) {
+      mine[r] = w.seg < 0 || own_seg[r] == -2 || own_seg[r] == w.seg;
+      limit[r] = w.seg < 0 || own_seg[r] == -2 ? 0x7fffffff : mine[r] ? own_limit[r] : -1;
+      sees = sees && limit[r] >= int(w.key0 + KT - 1);
+      fits = fits && (!mine[r] || limit[r] >= int(w.key0 + KT - 1));
+    }
+    const bool all_see = __all(sees) && !w.gone;  // every row, the whole tile: nothing to keep off
     bool masks = false;
     if (!all_see) {
       // A pair of scales per lane: keys' of dims .., values' of tokens 16 h + 4 i + 2 x and the next.
@@ -696,7 +723,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
         *vp = pair;
       }
       // Where the rows of its request see all of it and its keys are numbers, the other rows' weights are 0 by their bias.
-      masks = w.gone || !__all((!mine || limit >= int(w.key0 + KT - 1)) && !odd(*kp));
+      masks = w.gone || !__all(fits && !odd(*kp));
       if (__any(odd(pair))) {  // values of no number: 0 too; outputs of rows that see the first of them are no number
         const uint32_t at_token = (pair & 0x7c00u) == 0x7c00u ? first_token : odd(pair) ? first_token + 1 : 1000u;
         if ((pair & 0x7c00u) == 0x7c00u) pair &= 0xffff0000u;
@@ -705,60 +732,70 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
 #pragma unroll
         for (int c = 0; c < GR; ++c) {
           const uint32_t first = wave_reduce(int(lane / 2 % GR) == c ? at_token : 1000u, [](uint32_t x, uint32_t y) { return min(x, y); });
-          if (first < KT && limit >= int(w.key0 + first)) o[2 * c] = o[2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
+#pragma unroll
+          for (int r = 0; r < RG; ++r)
+            if (first < KT && limit[r] >= int(w.key0 + first)) o[r][2 * c] = o[r][2 * c + 1] = floatx4{NAN, NAN, NAN, NAN};
         }
       }
       asm volatile("" ::: "memory");  // (what is read below in other types is what was written here)
     }
     take_k(slot);
-    floatx4 s[2] = {};
+    floatx4 s[RG][2] = {};
 #pragma unroll
     for (int j = 0; j < GR; ++j) {
       half8 k8[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         k8[h] = key8(bits, kc[h][j], as_half2(ks[h][j / 2])[j % 2]);
-        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], ql[j], s[h], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RG; ++r) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], ql[r][j], s[r][h], 0, 0, 0);
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], qh[j], s[h], 0, 0, 0);
+      for (int r = 0; r < RG; ++r)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[r][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k8[h], qh[r][j], s[r][h], 0, 0, 0);
     }
     if (masks) {
       asm volatile("");
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
-        if (key > limit || ((w.gone >> (c / 4)) & 1u)) s[c / 4][c % 4] = -INFINITY;
+      for (int r = 0; r < RG; ++r)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int key = int(w.key0 + 16u * (c / 4) + 4u * q4 + (c % 4));
+          if (key > limit[r] || ((w.gone >> (c / 4)) & 1u)) s[r][c / 4][c % 4] = -INFINITY;
+        }
+    }
+    half8 ph[RG], pl[RG];  // the lane's four tokens of each half
+#pragma unroll
+    for (int r = 0; r < RG; ++r) {
+      float top = fmaxf(fmaxf(s[r][0][0], s[r][0][1]), s[r][0][2]), top1 = fmaxf(fmaxf(s[r][1][0], s[r][1][1]), s[r][1][2]);
+      top = fmaxf(fmaxf(top, s[r][0][3]), fmaxf(top1, s[r][1][3]));
+      const float mn = mine[r] ? fmaxf(m[r], quarter_max(top) * unscale[r]) : m[r];
+      const bool up = mn > m[r] + SLACK;
+      if (__any(up)) {
+        const float to = up ? floorf(mn) : m[r], f = up ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
+#pragma unroll
+        for (int c = 0; c < OT; ++c) o[r][c] *= f;
+        l[r] *= f;
+        m[r] = to;
       }
-    }
-    float top = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]), top1 = fmaxf(fmaxf(s[1][0], s[1][1]), s[1][2]);
-    top = fmaxf(fmaxf(top, s[0][3]), fmaxf(top1, s[1][3]));
-    const float mn = mine ? fmaxf(m, quarter_max(top) * unscale) : m;
-    const bool up = mn > m + SLACK;
-    if (__any(up)) {
-      const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+      // (a weight of a row that is not of the request: 2^-infinity)
+      const float bias = mine[r] ? LIFT - (m[r] == -INFINITY ? 0.0f : m[r]) : -INFINITY;
+      float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int c = 0; c < OT; ++c) o[c] *= f;
-      l *= f;
-      m = to;
+      for (int i = 0; i < 4; ++i) {
+        const int v = 2 * (i % 2);
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[r][i / 2][v], unscale[r], bias)), q = __builtin_amdgcn_exp2f(fmaf(s[r][i / 2][v + 1], unscale[r], bias));
+        sum[0] += p;
+        sum[1] += q;
+        const WeightParts w2 = split_weights(p, q);
+        ph[r][2 * i] = w2.hi[0];
+        ph[r][2 * i + 1] = w2.hi[1];
+        pl[r][2 * i] = w2.lo[0];
+        pl[r][2 * i + 1] = w2.lo[1];
+      }
+      l[r] += sum[0] + sum[1];
     }
-    // (a weight of a row that is not of the request: 2^-infinity)
-    const float bias = mine ? LIFT - (m == -INFINITY ? 0.0f : m) : -INFINITY;
-    half8 ph, pl;  // the lane's four tokens of each half
-    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int v = 2 * (i % 2);
-      const float p = __builtin_amdgcn_exp2f(fmaf(s[i / 2][v], unscale, bias)), q = __builtin_amdgcn_exp2f(fmaf(s[i / 2][v + 1], unscale, bias));
-      sum[0] += p;
-      sum[1] += q;
-      const WeightParts w2 = split_weights(p, q);
-      ph[2 * i] = w2.hi[0];
-      ph[2 * i + 1] = w2.hi[1];
-      pl[2 * i] = w2.lo[0];
-      pl[2 * i + 1] = w2.lo[1];
-    }
-    l += sum[0] + sum[1];
     lds_byte* const values = stage + slot * TILE;
 #pragma unroll
     for (int half_c = 0; half_c < GR / 2; ++half_c) {  // two groups of 32 dims
@@ -781,8 +818,11 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           const half8 v8 = {v[0][x][0], v[0][x][1], v[0][2 + x][0], v[0][2 + x][1], v[1][x][0], v[1][x][1], v[1][2 + x][0], v[1][2 + x][1]};
-          o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph, o[2 * c + x], 0, 0, 0);
-          o[2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl, o[2 * c + x], 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < RG; ++r) {
+            o[r][2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, ph[r], o[r][2 * c + x], 0, 0, 0);
+            o[r][2 * c + x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8, pl[r], o[r][2 * c + x], 0, 0, 0);
+          }
         }
       }
     }
@@ -794,56 +834,62 @@ __global__ __launch_bounds__(64 * STEP_WAVES, 3) void pg_step_kernel(PgAttendArg
     }
   }
 
-  // the block's four states as one
-  l = quarter_sum(l);
-  if (q4 == 0) {
-    ml[wave][r16][0] = m;
-    ml[wave][r16][1] = l;
+  // the block's four states as one, 16 rows at a time
+#pragma unroll
+  for (int r = 0; r < RG; ++r) {
+    l[r] = quarter_sum(l[r]);
+    if (q4 == 0) {
+      ml[wave][16 * r + r16][0] = m[r];
+      ml[wave][16 * r + r16][1] = l[r];
+    }
   }
-  __syncthreads();
-  float M = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < STEP_WAVES; ++i) M = fmaxf(M, ml[i][r16][0]);
-  const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-  float* os = reinterpret_cast<float*>(lds + wave * STAGE) + r16 * OP;
-#pragma unroll
-  for (int c = 0; c < GR; ++c)
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-      *reinterpret_cast<floatx4*>(os + 32 * c + 8 * q4 + 4 * x) =
-          floatx4{o[2 * c][2 * x] * f, o[2 * c + 1][2 * x] * f, o[2 * c][2 * x + 1] * f, o[2 * c + 1][2 * x + 1] * f};
-  __syncthreads();
-  const uint32_t jr = tid / 16, d0 = tid % 16 * 4;  // a row per 16 threads
-  const uint32_t out_row = tile * 16 + jr;
-  float M_row = -INFINITY, L_row = 0.0f;
-#pragma unroll
-  for (int i = 0; i < STEP_WAVES; ++i) M_row = fmaxf(M_row, ml[i][jr][0]);
-  const float M_base = M_row == -INFINITY ? 0.0f : M_row;  // (then every l is 0, or no number)
-#pragma unroll
-  for (int i = 0; i < STEP_WAVES; ++i) L_row = fmaf(ml[i][jr][1], __builtin_amdgcn_exp2f(ml[i][jr][0] - M_base), L_row);
-  const size_t part = (size_t(g) * sp.blocks + block) * 16 + jr;
   const bool last = sp.blocks == sp.tiles;
   if (sp.ranges && g == 0 && split == 0 && tid == 0) sp.ranges[tile] = make_uint2(share.first, share.count);
-  const uint32_t ob = pa.by_rows(out_row), ot = pa.by_rep(out_row - ob * per), oh = g * a.s.rep + out_row - (ob * a.c.n + ot) * a.s.rep;
-  const bool out_live = out_row < rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
-  if (last && !out_live) return;
-  float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
-  const float inv = last ? (M_row == -INFINITY ? NAN : 1.0f / L_row) : 1.0f;  // (it sees a key, its own)
+  const uint32_t jr = tid / 16, d0 = tid % 16 * 4;  // a row per 16 threads
 #pragma unroll
-  for (int c = 0; c < HD / 64; ++c) {
-    const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
-    floatx4 x = *reinterpret_cast<const floatx4*>(src);
+  for (int r = 0; r < RG; ++r) {
+    __syncthreads();
+    float M = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * (STAGE / 4));
-    *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
-  }
-  if (tid % 16 == 0 && !last) {
-    sp.ml[2 * part] = M_row - LIFT;
-    sp.ml[2 * part + 1] = L_row;
+    for (int i = 0; i < STEP_WAVES; ++i) M = fmaxf(M, ml[i][16 * r + r16][0]);
+    const float f = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - M);
+    float* os = reinterpret_cast<float*>(lds + wave * STAGE) + r16 * OP;
+#pragma unroll
+    for (int c = 0; c < GR; ++c)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        *reinterpret_cast<floatx4*>(os + 32 * c + 8 * q4 + 4 * x) =
+            floatx4{o[r][2 * c][2 * x] * f, o[r][2 * c + 1][2 * x] * f, o[r][2 * c][2 * x + 1] * f, o[r][2 * c + 1][2 * x + 1] * f};
+    __syncthreads();
+    float M_row = -INFINITY, L_row = 0.0f;
+#pragma unroll
+    for (int i = 0; i < STEP_WAVES; ++i) M_row = fmaxf(M_row, ml[i][16 * r + jr][0]);
+    const float M_base = M_row == -INFINITY ? 0.0f : M_row;  // (then every l is 0, or no number)
+#pragma unroll
+    for (int i = 0; i < STEP_WAVES; ++i) L_row = fmaf(ml[i][16 * r + jr][1], __builtin_amdgcn_exp2f(ml[i][16 * r + jr][0] - M_base), L_row);
+    const size_t part = (size_t(g) * sp.blocks + block) * ROWS + 16 * r + jr;
+    const uint32_t out_row = row0 + 16 * r + jr, ob = pa.by_rows(out_row), ot = pa.by_rep(out_row - ob * per), oh = g * a.s.rep + out_row - (ob * a.c.n + ot) * a.s.rep;
+    const bool out_live = 16 * r + jr < n_rows && ot < __shfl(run.rq.fresh, int(ob - b_lo) & 15, 64);
+    if (!last || out_live) {
+      float* dst = last ? a.out + ((size_t(ob) * a.c.n + ot) * a.s.H + oh) * HD : sp.o + part * HD;
+      const float inv = last ? (M_row == -INFINITY ? NAN : 1.0f / L_row) : 1.0f;  // (it sees a key, its own)
+#pragma unroll
+      for (int c = 0; c < HD / 64; ++c) {
+        const float* src = reinterpret_cast<const float*>(lds) + jr * OP + d0 + 64 * c;
+        floatx4 x = *reinterpret_cast<const floatx4*>(src);
+#pragma unroll
+        for (int i = 1; i < STEP_WAVES; ++i) x += *reinterpret_cast<const floatx4*>(src + i * (STAGE / 4));
+        *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
+      }
+      if (tid % 16 == 0 && !last) {
+        sp.ml[2 * part] = M_row - LIFT;
+        sp.ml[2 * part + 1] = L_row;
+      }
+    }
   }
 }
 
-// Many rows (turns, prompts).  A block of four waves owns up to 128 packed rows of a kv
+// Many rows (turns, prompts).  A block of four waves owns up to 128 rows of a request and kv
 // head, 32 per wave, and walks the run of tiles of 64 keys.  Each wave takes 16 of a
 // tile's keys and values from 4 bits to f16, once for the block, and leaves them in
 // LDS, the next tile's while this one's products run; codes are loaded another tile
@@ -869,9 +915,8 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), r32 = lane & 31u, h2 = lane >> 5, r16 = lane & 15u, q4 = lane >> 4;
   const uint32_t rest = pa.by_groups(blockIdx.x), g = blockIdx.x - rest * a.s.G;
   const uint32_t split = rest / sp.row_tiles, tile = sp.row_tiles - 1 - (rest - split * sp.row_tiles);  // later rows see more keys: they go first
-  const uint32_t splits = sp.each, per = a.c.n * a.s.rep, whose = sp.of_request ? tile / sp.of_request : 0u;
-  const uint32_t row0 = sp.of_request ? whose * per + (tile - whose * sp.of_request) * TILE_ROWS : tile * TILE_ROWS;
-  const uint32_t rows = sp.of_request ? (whose + 1) * per : a.c.R * per, n_rows = min(uint32_t(TILE_ROWS), rows - row0);
+  const uint32_t splits = sp.each, per = a.c.n * a.s.rep, whose = sp.by_of(tile), row0 = whose * per + (tile - whose * sp.of_request) * TILE_ROWS;
+  const uint32_t rows = (whose + 1) * per, n_rows = min(uint32_t(TILE_ROWS), rows - row0);
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
@@ -1233,9 +1278,10 @@ __global__ __launch_bounds__(256) void pg_join_kernel(KvAttendArgs a, PgShare sp
   const bool is_row = at < a.c.R * a.c.n * a.s.H;
   const uint32_t out = is_row ? at : 0u, bt = out / a.s.H, h = out % a.s.H, b = bt / a.c.n, t = bt % a.c.n, g = h / a.s.rep;
   const RawRequest raw = load_request(a.c, b);
-  const uint32_t row = bt * a.s.rep + h % a.s.rep, tile = row / 16;
+  const uint32_t row_b = t * a.s.rep + h % a.s.rep, row = sp.of_request ? row_b : b * a.c.n * a.s.rep + row_b, in_tile = row & ((1u << sp.shift) - 1u);
+  const uint32_t tile = (sp.of_request ? b * sp.of_request : 0u) + (row >> sp.shift);
   const uint2 range = sp.ranges ? sp.ranges[tile] : make_uint2(tile * sp.each, sp.each);
-  const size_t part = (size_t(g) * sp.blocks + range.x) * 16 + row % 16;
+  const size_t part = ((size_t(g) * sp.blocks + range.x) << sp.shift) + in_tile;
   float M = -INFINITY, L = 0.0f;
   floatx4 x = floatx4{0.f, 0.f, 0.f, 0.f};
   for (uint32_t s0 = team; s0 < range.y; s0 += 4 * TEAM) {
@@ -1244,8 +1290,9 @@ __global__ __launch_bounds__(256) void pg_join_kernel(KvAttendArgs a, PgShare sp
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t s = min(s0 + i * TEAM, range.y - 1);
-      ml[i] = *reinterpret_cast<const float2*>(sp.ml + 2 * (part + 16 * s));
-      if (TEAM > 1 || s0 + i < range.y) y[i] = *reinterpret_cast<const floatx4*>(sp.o + (part + 16 * s) * HD + 4 * d);
+      const size_t of = part + (size_t(s) << sp.shift);
+      ml[i] = *reinterpret_cast<const float2*>(sp.ml + 2 * of);
+      if (TEAM > 1 || s0 + i < range.y) y[i] = *reinterpret_cast<const floatx4*>(sp.o + of * HD + 4 * d);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -1745,33 +1792,44 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   PgShare sp{};
   sp.o = w.part;
   sp.ml = w.part_ml;
-  const uint32_t rows = a.c.R * a.c.n * a.s.rep;
-  sp.tiles = (rows + 15) / 16;
-  const uint32_t per = a.c.n * a.s.rep, of_request = (per + TILE_ROWS - 1) / TILE_ROWS;
-  // The tile kernel takes half as long for a score but 10 us more (128 rows' states), and where a request has few rows it
-  // does several requests' keys for all of them.  Step : tile kernel, us, heads 32 over 8 of 128: 1 x 1000 tokens over 1000
-  // (16 M scores) 50 : 55, 1 x 1200 over 1200 (23) 67 : 56, 2 x 100 over 4000 (25) 58 : 50, 8 x 40 over 2000 (20) 43 : 48; of
-  // 32 rows 8 x 8 over 6000 shared + 500 (13) 40 : 42, over 20000 + 500 (42) 86 : 64, over 16000 of their own (33) 64 : 99.
-  const size_t scores = size_t(a.s.G) * rows * (a.c.cap - min(a.c.n, a.c.cap) / 2);
-  const bool many = per >= 32 && scores / 64 * min(per, 64u) > 18000000u * size_t(128) / hd;
+  const uint32_t per = a.c.n * a.s.rep, rows = a.c.R * per;
   // A row tile with rows of two requests walks both's keys, twice as long as its neighbours; tiles of one request each have
-  // up to a third of their rows empty.  Tiles of two : of one, us: 8 x 500 over 4000 467 : 329, 8 x 100 (400 rows) over 4000
-  // 188 : 112, over 1500 shared + 500 79 : 70; 8 x 40 (160 rows, 96 of 256 empty) over 3500 + 500 60 : 69.
-  if (many && of_request * TILE_ROWS <= per + per / 3) sp.of_request = of_request;
-  sp.row_tiles = sp.of_request ? a.c.R * of_request : (rows + TILE_ROWS - 1) / TILE_ROWS;
-  const uint32_t kt = many ? 64 : 32, lots = a.s.G * (many ? sp.row_tiles : sp.tiles);
-  const uint32_t most = (a.c.cap + kt - 1) / kt * (many ? 1u : min(a.c.R, 15 / (a.c.n * a.s.rep) + 1));  // key tiles of a row tile, at most
+  // empty rows (the step kernel's up to a third, but where 32 rows hold the request).  Tiles of two : of one, us, heads 32 over 8
+  // of 128: 8 x 500 tokens over 4000 467 : 329, 8 x 100 (400 rows) over 4000 188 : 112, over 1500 shared + 500 79 : 70; of 16
+  // rows 16 x 3 (12 rows) over 4000 38 : 30.
+  auto apart = [&](uint32_t n) { return (per + n - 1) / n * n <= per + per / 3; };
+  // The tile kernel takes half as long for a score but 10 us more (128 rows' states).  Step : tile kernel: 1 x 1000 over 1000
+  // (20 M scores) 47 : 46, 1 x 1200 over 1200 (29) 61 : 55, 2 x 100 over 4000 (26) 57 : 50, heads 64 over 8, 2 x 50 over 3000 (20) 55 :
+  // 39; of 160 rows, which are two tiles, 8 x 40 over 4000 65 : 68, over 3500 shared + 500 84 : 69.  (Requests of fewer than 96
+  // rows, several to a tile: 8 x 20 over 16000 118 : 167, 8 x 8 over 20000 shared + 500 77 : 66.)
+  const size_t scores = size_t(a.s.G) * rows * (a.c.cap - min(a.c.n, a.c.cap) / 2);
+  const bool many = per >= 96 && scores > 18000000u * size_t(128) / hd;
+  // Rows of the step kernel's tiles.  32 take a key's four bits apart once for twice as many, but short runs want the waves of
+  // 16.  16 : 32, us: 16 x 5 over 32001 239 : 172, 8 x 8 over 16000 64 : 58, 1 x 100 over 4000 44 : 41, 8 x 8 over 4000 29 : 31,
+  // 2 x 6 over 500 10.6 : 13.0, 1 x 40 over 200 9.0 : 12.1; where 16 would have rows of two requests, 16 x 5 over 1000 28 : 20.
+  const bool two = !many && per > 16 && size_t(a.s.G) * ((rows + 15) / 16) * ((a.c.cap + 31) / 32) >= (apart(16) ? 16 : 4) * 1024;
+  const uint32_t tile_rows = many ? uint32_t(TILE_ROWS) : two ? 32 : 16, of_request = (per + tile_rows - 1) / tile_rows;
+  if (many || apart(tile_rows) || (two && of_request == 1)) sp.of_request = of_request;
+  sp.by_of = Div::by(of_request);
+  sp.row_tiles = sp.of_request ? a.c.R * of_request : (rows + tile_rows - 1) / tile_rows;
+  sp.tiles = many ? (rows + 15) / 16 : sp.row_tiles;
+  sp.shift = two ? 5 : 4;
+  const uint32_t kt = many ? 64 : 32, lots = a.s.G * sp.row_tiles;
+  const uint32_t most = (a.c.cap + kt - 1) / kt * (many || sp.of_request ? 1u : min(a.c.R, (tile_rows - 1) / per + 1));  // key tiles of a row tile, at most
   // Blocks of the step kernel, by the key tiles that a wave of 256 would walk at most: short runs end sooner with fewer
   // states to join, long ones want more waves to take turns.  256 : 512 : 768 blocks, us: 8 x 1 over 1500 + 512 (4 tiles) 13 :
   // 17 : 21, 16 x 1 over 1000 (5) 17 : 18 : 21, 1 x 1 over 30000 (7) 21 : 20 : 22, 16 x 1 over 6000 (24) 44 : 35 : 34, over
   // 32001 (126) 202 : 127 : 120.
   const size_t walk = size_t(lots) * most / 1024;
   const uint32_t fill = many || (walk >= 6 && walk < 24) ? 512 : walk < 6 ? 256 : 768;
-  uint32_t splits = max(1u, min(fill / lots, many ? max(1u, most / 2) : (most + STEP_WAVES - 1) / STEP_WAVES));
+  // (the tile kernel's: 8 key tiles each on average, or their states cost more than they save: 1 x 1000 in 1 : 2 46 : 54, 1 x 100
+  // over 4000 in 4 : 8 : 16 50 : 38 : 42)
+  uint32_t splits = max(1u, min(fill / lots, many ? (a.c.cap - min(a.c.n, a.c.cap) / 2) / (8 * kt) : (most + STEP_WAVES - 1) / STEP_WAVES));
   // One block, and no join, for short runs (in a graph, one : several, us: 1 x 1, table of 14 tiles 8.9 : 9.1, of 18 10.1 : 9.2;
   // heads of 64, 18 8.3 : 8.4, 26 10.1 : 8.4).
   if (!many && most <= (hd == 64 ? 24u : 16u)) splits = 1;
-  if (size_t(a.s.G) * sp.tiles * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / (a.s.G * sp.tiles)));
+  const size_t parts = size_t(a.s.G) * sp.tiles << (sp.shift - 4);  // (16 rows each)
+  if (parts * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / parts));
   sp.blocks = sp.tiles * splits;
   sp.each = splits;
   sp.by_each = Div::by(splits);
@@ -1781,11 +1839,22 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   return by_dim(hd, [&](auto HD) {
     if (many)
       hipLaunchKernelGGL(pg_tile_kernel<HD()>, dim3(lots * splits), dim3(256), 0, s, pa, sp);
-    else if (pa.p.shift == 4)  // a tile takes two pages
-      hipLaunchKernelGGL((pg_step_kernel<HD(), true>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
-    else
-      hipLaunchKernelGGL((pg_step_kernel<HD(), false>), dim3(a.s.G * sp.blocks), dim3(64 * STEP_WAVES), 0, s, pa, sp);
+    else {
+      const dim3 grid(a.s.G * sp.blocks), block(64 * STEP_WAVES);
+      auto step = [&](auto TWO, auto RG) { hipLaunchKernelGGL((pg_step_kernel<HD(), TWO(), RG()>), grid, block, 0, s, pa, sp); };
+      auto pages = [&](auto RG) {
+        if (pa.p.shift == 4)  // a tile takes two pages
+          step(std::true_type(), RG);
+        else
+          step(std::false_type(), RG);
+      };
+      if (two)
+        pages(std::integral_constant<int, 2>());
+      else
+        pages(std::integral_constant<int, 1>());
+    }
     // (several teams a row : one, us: 8 x 1 over 2000 16.7 : 18.6, 16 x 1 over 8000 40.3 : 44.7, 64 x 1 over 2000 43.0 : 42.6)
+    if (many) sp.of_request = 0;  // (its states go by rows alone)
     const uint32_t out_rows = a.c.R * a.c.n * a.s.H, teams = 256 / (HD() / 4);
     if (splits > 1 && out_rows <= 2048)
       hipLaunchKernelGGL((pg_join_kernel<HD(), 1024 / HD()>), dim3(out_rows), dim3(256), 0, s, a, sp);

@@ -199,7 +199,7 @@ def test_attend_turn_borders(extra, hd, page, room):
 @pytest.mark.parametrize("shared", [0, 5])
 @pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65, 95, 96, 97])
 def test_attend_row_tiles(n, shared):
-    """Tiles of 128 rows: of one request each, or of several, by how many rows a request has; idle ones among them."""
+    """Row tiles of one request each, or of several, by how many rows a request has; idle ones among them."""
     new = [n, 1, 0, n, n - 1, n // 2, n]
     Pool((8, 2, 64), 32, [shared * 32 + x + 10 * i if x else 0 for i, x in enumerate(new)], new, shared=shared, seed=n, width=4096).check_all()
     new = [n // 2, n // 2, 0, 1, n // 4, n // 2, n // 2, n // 2, n // 2]
