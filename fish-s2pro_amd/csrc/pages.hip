@@ -416,6 +416,11 @@ __device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
 struct PageWindow {
   uint32_t b = 0xffffffffu, first = 0;
   int32_t page = 0;
+  __device__ __forceinline__ void load(const PgPool& p, uint32_t req, uint32_t i) {
+    b = req;
+    first = i;
+    page = p.table[size_t(req) * p.width + min(i + (threadIdx.x & 63u), p.width - 1)];
+  }
   __device__ __forceinline__ void begin(const Pages64& early, uint32_t b_lo, uint32_t req) {  // (where req is one of the few)
     if (req - b_lo >= uint32_t(FEW)) return;
     b = req;
@@ -424,11 +429,7 @@ struct PageWindow {
       if (req - b_lo == uint32_t(j)) page = early.of[j];
   }
   __device__ __forceinline__ uint32_t get(const PgPool& p, uint32_t req, uint32_t i) {
-    if (req != b || i - first >= 64u) {
-      b = req;
-      first = i;
-      page = p.table[size_t(req) * p.width + min(i + (threadIdx.x & 63u), p.width - 1)];
-    }
+    if (req != b || i - first >= 64u) load(p, req, i);
     return lane_read_u32(uint32_t(page), int(i - first));
   }
 };
@@ -920,54 +921,36 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   const Chunk<HD> at{pa.p.shift};
   const Bits bits = code_bits();
 
-  const RawRequest raw = load_request(a.c, min(pa.by_rows(row0) + lane, a.c.R - 1));
-  const Pages64 early = load_pages(pa, pa.by_rows(row0));
+  const RawRequest raw = load_request(a.c, whose);
+  PageWindow window;
+  window.load(pa.p, whose, 0);
   const uint32_t my_row = row0 + wave * 32 + r32, row = min(my_row, rows - 1);
-  const uint32_t b_row = pa.by_rows(row), t_row = pa.by_rep(row - b_row * per), h_row = g * a.s.rep + row - (b_row * a.c.n + t_row) * a.s.rep;
-  const size_t at_row = (size_t(b_row) * a.c.n + t_row) * a.s.H + h_row;
+  const uint32_t t_row = pa.by_rep(row - whose * per), h_row = g * a.s.rep + row - (whose * a.c.n + t_row) * a.s.rep;
+  const size_t at_row = (size_t(whose) * a.c.n + t_row) * a.s.H + h_row;
   float4 qx[DS][2];  // dims 16 ks + 8 h2 ..
 #pragma unroll
   for (int ks = 0; ks < DS; ++ks)
 #pragma unroll
     for (int e = 0; e < 2; ++e) qx[ks][e] = *reinterpret_cast<const float4*>(a.q + at_row * HD + 16 * ks + 8 * h2 + 4 * e);
-  const PgRun run = pg_run<KT>(pa, row0, n_rows, raw, early, g == 0 && split == 0 && wave == 0 ? a.s.err : nullptr);
-  const uint64_t has = __ballot(run.seg_keys != 0);
-  if (!has) return;  // no row of a token
-  const uint32_t c_all = run.common / KT, c_lo = c_all * split / splits, n_com = c_all * (split + 1) / splits - c_lo;
-  const uint32_t o_lo = run.tiles * (splits - 1 - split) / splits, n_tiles = n_com + run.tiles * (splits - split) / splits - o_lo;
+  const Request rq = checked(a.c, raw, g == 0 && split == 0 && tid == 0 ? a.s.err : nullptr);
+  const uint32_t first_token = pa.by_rep(row0 - whose * per), last_token = pa.by_rep(row0 - whose * per + n_rows - 1);
+  if (first_token >= rq.fresh) return;  // no row of a token
+  const uint32_t seen = uniform(rq.len - rq.fresh + min(last_token, rq.fresh - 1) + 1);  // keys that its rows see, at most
+  const uint32_t all = (seen + KT - 1) / KT, lo = all * split / splits, n_tiles = all * (split + 1) / splits - lo;
 
-  uint32_t seg = 0;
-  const uint32_t lead = uint32_t(__ffsll((unsigned long long)has)) - 1;  // (with the others' pages in common)
-  PageWindow window;
-  if (n_com == 0) seg = owner(run, o_lo);
-  window.begin(early, run.b_lo, run.b_lo + (n_com ? lead : seg));
   // a tile, and where the wave's 16 keys of it are
   struct Tile {
     uint32_t key0, keys;
-    int seg;
     const uint8_t* part;
     uint32_t slot;
     bool gone;
   };
   auto where = [&](uint32_t i) {
     Tile w;
-    uint32_t req;
-    if (i < n_com) {
-      w.seg = -1;
-      req = run.b_lo + lead;
-      w.key0 = (c_lo + i) * KT;
-      w.keys = KT;
-    } else {
-      const uint32_t x = o_lo + (i - n_com);
-      seg = owner(run, x);
-      const uint32_t begin = seg ? lane_read_u32(run.seg_end, int(seg) - 1) : 0u;
-      w.seg = int(seg);
-      req = run.b_lo + seg;
-      w.key0 = run.common + (x - begin) * KT;
-      w.keys = min(uint32_t(KT), lane_read_u32(run.seg_keys, int(seg)) - w.key0);
-    }
+    w.key0 = (lo + i) * KT;
+    w.keys = min(uint32_t(KT), seen - w.key0);
     const uint32_t key = w.key0 + (16 * wave < w.keys ? 16 * wave : 0u);
-    const uint32_t page = window.get(pa.p, req, key >> pa.p.shift);
+    const uint32_t page = window.get(pa.p, whose, key >> pa.p.shift);
     w.gone = page >= pa.p.pages;
     w.part = pa.p.pool + (size_t(w.gone ? 0u : page) * a.s.G + g) * pa.p.chunk;
     w.slot = key & ((1u << pa.p.shift) - 1u);
@@ -1062,9 +1045,8 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
   };
 
   // this lane's row
-  const uint32_t len_row = __shfl(run.rq.len, int(b_row - run.b_lo) & 63, 64), fresh_row = __shfl(run.rq.fresh, int(b_row - run.b_lo) & 63, 64);
-  const bool live = my_row < rows && t_row < fresh_row;
-  const int own_seg = int(b_row - run.b_lo), own_limit = int(len_row - fresh_row + t_row);
+  const bool live = my_row < rows && t_row < rq.fresh;
+  const int limit = live ? int(rq.len - rq.fresh + t_row) : -1;  // the last key that it sees
   half8 qh[DS], ql[DS];  // dims 16 ks + 8 h2 + e
   float unscale;
   {
@@ -1116,7 +1098,6 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
     if (tid == 0) gone_tile[flag2] = 0;
     const uint32_t gone = uniform(gone_tile[flag]);  // (and bit 8)
     const bool more = i + 1 < n_tiles;
-    const int limit = !live ? -1 : cur.seg < 0 ? 0x7fffffff : cur.seg == own_seg ? own_limit : -1;
     const bool sees = __any(limit >= int(cur.key0));  // else nothing of it is for this wave's rows
     if (more && !sees) store(next, buf ^ 1u, flag1);
     uint32_t k_from = buf * BUF + k_at(r32, h2), v_from = buf * BUF + v_at(r32, h2);
