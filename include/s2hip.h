@@ -635,7 +635,8 @@ int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, con
  * no number makes that element of its row no number, a key all of them; so do a query
  * of no number and scores that are all below the range of f32.  A page that is not one
  * of the pool is not read: its tokens are not seen (a row that sees none is no
- * number).  Pages that requests have in common are read once for several of them.
+ * number).  Steps and short turns read pages that requests have in common once for
+ * several of them.
  * Products and sums are f32 or better. */
 int32_t s2hip_pages_attend(s2hip_pages* pages, const s2hip_pages_view* view, const float* q, uint32_t n_tokens,
                            float* out, void* stream, char* err, size_t err_cap);
