@@ -101,7 +101,7 @@ class Pool:
 
     def dense(self):
         """Keys and values [R][G][cap][hd] that the rows hold, zeros elsewhere."""
-        cap = self.width * self.page
+        cap = max(1, max(-(-n // self.page) for n in self.lens_h)) * self.page
         k = np.zeros((self.R, self.G, cap, self.hd))
         v = np.zeros_like(k)
         pool = self.pool.cpu().numpy()
@@ -204,6 +204,19 @@ def test_attend_row_tiles(n, shared):
     Pool((8, 2, 64), 32, [shared * 32 + x + 10 * i if x else 0 for i, x in enumerate(new)], new, shared=shared, seed=n, width=4096).check_all()
     new = [n // 2, n // 2, 0, 1, n // 4, n // 2, n // 2, n // 2, n // 2]
     Pool((4, 2, 128), 64, [shared * 64 + x + 10 * i if x else 0 for i, x in enumerate(new)], new, shared=shared, seed=n, width=4096).check_all()
+
+
+@pytest.mark.parametrize("shared", [0, 3])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n", [3, 4, 5, 6, 7, 8, 9, 11, 12, 13, 17, 23])
+def test_attend_speculative_steps(n, hd, page, shared):
+    """A few tokens of each request, in tables with room for long runs: row tiles of 16 and 32."""
+    new = [n, 1, 0, n, n - 1, n // 2, n]
+    lens = [shared * page + x + 70 * i if x else 0 for i, x in enumerate(new)]
+    Pool((8, 2, hd), page, lens, new, shared=shared, seed=n, width=131072 // page).check_all()
+    new, lens = new[:2], [lens[0] + 3000, lens[1]]
+    Pool((8, 2, hd), page, lens, new, shared=shared, seed=n, rows=n, width=16384 // page).check_all()
 
 
 def test_attend_many_requests():
