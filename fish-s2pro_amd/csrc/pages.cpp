@@ -18,7 +18,7 @@ namespace s2 {
 namespace {
 
 constexpr uint32_t PG_MAX_PAGES = 1u << 20, PG_MAX_SLOTS = 1u << 20, PG_MAX_REQUESTS = 256, PG_MAX_TOKENS = 65536, PG_MAX_REP = 64,
-                   PG_MAX_HEADS = 1024, PG_MAX_LAYERS = 1024;
+                   PG_MAX_HEADS = 1024, PG_MAX_LAYERS = 1024, PG_MAX_ROPE_DIMS = 1u << 16;
 
 struct Words {
   const void* p;
@@ -262,7 +262,7 @@ int32_t s2hip_rope_frequencies(uint32_t dims, double base, uint32_t scaling, dou
                                double high, double* freq, double* gain, char* err, size_t err_cap) {
   return kv_guarded(err, err_cap, [&] {
     if (!freq || !gain) throw std::runtime_error("NULL argument");
-    if (dims == 0 || dims % 2) s2::kfail("rope: dims %u is not even", dims);
+    if (dims == 0 || dims % 2 || dims > s2::PG_MAX_ROPE_DIMS) s2::kfail("rope: dims %u is not an even number of 2..%u", dims, s2::PG_MAX_ROPE_DIMS);
     if (!(base > 0.0) || !std::isfinite(base)) s2::kfail("rope: base is not positive");
     if (scaling > S2HIP_ROPE_PARTS) s2::kfail("rope: scaling %u is not known", scaling);
     if (scaling != S2HIP_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) s2::kfail("rope: factor is not at least 1");

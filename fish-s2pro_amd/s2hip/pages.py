@@ -27,6 +27,8 @@ ERR_PAGE = 8
 ERR_FULL = 16
 ERR_REFS = 32
 
+MAX_ROPE_DIMS = 1 << 16
+
 SCALINGS = {"none": 0, "linear": 1, "stretch": 2, "parts": 3}
 
 
@@ -37,7 +39,9 @@ def rope_frequencies(dims: int, base: float = 1.0e6, scaling: str = "none", fact
     L = _lib.load()
     if scaling not in SCALINGS:
         raise S2HipError(f"rope: scaling {scaling!r} is not one of {', '.join(SCALINGS)}")
-    freq, gain = np.zeros(max(1, dims // 2)), ctypes.c_double()
+    if not 2 <= dims <= MAX_ROPE_DIMS or dims % 2:  # (a C caller's dims are 32 bits without a sign)
+        raise S2HipError(f"rope: dims {dims} is not an even number of 2..{MAX_ROPE_DIMS}")
+    freq, gain = np.zeros(dims // 2), ctypes.c_double()
     err = ctypes.create_string_buffer(_lib.ERR_CAP)
     if not L.s2hip_rope_frequencies(dims, base, SCALINGS[scaling], factor, context, low, high, freq.ctypes.data,
                                     ctypes.byref(gain), err, _lib.ERR_CAP):

@@ -589,8 +589,8 @@ typedef struct {
   uint32_t requests;
 } s2hip_pages_view;
 
-/* Angles per position of dims / 2 pairs, base^(-2 i / dims), for s2hip_pages_config,
- * and the gain that belongs to them; for contexts `factor` (>= 1) times as long as the
+/* Angles per position of dims / 2 pairs (dims: even, 2..65536), base^(-2 i / dims), for
+ * s2hip_pages_config, and the gain that belongs to them; for contexts `factor` (>= 1) times as long as the
  * `context` positions that a model was trained on:
  *   S2HIP_ROPE_LINEAR   all over factor
  *   S2HIP_ROPE_STRETCH  base times factor^(dims / (dims - 2)): the slowest over factor (dims >= 4)

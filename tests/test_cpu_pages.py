@@ -1,13 +1,14 @@
 """The paged 4-bit cache without a device: rotation frequencies, what a handle
 refuses before it looks for one, and the 64-bit model of the layout."""
 
+import ctypes
 import math
 
 import numpy as np
 import pytest
 
 import pages_util
-from s2hip import PagedKv, S2HipError, rope_frequencies
+from s2hip import PagedKv, S2HipError, _lib, rope_frequencies
 
 GOOD = dict(heads=8, kv_heads=2, head_dim=64, page_tokens=16, pages=10, table_pages=4)
 
@@ -44,6 +45,22 @@ def test_scaled_frequencies():
 def test_frequencies_refused(bad, text):
     with pytest.raises(S2HipError, match=text):
         rope_frequencies(**dict(dict(dims=64, base=1.0e4), **bad))
+
+
+@pytest.mark.parametrize("dims", [-1, -2, -64, -(1 << 31), 1, (1 << 16) + 2, (1 << 32) - 2, (1 << 32) + 64, (1 << 33) + 2])
+def test_frequencies_of_impossible_dims(dims):
+    """Numbers below 0 and beyond what the C call's 32 bits hold: refused before anything is written."""
+    with pytest.raises(S2HipError, match="dims"):
+        rope_frequencies(dims, 1.0e4)
+
+
+@pytest.mark.parametrize("dims", [0, 3, (1 << 16) + 2, (1 << 32) - 2, (1 << 32) - 64])
+def test_frequencies_of_impossible_dims_in_c(dims):
+    """The C call itself writes to no frequency, whatever a caller's binding makes of its number."""
+    L = _lib.load()
+    freq, gain, err = np.full(4, 7.0), ctypes.c_double(7.0), ctypes.create_string_buffer(_lib.ERR_CAP)
+    assert L.s2hip_rope_frequencies(dims, 1.0e4, 0, 1.0, 8192.0, 1.0, 32.0, freq.ctypes.data, ctypes.byref(gain), err, _lib.ERR_CAP) == 0
+    assert b"dims" in err.value and (freq == 7.0).all() and gain.value == 7.0
 
 
 @pytest.mark.parametrize("bad, text", [
