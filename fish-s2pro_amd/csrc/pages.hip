@@ -1443,8 +1443,9 @@ __device__ __forceinline__ void copy_pages(const PgUpdateArgs& a, const int32_t*
   if (to_now) *to_now = now;
 }
 
-// One block, a wave per row at a time.  References are counted apart: what rows let go of is taken off, what they take
-// added; the rest of a row that stays its own counts as it is.  Of w rows that write to a page of r references, the
+// One block, a wave per row at a time.  References are counted apart: what every row holds is taken off, then what it will
+// hold added, also where that is the same: a count that goes below 0 on the way was below the rows that hold the page, and
+// two rows would each take the page for their own.  Of w rows that write to a page of r references, the
 // first r - 1 write to copies: the last writes in place if no one else holds it.
 //   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores; sixteen
 // waves share four vector units, so each instruction of a turn counts (64 rows of 102 pages 13 us, 16 of 32 pages 8, of a
@@ -1532,8 +1533,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
         const uint32_t i = i0 + 64 * k + lane;
         const bool in = uint32_t(e[k]) < a.p.pages && uint32_t(v[k]) < a.p.pages;
         if (!in) report(S2HIP_PAGES_ERR_PAGE);
-        if (in && i < n_old && (!same || i >= n_base)) atomicSub(refs(uint32_t(e[k])), 1);
-        if (in && i < n_base && !same) atomicAdd(refs(uint32_t(v[k])), 1);
+        if (in && i < n_old && atomicSub(refs(uint32_t(e[k])), 1) < 1) report(S2HIP_PAGES_ERR_REFS);
         if (i < n_base) *rows(b * width + i) = v[k];
       }
     }
@@ -1543,13 +1543,13 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     const uint32_t n = uniform(pages_of(kept[b]));
     for (uint32_t i0 = 0; i0 < n; i0 += 128) {
       const uint32_t i = i0 + lane;
-      const int32_t x = i < n ? count(uint32_t(*rows(b * width + i))) : 1, y = i + 64 < n ? count(uint32_t(*rows(b * width + i + 64))) : 1;
-      if (min(x, y) < 1) report(S2HIP_PAGES_ERR_REFS);
+      if (i < n) atomicAdd(refs(uint32_t(*rows(b * width + i))), 1);
+      if (i + 64 < n) atomicAdd(refs(uint32_t(*rows(b * width + i + 64))), 1);
     }
   }
   const bool grows = tid < a.R && add > 0 && (uint32_t(kept[tid]) & page_up) != 0;
   if (tid < a.R) last[tid] = grows ? *rows(tid * width + (uint32_t(kept[tid]) >> a.p.shift)) : -1;
-  __syncthreads();
+  turn_over();
   for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {  // earlier rows that grow into the same page
     uint32_t n = 0;
     for (uint32_t i = lane; i < (b + 63) / 64 * 64; i += 64) n += uint32_t(__popcll(__ballot(i < b && last[i] == last[b])));

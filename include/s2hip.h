@@ -561,7 +561,7 @@ typedef struct s2hip_pages s2hip_pages;
 #define S2HIP_PAGES_ERR_RANGE 4u    /* append: keys or values that 4 bits do not hold became no numbers */
 #define S2HIP_PAGES_ERR_PAGE 8u     /* a page of a token in use is not one of the pool */
 #define S2HIP_PAGES_ERR_FULL 16u    /* update: fewer free pages than the rows need */
-#define S2HIP_PAGES_ERR_REFS 32u    /* update, compact: refs below the rows that hold a page, or below 0 */
+#define S2HIP_PAGES_ERR_REFS 32u    /* refs below 0; update: below the rows that hold the page; compact: 0 of a page that one holds */
 
 typedef struct {
   int32_t device;

@@ -734,6 +734,46 @@ def test_update_refused(in_place):
     k.update(errors=ERR_REFS, in_place=in_place)
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("pages", [12, 20000])  # counts in a block's LDS, and in the workspace
+def test_update_counts_below_the_rows(pages, in_place):
+    """A page counted by fewer than the rows that hold it: no row takes it for its own, whatever the rows become."""
+    k = Book(4, 4, pages, layers=1)
+    k.update(add=[20, 0, 37, 0])
+    k.update(source=[0, 0, 2, 0])  # rows 0, 1 and 3 hold two pages in common, the second not full
+    first, second = k.table[0][:2]
+    assert k.refs[first] == k.refs[second] == 3
+    for page, refs in ((second, 2), (second, 1), (first, 2)):
+        short = list(k.refs)
+        short[page] = refs
+        for args in (dict(add=[1, 1, 0, 1]), dict(add=[1, 0, 0, 0]), dict(keep=[18, 99, 99, 99], add=[1, 0, 0, 0]), dict(), dict(add=[0, 0, 1, 0]),
+                     dict(source=[0, 1, 0, -1], add=[1, 1, 1, 0]), dict(source=[-1, 1, 2, 3]), dict(source=[0, -1, 2, -1], add=[1, 0, 0, 0])):
+            d, args = dict(k.d, refs=dev(short)), {x: dev(y) for x, y in args.items()}
+            before = {x: y.clone() for x, y in d.items()}
+            out = {x: (y if in_place else torch.full_like(y, 99)) for x, y in d.items()}
+            k.ops.update(k.ops.view(ptr(k.d_pool), ptr(d["table"]), ptr(d["lens"]), 4), ptr(d["refs"]), ptr(out["refs"]), ptr(out["table"]), ptr(out["lens"]),
+                         stream=stream(), **{x: ptr(y) for x, y in args.items()})
+            torch.cuda.synchronize()
+            assert k.ops.errors(stream()) == ERR_REFS, (page, refs, args)
+            assert all(torch.equal(out[x], before[x]) and torch.equal(d[x], before[x]) for x in d)
+            k.check()
+    k.update(add=[1, 1, 0, 1], in_place=in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_compact_counts_below_the_rows(in_place):
+    """Compact looks for pages that a row holds and no one counts; a count that is only too low moves with its page."""
+    k = Book(3, 4, 12)
+    k.update(add=[40, 20, 20])
+    k.update(source=[-1, 1, 1])
+    page = k.table[1][1]
+    assert page > 1 and k.refs[page] == 2
+    k.refs[page] = 1
+    k.d["refs"].copy_(dev(k.refs))
+    k.compact(in_place)
+    assert k.refs[:3] == [2, 1, 0]
+
+
 def test_update_full_to_the_last_page():
     k = Book(2, 8, 9)
     k.update(add=[128, 16, ])
