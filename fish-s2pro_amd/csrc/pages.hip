@@ -285,13 +285,18 @@ __device__ __forceinline__ void values8(Bits bits, uint32_t w, u32x2 d, half2v (
   v[2] = elements<2>(bits, w, d1, c1);
   v[3] = elements<3>(bits, w, d1, c1);
 }
+// A scale that append writes is at most 2048 by size.  One beyond that counts as no number where a row must not see it: 24 of
+// it is an infinity from 2730 on, and so are its elements, whose product with a weight of 0 is no number.
+constexpr uint32_t SCALE_MOST = 0x6800u;  // 2048
+__device__ __forceinline__ bool odd_scale(uint32_t half) { return (half & 0x7fffu) > SCALE_MOST; }
+__device__ __forceinline__ bool odd_scales(uint32_t pair) { return ((pair & 0x7fff7fffu) + 0x00010001u * (0x7fffu - SCALE_MOST)) & 0x80008000u; }
 // Of pair x of scales those of no number become 0; the first of them, or a large number.
 template <class Pairs>
 __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
   uint32_t first = 1000, pair = pairs[x];
 #pragma unroll
   for (int i = 1; i >= 0; --i)
-    if (((pair >> (16 * i)) & 0x7c00u) == 0x7c00u) {
+    if (odd_scale(pair >> (16 * i))) {
       pair &= ~(0xffffu << (16 * i));
       first = i;
     }
@@ -716,7 +721,6 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
       lds_u32* const kp = reinterpret_cast<lds_u32*>(stage + slot * TILE + KS_AT) + lane % PAIRS;
       lds_u32* const vp = reinterpret_cast<lds_u32*>(stage + slot * TILE + VS_AT) + lane % PAIRS;
       const uint32_t quad = lane % PAIRS / (2 * GR), first_token = 4 * quad + 2 * (lane & 1u);
-      auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
       uint32_t pair = *vp;
       if (w.keys < KT || w.gone) {  // scales of tokens that no row sees may hold anything: 0
         const int there = (w.gone >> (quad / 4)) & 1u ? 0 : int(w.keys) - int(first_token);
@@ -724,11 +728,11 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
         *vp = pair;
       }
       // Where the rows of its request see all of it and its keys are numbers, the other rows' weights are 0 by their bias.
-      masks = w.gone || !__all(fits && !odd(*kp));
-      if (__any(odd(pair))) {  // values of no number: 0 too; outputs of rows that see the first of them are no number
-        const uint32_t at_token = (pair & 0x7c00u) == 0x7c00u ? first_token : odd(pair) ? first_token + 1 : 1000u;
-        if ((pair & 0x7c00u) == 0x7c00u) pair &= 0xffff0000u;
-        if ((pair & 0x7c000000u) == 0x7c000000u) pair &= 0xffffu;
+      masks = w.gone || !__all(fits && !odd_scales(*kp));
+      if (__any(odd_scales(pair))) {  // values of no number: 0 too; outputs of rows that see the first of them are no number
+        const uint32_t at_token = odd_scale(pair) ? first_token : odd_scales(pair) ? first_token + 1 : 1000u;
+        if (odd_scale(pair)) pair &= 0xffff0000u;
+        if (odd_scale(pair >> 16)) pair &= 0xffffu;
         *vp = pair;
 #pragma unroll
         for (int c = 0; c < GR; ++c) {
@@ -1004,12 +1008,12 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
 #pragma unroll
       for (int c = 0; c < GR; ++c) vs[c] = u32x2{vs[c][0] & low, vs[c][1] & high};
     }
-    half2v z = half2v{};
+    float z = 0.0f;  // (their squares' sum: none is beyond 2048 where it is not beyond 2048^2, and most are far below)
 #pragma unroll
     for (int c = 0; c < GR; ++c)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) z = __builtin_elementwise_fma(as_half2(vs[c][x]), half2v{}, z);
-    if (__any(!(z[0] == _Float16(0)) || !(z[1] == _Float16(0)))) {  // of no number: 0 too, and noted
+      for (int x = 0; x < 2; ++x) z = __builtin_amdgcn_fdot2(as_half2(vs[c][x]), as_half2(vs[c][x]), z, false);
+    if (__any(!(z <= 0x1p22f))) {  // of no number: 0 too, and noted
 #pragma unroll
       for (int c = 0; c < GR; ++c)
 #pragma unroll

@@ -553,6 +553,9 @@ int32_t s2hip_kv_evict(s2hip_kv* kv, const s2hip_kv_view* view, uint32_t layers,
  * nearest to x / d (the even one of two), from -8 to 7, plus 8; d 0: all elements 0.
  * Where one of them is no number or not below 16384 by size, d is no number, and so
  * are the 32 elements.
+ * A page that the caller fills keeps to such scales: of one with more bits the
+ * elements are rounded once more, and one beyond 2048 by size may make anything of the
+ * rows that see its 32 elements (of no others).
  * ------------------------------------------------------------------------- */
 typedef struct s2hip_pages s2hip_pages;
 

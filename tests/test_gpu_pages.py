@@ -312,6 +312,32 @@ def _without(p, pool):
     return k, v
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("part", ["key", "value"])
+@pytest.mark.parametrize("room", [None, 4000])
+@pytest.mark.parametrize("n", [1, 5, 40])
+def test_attend_scales_beyond_the_format(n, room, part, hd):
+    """A finite scale that append never writes, in a slot of one request: rows that do not see it (its earlier tokens, and other
+    requests, before and behind it in a row tile) keep every bit."""
+    length, g, group = n + 40, 1, 1
+    p = Pool((8, 2, hd), 16, [length] * 3, [n] * 3, seed=n, width=room)
+    clean = p.attend().clone()
+    p.check(clean)
+    dims = slice(None) if part == "key" else slice(32 * group, 32 * group + 32)
+    for slot in (3, length - max(1, n // 2)):  # of request 1: in a tile that its rows see whole, and among the new ones
+        at = (p.lay.key_scale if part == "key" else p.lay.value_scale)[slot % 16, group]
+        hit = torch.zeros(3, n, 8, hd, dtype=torch.bool, device="cuda")
+        hit[1, max(0, slot - (length - n)) :, 4 * g : 4 * g + 4, dims] = True
+        for bits in (0x6801, 0x6955, 0x6C00, 0x7800, 0x7BFF, 0xF800, 0xE801):
+            pool = p.pool_h.copy()
+            pool[p.table_h[1][slot // 16], g, at : at + 2] = np.array([bits], np.uint16).view(np.uint8)
+            p.pool.copy_(torch.from_numpy(pool))
+            p.out.fill_(7.0)
+            out = p.attend()
+            assert torch.equal(out[~hit], clean[~hit]), (slot, hex(bits))
+    assert p.ops.errors(stream()) == 0
+
+
 @pytest.mark.parametrize("n", [3, 40])
 def test_attend_query_of_no_number(n):
     p = Pool((8, 2, 128), 16, [50, 50], [n, n], seed=9, width=2000)
