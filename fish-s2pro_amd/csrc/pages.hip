@@ -261,7 +261,14 @@ __device__ __forceinline__ half8 key8(Bits bits, uint32_t w, _Float16 d) {
   const half2v a = elements<0>(bits, w, dd, c), b = elements<1>(bits, w, dd, c), e = elements<2>(bits, w, dd, c), f = elements<3>(bits, w, dd, c);
   return half8{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
 }
-// Two weights' f16 parts and what those leave of them (f16 too: 2^-22 of the weight), both in one register each.
+// m follows a row's maximum as for the dense caches, but closer behind, and weights are 2^(s - m + LIFT), up to 2^15: the
+// largest of a row is 2^14 or more, and the lo part of a small one, of whole 2^-24, is exact to 2^-39 of it.  (Where one key
+// weighs e^16 times as much as any other and its value is 0, the output is the others': with m up to 2^8 behind and a lift of
+// 6 it was off by a thousandth.)  o is rescaled more often: slack and lift 1 14 : 4 11 : 8 6, us: 1 x 3999
+// 262.8 : 258.7 : 257.8, 8 x 250 over 1500 + 250 102.5 : 100.5 : 100.8, 16 x 1 over 32001 116.4 : 116.1 : 115.9.
+constexpr float LIFT = 14.0f, BEHIND = 1.0f;
+
+// Two weights' f16 parts and what those leave of them (f16 too: 2^-22 of the weight, or 2^-25), both in one register each.
 struct WeightParts {
   half2v hi, lo;
 };
@@ -492,7 +499,6 @@ template <int HD, bool TWO, int RG>
 __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kernel(PgAttendArgs pa, PgShare sp) {
   constexpr int ROWS = 16 * RG, KT = 32, OT = HD / 16, GR = HD / 32;  // key tile, 16 x 16 output tiles, scales of a head
   constexpr int OP = HD + 4;                          // padded row of the joined states
-  constexpr float LIFT = F16_LIFT;
   // A tile: key codes, value codes, key scales, value scales (and what the load of those leaves behind them); a wave's two, and in their place its
   // state in the end.
   constexpr uint32_t TILE = KT * HD + 1024, STAGE = 2 * TILE, K_AT = 0, V_AT = KT * HD / 2, KS_AT = KT * HD, VS_AT = KT * (HD + HD / 16);
@@ -776,7 +782,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
       float top = fmaxf(fmaxf(s[r][0][0], s[r][0][1]), s[r][0][2]), top1 = fmaxf(fmaxf(s[r][1][0], s[r][1][1]), s[r][1][2]);
       top = fmaxf(fmaxf(top, s[r][0][3]), fmaxf(top1, s[r][1][3]));
       const float mn = mine[r] ? fmaxf(m[r], quarter_max(top) * unscale[r]) : m[r];
-      const bool up = mn > m[r] + SLACK;
+      const bool up = mn > m[r] + BEHIND;
       if (__any(up)) {
         const float to = up ? floorf(mn) : m[r], f = up ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
 #pragma unroll
@@ -911,7 +917,6 @@ template <int HD>
 __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShare sp) {
   constexpr int KT = 64, GR = HD / 32, DS = HD / 16, DT = HD / 32;
   constexpr uint32_t RB = HD * 2, PLANE = KT * RB, BUF = 2 * PLANE;  // bytes of a key's row, of the keys (and of the values), of both
-  constexpr float LIFT = F16_LIFT;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
   // of tiles i, i + 1 and the one behind: bit w: the 16 keys of wave w lie in no page, bit 8: there are values of no number; a
   // group's first
@@ -1165,7 +1170,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       }
       top = fmaxf(top, top1) * unscale;
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
-      const bool up = mn > m + SLACK;
+      const bool up = mn > m + BEHIND;
       if (__any(up)) {
         const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
 #pragma unroll

@@ -640,7 +640,9 @@ int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, con
  * of the pool is not read: its tokens are not seen (a row that sees none is no
  * number).  Steps and short turns read pages that requests have in common once for
  * several of them.
- * Products and sums are f32 or better. */
+ * Queries and weights are taken as two f16 parts: exact to 2^-22, or to 2^-38 of the
+ * largest element of the query and 2^-39 of the largest weight of the row.  Sums are
+ * f32. */
 int32_t s2hip_pages_attend(s2hip_pages* pages, const s2hip_pages_view* view, const float* q, uint32_t n_tokens,
                            float* out, void* stream, char* err, size_t err_cap);
 /* The rows made anew, all at once: row b becomes the first keep[b] tokens (all, where it

@@ -402,6 +402,32 @@ def test_attend_scales(scale, n):
     p.check_all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("room", [None, 4000])
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("gap", [8, 12, 16, 20, 24])
+def test_attend_sink(gap, n, room, hd):
+    """A first key that outweighs all others together and whose value is 0: the output is the others', whose weights are far
+    below the row's largest.  Beside the bounds of sums in f32, a weight is held to 2^-22 of itself or 2^-39 of the largest of
+    its row (two f16 parts, the largest at 2^14 or above, half a step of the least f16 numbers 2^-25)."""
+    p = Pool((8, 2, hd), 16, [n + 1000, n + 90, n + 1], [n] * 3, seed=gap + n, width=room)
+    sign = np.where(np.random.default_rng(gap).random(hd) < 0.5, -7, 7)
+    pool = p.pool_h.copy()
+    for row in p.table_h:
+        for g in range(2):
+            p.lay.write(pool[row[0], g], 0, (sign + 8, np.ones(hd // 32)), (np.full(hd, 8), np.zeros(hd // 32)))
+    p.pool.copy_(torch.from_numpy(pool))
+    p.q.mul_(0.1).add_(torch.as_tensor(sign, device="cuda") * (gap / 49 / math.sqrt(hd)))
+    out = p.attend()
+    k, v = p.dense()
+    ref, tol = kv_util.attend(p.q, k, v, p.lens_h, p.new_h)[:2]
+    for b in range(3):
+        upto = v[b].abs().cumsum(1)[:, p.lens_h[b] - n : p.lens_h[b]]  # [G][n][hd]: of the values that a token sees
+        tol[b] += 2.0**-39 * upto.transpose(0, 1).repeat_interleave(4, 1)
+    p.check(out, (ref, tol))
+    assert p.ops.errors(stream()) == 0
+
+
 def test_attend_offsets_beyond_32_bits():
     """Pages that lie more than 4 GiB into the pool."""
     page, hd, G = 128, 128, 8
