@@ -35,6 +35,30 @@ void apart(const Words (&all)[N]) {
     for (size_t j = i + 1; j < N; ++j) apart(all[i], all[j]);
 }
 
+// An output that shares a word with an input.
+template <size_t N, size_t M>
+void outputs_apart(const Words (&outputs)[N], const Words (&inputs)[M]) {
+  for (const Words& out : outputs)
+    for (const Words& in : inputs) apart(in, out);
+}
+// A pool in every layer; what lies between the layers is the caller's.
+struct Layers {
+  const void* p;
+  uint64_t bytes, stride;
+  uint32_t n;
+};
+void pools_apart(const Layers& pools, const Words& x) {
+  if (!x.p) return;
+  const uint64_t base = reinterpret_cast<uintptr_t>(pools.p), at = reinterpret_cast<uintptr_t>(x.p), end = at + 4 * uint64_t(x.words);
+  // the first layer that ends behind the array's beginning
+  const uint64_t first = at < base + pools.bytes ? 0 : (at - base - pools.bytes) / pools.stride + 1;
+  if (first < pools.n && base + first * pools.stride < end) kfail("kv: %s overlaps pool", x.name);
+}
+template <size_t N>
+void pools_apart(const Layers& pools, const Words (&all)[N]) {
+  for (const Words& x : all) pools_apart(pools, x);
+}
+
 class Pages : DeviceArrays {
  public:
   explicit Pages(const s2hip_pages_config& c) {
@@ -127,6 +151,13 @@ class Pages : DeviceArrays {
     may(v_held, "v_held", 16);
     const size_t rows = size_t(v.requests) * n, q = rows * cfg_.heads * cfg_.head_dim, kv = rows * cfg_.kv_heads * cfg_.head_dim;
     apart({{qkv, q + 2 * kv, "qkv"}, {q_out, q, "q_out"}, {k_held, kv, "k_held"}, {v_held, kv, "v_held"}});
+    const Words outputs[] = {{q_out, q, "q_out"}, {k_held, kv, "k_held"}, {v_held, kv, "v_held"}};
+    const Words inputs[] = {{positions, rows, "positions"}, {qn, cfg_.head_dim, "q_norm"}, {kn, cfg_.head_dim, "k_norm"}, {v.table, table_words(v), "table"},
+                            {v.lens, v.requests, "lens"}, {v.new_lens, v.requests, "new_lens"}};
+    outputs_apart(outputs, inputs);
+    pools_apart(one_pool(v), outputs);
+    pools_apart(one_pool(v), inputs);
+    pools_apart(one_pool(v), Words{qkv, q + 2 * kv, "qkv"});
     a.s = shape_;
     a.rope = rope_;
     a.qkv = qkv;
@@ -148,6 +179,9 @@ class Pages : DeviceArrays {
     need(out, "out", 16);
     const size_t words = size_t(v.requests) * n * cfg_.heads * cfg_.head_dim;
     if (meet(q, words, out, words)) kfail("kv: out overlaps q");
+    const Words outputs[] = {{out, words, "out"}};
+    outputs_apart(outputs, {{v.table, table_words(v), "table"}, {v.lens, v.requests, "lens"}, {v.new_lens, v.requests, "new_lens"}});
+    pools_apart(one_pool(v), outputs);
     a.a.s = shape_;
     a.a.q = q;
     a.a.out = out;
@@ -170,6 +204,8 @@ class Pages : DeviceArrays {
       for (const Words& in : {Words{source, R, "source"}, Words{keep, R, "keep"}, Words{add, R, "add"}, Words{out.p == refs_out ? nullptr : refs, P, "refs"},
                               Words{out.p == table_out ? nullptr : v.table, T, "table"}, Words{out.p == lens_out ? nullptr : v.lens, R, "lens"}})
         apart(in, out);
+    pools_apart({v.pool, bytes() * P, a.layer_stride, layers},
+                {r, t, l, {source, R, "source"}, {keep, R, "keep"}, {add, R, "add"}, {refs, P, "refs"}, {v.table, T, "table"}, {v.lens, R, "lens"}});
     a.source = source;
     a.keep = keep;
     a.add = add;
@@ -189,6 +225,7 @@ class Pages : DeviceArrays {
     for (const Words& out : {r, t, u, m})
       for (const Words& in : {Words{out.p == refs_out ? nullptr : refs, P, "refs"}, Words{out.p == table_out ? nullptr : v.table, T, "table"}, Words{v.lens, R, "lens"}})
         apart(in, out);
+    pools_apart({v.pool, bytes() * P, a.layer_stride, layers}, {r, t, u, m, {refs, P, "refs"}, {v.table, T, "table"}, {v.lens, R, "lens"}});
     a.used_out = used_out;
     a.moved_to = moved_to;
     DeviceScope on(cfg_.device);
@@ -204,6 +241,9 @@ class Pages : DeviceArrays {
     need(v.lens, "lens", 4);
     return {static_cast<uint8_t*>(v.pool), v.table, shift_, cfg_.pages, cfg_.table_pages, chunk_};
   }
+
+  size_t table_words(const s2hip_pages_view& v) const { return size_t(v.requests) * cfg_.table_pages; }
+  Layers one_pool(const s2hip_pages_view& v) const { return {v.pool, bytes() * cfg_.pages, bytes() * cfg_.pages, 1}; }
 
   KvCaches tokens(const s2hip_pages_view& v, uint32_t n) const {
     if (n == 0 || uint64_t(v.requests) * n > cfg_.max_tokens)

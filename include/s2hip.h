@@ -633,7 +633,7 @@ int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, con
 /* Attention of the new tokens' queries q [requests][n_tokens][heads head_dim]:
  * token t of request b sees its request's slots 0 .. lens[b] - new_lens[b] + t; query
  * head h reads kv head h / (heads / kv_heads).  out like q; rows of tokens t >=
- * new_lens[b] stay as they were, out must not overlap q.  What a token does not see
+ * new_lens[b] stay as they were; out must not overlap an input.  What a token does not see
  * never reaches its row, whatever bits stand there.  A value that it sees and that is
  * no number makes that element of its row no number, a key all of them; so do a query
  * of no number and scores that are all below the range of f32.  A page that is not one
@@ -655,7 +655,8 @@ int32_t s2hip_pages_attend(s2hip_pages* pages, const s2hip_pages_view* view, con
  *   refs_out counts the new rows in place of the old.  Pages that no row holds any more
  * are free at once; the lowest free ones go to the rows in order, a copy's before the
  * slots behind it.  table_out [requests][table_pages] (-1 behind the pages in use),
- * lens_out; each array out is its array in or shares nothing with it.  Where a value is
+ * lens_out; each array out is its array in or shares nothing with it, and none shares
+ * anything with another array or with the pools.  Where a value is
  * out of range, refs do not fit, or too few pages are free, nothing changes (each array
  * out is as its array in) and the error bits say why.  view->new_lens is not looked at. */
 int32_t s2hip_pages_update(s2hip_pages* pages, const s2hip_pages_view* view, uint32_t layers, uint64_t layer_stride,

@@ -1214,6 +1214,61 @@ def test_calls_refused():
     p.check(p.attend())
 
 
+def test_overlaps_refused():
+    """Every output against every array of its call, by its last and its first word; and apart by none it goes."""
+    H, G, hd, page, pages, width, R, n = 4, 2, 64, 16, 6, 3, 2, 2
+    ops = PagedKv(H, G, hd, page, pages, width, max_requests=R, max_tokens=R * n)
+    rows, pool = R * n, pages * ops.page_bytes
+    base = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    spare = [ptr(base) + 65536 * (i + 4) for i in range(12)]  # the pool lies in front of them
+
+    up = lambda x: -(-x // 16) * 16  # noqa: E731
+
+    def check(call, sizes, outputs, same=()):
+        """call(addresses): arrays of `sizes` bytes by name; those of `outputs` share nothing with the others but for the pairs `same`."""
+        where = dict(zip(sizes, spare), pool=ptr(base))
+        call(where)
+        for out in outputs:
+            for other in sizes:
+                if out == other or (other, out) in same:
+                    continue
+                for at in (where[other] + up(1 - sizes[out]), where[other] + (sizes[other] - 4) // 16 * 16):
+                    if at >= ptr(base):
+                        with pytest.raises(S2HipError, match="overlap"):
+                            call(dict(where, **{out: at}))
+                for at in (where[other] - up(sizes[out]), where[other] + up(sizes[other])):
+                    if at >= ptr(base) and out != "pool":
+                        call(dict(where, **{out: at}))
+
+    def view(w):
+        return ops.view(w["pool"], w["table"], w["lens"], R, new_lens=w.get("new_lens", 0))
+
+    q, kv = rows * H * hd * 4, rows * G * hd * 4
+    batch = dict(table=R * width * 4, lens=4 * R, new_lens=4 * R, pool=pool)
+    check(lambda w: ops.append(view(w), w["qkv"], n, w["positions"], w["q_out"], q_norm=w["q_norm"], k_norm=w["k_norm"], k_held=w["k_held"], v_held=w["v_held"], stream=stream()),
+          dict(batch, qkv=q + 2 * kv, positions=rows * 4, q_norm=hd * 4, k_norm=hd * 4, q_out=q, k_held=kv, v_held=kv), ["q_out", "k_held", "v_held", "pool"])
+    check(lambda w: ops.attend(view(w), w["q"], n, w["out"], stream=stream()), dict(batch, q=q, out=q), ["out"])
+    batch = dict(table=R * width * 4, lens=4 * R, pool=pool, refs=4 * pages, refs_out=4 * pages, table_out=R * width * 4)
+    check(lambda w: ops.update(view(w), w["refs"], w["refs_out"], w["table_out"], w["lens_out"], source=w["source"], keep=w["keep"], add=w["add"], stream=stream()),
+          dict(batch, lens_out=4 * R, source=4 * R, keep=4 * R, add=4 * R), ["refs_out", "table_out", "lens_out", "pool"], [("lens", "lens_out")])
+    check(lambda w: ops.compact(view(w), w["refs"], w["refs_out"], w["table_out"], w["used_out"], moved_to=w["moved_to"], stream=stream()),
+          dict(batch, used_out=4, moved_to=4 * pages), ["refs_out", "table_out", "used_out", "moved_to", "pool"])
+    # layers apart: what lies between them is the caller's, what lies in one is not
+    where = dict(zip(("table", "lens", "refs"), spare), pool=ptr(base))
+    gap = up(pool)
+
+    def grow(refs_out):
+        ops.update(ops.view(where["pool"], where["table"], where["lens"], R), where["refs"], refs_out, spare[8], spare[9], layers=3, layer_stride=gap + 1024, stream=stream())
+
+    for at in (gap, gap + 1024 - 4 * pages, 2 * gap + 1024, 3 * gap + 2048):
+        grow(ptr(base) + at)
+    for at in (0, gap - 4, gap + 1024 - 4, gap + 1024, 2 * gap + 1020, 2 * gap + 2048 - 4 * pages + 4, 3 * gap + 2044):
+        with pytest.raises(S2HipError, match="refs_out overlaps pool"):
+            grow(ptr(base) + at)
+    torch.cuda.synchronize()
+    ops.errors(stream())
+
+
 def test_errors_refused_under_capture():
     p = Pool((8, 2, 64), 16, [9], [1], seed=5)
     side = torch.cuda.Stream()
