@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     const double angle = double(pos) * per_token;
     double sn, cs;
     sincospi(2.0 * (angle - rint(angle)), &sn, &cs);
-    turn[tid] = tid < half ? make_double2(cs * a.rope.gain, sn * a.rope.gain) : make_double2(1.0, 0.0);
+    turn[tid] = make_double2(cs * a.rope.gain, sn * a.rope.gain);
   }
   if (brings) *reinterpret_cast<float4*>(&gains[0][4 * tid]) = gain4;
   __syncthreads();
@@ -98,7 +98,6 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
 #pragma unroll
   for (int i = 0; i < PAIRS; ++i) {
     cs[i] = turn[HALF ? (second ? d0 - half + i : d0 + i) % (HD / 2) : d0 / 2 + i];
-    if (HALF && !turns) cs[i] = make_double2(1.0, 0.0);
     if (second) cs[i].y = -cs[i].y;  // the second of a pair takes the first's times sin, the first the second's times -sin
   }
   for (uint32_t h = h0; h < heads;) {  // whole rows of LP lanes take part
@@ -136,12 +135,15 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
       }
 #pragma unroll
       for (int e = 0; e < (HALF ? 8 : 4); ++e) {
+        // (dims that do not turn go past it: 0 times an infinity beside them is no number)
         if constexpr (HALF) {
-          y[e] = (y[e] * cs[e].x - w[e] * cs[e].y) * f;
+          const double r = y[e] * cs[e].x - w[e] * cs[e].y;
+          y[e] = (turns ? r : y[e]) * f;
         } else {
-          const double p = y[2 * e], q = y[2 * e + 1];
-          y[2 * e] = (p * cs[e].x - q * cs[e].y) * f;
-          y[2 * e + 1] = (p * cs[e].y + q * cs[e].x) * f;
+          const double p = y[2 * e], q = y[2 * e + 1], r0 = p * cs[e].x - q * cs[e].y, r1 = p * cs[e].y + q * cs[e].x;
+          const bool turned = d0 + 2 * e < a.rope.dims;
+          y[2 * e] = (turned ? r0 : p) * f;
+          y[2 * e + 1] = (turned ? r1 : q) * f;
         }
       }
     }

@@ -552,6 +552,26 @@ def test_append_few_dims(dims):
     a.check()
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("dims,hd", [(16, 64), (32, 128), (64, 128), (128, 128)])
+def test_append_infinities_beside_dims_that_do_not_turn(dims, hd, half):
+    """The rest of a head is as it is, whatever stands in the other dims and in itself."""
+    a = Append((4, 2, hd), 16, [5, 30], [5, 2], dims=dims, half=half, norms=False, seed=dims)
+    for t in range(2):
+        a.qkv[:, t, 0, hd - 2 :] = torch.tensor([[math.inf, 1.5], [-2.0, -math.inf]], device="cuda")[t]
+        a.qkv[:, t, 1, hd - 8 :: 3] = math.nan
+        a.qkv[:, t, 2, min(dims, hd - 1)] = -math.inf
+        a.qkv[:, t, 3, t] = math.inf
+    a.run()
+    x = a.qkv.cpu()[:, :, :4]
+    want = pages_util.rotated(x, a.pos.cpu(), None, dims, half, a.freq, a.mult, 0.0).float()
+    for b, new in enumerate(a.pool.new_h):
+        got = a.q[b, :new].cpu()
+        assert np.array_equal(got[..., dims:].numpy(), x[b, :new, :, dims:].numpy(), equal_nan=True)
+        assert torch.equal(got.isnan(), want[b, :new].isnan()) and torch.equal(got.isinf(), want[b, :new].isinf())
+    assert a.pool.ops.errors(stream()) == 0  # (no key and no value of no number)
+
+
 def test_append_without_norms_or_held():
     a = Append((8, 2, 128), 32, [9, 70], [9, 40], norms=False, held=False, seed=3)
     a.run()
