@@ -111,9 +111,8 @@ class Pages : DeviceArrays {
     CHK(hipMemset(shape_.err, 0, 2 * sizeof(uint32_t)));
     while ((1u << shift_) < c.page_tokens) ++shift_;
     chunk_ = c.page_tokens * (c.head_dim + c.head_dim / 8);
-    work_.cap_parts = 8192;
-    work_.part = alloc<float>(work_.cap_parts * 16 * c.head_dim);
-    work_.part_ml = alloc<float>(work_.cap_parts * 16 * 2);
+    work_.part = alloc<float>(size_t(PG_STATES) * 16 * c.head_dim);
+    work_.part_ml = alloc<float>(size_t(PG_STATES) * 16 * 2);
     work_.ranges = alloc<uint2>(64);
     work_.refs = alloc<int32_t>(c.pages);
     work_.list = alloc<int32_t>(size_t(c.pages) * 2);

@@ -74,10 +74,14 @@ struct PgUpdateArgs {
   uint32_t* err;
 };
 
+// Blocks that an attention in several splits is shared out to, and the 16-row states that they leave, at most: the tile kernel's
+// 8 each (128 rows), the step kernel's 1 or 2.  (Calls of more row tiles have one split, and no states.)
+constexpr uint32_t PG_TILE_BLOCKS = 512, PG_STEP_BLOCKS = 768, PG_STATES = 8 * PG_TILE_BLOCKS;
+static_assert(PG_STATES >= 2 * PG_STEP_BLOCKS, "the step kernel's states fit");
+
 struct PgWorkspace {
-  float* part;     // [cap_parts][16][hd]: attention states
-  float* part_ml;  // [cap_parts][16][2]
-  size_t cap_parts;
+  float* part;     // [PG_STATES][16][hd]: attention states
+  float* part_ml;  // [PG_STATES][16][2]
   uint2* ranges;   // [64]: a row tile's states
   int32_t* refs;   // [pages]
   int32_t* list;   // [2][pages]: free pages; holes and movers

@@ -1813,7 +1813,7 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   // 17 : 21, 16 x 1 over 1000 (5) 17 : 18 : 21, 1 x 1 over 30000 (7) 21 : 20 : 22, 16 x 1 over 6000 (24) 44 : 35 : 34, over
   // 32001 (126) 202 : 127 : 120.
   const size_t walk = size_t(lots) * most / 1024;
-  const uint32_t fill = many || (walk >= 6 && walk < 24) ? 512 : walk < 6 ? 256 : 768;
+  const uint32_t fill = many ? PG_TILE_BLOCKS : walk < 6 ? 256 : walk < 24 ? 512 : PG_STEP_BLOCKS;
   // (the tile kernel's: 8 key tiles each on average, or their states cost more than they save: 1 x 1000 in 1 : 2 46 : 54, 1 x 100
   // over 4000 in 4 : 8 : 16 50 : 38 : 42)
   uint32_t splits = max(1u, min(fill / lots, many ? (a.c.cap - min(a.c.n, a.c.cap) / 2) / (8 * kt) : (most + STEP_WAVES - 1) / STEP_WAVES));
@@ -1821,7 +1821,7 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   // heads of 64, 18 8.3 : 8.4, 26 10.1 : 8.4).
   if (!many && most <= (hd == 64 ? 24u : 16u)) splits = 1;
   const size_t parts = size_t(a.s.G) * sp.tiles << (sp.shift - 4);  // (16 rows each)
-  if (parts * splits > w.cap_parts) splits = uint32_t(max(size_t(1), w.cap_parts / parts));
+  if (splits > 1 && parts * splits > PG_STATES) return hipErrorInvalidValue;  // (lots splits is at most fill)
   sp.blocks = sp.tiles * splits;
   sp.each = splits;
   sp.by_each = Div::by(splits);

@@ -454,6 +454,23 @@ def test_attend_offsets_beyond_32_bits():
     assert ops.errors(stream()) == 0
 
 
+@pytest.mark.parametrize("shape,n", [((64, 1, 64), 2), ((4, 4, 128), 100), ((64, 1, 64), 1), ((8, 1, 128), 3)])
+def test_attend_most_states(shape, n):
+    """Tables of 2^20 slots, runs far shorter: as many splits of a row tile, and states, as a call has."""
+    Pool(shape, 128, [3000 + n], [n], seed=n, width=8192).check_all()
+
+
+def test_memory_of_a_handle():
+    """What a handle keeps at head dim 128: no more attention states than calls leave."""
+    torch.cuda.synchronize()
+    PagedKv(8, 2, 128, 16, 10, 4, max_requests=1).close()  # (what the runtime takes with the first)
+    before = torch.cuda.mem_get_info()[0]
+    ops = PagedKv(8, 2, 128, 16, 10, 4, max_requests=1)
+    taken = before - torch.cuda.mem_get_info()[0]
+    ops.close()
+    assert taken <= 40 << 20, taken  # 4096 states of 16 rows of 130 numbers are 32.5 MiB, the rest below 10 KB in arrays of their own
+
+
 def test_attend_most_tokens():
     """The most tokens of a call, 4 M packed rows; a few of them against 64 bits."""
     n, page, hd = 32768, 128, 64
