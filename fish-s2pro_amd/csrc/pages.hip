@@ -1460,14 +1460,15 @@ __device__ __forceinline__ void copy_pages(const PgUpdateArgs& a, const int32_t*
 // first r - 1 write to copies: the last writes in place if no one else holds it.
 //   All latency: two loads one after the other (the rows' lengths, their pages), a few turns over LDS, the stores; sixteen
 // waves share four vector units, so each instruction of a turn counts (64 rows of 102 pages 13 us, 16 of 32 pages 8, of a
-// pool of 7000).  FITS: counts, free pages and new rows are in LDS; else in the workspace, where each turn is a trip to the
-// second-level cache (64 rows of 102 pages of a pool of 15800, which fits, 14.5 us; of 15900, which does not, 21).
+// pool of 7000).  FITS: counts, free pages and new rows are in LDS.  COUNTS: the counts alone, the rest in the workspace (64
+// rows of 32 pages, tables of 512, in a pool of 20000: 19 us; the counts there too, 32).  Else each turn is a trip to the
+// second-level cache (64 rows of 102 pages of a pool of 38400, the most for COUNTS, 20 us, of 38401 36).
 //   MOVES (arrays out apart from those in): every block works it all out for itself, the first writes it down, and all of
 // them copy pages: one launch (16 rows 8.5 us; in place, with a second launch that copies, 9.3, and the caller's own 2.7 for
 // it).  64 rows that each copy a page in 36 layers: 31 us, 122 MB in 18 of them.
 constexpr uint32_t ROWS_LDS = 150 * 1024;  // bytes: counts, free pages, rows
 
-template <bool FITS, bool MOVES>
+template <bool COUNTS, bool FITS, bool MOVES>
 __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a, PgWorkspace w, uint32_t bytes) {
   extern __shared__ int32_t dyn[];
   __shared__ int32_t source[MAX_ROWS], lens[MAX_ROWS], kept[MAX_ROWS], total[MAX_ROWS], last[MAX_ROWS], before[MAX_ROWS];
@@ -1476,7 +1477,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), width = a.p.width, page_up = (1u << a.p.shift) - 1u;
   const int64_t cap = int64_t(width) << a.p.shift;
   auto refs = [&](uint32_t p) -> int32_t* {
-    if constexpr (FITS) return dyn + p;
+    if constexpr (COUNTS) return dyn + p;
     return w.refs + p;
   };
   auto list = [&](uint32_t i) -> int32_t* {
@@ -1488,7 +1489,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     return w.table + x;
   };
   auto count = [&](uint32_t p) {  // now, with what others have added
-    if constexpr (FITS) return *refs(p);
+    if constexpr (COUNTS) return *refs(p);
     return load_now(refs(p));
   };
   auto pages_of = [&](int32_t n) { return (uint32_t(n) + page_up) >> a.p.shift; };
@@ -1544,19 +1545,57 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
         const uint32_t i = i0 + 64 * k + lane;
         const bool in = uint32_t(e[k]) < a.p.pages && uint32_t(v[k]) < a.p.pages;
         if (!in) report(S2HIP_PAGES_ERR_PAGE);
-        if (in && i < n_old && atomicSub(refs(uint32_t(e[k])), 1) < 1) report(S2HIP_PAGES_ERR_REFS);
+        if (COUNTS && in && i < n_old && atomicSub(refs(uint32_t(e[k])), 1) < 1) report(S2HIP_PAGES_ERR_REFS);
         if (i < n_base) *rows(b * width + i) = v[k];
       }
     }
   }
   if (stops()) return;
-  for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
-    const uint32_t n = uniform(pages_of(kept[b]));
-    for (uint32_t i0 = 0; i0 < n; i0 += 128) {
-      const uint32_t i = i0 + lane;
-      if (i < n) atomicAdd(refs(uint32_t(*rows(b * width + i))), 1);
-      if (i + 64 < n) atomicAdd(refs(uint32_t(*rows(b * width + i + 64))), 1);
+  if constexpr (COUNTS) {
+    for (uint32_t b = wave; b < a.R; b += ROWS_THREADS / 64) {
+      const uint32_t n = uniform(pages_of(kept[b]));
+      for (uint32_t i0 = 0; i0 < n; i0 += 128) {
+        const uint32_t i = i0 + lane;
+        if (i < n) atomicAdd(refs(uint32_t(*rows(b * width + i))), 1);
+        if (i + 64 < n) atomicAdd(refs(uint32_t(*rows(b * width + i + 64))), 1);
+      }
     }
+  } else {
+    // f(page, how many) of the entries table[b][i], i below the pages of n[b] tokens: a lane takes a column of the wave's rows,
+    // and those that have a page in common there, as rows that begin alike do, are one change of its count.  (One change
+    // each, 64 rows with 93 pages in common made anew in a pool of 38401: 47 us, so 36.)
+    auto by_columns = [&](const int32_t* table, const int32_t* n, auto&& f) {
+      constexpr uint32_t WAVES = ROWS_THREADS / 64;
+      uint32_t most = 0;
+      for (uint32_t b = wave; b < a.R; b += WAVES) most = max(most, uniform(pages_of(n[b])));
+      for (uint32_t i0 = 0; i0 < most; i0 += 64) {
+        const uint32_t i = i0 + lane;
+        int32_t page = -1, count = 0;
+        for (uint32_t b0 = wave; b0 < a.R; b0 += 4 * WAVES) {
+          int32_t e[4];
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {
+            const uint32_t b = b0 + k * WAVES;
+            e[k] = b < a.R && i < uniform(pages_of(n[min(b, a.R - 1)])) ? table[size_t(b) * width + i] : -1;
+          }
+#pragma unroll
+          for (uint32_t k = 0; k < 4; ++k) {
+            if (e[k] != page) {
+              if (page >= 0) f(uint32_t(page), count);
+              page = e[k];
+              count = 0;
+            }
+            ++count;
+          }
+        }
+        if (page >= 0) f(uint32_t(page), count);
+      }
+    };
+    by_columns(a.p.table, lens, [&](uint32_t p, int32_t n) {
+      if (atomicSub(refs(p), n) < n) report(S2HIP_PAGES_ERR_REFS);
+    });
+    if (stops()) return;
+    by_columns(w.table, kept, [&](uint32_t p, int32_t n) { atomicAdd(refs(p), n); });
   }
   const bool grows = tid < a.R && add > 0 && (uint32_t(kept[tid]) & page_up) != 0;
   if (tid < a.R) last[tid] = grows ? *rows(tid * width + (uint32_t(kept[tid]) >> a.p.shift)) : -1;
@@ -1577,7 +1616,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
   const uint32_t begin = block_scan(needs, all);
   if (tid < a.R) offset[tid] = begin;
   // the free pages: each wave counts those of a run of pages, then says which they are
-  if constexpr (!FITS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (plain loads of what atomics have changed)
+  if constexpr (!COUNTS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");  // (plain loads of what atomics have changed)
   uint32_t mine = 0;
   bool below = false;
   by_waves(refs(0), a.p.pages, 1, [&](uint32_t, int32_t r) {
@@ -1623,7 +1662,7 @@ __global__ __launch_bounds__(ROWS_THREADS) void pg_update_kernel(PgUpdateArgs a,
     for (uint32_t i = lane; i < width; i += 64) a.table_out[size_t(b) * width + i] = i < from ? *rows(b * width + i) : i < n ? *list(at + i - from) : -1;
   }
   turn_over();
-  if constexpr (!FITS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  if constexpr (!COUNTS) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
   each_page(refs(0), a.p.pages, [&](uint32_t p, auto x) { store_counts(a.refs_out + p, x); });
 }
 
@@ -1864,10 +1903,10 @@ static bool meets(const void* p, const void* q, size_t n) {
 
 // Once per device, before the launches there.
 hipError_t prepare_pg() {
-  static std::atomic<uint64_t> devices[3];
-  const void* kernels[3] = {reinterpret_cast<const void*>(pg_update_kernel<true, true>), reinterpret_cast<const void*>(pg_update_kernel<true, false>),
-                            reinterpret_cast<const void*>(pg_pack_kernel<true>)};
-  for (int i = 0; i < 3; ++i) {
+  static std::atomic<uint64_t> devices[4];
+  const void* kernels[4] = {reinterpret_cast<const void*>(pg_update_kernel<true, true, true>), reinterpret_cast<const void*>(pg_update_kernel<true, true, false>),
+                            reinterpret_cast<const void*>(pg_update_kernel<true, false, false>), reinterpret_cast<const void*>(pg_pack_kernel<true>)};
+  for (int i = 0; i < 4; ++i) {
     const hipError_t e = allow_lds(kernels[i], ROWS_LDS, devices[i]);
     if (e != hipSuccess) return e;
   }
@@ -1884,9 +1923,11 @@ static hipError_t launch_rows(K kernel, uint32_t blocks, size_t lds, hipStream_t
 hipError_t launch_pg_update(const PgUpdateArgs& a, const PgWorkspace& w, uint32_t page_bytes, hipStream_t s) {
   const size_t words = size_t(a.R) * a.p.width, lds = (2 * size_t(a.p.pages) + words) * 4;
   const bool fits = lds <= ROWS_LDS, in_place = meets(a.refs, a.refs_out, a.p.pages) || meets(a.p.table, a.table_out, words) || meets(a.lens, a.lens_out, a.R);
-  if (fits && !in_place) return launch_rows(pg_update_kernel<true, true>, 256, lds, s, a, w, page_bytes);
-  const hipError_t e = fits ? launch_rows(pg_update_kernel<true, false>, 1, lds, s, a, w, page_bytes)
-                            : launch_rows(pg_update_kernel<false, false>, 1, 0, s, a, w, page_bytes);
+  if (fits && !in_place) return launch_rows(pg_update_kernel<true, true, true>, 256, lds, s, a, w, page_bytes);
+  const size_t counts = size_t(a.p.pages) * 4;
+  const hipError_t e = fits                 ? launch_rows(pg_update_kernel<true, true, false>, 1, lds, s, a, w, page_bytes)
+                       : counts <= ROWS_LDS ? launch_rows(pg_update_kernel<true, false, false>, 1, counts, s, a, w, page_bytes)
+                                            : launch_rows(pg_update_kernel<false, false, false>, 1, 0, s, a, w, page_bytes);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(pg_copy_kernel, dim3((page_bytes + 16383) / 16384, a.R, a.layers), dim3(256), 0, s, a, w.moves, page_bytes);
   return hipGetLastError();

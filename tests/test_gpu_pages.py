@@ -788,6 +788,12 @@ def test_update_and_compact_at_random(seed, pages, in_place):
 
 
 @pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("seed", range(2))
+def test_update_and_compact_counts_beyond_lds(seed, in_place):
+    test_update_and_compact_at_random(seed, 40000, in_place)
+
+
+@pytest.mark.parametrize("in_place", [True, False])
 def test_update_refused(in_place):
     """Whatever is wrong: nothing changes."""
     k = Book(3, 4, 9)
@@ -824,7 +830,7 @@ def test_update_refused(in_place):
 
 
 @pytest.mark.parametrize("in_place", [True, False])
-@pytest.mark.parametrize("pages", [12, 20000])  # counts in a block's LDS, and in the workspace
+@pytest.mark.parametrize("pages", [12, 20000, 40000])  # all in a block's LDS, the counts alone, nothing
 def test_update_counts_below_the_rows(pages, in_place):
     """A page counted by fewer than the rows that hold it: no row takes it for its own, whatever the rows become."""
     k = Book(4, 4, pages, layers=1)
