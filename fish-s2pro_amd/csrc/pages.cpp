@@ -51,7 +51,7 @@ void pools_apart(const Layers& pools, const Words& x) {
   if (!x.p) return;
   const uint64_t base = reinterpret_cast<uintptr_t>(pools.p), at = reinterpret_cast<uintptr_t>(x.p), end = at + 4 * uint64_t(x.words);
   // the first layer that ends behind the array's beginning
-  const uint64_t first = at < base + pools.bytes ? 0 : (at - base - pools.bytes) / pools.stride + 1;
+  const uint64_t first = at < base + pools.bytes ? 0 : pools.n == 1 ? 1 : (at - base - pools.bytes) / pools.stride + 1;
   if (first < pools.n && base + first * pools.stride < end) kfail("kv: %s overlaps pool", x.name);
 }
 template <size_t N>

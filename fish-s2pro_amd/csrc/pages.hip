@@ -184,8 +184,9 @@ __global__ __launch_bounds__(256) void pg_append_kernel(PgAppendArgs a) {
     }
     const double size = rounded8(big * 0.125), d = negative ? size : -size;
     const double inv = odd || size == 0.0 ? 0.0 : 1.0 / d;
-    // y / d is y inv but for 2^-52 of it.  It is at most 8 2^9 / (2^9 - 1): taken to a multiple of 2^-40 first, one that is
-    // halfway between whole numbers is so again (no other quotient of a value's 24 bits by 8 comes so near).  Then to a whole
+    // y / d is y inv but for 2^-52 of it.  It is at most 8 2^9 / (2^9 - 1), and below 12 where d is a few times 2^-24 and rounded
+    // by up to a third (a code of 8 and more is 7 then).  Beside 1.5 2^12 it is taken to a multiple of 2^-40: one that is halfway
+    // between whole numbers is so again (no other quotient of a value's 24 bits by 8 comes nearer than 2^-25).  Then to a whole
     // number, ties to even, which stands in the low bits of the sum with 1.5 2^52.
     int code[8];  // less 8
 #pragma unroll
@@ -323,8 +324,8 @@ __device__ __forceinline__ uint32_t take_odd_scales(Pairs& pairs, int x) {
 // of each 16, as the weights stand in the registers): both go from memory to operands
 // with no exchange.
 //   Vector instructions bound it: 4 bits become f16 numbers, and a weight two of them, at one
-// issue of four units (16 x 1 over 32001 slots: 105 us for 450 MB, 4.3 TB/s, vector units 60 %
-// busy, matrix units 19 %; its loads alone take 97).  Short runs are latency: of 10 us of 8 x 1
+// issue of four units (16 x 1 over 32001 slots: 105 to 116 us by the card for 450 MB, 3.9 to 4.3 TB/s, vector units 59 %
+// busy, matrix units 19 %; its loads alone took 97 on the quickest).  Short runs are latency: of 10 us of 8 x 1
 // over 1500 + 512, 2.5 go before the first load of a page (lengths, tables, queries), 1 in it, 1 to
 // a tile (a wave alone on its unit issues every fifth cycle), 1 at the end, and 3.5 in the join.
 //   The run: first the tiles that all requests of the rows have in common (the same
@@ -907,9 +908,9 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
 // tile's keys and values from 4 bits to f16, once for the block, and leaves them in
 // LDS, the next tile's while this one's products run; codes are loaded another tile
 // ahead.
-//   Its products bound it (two for a term: hi and lo): a prompt of 3999 takes 254 us, the products
-// alone, at the rate that the card's power allows, 226; matrix units 48 % busy by cycles, vector units 42.
-// Of 8 x 250 tokens over 1500 + 250 (97 us) 380 blocks have rows: a second one on half of the CUs.
+//   Its products bound it (two for a term: hi and lo): a prompt of 3999 takes 263 us, the products
+// alone, at the rate that the card's power allows, 226; matrix units 48 % busy by cycles, vector units 46.
+// Of 8 x 250 tokens over 1500 + 250 (100 us) 380 blocks have rows: a second one on half of the CUs.
 //   v_mfma_f32_32x32x16_f16, S^T = K Q^T and O^T += V^T P^T, a lane holds one row
 // (lane % 32).  Values stand transposed, a row of 64 tokens per dim, each 16 bytes the
 // 8 tokens that a lane's 8 weights belong to.
@@ -1673,7 +1674,7 @@ __global__ __launch_bounds__(256) void pg_copy_kernel(PgUpdateArgs a, const int3
 }
 
 // The pages in use, the lists of holes and movers, refs.  A short call is three trips over refs (1 layer of a few hundred
-// pages 6 us), a long one memory (36 layers, 12 x 3500 tokens, half of the pages moved: 270 to 280 us, 1.36 GB: 4.9 TB/s).  MOVES (arrays out apart from those in, and few enough pages):
+// pages 6 us), a long one memory (36 layers, 12 x 3500 tokens, half of the pages moved: 270 to 290 us, 1.36 GB: 4.7 to 5 TB/s).  MOVES (arrays out apart from those in, and few enough pages):
 // every block works them out in its LDS, and all of them move pages and rewrite the table; else one block leaves the
 // lists in the workspace.
 template <bool MOVES>
@@ -1846,7 +1847,7 @@ hipError_t launch_pg_attend(uint32_t hd, PgAttendArgs pa, const PgWorkspace& w, 
   sp.tiles = many ? (rows + 15) / 16 : sp.row_tiles;
   sp.shift = two ? 5 : 4;
   const uint32_t kt = many ? 64 : 32, lots = a.s.G * sp.row_tiles;
-  const uint32_t most = (a.c.cap + kt - 1) / kt * (many || sp.of_request ? 1u : min(a.c.R, (tile_rows - 1) / per + 1));  // key tiles of a row tile, at most
+  const uint32_t most = (a.c.cap + kt - 1) / kt * (many || sp.of_request ? 1u : min(a.c.R, (tile_rows - 1) / per + 1));  // key tiles of a row tile (one that begins inside a request may have a request more)
   // Blocks of the step kernel, by the key tiles that a wave of 256 would walk at most: short runs end sooner with fewer
   // states to join, long ones want more waves to take turns.  256 : 512 : 768 blocks, us: 8 x 1 over 1500 + 512 (4 tiles) 13 :
   // 17 : 21, 16 x 1 over 1000 (5) 17 : 18 : 21, 1 x 1 over 30000 (7) 21 : 20 : 22, 16 x 1 over 6000 (24) 44 : 35 : 34, over

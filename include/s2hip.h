@@ -485,13 +485,14 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * of its row no number, in a key all of them, with the weights that the row
  * gives; so do scores that are all below the range of f32.  The shared prefix is
  * read once for several requests' queries.  out must not overlap q.
- *   Products and sums are f32 or better, but for f32 caches where each request
- * brings 32 rows or more to a kv head (n_tokens heads / kv_heads: one token of 32
- * heads over one does) and the capacities make a call large, and for the weights
- * of calls whose scores are too many to be kept (by rows and capacities; a step
- * over large caches can be one): there each term is exact to 2^-22, or to 2^-39
- * of the largest element of the key, the value and the query that it comes from
- * and of the values that its token sees.  Values of f32 caches below 2^-80 may
+ *   Products and sums are f32 or better, but for queries and weights over f16
+ * caches, for f32 caches where each request brings 32 rows or more to a kv head
+ * (n_tokens heads / kv_heads: one token of 32 heads over one does) and the
+ * capacities make a call large, and for the weights of calls whose scores are too
+ * many to be kept (by rows and capacities; a step over large caches can be one):
+ * there each term is exact to 2^-22, or to 2^-39 of the largest element of the
+ * key, the value and the query that it comes from and of the values that its token
+ * sees, and a weight to 2^-22 or 2^-31 of the largest of its row.  Values of f32 caches below 2^-80 may
  * count as 0.  Which kernels run, and so the last bits, goes by the view's
  * capacities and prefix_len, not only by the lengths in use. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
@@ -642,7 +643,8 @@ int32_t s2hip_pages_append(s2hip_pages* pages, const s2hip_pages_view* view, con
  * several of them.
  * Queries and weights are taken as two f16 parts: exact to 2^-22, or to 2^-38 of the
  * largest element of the query and 2^-39 of the largest weight of the row.  Sums are
- * f32. */
+ * f32.  Which kernels run, and so the time and the last bits, goes by n_tokens, requests
+ * and table_pages, not by the lengths in use. */
 int32_t s2hip_pages_attend(s2hip_pages* pages, const s2hip_pages_view* view, const float* q, uint32_t n_tokens,
                            float* out, void* stream, char* err, size_t err_cap);
 /* The rows made anew, all at once: row b becomes the first keep[b] tokens (all, where it
