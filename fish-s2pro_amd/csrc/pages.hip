@@ -264,12 +264,19 @@ __device__ __forceinline__ half8 key8(Bits bits, uint32_t w, _Float16 d) {
   const half2v a = elements<0>(bits, w, dd, c), b = elements<1>(bits, w, dd, c), e = elements<2>(bits, w, dd, c), f = elements<3>(bits, w, dd, c);
   return half8{a[0], a[1], b[0], b[1], e[0], e[1], f[0], f[1]};
 }
-// m follows a row's maximum as for the dense caches, but closer behind, and weights are 2^(s - m + LIFT), up to 2^15: the
-// largest of a row is 2^14 or more, and the lo part of a small one, of whole 2^-24, is exact to 2^-39 of it.  (Where one key
-// weighs e^16 times as much as any other and its value is 0, the output is the others': with m up to 2^8 behind and a lift of
-// 6 it was off by a thousandth.)  o is rescaled more often: slack and lift 1 14 : 4 11 : 8 6, us: 1 x 3999
-// 262.8 : 258.7 : 257.8, 8 x 250 over 1500 + 250 102.5 : 100.5 : 100.8, 16 x 1 over 32001 116.4 : 116.1 : 115.9.
+// Weights are 2^(s - m), up to 2^15: m, a whole number, follows LIFT below a row's maximum, by BEHIND at most.  So the largest
+// of a row is 2^14 or more, and the lo part of a small one, of whole 2^-24, is exact to 2^-39 of it.  (Where one key weighs e^16
+// times as much as any other and its value is 0, the output is the others': with a lift of 6, the maximum up to 2^8 behind, it was
+// off by a thousandth.)  o is rescaled more often: lift and slack 14 1 : 11 4 : 6 8, us: 1 x 3999 262.8 : 258.7 : 257.8, 8 x 250
+// over 1500 + 250 102.5 : 100.5 : 100.8, 16 x 1 over 32001 116.4 : 116.1 : 115.9.
 constexpr float LIFT = 14.0f, BEHIND = 1.0f;
+
+// The m of a maximum.  From 2^25 on f32 has every 4th whole number or fewer, and LIFT less may be 16 less: a weight of 2^16, which
+// is no f16 number, so the maximum itself then.
+__device__ __forceinline__ float base_of(float most) {
+  const float to = floorf(most) - LIFT;
+  return most - to > LIFT + BEHIND ? to + 16.0f : to;
+}
 
 // Two weights' f16 parts and what those leave of them (f16 too: 2^-22 of the weight, or 2^-25), both in one register each.
 struct WeightParts {
@@ -785,16 +792,16 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
       float top = fmaxf(fmaxf(s[r][0][0], s[r][0][1]), s[r][0][2]), top1 = fmaxf(fmaxf(s[r][1][0], s[r][1][1]), s[r][1][2]);
       top = fmaxf(fmaxf(top, s[r][0][3]), fmaxf(top1, s[r][1][3]));
       const float mn = mine[r] ? fmaxf(m[r], quarter_max(top) * unscale[r]) : m[r];
-      const bool up = mn > m[r] + BEHIND;
+      const bool up = mn - m[r] > LIFT + BEHIND;
       if (__any(up)) {
-        const float to = up ? floorf(mn) : m[r], f = up ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
+        const float to = up ? base_of(mn) : m[r], f = up ? __builtin_amdgcn_exp2f(m[r] - to) : 1.0f;
 #pragma unroll
         for (int c = 0; c < OT; ++c) o[r][c] *= f;
         l[r] *= f;
         m[r] = to;
       }
       // (a weight of a row that is not of the request: 2^-infinity)
-      const float bias = mine[r] ? LIFT - (m[r] == -INFINITY ? 0.0f : m[r]) : -INFINITY;
+      const float bias = mine[r] ? (m[r] == -INFINITY ? 0.0f : -m[r]) : -INFINITY;
       float sum[2] = {0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -896,7 +903,7 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
         *reinterpret_cast<floatx4*>(dst + d0 + 64 * c) = x * inv;
       }
       if (tid % 16 == 0 && !last) {
-        sp.ml[2 * part] = M_row - LIFT;
+        sp.ml[2 * part] = M_row;
         sp.ml[2 * part + 1] = L_row;
       }
     }
@@ -1173,15 +1180,15 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       }
       top = fmaxf(top, top1) * unscale;
       const float mn = fmaxf(m, half_reduce(top, [](float p, float q) { return fmaxf(p, q); }));
-      const bool up = mn > m + BEHIND;
+      const bool up = mn - m > LIFT + BEHIND;
       if (__any(up)) {
-        const float to = up ? floorf(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
+        const float to = up ? base_of(mn) : m, f = up ? __builtin_amdgcn_exp2f(m - to) : 1.0f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
         l *= f;
         m = to;
       }
-      const float bias = LIFT - (m == -INFINITY ? 0.0f : m);
+      const float bias = m == -INFINITY ? 0.0f : -m;
       if (gone >> 8) {  // values of no number
         asm volatile("");
 #pragma unroll
@@ -1254,7 +1261,7 @@ __global__ __launch_bounds__(256, 2) void pg_tile_kernel(PgAttendArgs pa, PgShar
       *reinterpret_cast<floatx4*>(dst + 32 * dt + 8 * c + 4 * h2) =
           floatx4{o[dt][4 * c] * f, o[dt][4 * c + 1] * f, o[dt][4 * c + 2] * f, o[dt][4 * c + 3] * f};
   if (h2 == 0 && !last) {
-    sp.ml[2 * part] = m - LIFT;
+    sp.ml[2 * part] = m;
     sp.ml[2 * part + 1] = l;
   }
 }

@@ -428,6 +428,42 @@ def test_attend_sink(gap, n, room, hd):
     assert p.ops.errors(stream()) == 0
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("room", [None, 4000])
+@pytest.mark.parametrize("n", [1, 5, 40])
+@pytest.mark.parametrize("below", [False, True])  # 0: all scores are negative
+def test_attend_large_scores(below, n, room, hd):
+    """Scores of 2^12 to 2^40 (where f32 has whole numbers, then every 2nd, 4th ..): the largest, a sixth or more above the others,
+    takes all of the weight, and its value comes out."""
+    p = Pool((8, 2, hd), 16, [n + 1000, n + 90, n + 6], [n] * 3, seed=n, width=room)
+    r = np.random.default_rng(n)
+    pool, best = p.pool_h.copy(), 5
+    code = np.full(hd, 8)
+    zero = code, np.zeros(hd // 32)
+    for b, row in enumerate(p.table_h):
+        for s in range(p.lens_h[b]):
+            for g in range(2):
+                part, lay = pool[row[s // 16], g], p.lay
+                at, shift = lay.key[0][s % 16, :32], lay.key[1][s % 16, :32]  # the first group: one dim, the other groups' scales are 0
+                part[lay.key_scale[s % 16][:, None] + np.arange(2)] = 0
+                part[lay.key_scale[s % 16, 0] + np.arange(2)] = np.array([1.0], np.float16).view(np.uint8)
+                c = (7 if s == best else r.integers(-8, 7)) if not below else (-1 if s == best else -r.integers(2, 9))
+                part[at] = 0x88
+                part[at[0]] = (0x88 & ~(15 << int(shift[0])) & 255) | int(c + 8) << int(shift[0])
+    p.pool.copy_(torch.from_numpy(pool))
+    v = p.dense()[1]
+    want = v[:, :, best].repeat_interleave(4, 1)[:, None].expand(p.out.shape)
+    mantissa = 1 + torch.rand(p.q.shape[:3], generator=gen(n), device="cuda")
+    for e in range(12, 40):
+        p.q.zero_()
+        p.q[..., 0] = mantissa * 2.0**e
+        p.out.fill_(7.0)
+        out = p.attend()
+        far = (out.double() - want).abs()
+        assert bool((far <= 4 * U * want.abs()).all()), (e, far.max().item())
+    assert p.ops.errors(stream()) == 0
+
+
 def test_attend_offsets_beyond_32_bits():
     """Pages that lie more than 4 GiB into the pool."""
     page, hd, G = 128, 128, 8
