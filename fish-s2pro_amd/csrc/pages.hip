@@ -915,8 +915,8 @@ __global__ __launch_bounds__(64 * STEP_WAVES, RG == 1 ? 3 : 2) void pg_step_kern
 // tile's keys and values from 4 bits to f16, once for the block, and leaves them in
 // LDS, the next tile's while this one's products run; codes are loaded another tile
 // ahead.
-//   Its products bound it (two for a term: hi and lo): a prompt of 3999 takes 263 us, the products
-// alone, at the rate that the card's power allows, 226; matrix units 48 % busy by cycles, vector units 46.
+//   Its products bound it (two for a term: hi and lo): a prompt of 3999 takes 255 to 263 us by the card,
+// the products alone, at the rate that the card's power allows, 226; matrix units 48 % busy by cycles, vector units 46.
 // Of 8 x 250 tokens over 1500 + 250 (100 us) 380 blocks have rows: a second one on half of the CUs.
 //   v_mfma_f32_32x32x16_f16, S^T = K Q^T and O^T += V^T P^T, a lane holds one row
 // (lane % 32).  Values stand transposed, a row of 64 tokens per dim, each 16 bytes the
