@@ -66,8 +66,8 @@ using Elem = std::conditional_t<KH, _Float16, float>;
 // 2^SLACK and the o registers are hardly ever rescaled.  It is a whole number, so
 // that taking it off and the factors between states round nothing, and each row's
 // goes by the keys that the row sees alone.  f16 parts of
-// weights are of 2^(s - m + F16_LIFT), up to 2^14: the lo part of a small weight is
-// exact to 2^-25, 2^-31 of the largest.  The o of f32 values leave (and in
+// weights are of 2^(s - m + F16_LIFT), up to 2^14: the hi and the lo part of a small
+// weight are exact to 2^-25 each, together 2^-30 of the largest.  The o of f32 values leave (and in
 // kv_step_kernel grow) times F32_DOWN: 65536 weights then add no more than the
 // largest value.
 constexpr float SLACK = 8.0f, F16_LIFT = 6.0f, F32_DOWN = 0x1p-30f, F32_UP = 0x1p30f;

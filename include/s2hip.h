@@ -492,8 +492,8 @@ int32_t s2hip_kv_append(s2hip_kv* kv, const s2hip_kv_view* view, const float* qk
  * many to be kept (by rows and capacities; a step over large caches can be one):
  * there each term is exact to 2^-22, or to 2^-39 of the largest element of the
  * key, the value and the query that it comes from and of the values that its token
- * sees, and a weight to 2^-22 or 2^-31 of the largest of its row.  Values of f32 caches below 2^-80 may
- * count as 0.  Which kernels run, and so the last bits, goes by the view's
+ * sees, and a weight to 2^-22 or 2^-30 of the largest of its row.  Values of f32
+ * caches below 2^-80 may count as 0.  Which kernels run, and so the last bits, goes by the view's
  * capacities and prefix_len, not only by the lengths in use. */
 int32_t s2hip_kv_attend(s2hip_kv* kv, const s2hip_kv_view* view, const float* q, uint32_t n_tokens, float* out,
                         void* stream, char* err, size_t err_cap);

@@ -1162,3 +1162,26 @@ def test_step_weights_computed_once_more(f16):
     used = (torch.arange(b.cap, device="cuda")[None, None] < b.lens[:, None, None]).expand(w.shape)
     assert bool(((w.double() - want[2]).abs() <= want[3] + U * want[2])[used].all())
     assert bool(((pw.double() - want[4]).abs() <= want[5] + U * want[4]).all())
+
+
+@pytest.mark.parametrize("cap", [None, 32768])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 40, 300])
+@pytest.mark.parametrize("gap", [8, 16, 24])
+def test_attend_sink(gap, n, f16, cap):
+    """A first key that outweighs all others together and whose value is 0: the output is the others'.  Weights as two f16 parts
+    are held to 2^-30 of the largest of their row: it is 2^6 or above; a small one's upper 11 bits and the rest become f16 numbers,
+    each off by up to half a step of the least ones, 2^-25, so 2^-24 together.  Beside that the bounds of sums in f32, and 2^-22 or
+    2^-39 of what a token sees for parts of keys and values."""
+    b = Batch((8, 2, 128), f16, [n + 1000, n + 90, n + 1], [n] * 3, cap=cap, seed=gap + n, spread=0.15)
+    sign = torch.where(torch.rand(128, generator=gen(gap), device="cuda") < 0.5, -7.0, 7.0)
+    b.k *= 0.6
+    b.k[:, :, 0], b.v[:, :, 0] = sign.to(b.k.dtype), 0
+    b.q += sign * (gap / 49 / math.sqrt(128))
+    want = b.expect()
+    for r in range(3):
+        v = b.v[r, :, : b.lens_h[r]].double().abs()
+        upto = v.cumsum(1)[:, b.lens_h[r] - n :]  # [G][n][hd]: of the values that a token sees
+        want[1][r] += (2.0**-30 * upto + 2.0**-38 * v.amax((1, 2), keepdim=True)).transpose(0, 1).repeat_interleave(4, 1)
+    b.check(b.attend(), want)
+    assert b.ops.errors(stream()) == 0
